@@ -515,6 +515,122 @@ int ponni_plan_host_model(ponni_plan plan, ponni_device_model* out);
 int ponni_forward_host(ponni_plan plan, const void* x, int64_t ld_in, void* y, int64_t ld_out, int64_t batch,
                        int32_t threads);
 
+/* --- routing and expert networks ------------------------------------------- */
+
+/* Operators without a counterpart in the reference: a batch whose samples go
+ * through different networks of one architecture (a mixture of experts, an
+ * emulator per regime), and weights and activations in 4 bits.  Their work
+ * buffers are the caller's: a call keeps nothing from one to the next, so
+ * calls on different streams and captured graphs need only have buffers of
+ * their own.  Every call is asynchronous on `stream` and can be captured,
+ * except where it says otherwise. */
+
+/* Where the samples of a batch go: filled by ponni_route, or by the caller.
+ * Device arrays, owned by the caller.  The k * batch assignments are sorted by
+ * expert, within an expert by sample; those of expert e are the sorted columns
+ * offsets[e] <= c < offsets[e + 1]. */
+typedef struct ponni_routing {
+  int32_t num_experts; /* 1 .. PONNI_MAX_EXPERTS                                       */
+  int32_t top_k;       /* 1 .. min(PONNI_MAX_TOP_K, num_experts)                        */
+  int64_t batch;       /* top_k * batch <= INT32_MAX                                    */
+  int32_t* experts;    /* [top_k, batch]: the sample's j-th expert, -1 for none         */
+  float* weights;      /* [top_k, batch]: its weight, 0 for none                        */
+  int32_t* slots;      /* [top_k, batch]: its sorted column, -1 for none                */
+  int32_t* source;     /* [top_k * batch]: a sorted column's sample, -1 past the last   */
+  int32_t* offsets;    /* [num_experts + 1]                                             */
+} ponni_routing;
+#define PONNI_MAX_EXPERTS 1024
+#define PONNI_MAX_TOP_K 16
+
+/* The top_k experts of each sample from scores [num_experts, batch] of `dtype`
+ * (F32, F16, BF16) with row stride ld: the largest scores, in descending
+ * order, of equal ones that of the lower index first.  A score of -inf or NaN rules the
+ * expert out for that sample; a sample may have fewer than top_k experts, or
+ * none.  weights[j, b] = exp(s_j - max) / sum, the sum over the sample's chosen experts
+ * (PONNI_ROUTE_CHOSEN) or over all that are not ruled out (PONNI_ROUTE_ALL), in fp32;
+ * scores of +inf share the weight equally.  The order of the results does
+ * not depend on the order of execution.  `workspace`: device memory of at
+ * least ponni_route_workspace_bytes, at a multiple of 16 bytes. */
+#define PONNI_ROUTE_CHOSEN 0
+#define PONNI_ROUTE_ALL 1
+int ponni_route(const void* scores, int64_t ld, int32_t dtype, int32_t normalize, const ponni_routing* routing,
+                void* workspace, int64_t workspace_bytes, hipStream_t stream);
+/* (-1 for sizes that ponni_route refuses) */
+int64_t ponni_route_workspace_bytes(int32_t num_experts, int32_t top_k, int64_t batch);
+
+/* Microscaled 4-bit rows (the OCP MXFP4 format): 32 consecutive features of a
+ * sample share a scale 2^(s - 127), s = 255 for NaN, and are held as sign, two exponent
+ * bits and one mantissa bit: 0, 0.5, 1, 1.5, 2, 3, 4, 6.  Sample c of a
+ * [features, columns] array is
+ *   codes  + c * ponni_mx4_code_bytes(features):  feature f in the low (even f) or
+ *                                                 high half of byte f / 2
+ *   scales + c * ponni_mx4_scale_bytes(features): feature f's scale in byte f / 32
+ * with codes and scales zero past the last feature, up to a multiple of 128.
+ * codes and scales are device memory at multiples of 16 bytes. */
+int64_t ponni_mx4_code_bytes(int64_t features);
+int64_t ponni_mx4_scale_bytes(int64_t features);
+
+/* x [features, columns] of `dtype` (F32, F16, BF16), row stride ld, as 4-bit
+ * rows.  A block's scale is 2^(floor(log2 a) - 2), a its largest magnitude, at
+ * least 2^-127; its elements are x / scale rounded to nearest, ties to the even
+ * code, magnitudes beyond 6 to 6.  A block that holds NaN or an infinity is NaN. */
+int ponni_mx4_quantize(const void* x, int64_t ld, int32_t dtype, int64_t features, int64_t columns, void* codes,
+                       void* scales, hipStream_t stream);
+/* The values that 4-bit rows stand for, as y [features, columns] of `dtype`. */
+int ponni_mx4_dequantize(const void* codes, const void* scales, int64_t features, int64_t columns, void* y, int64_t ld,
+                         int32_t dtype, hipStream_t stream);
+
+typedef struct ponni_experts_s* ponni_experts;
+
+/* How the layers' operands are held. */
+#define PONNI_WEIGHTS_SAME 0 /* weights and states in the model's type                  */
+#define PONNI_WEIGHTS_MX4 1  /* both in 4-bit blocks along the contracted features: weights
+                                when they are set, each layer's input from its fp32 value;
+                                x and y F16 or BF16                                     */
+
+/* num_experts networks of one architecture: `layers` is a chain of
+ * PONNI_LAYER_MATVEC, each followed by an optional PONNI_LAYER_BIAS and an optional activation
+ * (RELU, LEAKY_RELU, GELU, SILU, SIGMOID, TANH), with the sizes of one
+ * expert, up to 65536 features.  dtype F32, F16 or BF16: the type of x, y and (PONNI_WEIGHTS_SAME)
+ * the products' operands; sums, biases and activations are fp32.  num_experts = 1
+ * is a plain dense chain.  Touches no device. */
+int ponni_experts_create(const ponni_layer_desc* layers, int32_t num_layers, int32_t num_experts, int32_t dtype,
+                         int32_t weights, ponni_experts* out_experts);
+void ponni_experts_destroy(ponni_experts experts);
+
+/* All experts' parameters of a layer: MATVEC W [num_experts, n_in, n_out], BIAS
+ * b [num_experts, n], contiguous, of `dtype` (F32, F64, F16, BF16), in host or
+ * device memory (of the current device, which the object is bound to from the
+ * first call on).  Device memory is read on `stream`.  Weights are rounded to
+ * the model's operand type.  Synchronous with respect to the host; not for
+ * captured streams.  A bias that was never set is zero. */
+int ponni_experts_set_layer_params(ponni_experts experts, int32_t layer, const void* values, int32_t dtype,
+                                   int64_t count, int32_t on_device, hipStream_t stream);
+int64_t ponni_experts_layer_param_count(ponni_experts experts, int32_t layer);
+
+/* y[:, c] = chain of expert e at x[:, c] for offsets[e] <= c < offsets[e + 1]: x [n_in,
+ * columns] and y [n_out, columns] with row strides ld_in and ld_out, columns
+ * sorted by expert.  offsets: device array [num_experts + 1], ascending, of values in
+ * 0 .. columns; null with one expert: all columns.  Columns in no group are
+ * left as they were.  Groups may be empty.  x, y and the workspace must not overlap. */
+int ponni_experts_forward(ponni_experts experts, const void* x, int64_t ld_in, const int32_t* offsets, void* y,
+                          int64_t ld_out, int64_t columns, void* workspace, int64_t workspace_bytes,
+                          hipStream_t stream);
+/* The same of x as 4-bit rows (PONNI_WEIGHTS_MX4). */
+int ponni_experts_forward_mx4(ponni_experts experts, const void* codes, const void* scales, const int32_t* offsets,
+                              void* y, int64_t ld_out, int64_t columns, void* workspace, int64_t workspace_bytes,
+                              hipStream_t stream);
+int64_t ponni_experts_workspace_bytes(ponni_experts experts, int64_t columns);
+
+/* y[:, b] = sum over j, in that order, of weights[j, b] * chain of expert experts[j, b] at x[:, b],
+ * x [n_in, batch], y [n_out, batch]; a sample without experts gives zero.
+ * Reads routing->weights, slots, source and offsets.  The chains' outputs are
+ * held in the model's type, their sum in fp32. */
+int ponni_experts_forward_mixture(ponni_experts experts, const void* x, int64_t ld_in, const ponni_routing* routing,
+                                  void* y, int64_t ld_out, void* workspace, int64_t workspace_bytes,
+                                  hipStream_t stream);
+int64_t ponni_experts_mixture_workspace_bytes(ponni_experts experts, int32_t top_k, int64_t batch);
+
 /* --- synthetic data (bench and tests) ------------------------------------- */
 
 /* Fill n elements of a device buffer of `dtype` with the counter-based

@@ -13,5 +13,9 @@ from .model import (  # noqa: F401
     Save_State, Selu, Sigmoid, Silu, Softmax, Softplus, Tanh, concat_params, create_inference_model, descs,
     fill_synthetic,
 )
+from .experts import (  # noqa: F401
+    ExpertBias, ExpertInference, ExpertMatvec, MixtureOfExperts, Mx4, Routing, create_expert_model, quantize_mx4,
+    route_experts,
+)
 
 __all__ = [n for n in dir() if not n.startswith("_")] + ["_abi"]

@@ -139,6 +139,18 @@ class DeviceModel(ctypes.Structure):
                 ("slot_rows", ctypes.c_void_p)]
 
 
+MAX_EXPERTS, MAX_TOP_K = 1024, 16
+ROUTE_CHOSEN, ROUTE_ALL = 0, 1
+WEIGHTS_SAME, WEIGHTS_MX4 = 0, 1
+
+
+class RoutingArrays(ctypes.Structure):
+    """ponni_routing (include/ponni_hip.h)."""
+    _fields_ = [("num_experts", ctypes.c_int32), ("top_k", ctypes.c_int32), ("batch", ctypes.c_int64),
+                ("experts", ctypes.c_void_p), ("weights", ctypes.c_void_p), ("slots", ctypes.c_void_p),
+                ("source", ctypes.c_void_p), ("offsets", ctypes.c_void_p)]
+
+
 def lib() -> ctypes.CDLL:
     """Load the in-tree libponni_hip.so; fail loudly when it is missing."""
     global _lib
@@ -219,6 +231,37 @@ def lib() -> ctypes.CDLL:
                                            ctypes.c_char_p, ctypes.c_char_p]
     L.ponni_file_read_tensors.restype = ctypes.c_int
     L.ponni_file_read_tensors.argtypes = [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(TensorSpec), i32, vp, i32]
+    routing = ctypes.POINTER(RoutingArrays)
+    L.ponni_route.restype = ctypes.c_int
+    L.ponni_route.argtypes = [vp, i64, i32, i32, routing, vp, i64, vp]
+    L.ponni_route_workspace_bytes.restype = i64
+    L.ponni_route_workspace_bytes.argtypes = [i32, i32, i64]
+    L.ponni_mx4_code_bytes.restype = i64
+    L.ponni_mx4_code_bytes.argtypes = [i64]
+    L.ponni_mx4_scale_bytes.restype = i64
+    L.ponni_mx4_scale_bytes.argtypes = [i64]
+    L.ponni_mx4_quantize.restype = ctypes.c_int
+    L.ponni_mx4_quantize.argtypes = [vp, i64, i32, i64, i64, vp, vp, vp]
+    L.ponni_mx4_dequantize.restype = ctypes.c_int
+    L.ponni_mx4_dequantize.argtypes = [vp, vp, i64, i64, vp, i64, i32, vp]
+    L.ponni_experts_create.restype = ctypes.c_int
+    L.ponni_experts_create.argtypes = [ctypes.POINTER(LayerDesc), i32, i32, i32, i32, ctypes.POINTER(vp)]
+    L.ponni_experts_destroy.restype = None
+    L.ponni_experts_destroy.argtypes = [vp]
+    L.ponni_experts_set_layer_params.restype = ctypes.c_int
+    L.ponni_experts_set_layer_params.argtypes = [vp, i32, vp, i32, i64, i32, vp]
+    L.ponni_experts_layer_param_count.restype = i64
+    L.ponni_experts_layer_param_count.argtypes = [vp, i32]
+    L.ponni_experts_forward.restype = ctypes.c_int
+    L.ponni_experts_forward.argtypes = [vp, vp, i64, vp, vp, i64, i64, vp, i64, vp]
+    L.ponni_experts_forward_mx4.restype = ctypes.c_int
+    L.ponni_experts_forward_mx4.argtypes = [vp, vp, vp, vp, vp, i64, i64, vp, i64, vp]
+    L.ponni_experts_workspace_bytes.restype = i64
+    L.ponni_experts_workspace_bytes.argtypes = [vp, i64]
+    L.ponni_experts_forward_mixture.restype = ctypes.c_int
+    L.ponni_experts_forward_mixture.argtypes = [vp, vp, i64, routing, vp, i64, vp, i64, vp]
+    L.ponni_experts_mixture_workspace_bytes.restype = i64
+    L.ponni_experts_mixture_workspace_bytes.argtypes = [vp, i32, i64]
     _lib = L
     return L
 

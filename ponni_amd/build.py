@@ -34,6 +34,10 @@ SOURCES = [
     "static_scratch.hip",
     "kernels_gather.hip",
     "kernels_peaks.hip",
+    "experts.cpp",
+    "kernels_experts.hip",
+    "kernels_route.hip",
+    "kernels_mx4.hip",
 ]
 
 # Headers embedded in the library for the run-time (hipRTC) compiler.

@@ -1,0 +1,501 @@
+// Layers of expert networks over columns grouped by expert:
+// y[f, c] = act(bias_e[f] + sum_k W_e[k][f] x[k, c]), e the expert whose group
+// holds column c.
+//
+// Operands are fragments of 16 bytes: 8 features of a 16-bit type, 4 of fp32,
+// 32 of 4 bits.  Samples are rows, 64 bytes (4 fragments) a contraction step,
+// so that a column taken from anywhere (a mixture gathers its samples by
+// expert) is one whole 64-byte piece.  Weights are packed in fragment order.
+// Output features are dealt to the MFMA tiles of a block of 64 so that a lane,
+// which holds rows 4g .. 4g + 3 of every 16 x 16 tile, holds 16 consecutive
+// features 16g + 4i + e of its column: rows are written in whole 16-byte
+// pieces from the accumulators, 128 bytes of a row by the four lane groups.
+//
+// A workgroup computes 16 MI WM features x 16 NJ WN columns of one group; a
+// step's weights and rows go from memory straight into LDS two steps ahead,
+// one barrier a step.
+#include <hip/hip_runtime.h>
+
+#include <type_traits>
+
+#include "activations.h"
+#include "experts.h"
+#include "lds_requests.h"
+#include "operand_types.h"
+#include "program.h"
+
+namespace ponni_hip {
+namespace {
+
+typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) void* lds_void;
+
+// acc += A B for one step's fragments of a 16 x 16 tile.  mx4: a_scale holds the
+// scales of the 4 tiles of a block (TILE picks its byte), b_scale the column's in its first byte.
+template <Operand OP, int TILE>
+__device__ inline f32x4 multiply(i32x4 a, i32x4 b, f32x4 acc, int a_scale, int b_scale) {
+  if constexpr (OP == OPERAND_F16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), acc, 0, 0, 0);
+  } else if constexpr (OP == OPERAND_BF16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), acc, 0, 0, 0);
+  } else if constexpr (OP == OPERAND_MX4) {
+    i32x8 const a8 = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, b8 = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, acc, 4, 4, TILE, a_scale, 0, b_scale);
+  } else {
+    f32x4 const af = __builtin_bit_cast(f32x4, a), bf = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int e = 0; e < 4; e++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(af[e], bf[e], acc, 0, 0, 0);
+    return acc;
+  }
+}
+
+// Columns of an expert's group, from offsets that a caller's program wrote:
+// whatever they hold, a group lies within [0, columns).
+struct Group {
+  int32_t first, last;
+};
+__device__ inline Group group_of(int32_t const* offsets, int expert, int32_t columns) {
+  auto clamp = [&](int32_t v) { return v < 0 ? 0 : v > columns ? columns : v; };
+  if (offsets == nullptr) return {0, columns};
+  int32_t const a = clamp(offsets[expert]), b = clamp(offsets[expert + 1]);
+  return {a, b < a ? a : b};
+}
+
+struct Tile {
+  int expert;
+  int32_t first, last;  // columns [first, last), at most the tile's width
+  int block;            // of output features
+  bool none;
+};
+
+// This workgroup's tile.  Every group has ceil(columns / width) column tiles; the
+// grid holds as many as any offsets can give.  Each XCD (workgroups go to the
+// eight in turn) takes a contiguous share of the tiles, output blocks of a column
+// tile first: its rows are read into one L2 only, and an expert's weights by few.
+template <int WIDTH>
+__device__ inline Tile find_tile(ContractArgs const& a, int out_blocks) {
+  int const lane = threadIdx.x & 63;
+  int32_t const columns = static_cast<int32_t>(a.columns);
+  auto tiles = [&](int base) {
+    if (base + lane >= a.experts) return 0;
+    Group const g = group_of(a.offsets, base + lane, columns);
+    return int((int64_t(g.last) - g.first + WIDTH - 1) / WIDTH);
+  };
+  auto scan = [&](int n) {  // inclusive, over the wave
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      int const t = __shfl_up(n, d);
+      n += lane >= d ? t : 0;
+    }
+    return n;
+  };
+  int64_t total = 0;
+  for (int base = 0; base < a.experts; base += 64) total += __shfl(scan(tiles(base)), 63);
+  total *= out_blocks;
+  int64_t const q = total / 8, r = total % 8, xcd = blockIdx.x % 8, at = blockIdx.x / 8;
+  Tile t{};
+  t.none = true;
+  if (at >= q + (xcd < r ? 1 : 0)) return t;
+  int64_t const index = xcd * q + (xcd < r ? xcd : r) + at;
+  int column_tile = static_cast<int>(index / out_blocks);
+  t.block = static_cast<int>(index % out_blocks);
+  for (int base = 0; base < a.experts; base += 64) {
+    int const n = tiles(base), end = scan(n);
+    int const all = __shfl(end, 63);
+    if (column_tile < all) {
+      int const l = __builtin_ctzll(__ballot(column_tile < end));
+      t.expert = __builtin_amdgcn_readfirstlane(base + l);
+      int const within = __builtin_amdgcn_readfirstlane(column_tile - (__shfl(end, l) - __shfl(n, l)));
+      Group const g = group_of(a.offsets, t.expert, columns);
+      t.first = g.first + within * WIDTH;
+      t.last = g.last - t.first < WIDTH ? g.last : t.first + WIDTH;
+      t.none = false;
+      return t;
+    }
+    column_tile -= all;
+  }
+  return t;
+}
+
+template <bool Precise, class Each>
+__device__ inline void activate(int act, float slope, Each&& each) {
+  switch (act) {
+    case ACT_RELU: each([](float v) { return act_relu(v); }); break;
+    case ACT_LEAKY_RELU: each([slope](float v) { return act_leaky_relu(v, slope); }); break;
+    case ACT_TANH: each([](float v) { return Precise ? tanh_f32(v) : tanh_half(v); }); break;
+    case ACT_SIGMOID: each([](float v) { return Precise ? sigmoid_f32(v) : act_sigmoid_fast(v); }); break;
+    case ACT_SILU: each([](float v) { return Precise ? silu_f32(v) : act_silu_fast(v); }); break;
+    case ACT_GELU_TANH: each([](float v) { return Precise ? gelu_tanh_f32(v) : act_gelu_tanh_fast(v); }); break;
+    case ACT_GELU_ERF: each([](float v) { return act_gelu_erf(v); }); break;
+    default: break;
+  }
+}
+
+// 16 consecutive features from feature f0 of row `col` (v: zero past n_out).
+template <OutputKind KIND, class S>
+__device__ inline void store_features(ContractArgs const& a, int64_t col, int f0, f32x4 (&v)[4]) {
+  if constexpr (KIND == OUT_FEATURES) {
+    S* __restrict__ y = static_cast<S*>(a.y) + col;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (f0 + 4 * i + e < a.n_out) y[int64_t(f0 + 4 * i + e) * a.ldy] = S(v[i][e]);
+  } else if constexpr (KIND == OUT_ROWS) {
+    typedef S Piece __attribute__((ext_vector_type(16 / sizeof(S))));
+    constexpr int N = 16 / sizeof(S);
+#pragma unroll
+    for (int p = 0; p < 16 / N; p++) {
+      Piece o;
+#pragma unroll
+      for (int e = 0; e < N; e++) o[e] = S(v[(p * N + e) / 4][(p * N + e) % 4]);
+      if (f0 + p * N < a.row_features)
+        *reinterpret_cast<Piece*>(a.y_rows.data + col * a.y_rows.stride + (f0 + p * N) * sizeof(S)) = o;
+    }
+  }
+}
+
+// The same as half a block of 32: lanes 16 apart hold its two halves.
+__device__ inline void store_mx4(ContractArgs const& a, int64_t col, bool valid, int f0, f32x4 (&v)[4]) {
+  float amax = 0.0f;
+  bool finite = true;
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      amax = fmaxf(amax, __builtin_fabsf(v[i][e]));
+      finite = finite && v[i][e] == v[i][e];
+    }
+  if (!finite) amax = __builtin_inff();
+  amax = fmaxf(amax, __shfl_xor(amax, 16));
+  unsigned const scale = mx4_scale(amax);
+  float const inverse = mx4_inverse(scale);
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  i32x2 codes = {0, 0};
+  if (scale != 255u) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) codes[i / 8] |= mx4_code(v[i / 4][i % 4] * inverse) << (4 * (i % 8));
+  }
+  if (!valid || f0 >= a.row_features) return;
+  *reinterpret_cast<i32x2*>(a.y_rows.data + col * a.y_rows.stride + f0 / 2) = codes;
+  if (f0 % kMx4Block == 0)
+    a.y_rows.scales[col * a.y_rows.scale_stride + f0 / kMx4Block] = static_cast<unsigned char>(scale);
+}
+
+constexpr int kSlots = 3;  // steps in LDS: computed, landed, in flight
+
+template <Operand OP, class S, OutputKind KIND, int MI, int NJ, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void contract(ContractArgs a) {
+  static_assert(MI % 4 == 0, "whole blocks of 64 features");
+  constexpr int W = WM * WN, BM = 16 * MI * WM, BN = 16 * NJ * WN;
+  constexpr bool MX = OP == OPERAND_MX4;
+  constexpr int A_BYTES = BM * 64, B_BYTES = BN * 64, AS_BYTES = MX ? BM * 4 : 0, BS_BYTES = MX ? BN * 4 : 0;
+  constexpr int SLOT = A_BYTES + B_BYTES + AS_BYTES + BS_BYTES;
+  constexpr int A_REQ = A_BYTES / 1024 / W, B_REQ = B_BYTES / 1024 / W, S_REQ = MX ? (BM + BN) / 64 / W : 0;
+  constexpr int REQ = A_REQ + B_REQ + S_REQ;
+  static_assert(A_BYTES % (1024 * W) == 0 && B_BYTES % (1024 * W) == 0 && (!MX || (BM + BN) % (64 * W) == 0), "whole requests");
+  __shared__ __attribute__((aligned(16))) char lds[kSlots * SLOT];
+  int const lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int const wm = wave / WN, wn = wave % WN;
+  Tile const t = find_tile<BN>(a, (a.blocks * 64 + BM - 1) / BM);
+  if (t.none) return;
+  unsigned const lds0 = static_cast<unsigned>(reinterpret_cast<uint64_t>((lds_void)lds));
+  int const steps = a.steps;
+
+  // Columns past the tile's last repeat it.
+  auto row_of = [&](int local) {
+    int32_t const col = t.first + local < t.last ? t.first + local : t.last - 1;
+    int64_t const row = a.source != nullptr ? a.source[col] : col;
+    return row < 0 || row >= a.x_rows ? int64_t(0) : row;
+  };
+  auto block_of = [&](int local) {  // (blocks past the last one are computed and dropped)
+    int const b = t.block * (BM / 64) + local;
+    return int64_t(t.expert) * a.blocks + (b < a.blocks ? b : a.blocks - 1);
+  };
+  char const* pa[A_REQ];
+  char const* pb[B_REQ];
+  char const* ps[MX ? S_REQ : 1];
+#pragma unroll
+  for (int r = 0; r < A_REQ; r++) {
+    int const piece = wave + W * r;
+    pa[r] = a.weights + block_of(piece / 4) * steps * 4096 + piece % 4 * 1024 + 16 * lane;
+  }
+#pragma unroll
+  for (int r = 0; r < B_REQ; r++) {
+    int const piece = (wave + W * r) * 64 + lane, col = piece >> 2;
+    // A row's four fragments are kept at places that depend on its column, so
+    // that 16 columns' reads of one fragment fall into different banks.
+    pb[r] = a.x.data + row_of(col) * a.x.stride + 16 * ((piece & 3) ^ ((col >> 2) & 3));
+  }
+  if constexpr (MX) {
+#pragma unroll
+    for (int r = 0; r < S_REQ; r++) {
+      int const q = wave + W * r;
+      ps[r] = q < BM / 64 ? reinterpret_cast<char const*>(a.w_scales) + block_of(q) * steps * 256 + 4 * lane
+                          : reinterpret_cast<char const*>(a.x.scales) + row_of((q - BM / 64) * 64 + lane) * a.x.scale_stride;
+    }
+  }
+  auto request = [&](int s) {
+    unsigned const slot = lds0 + s % kSlots * SLOT;
+#pragma unroll
+    for (int r = 0; r < A_REQ; r++) {
+      dma16(pa[r], slot + (wave + W * r) * 1024);
+      pa[r] += 4096;
+    }
+#pragma unroll
+    for (int r = 0; r < B_REQ; r++) {
+      dma16(pb[r], slot + A_BYTES + (wave + W * r) * 1024);
+      pb[r] += 64;
+    }
+    if constexpr (MX) {
+#pragma unroll
+      for (int r = 0; r < S_REQ; r++) {
+        int const q = wave + W * r;
+        dma4(ps[r], slot + A_BYTES + B_BYTES + q * 256);
+        ps[r] += q < BM / 64 ? 256 : 4;
+      }
+    }
+  };
+  f32x4 acc[MI][NJ];
+#pragma unroll
+  for (int i = 0; i < MI; i++) {
+    // bias of features 16 g + 4 i .. + 3 of the block
+    f32x4 seed = {0, 0, 0, 0};
+    if (a.bias != nullptr)
+      seed = *reinterpret_cast<f32x4 const*>(a.bias + block_of((wm * MI + i) / 4) * 64 + 16 * g + 4 * (i % 4));
+#pragma unroll
+    for (int j = 0; j < NJ; j++) acc[i][j] = seed;
+  }
+  request(0);
+  if (steps > 1) request(1);
+  for (int s = 0; s < steps; s++) {
+    // This wave's requests for step s have landed once only those for step
+    // s + 1 are outstanding; the barrier makes that true of every wave, and
+    // ends every wave's reads of the slot that step s + 2 takes.
+    if (s + 1 < steps) wait_requests<REQ>();
+    else wait_requests<0>();
+    workgroup_barrier();
+    if (s + 2 < steps) request(s + 2);
+    char const* __restrict__ slot = lds + s % kSlots * SLOT;
+    i32x4 av[MI], bv[NJ];
+    int as[MI / 4] = {}, bs[NJ] = {};
+#pragma unroll
+    for (int i = 0; i < MI; i++) av[i] = reinterpret_cast<i32x4 const*>(slot + (wm * MI + i) * 1024)[lane];
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      int const col = 16 * (wn * NJ + j) + c;
+      bv[j] = *reinterpret_cast<i32x4 const*>(slot + A_BYTES + 64 * col + 16 * (g ^ ((c >> 2) & 3)));
+      if constexpr (MX) bs[j] = reinterpret_cast<unsigned char const*>(slot)[A_BYTES + B_BYTES + AS_BYTES + 4 * col + g];
+    }
+    if constexpr (MX) {
+#pragma unroll
+      for (int n = 0; n < MI / 4; n++)
+        as[n] = reinterpret_cast<int const*>(slot + A_BYTES + B_BYTES + (wm * MI / 4 + n) * 256)[lane];
+    }
+#pragma unroll
+    for (int n = 0; n < MI / 4; n++)
+#pragma unroll
+      for (int j = 0; j < NJ; j++) {
+        acc[4 * n][j] = multiply<OP, 0>(av[4 * n], bv[j], acc[4 * n][j], as[n], bs[j]);
+        acc[4 * n + 1][j] = multiply<OP, 1>(av[4 * n + 1], bv[j], acc[4 * n + 1][j], as[n], bs[j]);
+        acc[4 * n + 2][j] = multiply<OP, 2>(av[4 * n + 2], bv[j], acc[4 * n + 2][j], as[n], bs[j]);
+        acc[4 * n + 3][j] = multiply<OP, 3>(av[4 * n + 3], bv[j], acc[4 * n + 3][j], as[n], bs[j]);
+      }
+  }
+  activate<OP == OPERAND_F32>(a.act, a.act_a, [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < MI; i++)
+#pragma unroll
+      for (int j = 0; j < NJ; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[i][j][e] = f(acc[i][j][e]);
+  });
+#pragma unroll
+  for (int n = 0; n < MI / 4; n++) {
+    int const f0 = t.block * BM + (wm * MI / 4 + n) * 64 + 16 * g;
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+      int64_t const col = int64_t(t.first) + 16 * (wn * NJ + j) + c;
+      f32x4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[i][e] = f0 + 4 * i + e < a.n_out ? acc[4 * n + i][j][e] : 0.0f;
+      if constexpr (KIND == OUT_MX4) store_mx4(a, col, col < t.last, f0, v);
+      else if (col < t.last) store_features<KIND, S>(a, col, f0, v);
+    }
+  }
+}
+
+template <Operand OP, class S, OutputKind KIND, int MI, int NJ, int WM, int WN>
+hipError_t launch_tiled(ContractArgs const& a, hipStream_t stream) {
+  constexpr int BM = 16 * MI * WM, BN = 16 * NJ * WN;
+  int64_t const out_blocks = (int64_t(a.blocks) * 64 + BM - 1) / BM;
+  // ceil(n / BN) summed over the groups: at most one more than n / BN for each that has columns
+  int64_t const partial = a.experts < a.columns ? a.experts : a.columns;
+  int64_t const tiles = (a.columns / BN + partial) * out_blocks;
+  if (tiles > INT32_MAX) return hipErrorInvalidValue;
+  // (a share per XCD is rounded up: the grid is whole rounds of the eight)
+  dim3 const grid(static_cast<unsigned>((tiles + 7) / 8 * 8)), block(64 * WM * WN);
+  hipLaunchKernelGGL((contract<OP, S, KIND, MI, NJ, WM, WN>), grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+
+template <Operand OP, class S>
+hipError_t launch_kind(OutputKind kind, ContractArgs const& a, hipStream_t stream) {
+  switch (kind) {
+    case OUT_FEATURES: return launch_tiled<OP, S, OUT_FEATURES, 4, 4, 2, 2>(a, stream);
+    case OUT_ROWS: return launch_tiled<OP, S, OUT_ROWS, 4, 4, 2, 2>(a, stream);
+    default:
+      if constexpr (OP == OPERAND_MX4) return launch_tiled<OP, S, OUT_MX4, 4, 4, 2, 2>(a, stream);
+      return hipErrorInvalidValue;
+  }
+}
+
+// 64 samples x 64 features: a lane sums 8 features of one sample's rows, the
+// tile turns in LDS.
+template <class S>
+__global__ __launch_bounds__(256) void combine(Rows rows, int64_t num_rows, ponni_routing r, int64_t features,
+                                               S* __restrict__ y, int64_t ld) {
+  __shared__ float tile[64][65];  // [feature][sample]
+  int64_t const b0 = int64_t(blockIdx.x) * 64, f0 = int64_t(blockIdx.y) * 64;
+  for (int p = threadIdx.x; p < 64 * 8; p += 256) {
+    int const s = p >> 3, q = (p & 7) * 8;
+    int64_t const b = b0 + s;
+    float sum[8] = {};
+    if (b < r.batch && f0 + q < features)
+      for (int j = 0; j < r.top_k; j++) {
+        int64_t const slot = r.slots[j * r.batch + b];
+        if (slot < 0 || slot >= num_rows) continue;
+        float const w = r.weights[j * r.batch + b];
+        S const* row = reinterpret_cast<S const*>(rows.data + slot * rows.stride) + f0 + q;
+#pragma unroll
+        for (int i = 0; i < 8; i++) sum[i] = fmaf(w, float(row[i]), sum[i]);  // (rows are whole 64-byte pieces)
+      }
+#pragma unroll
+    for (int i = 0; i < 8; i++) tile[q + i][s] = sum[i];
+  }
+  __syncthreads();
+  int const s = threadIdx.x & 63;
+  if (b0 + s >= r.batch) return;
+  for (int f = threadIdx.x >> 6; f < 64 && f0 + f < features; f += 4) y[(f0 + f) * ld + b0 + s] = S(tile[f][s]);
+}
+
+// One lane per 16-byte piece of the packed weights.
+template <Operand OP, class T>
+__global__ __launch_bounds__(256) void pack_weights(T const* __restrict__ w, int64_t experts, int64_t n_in,
+                                                    int64_t n_out, int64_t blocks, int64_t steps, char* weights,
+                                                    unsigned char* scales) {
+  int64_t const piece = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (piece >= experts * blocks * steps * 256) return;
+  int const lane = piece % 64, i = piece / 64 % 4, g = lane >> 4, row = lane & 15;
+  int64_t const step = piece / 256 % steps, block = piece / 256 / steps % blocks, e = piece / 256 / steps / blocks;
+  int64_t const f = block * 64 + 16 * (row >> 2) + 4 * i + (row & 3);
+  constexpr int N = OP == OPERAND_F32 ? 4 : OP == OPERAND_MX4 ? 32 : 8;
+  int64_t const k0 = step * 4 * N + g * N;
+  float v[N];
+#pragma unroll
+  for (int k = 0; k < N; k++) v[k] = f < n_out && k0 + k < n_in ? float(w[(e * n_in + k0 + k) * n_out + f]) : 0.0f;
+  i32x4 out = {0, 0, 0, 0};
+  if constexpr (OP == OPERAND_MX4) {
+    float amax = 0.0f;
+    bool finite = true;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      amax = fmaxf(amax, __builtin_fabsf(v[k]));
+      finite = finite && v[k] == v[k];
+    }
+    unsigned const scale = finite ? mx4_scale(amax) : 255u;
+    float const inverse = mx4_inverse(scale);
+    if (scale != 255u) {
+#pragma unroll
+      for (int k = 0; k < N; k++) out[k / 8] |= mx4_code(v[k] * inverse) << (4 * (k % 8));
+    }
+    scales[(piece / 256 * 64 + lane) * 4 + i] = static_cast<unsigned char>(scale);
+  } else {
+    using S = std::conditional_t<OP == OPERAND_F32, float, std::conditional_t<OP == OPERAND_F16, _Float16, __bf16>>;
+    typedef S Piece __attribute__((ext_vector_type(N)));
+    Piece p;
+#pragma unroll
+    for (int k = 0; k < N; k++) p[k] = S(v[k]);
+    out = __builtin_bit_cast(i32x4, p);
+  }
+  reinterpret_cast<i32x4*>(weights)[piece] = out;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void pack_bias(T const* __restrict__ b, int64_t experts, int64_t n, int64_t padded,
+                                                 float* __restrict__ bias) {
+  int64_t const i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= experts * padded) return;
+  bias[i] = i % padded < n ? float(b[i / padded * n + i % padded]) : 0.0f;
+}
+
+template <class F> bool with_parameter_dtype(int dtype, F&& f) {
+  if (dtype == PONNI_F64) {
+    f(double{});
+    return true;
+  }
+  return with_dtype(dtype, f);
+}
+
+}  // namespace
+
+hipError_t launch_contraction(Operand op, int out_type, OutputKind kind, ContractArgs const& a, hipStream_t stream) {
+  switch (op) {
+    case OPERAND_F32: return launch_kind<OPERAND_F32, float>(kind, a, stream);
+    case OPERAND_F16: return launch_kind<OPERAND_F16, _Float16>(kind, a, stream);
+    case OPERAND_BF16: return launch_kind<OPERAND_BF16, __bf16>(kind, a, stream);
+    default:
+      return out_type == PONNI_F16 ? launch_kind<OPERAND_MX4, _Float16>(kind, a, stream)
+                                   : launch_kind<OPERAND_MX4, __bf16>(kind, a, stream);
+  }
+}
+
+hipError_t launch_combine(int dtype, Rows const& rows, int64_t num_rows, const ponni_routing& r, int64_t features,
+                          void* y, int64_t ld, hipStream_t stream) {
+  dim3 const grid(unsigned((r.batch + 63) / 64), unsigned((features + 63) / 64));
+  with_dtype(dtype, [&](auto s) {
+    using S = decltype(s);
+    hipLaunchKernelGGL(combine<S>, grid, dim3(256), 0, stream, rows, num_rows, r, features, static_cast<S*>(y), ld);
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_pack_weights(Operand op, int dtype, const void* w, int64_t experts, int64_t n_in, int64_t n_out,
+                               int64_t blocks, char* weights, unsigned char* scales, hipStream_t stream) {
+  int64_t const steps = contraction_steps(op, n_in), groups = experts * blocks * steps;
+  if (groups > INT32_MAX) return hipErrorInvalidValue;
+  dim3 const grid(static_cast<unsigned>(groups)), block(256);
+  with_parameter_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, block, 0, stream, static_cast<T const*>(w), experts, n_in, n_out, blocks, steps,
+                         weights, scales);
+    };
+    switch (op) {
+      case OPERAND_F32: launch(pack_weights<OPERAND_F32, T>); break;
+      case OPERAND_F16: launch(pack_weights<OPERAND_F16, T>); break;
+      case OPERAND_BF16: launch(pack_weights<OPERAND_BF16, T>); break;
+      default: launch(pack_weights<OPERAND_MX4, T>); break;
+    }
+  });
+  return hipGetLastError();
+}
+
+hipError_t launch_pack_bias(int dtype, const void* b, int64_t experts, int64_t n, int64_t padded, float* bias,
+                            hipStream_t stream) {
+  int64_t const blocks = (experts * padded + 255) / 256;
+  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  with_parameter_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    hipLaunchKernelGGL(pack_bias<T>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
+                       static_cast<T const*>(b), experts, n, padded, bias);
+  });
+  return hipGetLastError();
+}
+
+}  // namespace ponni_hip

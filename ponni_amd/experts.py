@@ -1,0 +1,394 @@
+"""Routing, expert networks and 4-bit rows over libponni_hip.
+
+    model = create_expert_model(ExpertMatvec(W1), ExpertBias(b1), Silu(n), ExpertMatvec(W2), ExpertBias(b2),
+                                dtype="bf16")              # W [experts, n_in, n_out], b [experts, n_out]
+    y = model.forward_batch_parallel(x, offsets)           # x [n_in, columns], columns sorted by expert
+    routing = route_experts(scores, top_k=2)               # scores [experts, B], e.g. of an Inference model
+    y = model.forward_mixture(x, routing)                  # x [n_in, B]
+
+GPU tensors are [features, columns] with contiguous rows, as for
+Inference.forward_batch_parallel.  Work buffers are allocated by torch for
+each call, on the current stream.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass, field
+from typing import Sequence
+
+import numpy as np
+
+from . import _abi as A
+from .model import _DTYPES, Inference, Layer, _current_stream
+
+_torch = None  # (dtype name -> torch dtype, torch dtype -> ABI code), filled on first use
+
+
+def _types():
+    global _torch
+    if _torch is None:
+        import torch
+
+        _torch = ({"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16},
+                  {torch.float32: A.F32, torch.float16: A.F16, torch.bfloat16: A.BF16, torch.float64: A.F64})
+    return _torch
+
+
+class _on:
+    """The device of a tensor as the current one, where it is not."""
+
+    def __init__(self, t):
+        import torch
+
+        self.index = t.device.index
+        self.device = None if torch.cuda.current_device() == self.index else torch.cuda.device(self.index)
+
+    def __enter__(self):
+        if self.device is not None:
+            self.device.__enter__()
+
+    def __exit__(self, *a):
+        if self.device is not None:
+            self.device.__exit__(*a)
+
+
+def _rows(t, what: str, rows: int | None = None, columns: int | None = None):
+    """Checks a [features, columns] GPU tensor with contiguous rows; its row stride."""
+    if t.dim() != 2 or not t.is_cuda:
+        raise ValueError(f"{what} must be a two-dimensional GPU tensor [features, columns]")
+    if (rows is not None and t.shape[0] != rows) or (columns is not None and t.shape[1] != columns):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected "
+                         f"({'any' if rows is None else rows}, {'any' if columns is None else columns})")
+    if t.shape[1] == 0:
+        raise A.PonniError(A.PONNI_ERR_SHAPE, f"{what} has no columns")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what} needs contiguous rows")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _same_device(t, other, what: str):
+    if t.device != other.device:
+        raise ValueError(f"{what} is on {t.device}, the input on {other.device}")
+
+
+def _int_array(t, shape, other, what: str):
+    import torch
+
+    if t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor of shape {tuple(shape)}")
+    _same_device(t, other, what)
+
+
+# -- routing ---------------------------------------------------------------------------
+
+
+@dataclass(frozen=True)
+class Routing:
+    """Where the samples of a batch go (ponni_routing): experts (int32), weights
+    (float32) and slots (int32) [top_k, batch], source [top_k * batch] and offsets
+    [num_experts + 1] (int32), on the GPU.  From route_experts, or a program's own."""
+
+    experts: "object"
+    weights: "object"
+    slots: "object"
+    source: "object"
+    offsets: "object"
+    checked: bool = field(default=False, repr=False)
+
+    @property
+    def num_experts(self) -> int:
+        return self.offsets.shape[0] - 1
+
+    @property
+    def top_k(self) -> int:
+        return self.slots.shape[0]
+
+    @property
+    def batch(self) -> int:
+        return self.slots.shape[1]
+
+    def arrays(self) -> A.RoutingArrays:
+        if not self.checked:
+            import torch
+
+            if self.slots.dim() != 2 or self.offsets.dim() != 1 or not self.slots.is_cuda:
+                raise ValueError("slots must be a GPU tensor [top_k, batch], offsets [num_experts + 1]")
+            _int_array(self.slots, self.slots.shape, self.slots, "slots")
+            _int_array(self.experts, self.slots.shape, self.slots, "experts")
+            _int_array(self.source, (self.top_k * self.batch,), self.slots, "source")
+            _int_array(self.offsets, self.offsets.shape, self.slots, "offsets")
+            if (self.weights.dtype != torch.float32 or self.weights.shape != self.slots.shape
+                    or not self.weights.is_contiguous()):
+                raise ValueError(f"weights must be a contiguous float32 tensor of shape {tuple(self.slots.shape)}")
+            _same_device(self.weights, self.slots, "weights")
+        return A.RoutingArrays(self.num_experts, self.top_k, self.batch, self.experts.data_ptr(),
+                               self.weights.data_ptr(), self.slots.data_ptr(), self.source.data_ptr(),
+                               self.offsets.data_ptr())
+
+
+def route_experts(scores, top_k: int, normalize: str = "chosen") -> Routing:
+    """The top_k experts of each sample from scores [num_experts, batch] (f32, f16
+    or bf16), and the samples sorted by expert (ponni_route).  normalize: the
+    weights are softmax values over the sample's "chosen" experts or over "all"."""
+    import torch
+
+    codes = _types()[1]
+    ld = _rows(scores, "scores")
+    if scores.dtype not in codes:
+        raise ValueError(f"scores of type {scores.dtype}")
+    if normalize not in ("chosen", "all"):
+        raise ValueError(f"normalize must be 'chosen' or 'all', not {normalize!r}")
+    e, b = scores.shape
+    L = A.lib()
+    need = L.ponni_route_workspace_bytes(e, top_k, b)
+    if need < 0:
+        raise A.PonniError(A.PONNI_ERR_INVALID_ARGUMENT, L.ponni_last_error().decode())
+    n = top_k * b
+    # One allocation: the integer arrays and weights, then the work buffer (16-byte aligned).
+    ints = torch.empty(4 * n + (e + 4) // 4 * 4 + 16 + need // 4, dtype=torch.int32, device=scores.device)
+    at = (4 * n + e + 1 + 3) // 4 * 4
+    r = Routing(ints[:n].view(top_k, b), ints[n:2 * n].view(torch.float32).view(top_k, b),
+                ints[2 * n:3 * n].view(top_k, b), ints[3 * n:4 * n], ints[4 * n:4 * n + e + 1], checked=True)
+    with _on(scores):
+        arrays = r.arrays()
+        A.check(L.ponni_route(scores.data_ptr(), ld, codes[scores.dtype],
+                              A.ROUTE_ALL if normalize == "all" else A.ROUTE_CHOSEN, ctypes.byref(arrays),
+                              ints.data_ptr() + 4 * at, need, _current_stream(scores)))
+    return r
+
+
+# -- 4-bit rows ------------------------------------------------------------------------
+
+
+@dataclass
+class Mx4:
+    """Samples as microscaled 4-bit rows (ponni_mx4_quantize): codes [columns,
+    code bytes] and scales [columns, scale bytes], uint8."""
+
+    codes: "object"
+    scales: "object"
+    features: int
+
+    @property
+    def columns(self) -> int:
+        return self.codes.shape[0]
+
+    def dequantize(self, dtype=None):
+        """The values as a [features, columns] tensor (float32, float16 or bfloat16)."""
+        import torch
+
+        y = torch.empty((self.features, self.columns), dtype=dtype or torch.float32, device=self.codes.device)
+        if y.dtype not in _types()[1]:
+            raise ValueError(f"values of type {y.dtype}")
+        with _on(y):
+            A.check(A.lib().ponni_mx4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), self.features,
+                                                 self.columns, y.data_ptr(), self.columns, _types()[1][y.dtype],
+                                                 _current_stream(y)))
+        return y
+
+
+def quantize_mx4(x) -> Mx4:
+    """x [features, columns] (f32, f16 or bf16) in microscaled 4-bit floating
+    point: blocks of 32 features of a sample share a power-of-two scale."""
+    import torch
+
+    ld = _rows(x, "x")
+    if x.dtype not in _types()[1]:
+        raise ValueError(f"x of type {x.dtype}")
+    k, n = x.shape
+    L = A.lib()
+    q = Mx4(torch.empty((n, L.ponni_mx4_code_bytes(k)), dtype=torch.uint8, device=x.device),
+            torch.empty((n, L.ponni_mx4_scale_bytes(k)), dtype=torch.uint8, device=x.device), k)
+    with _on(x):
+        A.check(L.ponni_mx4_quantize(x.data_ptr(), ld, _types()[1][x.dtype], k, n, q.codes.data_ptr(),
+                                     q.scales.data_ptr(), _current_stream(x)))
+    return q
+
+
+# -- expert networks ---------------------------------------------------------------------
+
+
+def _host_or_device(values, dims: int, what: str):
+    """A contiguous numpy array or torch tensor of `dims` dimensions."""
+    if hasattr(values, "data_ptr"):
+        values = values.detach()
+        v = values.contiguous() if values.dtype in _types()[1] else values.double().contiguous()
+    else:
+        v = np.ascontiguousarray(values)
+        if v.dtype not in (np.float32, np.float64, np.float16):
+            v = v.astype(np.float64)
+    if len(v.shape) != dims:
+        raise ValueError(f"{what} must have {dims} dimensions, got shape {tuple(v.shape)}")
+    return v
+
+
+@dataclass
+class ExpertLayer(Layer):
+    """A layer with parameters of every expert: `values`, a numpy array or torch tensor."""
+
+    values: "object" = None
+
+
+def ExpertMatvec(weights) -> ExpertLayer:
+    """One Matvec per expert: weights [experts, n_in, n_out] (numpy or torch, host or GPU)."""
+    w = _host_or_device(weights, 3, "ExpertMatvec weights")
+    return ExpertLayer(A.LAYER_MATVEC, w.shape[1], w.shape[2], label="Matvec", values=w)
+
+
+def ExpertBias(bias) -> ExpertLayer:
+    """One Bias per expert: bias [experts, n]."""
+    b = _host_or_device(bias, 2, "ExpertBias values")
+    return ExpertLayer(A.LAYER_BIAS, b.shape[1], b.shape[1], label="Bias", values=b)
+
+
+class ExpertInference:
+    """Networks of one architecture, one per expert (ponni_experts).  The layers'
+    arrays are read by the constructor and not kept."""
+
+    def __init__(self, layers: Sequence[Layer], dtype: str = "f32", weights: str = "same"):
+        if weights not in ("same", "mx4"):
+            raise ValueError(f"weights must be 'same' or 'mx4', not {weights!r}")
+        held = [l for l in layers if getattr(l, "values", None) is not None]
+        if not held:
+            raise A.PonniError(A.PONNI_ERR_INVALID_MODEL, "the chain must begin with a Matvec")
+        self.num_experts = int(held[0].values.shape[0])
+        if any(l.values.shape[0] != self.num_experts for l in held):
+            raise A.PonniError(A.PONNI_ERR_INVALID_MODEL, "the layers hold parameters of different numbers of experts")
+        self.dtype, self.weights = dtype, weights
+        self.n_in, self.n_out = layers[0].n_in, layers[-1].n_out
+        descs = (A.LayerDesc * len(layers))(*[l.desc() for l in layers])
+        self._experts = ctypes.c_void_p()
+        A.check(A.lib().ponni_experts_create(descs, len(layers), self.num_experts, _DTYPES[dtype],
+                                             A.WEIGHTS_MX4 if weights == "mx4" else A.WEIGHTS_SAME,
+                                             ctypes.byref(self._experts)))
+        self._pending = [(i, l.values) for i, l in enumerate(layers) if getattr(l, "values", None) is not None]
+        device = next((v.device for _, v in self._pending if hasattr(v, "data_ptr") and v.is_cuda), None)
+        import torch
+
+        if device is not None or torch.cuda.is_available():
+            self._push(device)
+
+    def _push(self, device):
+        import torch
+
+        with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
+            for i, v in self._pending:
+                self.set_layer_params(i, v)
+        self._pending = []
+
+    def __del__(self):
+        e = getattr(self, "_experts", None)
+        if e is not None and e.value:
+            try:
+                A.lib().ponni_experts_destroy(e)
+            except (AttributeError, TypeError):  # interpreter shutdown: the module is gone
+                pass
+            self._experts = None
+
+    def set_layer_params(self, i: int, values) -> None:
+        """All experts' parameters of layer i (numpy or torch, host or GPU)."""
+        if hasattr(values, "data_ptr"):
+            v = values.detach().contiguous()
+            code, ptr, n, on_device = _types()[1][v.dtype], v.data_ptr(), v.numel(), int(v.is_cuda)
+            stream = _current_stream(v) if on_device else 0
+        else:
+            v = np.ascontiguousarray(values)
+            code = {np.dtype(np.float32): A.F32, np.dtype(np.float64): A.F64, np.dtype(np.float16): A.F16}[v.dtype]
+            ptr, n, on_device, stream = v.ctypes.data, v.size, 0, 0
+        A.check(A.lib().ponni_experts_set_layer_params(self._experts, i, ptr, code, n, on_device, stream))
+
+    def get_num_inputs(self) -> int:
+        return self.n_in
+
+    def get_num_outputs(self) -> int:
+        return self.n_out
+
+    def _buffers(self, like, columns, y):
+        import torch
+
+        dtype = _types()[0][self.dtype]
+        if y is None:
+            y = torch.empty((self.n_out, columns), dtype=dtype, device=like.device)
+        ld = _rows(y, "y", self.n_out, columns)
+        if y.dtype != dtype:
+            raise ValueError(f"y is {y.dtype}, the model {dtype}")
+        _same_device(y, like, "y")
+        return y, ld
+
+    def forward_batch_parallel(self, x, offsets=None, y=None):
+        """x [n_in, columns] of the model's type, or Mx4 rows (4-bit weights), columns
+        sorted by expert; offsets int32 [num_experts + 1] on the GPU (None with one
+        expert: all columns).  Returns y [n_out, columns]; columns in no group are
+        left as they were (undefined in a new y)."""
+        import torch
+
+        L = A.lib()
+        rows = isinstance(x, Mx4)
+        if rows:
+            like, columns = x.codes, x.columns
+            if x.features != self.n_in:
+                raise ValueError(f"x has {x.features} features, the model {self.n_in} inputs")
+        else:
+            like, columns = x, x.shape[1] if x.dim() == 2 else 0
+            ld_in = _rows(x, "x", self.n_in)
+            if x.dtype != _types()[0][self.dtype]:
+                raise ValueError(f"x is {x.dtype}, the model {_types()[0][self.dtype]}")
+        if offsets is not None:
+            _int_array(offsets, (self.num_experts + 1,), like, "offsets")
+        y, ld = self._buffers(like, columns, y)
+        need = L.ponni_experts_workspace_bytes(self._experts, columns)
+        work = torch.empty(max(need, 1), dtype=torch.uint8, device=like.device)
+        at = 0 if offsets is None else offsets.data_ptr()
+        with _on(like):
+            stream = _current_stream(like)
+            if rows:
+                A.check(L.ponni_experts_forward_mx4(self._experts, x.codes.data_ptr(), x.scales.data_ptr(), at,
+                                                    y.data_ptr(), ld, columns, work.data_ptr(), need, stream))
+            else:
+                A.check(L.ponni_experts_forward(self._experts, x.data_ptr(), ld_in, at, y.data_ptr(), ld, columns,
+                                                work.data_ptr(), need, stream))
+        return y
+
+    def forward_mixture(self, x, routing: Routing, y=None):
+        """x [n_in, batch]: the weighted sum of each sample's experts (ponni_experts_forward_mixture)."""
+        import torch
+
+        L = A.lib()
+        ld_in = _rows(x, "x", self.n_in, routing.batch)
+        if x.dtype != _types()[0][self.dtype]:
+            raise ValueError(f"x is {x.dtype}, the model {_types()[0][self.dtype]}")
+        _same_device(routing.slots, x, "routing")
+        y, ld = self._buffers(x, routing.batch, y)
+        need = L.ponni_experts_mixture_workspace_bytes(self._experts, routing.top_k, routing.batch)
+        work = torch.empty(max(need, 1), dtype=torch.uint8, device=x.device)
+        with _on(x):
+            arrays = routing.arrays()
+            A.check(L.ponni_experts_forward_mixture(self._experts, x.data_ptr(), ld_in, ctypes.byref(arrays),
+                                                    y.data_ptr(), ld, work.data_ptr(), need, _current_stream(x)))
+        return y
+
+
+def create_expert_model(*layers: Layer, dtype: str = "f32", weights: str = "same") -> ExpertInference:
+    """ExpertMatvec, each followed by an optional ExpertBias and an optional
+    activation.  dtype "f32", "f16" or "bf16"; weights "same" (as dtype) or "mx4"
+    (weights and every layer's input in 4 bits)."""
+    return ExpertInference(layers, dtype=dtype, weights=weights)
+
+
+class MixtureOfExperts:
+    """A router (an Inference model of num_experts outputs), and the experts it chooses among.
+
+        model = MixtureOfExperts(create_inference_model(Matvec(R), dtype="bf16"), experts, top_k=2)
+        y = model.forward_batch_parallel(x)
+    """
+
+    def __init__(self, router: Inference, experts: ExpertInference, top_k: int, normalize: str = "chosen"):
+        if router.get_num_outputs() != experts.num_experts:
+            raise A.PonniError(A.PONNI_ERR_INVALID_MODEL, "the router's outputs are not the experts")
+        if router.get_num_inputs() != experts.get_num_inputs() or router.dtype != experts.dtype:
+            raise A.PonniError(A.PONNI_ERR_INVALID_MODEL, "router and experts take different inputs")
+        self.router, self.experts, self.top_k, self.normalize = router, experts, top_k, normalize
+
+    def forward_batch_parallel(self, x, y=None):
+        routing = route_experts(self.router.forward_batch_parallel(x), self.top_k, self.normalize)
+        return self.experts.forward_mixture(x, routing, y)
