@@ -13,6 +13,15 @@ namespace ponni_hip {
 __device__ inline void dma16(void const* g, unsigned lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "{m0}"(lds) : "memory");
 }
+// The same at a uniform address and a 32-bit offset per lane.  (Five wait states:
+// those between a VALU write of a scalar register, as v_readfirstlane's of the
+// address, and a memory instruction's read of it, which the hardware does not check.)
+__device__ inline void dma16(void const* base, unsigned offset, unsigned lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "{m0}"(lds) : "memory");
+}
+__device__ inline void dma4(void const* base, unsigned offset, unsigned lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "{m0}"(lds) : "memory");
+}
 __device__ inline void dma4(void const* g, unsigned lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "{m0}"(lds) : "memory");
 }
