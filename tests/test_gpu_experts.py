@@ -53,7 +53,8 @@ def check_routing(r, scores, top_k, normalize):
 @pytest.mark.parametrize("normalize", ["chosen", "all"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("E,k,B", [(1, 1, 1), (2, 2, 3), (5, 1, 255), (8, 2, 1000), (64, 4, 257), (65, 3, 513),
-                                   (256, 8, 300), (1000, 16, 70), (1024, 5, 2), (3, 2, 70_001)])
+                                   (256, 8, 300), (1000, 16, 70), (1024, 5, 2), (6, 2, 4097), (5, 3, 70_001),
+                                   (3, 2, 131_073)])
 def test_routing(cuda, E, k, B, dtype, normalize):
     print(f"routing: E={E} k={k} B={B} {dtype} {normalize}", flush=True)
     r = np.random.default_rng(E * 1000 + B)
