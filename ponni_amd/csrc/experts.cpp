@@ -113,7 +113,8 @@ int check_routing_sizes(int32_t experts, int32_t top_k, int64_t batch) {
 }
 
 // The layers over `columns` sorted columns of `input` (row source[c], or c itself).
-int run_layers(ponni_experts_s const& e, Rows input, int64_t input_rows, int32_t const* source, int32_t const* offsets,
+// (x, if not null: the input itself, [features, input_rows], instead of rows)
+int run_layers(ponni_experts_s const& e, void const* x, int64_t ld_in, Rows input, int64_t input_rows, int32_t const* source, int32_t const* offsets,
                int64_t columns, void* y, int64_t ld_out, bool rows_out, char* base, Workspace const& w,
                Rows* result, hipStream_t stream) {
   bool const mx4 = e.operand == OPERAND_MX4;
@@ -125,6 +126,9 @@ int run_layers(ponni_experts_s const& e, Rows input, int64_t input_rows, int32_t
     a.w_scales = l.scales;
     a.bias = l.d_bias;
     a.x = input;
+    a.features = x;
+    a.ldx = ld_in;
+    a.n_in = l.n_in;
     a.x_rows = input_rows;
     a.source = source;
     a.offsets = offsets;
@@ -145,12 +149,14 @@ int run_layers(ponni_experts_s const& e, Rows input, int64_t input_rows, int32_t
       a.y_rows.data = base + w.state[i % 2];
       a.y_rows.scales = reinterpret_cast<unsigned char*>(base + w.state_scales[i % 2]);
       a.y_rows.stride = i < last ? int64_t(next) * 64 : round_up(l.n_out * element_bytes(e.dtype), 64);
-      a.y_rows.scale_stride = int64_t(next) * 4;
+      a.y_rows.scale_stride = 4;
+      a.y_rows.scale_step = columns * 4;
       a.row_features = i < last ? next * step_features(e.operand)
                                 : static_cast<int32_t>(a.y_rows.stride / element_bytes(e.dtype));
     }
     hipError_t const err = launch_contraction(e.operand, e.dtype, kind, a, stream);
     if (err != hipSuccess) return device_error("expert layer", err);
+    x = nullptr;
     input = a.y_rows;
     input_rows = columns;
     source = nullptr;
@@ -193,17 +199,19 @@ int forward_impl(ponni_experts e, const void* x, int64_t ld_in, const void* code
   char* base = static_cast<char*>(workspace);
   Rows rows;
   rows.stride = int64_t(first.steps) * 64;
-  rows.scale_stride = int64_t(first.steps) * 4;
+  rows.scale_stride = mx4_rows ? int64_t(first.steps) * 4 : 4;
+  rows.scale_step = mx4_rows ? 4 : columns * 4;
+  bool const direct = !mx4_rows && takes_features(columns, e->num_experts, first.blocks);
   if (mx4_rows) {
     rows.data = static_cast<char*>(const_cast<void*>(codes));
     rows.scales = static_cast<unsigned char*>(const_cast<void*>(scales));
-  } else {
+  } else if (!direct) {
     rows.data = base + w.input;
     rows.scales = reinterpret_cast<unsigned char*>(base + w.input_scales);
     hipError_t const err = launch_to_rows(e->operand, e->dtype, x, ld_in, first.n_in, columns, rows, stream);
     if (err != hipSuccess) return device_error("input rows", err);
   }
-  return run_layers(*e, rows, columns, nullptr, offsets, columns, y, ld_out, false, base, w, nullptr, stream);
+  return run_layers(*e, direct ? x : nullptr, ld_in, rows, columns, nullptr, offsets, columns, y, ld_out, false, base, w, nullptr, stream);
 }
 
 int mixture_impl(ponni_experts e, const void* x, int64_t ld_in, const ponni_routing* r, void* y, int64_t ld_out,
@@ -235,10 +243,13 @@ int mixture_impl(ponni_experts e, const void* x, int64_t ld_in, const ponni_rout
   rows.data = base + w.input;
   rows.scales = reinterpret_cast<unsigned char*>(base + w.input_scales);
   rows.stride = int64_t(first.steps) * 64;
-  rows.scale_stride = int64_t(first.steps) * 4;
-  hipError_t err = launch_to_rows(e->operand, e->dtype, x, ld_in, first.n_in, r->batch, rows, stream);
+  rows.scale_stride = 4;
+  rows.scale_step = r->batch * 4;
+  bool const direct = takes_features(columns, e->num_experts, first.blocks);
+  hipError_t err = hipSuccess;
+  if (!direct) err = launch_to_rows(e->operand, e->dtype, x, ld_in, first.n_in, r->batch, rows, stream);
   if (err != hipSuccess) return device_error("input rows", err);
-  st = run_layers(*e, rows, r->batch, r->source, r->offsets, columns, nullptr, 0, true, base, w, &result, stream);
+  st = run_layers(*e, direct ? x : nullptr, ld_in, rows, r->batch, r->source, r->offsets, columns, nullptr, 0, true, base, w, &result, stream);
   if (st != PONNI_OK) return st;
   err = launch_combine(e->dtype, result, columns, *r, last.n_out, y, ld_out, stream);
   return err == hipSuccess ? PONNI_OK : device_error("weighted sum", err);
@@ -402,6 +413,7 @@ Rows mx4_rows(const void* codes, const void* scales, int64_t features) {
   r.scales = static_cast<unsigned char*>(const_cast<void*>(scales));
   r.stride = contraction_steps(OPERAND_MX4, features) * 64;
   r.scale_stride = contraction_steps(OPERAND_MX4, features) * 4;
+  r.scale_step = 4;
   return r;
 }
 

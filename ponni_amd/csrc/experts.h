@@ -22,12 +22,14 @@ inline int64_t contraction_steps(Operand o, int64_t features) {
 }
 
 // Samples as rows: 64 bytes a step, features past the last one zero; mx4 rows
-// have 4 scale bytes a step beside them.
+// have 4 scale bytes a step beside them (a caller's row by row; the library's own step by
+// step, so that a tile's are consecutive).
 struct Rows {
   char* data = nullptr;
   unsigned char* scales = nullptr;  // mx4
   int64_t stride = 0;               // bytes from row to row of `data`
-  int64_t scale_stride = 0;
+  int64_t scale_stride = 0;         // bytes from a row's 4 scales to the next row's of a step,
+  int64_t scale_step = 0;           // and to those of the next step
 };
 
 enum OutputKind { OUT_FEATURES = 0, OUT_ROWS = 1, OUT_MX4 = 2 };
@@ -39,6 +41,9 @@ struct ContractArgs {
   const unsigned char* w_scales; // mx4: [experts][blocks][steps][64 lanes][4 tiles]
   const float* bias;             // [experts][64 blocks], or null
   Rows x;
+  const void* features;  // or the input as [features, x_rows] of the model's type, row stride ldx (takes_features)
+  int64_t ldx;
+  int32_t n_in;
   int64_t x_rows;
   const int32_t* source;   // row of each column (null: the column itself)
   const int32_t* offsets;  // [experts + 1] (null: one group of all columns)
@@ -57,6 +62,8 @@ struct ContractArgs {
   int32_t row_features;
 };
 
+// Whether a layer of these sizes reads its input as [features, columns] itself.
+bool takes_features(int64_t columns, int32_t experts, int32_t blocks);
 hipError_t launch_contraction(Operand op, int out_type, OutputKind kind, ContractArgs const& a, hipStream_t stream);
 
 // x [features, columns] of `dtype` as rows of `op`, `row_bytes` a row.

@@ -179,17 +179,16 @@ __device__ inline void store_mx4(ContractArgs const& a, int64_t col, bool valid,
   if (!finite) amax = __builtin_inff();
   amax = fmaxf(amax, __shfl_xor(amax, 16));
   unsigned const scale = mx4_scale(amax);
-  float const inverse = mx4_inverse(scale);
+  float const scale_value = mx4_scale_value(scale);
   typedef int i32x2 __attribute__((ext_vector_type(2)));
-  i32x2 codes = {0, 0};
-  if (scale != 255u) {
+  i32x2 codes;
 #pragma unroll
-    for (int i = 0; i < 16; i++) codes[i / 8] |= mx4_code(v[i / 4][i % 4] * inverse) << (4 * (i % 8));
-  }
+  for (int w = 0; w < 2; w++) codes[w] = mx4_word(scale_value, [&](int e) { return v[2 * w + e / 4][e % 4]; });
+  if (scale == 255u) codes = {0, 0};
   if (!valid || f0 >= a.row_features) return;
   *reinterpret_cast<i32x2*>(a.y_rows.data + col * a.y_rows.stride + f0 / 2) = codes;
   if (f0 % kMx4Block == 0)
-    a.y_rows.scales[col * a.y_rows.scale_stride + f0 / kMx4Block] = static_cast<unsigned char>(scale);
+    a.y_rows.scales[col * a.y_rows.scale_stride + f0 / 128 * a.y_rows.scale_step + f0 / kMx4Block % 4] = static_cast<unsigned char>(scale);
 }
 
 // Steps a turn of the loop: 128 bytes of a row, one whole line of the L2's.
@@ -245,7 +244,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void contract(ContractArgs a) {
       int const q = (wave + W * r) / D, h = (wave + W * r) % D;  // [block or 64 columns][step of the turn]
       ps[r] = q < BM / 64 ? reinterpret_cast<char const*>(a.w_scales) + (block_of(q) * steps + h) * 256 + 4 * lane
                           : reinterpret_cast<char const*>(a.x.scales) +
-                                row_of((q - BM / 64) * 64 + lane) * a.x.scale_stride + 4 * h;
+                                row_of((q - BM / 64) * 64 + lane) * a.x.scale_stride + h * a.x.scale_step;
     }
   }
   // Request r of a turn: its weights first, then its rows and scales.  The second
@@ -267,7 +266,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void contract(ContractArgs a) {
       r -= A_REQ + B_REQ;
       int const q = wave + W * r;
       if (whole || q % D == 0) dma4(ps[r], slot + A_BYTES + B_BYTES + q * 256);
-      ps[r] += q / D < BM / 64 ? 256 * D : 4 * D;
+      ps[r] += q / D < BM / 64 ? int64_t(256 * D) : D * a.x.scale_step;
     }
   };
   f32x4 acc[MI][NJ];
@@ -356,22 +355,167 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void contract(ContractArgs a) {
   }
 }
 
+// Few columns: 64 output features x 16 NJ columns a workgroup, whose W waves
+// share the contraction: what bounds these is the weights' way from memory, so each
+// wave has several steps' fragments under way at once, straight into registers, and
+// no wave waits for another before the sums meet in LDS (in the order of the
+// waves).  FEATURES: the input as the caller holds it, without rows made of it
+// first; 4-bit fragments are quantised as they are read.
+template <Operand OP, class S, OutputKind KIND, bool FEATURES, int NJ, int W>
+__global__ __launch_bounds__(64 * W) void contract_thin(ContractArgs a) {
+  constexpr bool MX = OP == OPERAND_MX4;
+  constexpr int U = NJ == 1 ? 4 : 2;  // steps under way
+  constexpr int N = OP == OPERAND_F32 ? 4 : MX ? 32 : 8;
+  __shared__ f32x4 sums[W][4 * NJ][64];
+  int const lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Tile const t = find_tile<16 * NJ>(a, a.blocks);
+  if (t.none) return;
+  int const steps = a.steps;
+  int64_t const block = int64_t(t.expert) * a.blocks + t.block;
+  char const* const weights = a.weights + block * steps * 4096 + 16 * lane;
+  int64_t row[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; j++) {
+    int32_t const col = t.first + 16 * j + c < t.last ? t.first + 16 * j + c : t.last - 1;
+    int64_t const r = a.source != nullptr ? a.source[col] : col;
+    row[j] = r < 0 || r >= a.x_rows ? int64_t(0) : r;
+  }
+  // This lane's fragment of step s of column j's row, and its scale.
+  auto read_row = [&](int s, int j, i32x4& v, int& scale) {
+    if constexpr (FEATURES) {
+      S const* x = static_cast<S const*>(a.features) + row[j];
+      S e[N];
+#pragma unroll
+      for (int k = 0; k < N; k++) {
+        int const f = (4 * s + g) * N + k;
+        e[k] = f < a.n_in ? x[f * a.ldx] : S(0.0f);
+      }
+      if constexpr (MX) {
+        float amax = 0.0f;
+        bool finite = true;
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+          amax = fmaxf(amax, __builtin_fabsf(float(e[k])));
+          finite = finite && e[k] == e[k];
+        }
+        scale = finite ? mx4_scale(amax) : 255u;
+        float const scale_value = mx4_scale_value(scale);
+#pragma unroll
+        for (int w = 0; w < 4; w++) v[w] = mx4_word(scale_value, [&](int k) { return e[8 * w + k]; });
+        if (scale == 255) v = {0, 0, 0, 0};
+      } else {
+        typedef S Piece __attribute__((ext_vector_type(N)));
+        Piece p;
+#pragma unroll
+        for (int k = 0; k < N; k++) p[k] = e[k];
+        v = __builtin_bit_cast(i32x4, p);
+      }
+    } else {
+      v = *reinterpret_cast<i32x4 const*>(a.x.data + row[j] * a.x.stride + s * 64 + 16 * g);
+      if constexpr (MX) scale = a.x.scales[row[j] * a.x.scale_stride + s * a.x.scale_step + g];
+    }
+  };
+  f32x4 acc[4][NJ] = {};
+  for (int s0 = wave; s0 < steps; s0 += U * W) {
+    i32x4 av[U][4], bv[U][NJ];
+    int as[U] = {}, bs[U][NJ] = {};
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      int const s = s0 + u * W;
+      if (s >= steps) continue;
+#pragma unroll
+      for (int i = 0; i < 4; i++) av[u][i] = *reinterpret_cast<i32x4 const*>(weights + int64_t(s) * 4096 + i * 1024);
+      if constexpr (MX) as[u] = reinterpret_cast<int const*>(a.w_scales + (block * steps + s) * 256)[lane];
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (s0 + u * W >= steps) continue;
+#pragma unroll
+      for (int j = 0; j < NJ; j++) read_row(s0 + u * W, j, bv[u][j], bs[u][j]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (s0 + u * W >= steps) continue;
+#pragma unroll
+      for (int j = 0; j < NJ; j++) {
+        acc[0][j] = multiply<OP, 0>(av[u][0], bv[u][j], acc[0][j], as[u], bs[u][j]);
+        acc[1][j] = multiply<OP, 1>(av[u][1], bv[u][j], acc[1][j], as[u], bs[u][j]);
+        acc[2][j] = multiply<OP, 2>(av[u][2], bv[u][j], acc[2][j], as[u], bs[u][j]);
+        acc[3][j] = multiply<OP, 3>(av[u][3], bv[u][j], acc[3][j], as[u], bs[u][j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+#pragma unroll
+    for (int j = 0; j < NJ; j++) sums[wave][4 * j + i][lane] = acc[i][j];
+  __syncthreads();
+  if (wave >= NJ) return;
+  // Wave j finishes the columns of tile j.
+  int const f0 = t.block * 64 + 16 * g;
+  f32x4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    v[i] = a.bias != nullptr ? *reinterpret_cast<f32x4 const*>(a.bias + block * 64 + 16 * g + 4 * i) : f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < W; w++) v[i] += sums[w][4 * wave + i][lane];
+  }
+  activate<OP == OPERAND_F32>(a.act, a.act_a, [&](auto f) {
+#pragma unroll
+    for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f(v[e / 4][e % 4]);
+  });
+#pragma unroll
+  for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f0 + e < a.n_out ? v[e / 4][e % 4] : 0.0f;
+  int64_t const col = int64_t(t.first) + 16 * wave + c;
+  if constexpr (KIND == OUT_MX4) store_mx4(a, col, col < t.last, f0, v);
+  else if (col < t.last) store_features<KIND, S>(a, col, f0, v);
+}
+
+// The grid of tiles of `width` columns x `out_blocks` blocks, at least as many as any offsets give.
+inline int64_t grid_of(ContractArgs const& a, int64_t width, int64_t out_blocks) {
+  // ceil(n / width) summed over the groups: at most one more than n / width for each that has columns
+  int64_t const partial = a.experts < a.columns ? a.experts : a.columns;
+  // (a share per XCD is rounded up: the grid is whole rounds of the eight)
+  return ((a.columns / width + partial) * out_blocks + 7) / 8 * 8;
+}
+
 template <Operand OP, class S, OutputKind KIND, int MI, int NJ, int WM, int WN>
 hipError_t launch_tiled(ContractArgs const& a, hipStream_t stream) {
   constexpr int BM = 16 * MI * WM, BN = 16 * NJ * WN;
-  int64_t const out_blocks = (int64_t(a.blocks) * 64 + BM - 1) / BM;
-  // ceil(n / BN) summed over the groups: at most one more than n / BN for each that has columns
-  int64_t const partial = a.experts < a.columns ? a.experts : a.columns;
-  int64_t const tiles = (a.columns / BN + partial) * out_blocks;
+  int64_t const tiles = grid_of(a, BN, (int64_t(a.blocks) * 64 + BM - 1) / BM);
   if (tiles > INT32_MAX) return hipErrorInvalidValue;
-  // (a share per XCD is rounded up: the grid is whole rounds of the eight)
-  dim3 const grid(static_cast<unsigned>((tiles + 7) / 8 * 8)), block(64 * WM * WN);
+  dim3 const grid(static_cast<unsigned>(tiles)), block(64 * WM * WN);
   hipLaunchKernelGGL((contract<OP, S, KIND, MI, NJ, WM, WN>), grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+
+// Columns of a thin tile, 0 where the other kernels' tiles serve better.
+inline int thin_columns(int64_t columns, int32_t experts, int32_t blocks) {
+  int64_t const groups = experts < columns ? experts : columns;
+  if (columns > 32 * groups || (columns / 128 + groups) * ((blocks + 1) / 2) >= 1024) return 0;
+  return columns <= 16 * groups ? 16 : 32;
+}
+
+template <Operand OP, class S, OutputKind KIND, bool FEATURES, int NJ>
+hipError_t launch_thin(ContractArgs const& a, hipStream_t stream) {
+  constexpr int W = 8;
+  int64_t const tiles = grid_of(a, 16 * NJ, a.blocks);
+  if (tiles > INT32_MAX) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((contract_thin<OP, S, KIND, FEATURES, NJ, W>), dim3(static_cast<unsigned>(tiles)), dim3(64 * W), 0,
+                     stream, a);
   return hipGetLastError();
 }
 
 template <Operand OP, class S, OutputKind KIND>
 hipError_t launch_sized(ContractArgs const& a, hipStream_t stream) {
+  bool const features = a.features != nullptr;
+  switch (thin_columns(a.columns, a.experts, a.blocks)) {
+    case 16: return features ? launch_thin<OP, S, KIND, true, 1>(a, stream) : launch_thin<OP, S, KIND, false, 1>(a, stream);
+    case 32: return features ? launch_thin<OP, S, KIND, true, 2>(a, stream) : launch_thin<OP, S, KIND, false, 2>(a, stream);
+    default: break;
+  }
+  if (features) return hipErrorInvalidValue;  // (takes_features)
   // 256 x 256 tiles, which read half as much from L2 per multiply-add, where two
   // rounds of the 256 CUs have one each; else 128 x 128.  bf16 1024-1024, 16 experts,
   // 65,536 columns: 195 us against 241.
@@ -445,10 +589,10 @@ __global__ __launch_bounds__(256) void pack_weights(T const* __restrict__ w, int
       finite = finite && v[k] == v[k];
     }
     unsigned const scale = finite ? mx4_scale(amax) : 255u;
-    float const inverse = mx4_inverse(scale);
+    float const scale_value = mx4_scale_value(scale);
     if (scale != 255u) {
 #pragma unroll
-      for (int k = 0; k < N; k++) out[k / 8] |= mx4_code(v[k] * inverse) << (4 * (k % 8));
+      for (int w = 0; w < 4; w++) out[w] = mx4_word(scale_value, [&](int k) { return v[8 * w + k]; });
     }
     scales[(piece / 256 * 64 + lane) * 4 + i] = static_cast<unsigned char>(scale);
   } else {
@@ -479,6 +623,8 @@ template <class F> bool with_parameter_dtype(int dtype, F&& f) {
 }
 
 }  // namespace
+
+bool takes_features(int64_t columns, int32_t experts, int32_t blocks) { return thin_columns(columns, experts, blocks) > 0; }
 
 hipError_t launch_contraction(Operand op, int out_type, OutputKind kind, ContractArgs const& a, hipStream_t stream) {
   switch (op) {

@@ -3,6 +3,8 @@
 
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "../../include/ponni_hip.h"
 
 namespace ponni_hip {
@@ -29,18 +31,22 @@ __device__ inline unsigned mx4_scale(float amax) {
   unsigned const e = (__builtin_bit_cast(unsigned, amax) >> 23) & 255u;
   return e == 255u ? 255u : e > 2u ? e - 2u : 0u;
 }
-// 2^(127 - scale): exact, also for scale 0 (2^127); 0 for a NaN block.
-__device__ inline float mx4_inverse(unsigned scale) {
-  return scale == 255u ? 0.0f : __builtin_bit_cast(float, (254u - scale) << 23);
+// Two elements into byte AT of `word`: a, b over scale_value, a power of two, to
+// nearest, ties to the even code, at most 6, by the hardware's conversion.
+template <int AT, class S> __device__ inline unsigned mx4_pair(unsigned word, S a, S b, float scale_value) {
+  typedef S S2 __attribute__((ext_vector_type(2)));
+  if constexpr (std::is_same_v<S, float>) return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, a, b, scale_value, AT);
+  else if constexpr (std::is_same_v<S, _Float16>)
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(word, S2{a, b}, scale_value, AT);
+  else return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(word, S2{a, b}, scale_value, AT);
 }
-// Sign and 3 bits of v = x * 2^(127 - scale), to nearest, ties to the even code,
-// at most 6: the values are 0, 0.5, ..., 2 in steps of 0.5, to 4 in steps of 1, 6.
-__device__ inline unsigned mx4_code(float v) {
-  float const s = __builtin_fabsf(v);
-  float const c = s < 2.0f ? __builtin_rintf(2.0f * s) : s < 4.0f ? 2.0f + __builtin_rintf(s)
-                                                                  : 4.0f + __builtin_rintf(0.5f * s);
-  unsigned const m = unsigned(c < 7.0f ? c : 7.0f);
-  return m | ((__builtin_bit_cast(unsigned, v) >> 31) << 3);
+// Eight elements, element(i) the i-th, as a word.
+template <class F> __device__ inline unsigned mx4_word(float scale_value, F&& element) {
+  unsigned w = 0;
+  w = mx4_pair<0>(w, element(0), element(1), scale_value);
+  w = mx4_pair<1>(w, element(2), element(3), scale_value);
+  w = mx4_pair<2>(w, element(4), element(5), scale_value);
+  return mx4_pair<3>(w, element(6), element(7), scale_value);
 }
 // Value of a 4-bit element: its three bits are the last exponent and first
 // mantissa bits of a float 2^126 times smaller (also below the binades: 0.5).
