@@ -34,36 +34,42 @@ def _types():
     return _torch
 
 
-class _on:
-    """The device of a tensor as the current one, where it is not."""
+_current_device = None  # () -> the current device's index
 
-    def __init__(self, t):
+
+def _call(like, fn, *args) -> None:
+    """fn(*args, current stream) with the tensor's device as the current one."""
+    global _current_device
+    if _current_device is None:
         import torch
 
-        self.index = t.device.index
-        self.device = None if torch.cuda.current_device() == self.index else torch.cuda.device(self.index)
+        _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+    index = like.get_device()
+    if _current_device() == index:
+        status = fn(*args, _current_stream(like))
+    else:
+        import torch
 
-    def __enter__(self):
-        if self.device is not None:
-            self.device.__enter__()
-
-    def __exit__(self, *a):
-        if self.device is not None:
-            self.device.__exit__(*a)
+        with torch.cuda.device(index):
+            status = fn(*args, _current_stream(like))
+    if status != A.PONNI_OK:
+        A.check(status)
 
 
 def _rows(t, what: str, rows: int | None = None, columns: int | None = None):
     """Checks a [features, columns] GPU tensor with contiguous rows; its row stride."""
-    if t.dim() != 2 or not t.is_cuda:
+    shape = t.shape
+    if len(shape) != 2 or not t.is_cuda:
         raise ValueError(f"{what} must be a two-dimensional GPU tensor [features, columns]")
-    if (rows is not None and t.shape[0] != rows) or (columns is not None and t.shape[1] != columns):
-        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected "
+    if (rows is not None and shape[0] != rows) or (columns is not None and shape[1] != columns):
+        raise ValueError(f"{what} has shape {tuple(shape)}, expected "
                          f"({'any' if rows is None else rows}, {'any' if columns is None else columns})")
-    if t.shape[1] == 0:
-        raise A.PonniError(A.PONNI_ERR_SHAPE, f"{what} has no columns")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    if shape[0] == 0 or shape[1] == 0:
+        raise A.PonniError(A.PONNI_ERR_SHAPE, f"{what} of shape {tuple(shape)} is empty")
+    stride = t.stride()
+    if shape[1] > 1 and stride[1] != 1:
         raise ValueError(f"{what} needs contiguous rows")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return stride[0] if shape[0] > 1 else shape[1]
 
 
 def _same_device(t, other, what: str):
@@ -143,24 +149,22 @@ def route_experts(scores, top_k: int, normalize: str = "chosen") -> Routing:
     need = L.ponni_route_workspace_bytes(e, top_k, b)
     if need < 0:
         raise A.PonniError(A.PONNI_ERR_INVALID_ARGUMENT, L.ponni_last_error().decode())
-    n = top_k * b
-    # One allocation: the integer arrays and weights, then the work buffer (16-byte aligned).
-    ints = torch.empty(4 * n + (e + 4) // 4 * 4 + 16 + need // 4, dtype=torch.int32, device=scores.device)
-    at = (4 * n + e + 1 + 3) // 4 * 4
-    r = Routing(ints[:n].view(top_k, b), ints[n:2 * n].view(torch.float32).view(top_k, b),
-                ints[2 * n:3 * n].view(top_k, b), ints[3 * n:4 * n], ints[4 * n:4 * n + e + 1], checked=True)
-    with _on(scores):
-        arrays = r.arrays()
-        A.check(L.ponni_route(scores.data_ptr(), ld, codes[scores.dtype],
-                              A.ROUTE_ALL if normalize == "all" else A.ROUTE_CHOSEN, ctypes.byref(arrays),
-                              ints.data_ptr() + 4 * at, need, _current_stream(scores)))
+    # Two allocations: the [top_k, batch] arrays and the source; offsets, then the work buffer (16-byte aligned).
+    made = torch.empty((4, top_k, b), dtype=torch.int32, device=scores.device)
+    at = (e + 4) // 4 * 4
+    more = torch.empty(at + need // 4, dtype=torch.int32, device=scores.device)
+    experts, weights, slots, source = made.unbind()
+    r = Routing(experts, weights.view(torch.float32), slots, source.view(-1), more[:e + 1], checked=True)
+    arrays, base = r.arrays(), more.data_ptr()
+    _call(scores, L.ponni_route, scores.data_ptr(), ld, codes[scores.dtype], A.ROUTE_ALL if normalize == "all" else
+          A.ROUTE_CHOSEN, ctypes.byref(arrays), base + 4 * at, need)
     return r
 
 
 # -- 4-bit rows ------------------------------------------------------------------------
 
 
-@dataclass
+@dataclass(frozen=True)
 class Mx4:
     """Samples as microscaled 4-bit rows (ponni_mx4_quantize): codes [columns,
     code bytes] and scales [columns, scale bytes], uint8."""
@@ -168,22 +172,32 @@ class Mx4:
     codes: "object"
     scales: "object"
     features: int
+    checked: bool = field(default=False, repr=False)
 
     @property
     def columns(self) -> int:
         return self.codes.shape[0]
 
+    def check(self) -> None:
+        if not self.checked:
+            import torch
+
+            for t, n, what in ((self.codes, A.lib().ponni_mx4_code_bytes(self.features), "codes"),
+                               (self.scales, A.lib().ponni_mx4_scale_bytes(self.features), "scales")):
+                if t.dtype != torch.uint8 or tuple(t.shape) != (self.columns, n) or not t.is_contiguous() or not t.is_cuda:
+                    raise ValueError(f"{what} must be a contiguous uint8 GPU tensor of shape ({self.columns}, {n})")
+            _same_device(self.scales, self.codes, "scales")
+
     def dequantize(self, dtype=None):
         """The values as a [features, columns] tensor (float32, float16 or bfloat16)."""
         import torch
 
+        self.check()
         y = torch.empty((self.features, self.columns), dtype=dtype or torch.float32, device=self.codes.device)
         if y.dtype not in _types()[1]:
             raise ValueError(f"values of type {y.dtype}")
-        with _on(y):
-            A.check(A.lib().ponni_mx4_dequantize(self.codes.data_ptr(), self.scales.data_ptr(), self.features,
-                                                 self.columns, y.data_ptr(), self.columns, _types()[1][y.dtype],
-                                                 _current_stream(y)))
+        _call(y, A.lib().ponni_mx4_dequantize, self.codes.data_ptr(), self.scales.data_ptr(), self.features, self.columns,
+              y.data_ptr(), self.columns, _types()[1][y.dtype])
         return y
 
 
@@ -198,10 +212,8 @@ def quantize_mx4(x) -> Mx4:
     k, n = x.shape
     L = A.lib()
     q = Mx4(torch.empty((n, L.ponni_mx4_code_bytes(k)), dtype=torch.uint8, device=x.device),
-            torch.empty((n, L.ponni_mx4_scale_bytes(k)), dtype=torch.uint8, device=x.device), k)
-    with _on(x):
-        A.check(L.ponni_mx4_quantize(x.data_ptr(), ld, _types()[1][x.dtype], k, n, q.codes.data_ptr(),
-                                     q.scales.data_ptr(), _current_stream(x)))
+            torch.empty((n, L.ponni_mx4_scale_bytes(k)), dtype=torch.uint8, device=x.device), k, checked=True)
+    _call(x, L.ponni_mx4_quantize, x.data_ptr(), ld, _types()[1][x.dtype], k, n, q.codes.data_ptr(), q.scales.data_ptr())
     return q
 
 
@@ -325,6 +337,7 @@ class ExpertInference:
         L = A.lib()
         rows = isinstance(x, Mx4)
         if rows:
+            x.check()
             like, columns = x.codes, x.columns
             if x.features != self.n_in:
                 raise ValueError(f"x has {x.features} features, the model {self.n_in} inputs")
@@ -339,14 +352,12 @@ class ExpertInference:
         need = L.ponni_experts_workspace_bytes(self._experts, columns)
         work = torch.empty(max(need, 1), dtype=torch.uint8, device=like.device)
         at = 0 if offsets is None else offsets.data_ptr()
-        with _on(like):
-            stream = _current_stream(like)
-            if rows:
-                A.check(L.ponni_experts_forward_mx4(self._experts, x.codes.data_ptr(), x.scales.data_ptr(), at,
-                                                    y.data_ptr(), ld, columns, work.data_ptr(), need, stream))
-            else:
-                A.check(L.ponni_experts_forward(self._experts, x.data_ptr(), ld_in, at, y.data_ptr(), ld, columns,
-                                                work.data_ptr(), need, stream))
+        if rows:
+            _call(like, L.ponni_experts_forward_mx4, self._experts, x.codes.data_ptr(), x.scales.data_ptr(), at,
+                  y.data_ptr(), ld, columns, work.data_ptr(), need)
+        else:
+            _call(like, L.ponni_experts_forward, self._experts, x.data_ptr(), ld_in, at, y.data_ptr(), ld, columns,
+                  work.data_ptr(), need)
         return y
 
     def forward_mixture(self, x, routing: Routing, y=None):
@@ -361,10 +372,9 @@ class ExpertInference:
         y, ld = self._buffers(x, routing.batch, y)
         need = L.ponni_experts_mixture_workspace_bytes(self._experts, routing.top_k, routing.batch)
         work = torch.empty(max(need, 1), dtype=torch.uint8, device=x.device)
-        with _on(x):
-            arrays = routing.arrays()
-            A.check(L.ponni_experts_forward_mixture(self._experts, x.data_ptr(), ld_in, ctypes.byref(arrays),
-                                                    y.data_ptr(), ld, work.data_ptr(), need, _current_stream(x)))
+        arrays = routing.arrays()
+        _call(x, L.ponni_experts_forward_mixture, self._experts, x.data_ptr(), ld_in, ctypes.byref(arrays), y.data_ptr(),
+              ld, work.data_ptr(), need)
         return y
 
 
