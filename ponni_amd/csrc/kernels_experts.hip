@@ -13,7 +13,7 @@
 //
 // A workgroup computes 16 MI WM features x 16 NJ WN columns of one group; two
 // steps' weights and rows, whole 128-byte lines, go from memory straight into
-// LDS a turn ahead, one barrier a turn.
+// LDS a turn and a half ahead, fragments into registers a step ahead.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -247,8 +247,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void contract(ContractArgs a) {
                                 row_of((q - BM / 64) * 64 + lane) * a.x.scale_stride + h * a.x.scale_step;
     }
   }
-  // Request r of a turn: its weights first, then its rows and scales.  The second
-  // half of the last turn only where there is one.
+  // Request r of a turn: its weights first, then its rows and scales; of a last turn
+  // of one step, those of that step.
   constexpr int REQ = A_REQ + B_REQ + (MX ? S_REQ : 0);
   auto request = [&](int turn, int r) {
     unsigned const slot = lds0 + turn % 2 * SLOT;
@@ -279,62 +279,74 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void contract(ContractArgs a) {
 #pragma unroll
     for (int j = 0; j < NJ; j++) acc[i][j] = seed;
   }
-  // Fragments of a step: its rows, and the weights of a block of 64 features.
-  i32x4 bv[2][NJ], av[2][4];
-  int bs[2][NJ] = {}, as[2] = {};
-  auto read_rows = [&](char const* slot, int h, i32x4(&v)[NJ], int(&s)[NJ]) {
-#pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      int const col = 16 * (wn * NJ + j) + c;
-      v[j] = *reinterpret_cast<i32x4 const*>(slot + A_BYTES + 64 * D * col + 16 * (((4 * h + g) ^ col) % (4 * D)));
+  // The fragments of a step, in one of two sets: read r is a tile's weights, then a tile's rows.
+  static_assert(D == 2, "one set a step of the turn");
+  constexpr int READS = MI + NJ;
+  i32x4 av[D][MI], bv[D][NJ];
+  int as[D][MI / 4] = {}, bs[D][NJ] = {};
+  auto read = [&](char const* slot, int h, int r) {
+    if (r < MI) {
+      int const at = (wm * MI + r) / 4 * D + h;
+      av[h][r] = reinterpret_cast<i32x4 const*>(slot + (4 * at + r % 4) * 1024)[lane];
       if constexpr (MX)
-        s[j] = reinterpret_cast<unsigned char const*>(slot)[A_BYTES + B_BYTES + AS_BYTES + (col / 64 * D + h) * 256 +
-                                                            4 * (col % 64) + g];
+        if (r % 4 == 0) as[h][r / 4] = reinterpret_cast<int const*>(slot + A_BYTES + B_BYTES + at * 256)[lane];
+    } else {
+      int const j = r - MI, col = 16 * (wn * NJ + j) + c;
+      bv[h][j] = *reinterpret_cast<i32x4 const*>(slot + A_BYTES + 64 * D * col + 16 * (((4 * h + g) ^ col) % (4 * D)));
+      if constexpr (MX)
+        bs[h][j] = reinterpret_cast<unsigned char const*>(slot)[A_BYTES + B_BYTES + AS_BYTES +
+                                                                (col / 64 * D + h) * 256 + 4 * (col % 64) + g];
     }
   };
-  auto read_weights = [&](char const* slot, int h, int n, i32x4(&v)[4], int& s) {
-    int const block = wm * MI / 4 + n;
+  // A step's MFMAs, a column tile at a time; `between` makes the reads and requests of that quarter.
+  auto multiply_step = [&](int h, auto&& between) {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      v[i] = reinterpret_cast<i32x4 const*>(slot + (block * 4 * D + 4 * h + i) * 1024)[lane];
-    if constexpr (MX) s = reinterpret_cast<int const*>(slot + A_BYTES + B_BYTES + (block * D + h) * 256)[lane];
+    for (int j = 0; j < NJ; j++) {
+      between(j);
+#pragma unroll
+      for (int n = 0; n < MI / 4; n++) {
+        acc[4 * n][j] = multiply<OP, 0>(av[h][4 * n], bv[h][j], acc[4 * n][j], as[h][n], bs[h][j]);
+        acc[4 * n + 1][j] = multiply<OP, 1>(av[h][4 * n + 1], bv[h][j], acc[4 * n + 1][j], as[h][n], bs[h][j]);
+        acc[4 * n + 2][j] = multiply<OP, 2>(av[h][4 * n + 2], bv[h][j], acc[4 * n + 2][j], as[h][n], bs[h][j]);
+        acc[4 * n + 3][j] = multiply<OP, 3>(av[h][4 * n + 3], bv[h][j], acc[4 * n + 3][j], as[h][n], bs[h][j]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
 #pragma unroll
   for (int r = 0; r < REQ; r++) request(0, r);
-  constexpr int PARTS = D * MI / 4;  // of a turn: a block of 64 features in one step
+  if (turns > 1) {
+#pragma unroll
+    for (int r = 0; r < REQ; r++) request(1, r);
+  }
+  if (2 * D <= steps) wait_requests<REQ>();
+  else wait_requests<0>();
+  workgroup_barrier();
+#pragma unroll
+  for (int r = 0; r < READS; r++) read(lds, 0, r);
+  // One barrier a turn, between its two steps: the next turn's data has landed for every
+  // wave, and every wave has this turn's in registers, so its slot takes
+  // the turn after the next.  While a step's MFMAs run, the next step's fragments are
+  // read (behind the last step: whatever the slot holds, for no use).
   for (int turn = 0; turn < turns; turn++) {
-    // This wave's requests for the turn have landed; the barrier makes that true
-    // of every wave, and ends every wave's reads of the slot that the next takes.
+    char const* __restrict__ slot = lds + turn % 2 * SLOT;
+    char const* __restrict__ next = lds + (turn + 1) % 2 * SLOT;
+    multiply_step(0, [&](int j) {
+#pragma unroll
+      for (int r = j * READS / NJ; r < (j + 1) * READS / NJ; r++) read(slot, 1, r);
+    });
+    wait_lds();
     wait_requests<0>();
     workgroup_barrier();
-    char const* __restrict__ slot = lds + turn % 2 * SLOT;
-    bool const more = turn + 1 < turns, odd = D * turn + D > steps;
-    read_rows(slot, 0, bv[0], bs[0]);
-    read_weights(slot, 0, 0, av[0], as[0]);
-    // Each part reads the next one's fragments and makes its share of the next
-    // turn's requests before its own MFMAs.
+    if (D * turn + 1 >= steps) break;
+    multiply_step(1, [&](int j) {
+      if (turn + 2 < turns) {
 #pragma unroll
-    for (int p = 0; p < PARTS; p++) {
-      int const h = p / (MI / 4), n = p % (MI / 4);
-      if (h > 0 && odd) break;
-      if (p + 1 < PARTS) {
-        int const hn = (p + 1) / (MI / 4);
-        if (hn > h) read_rows(slot, hn, bv[hn % 2], bs[hn % 2]);
-        read_weights(slot, hn, (p + 1) % (MI / 4), av[(p + 1) % 2], as[(p + 1) % 2]);
+        for (int r = j * REQ / NJ; r < (j + 1) * REQ / NJ; r++) request(turn + 2, r);
       }
-      if (h == 0 && more) {
 #pragma unroll
-        for (int r = n * REQ / (MI / 4); r < (n + 1) * REQ / (MI / 4); r++) request(turn + 1, r);
-      }
-      i32x4(&w)[4] = av[p % 2];
-#pragma unroll
-      for (int j = 0; j < NJ; j++) {
-        acc[4 * n][j] = multiply<OP, 0>(w[0], bv[h % 2][j], acc[4 * n][j], as[p % 2], bs[h % 2][j]);
-        acc[4 * n + 1][j] = multiply<OP, 1>(w[1], bv[h % 2][j], acc[4 * n + 1][j], as[p % 2], bs[h % 2][j]);
-        acc[4 * n + 2][j] = multiply<OP, 2>(w[2], bv[h % 2][j], acc[4 * n + 2][j], as[p % 2], bs[h % 2][j]);
-        acc[4 * n + 3][j] = multiply<OP, 3>(w[3], bv[h % 2][j], acc[4 * n + 3][j], as[p % 2], bs[h % 2][j]);
-      }
-    }
+      for (int r = j * READS / NJ; r < (j + 1) * READS / NJ; r++) read(next, 0, r);
+    });
   }
 #pragma unroll
   for (int n = 0; n < MI / 4; n++) {

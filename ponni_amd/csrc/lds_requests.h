@@ -31,6 +31,11 @@ __device__ inline void wait_requests() {
   static_assert(N >= 0 && N < 16, "vmcnt field");
   __builtin_amdgcn_s_waitcnt(0x0070 | N);
 }
+// This wave's LDS reads have their data.
+__device__ inline void wait_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xc07f);
+}
 __device__ inline void workgroup_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
