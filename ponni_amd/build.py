@@ -36,6 +36,11 @@ SOURCES = [
     "kernels_peaks.hip",
     "experts.cpp",
     "kernels_experts.hip",
+    "kernels_chain_f32.hip",
+    "kernels_chain_f16.hip",
+    "kernels_chain_bf16.hip",
+    "kernels_chain_mx4_f16.hip",
+    "kernels_chain_mx4_bf16.hip",
     "kernels_route.hip",
     "kernels_mx4.hip",
 ]

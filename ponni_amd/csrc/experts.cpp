@@ -55,8 +55,27 @@ struct Workspace {
   int64_t input = 0, input_scales = 0, state[2] = {0, 0}, state_scales[2] = {0, 0}, total = 0;
 };
 
+// The chain's layers, and the columns of its tiles where one kernel takes it whole (0: layer by layer).
+int chain_of(ponni_experts_s const& e, int64_t columns, ChainArgs& a) {
+  a = ChainArgs{};
+  if (e.layers.size() > kChainLayers) return 0;
+  a.num_layers = static_cast<int32_t>(e.layers.size());
+  for (int32_t i = 0; i < a.num_layers; i++) {
+    auto const& l = e.layers[i];
+    a.layers[i] = {l.weights, l.scales, l.d_bias, l.steps, l.blocks, l.n_out, l.act, l.act_a};
+    a.state_bytes = std::max(a.state_bytes, l.steps * 64);
+  }
+  a.io.columns = columns;
+  a.io.experts = e.num_experts;
+  return chain_columns(e.operand, a);
+}
+
 Workspace workspace_of(ponni_experts_s const& e, int64_t rows, int64_t columns, bool mixture) {
   Workspace w;
+  ChainArgs chain;
+  bool const whole = chain_of(e, columns, chain) > 0;
+  bool const direct = whole ? !mixture : takes_features(columns, e.num_experts, e.layers[0].blocks);
+  if (direct) rows = 0;
   auto take = [&](int64_t n) {
     int64_t const at = w.total;
     w.total += round_up(n, 256);
@@ -67,7 +86,7 @@ Workspace workspace_of(ponni_experts_s const& e, int64_t rows, int64_t columns, 
   w.input_scales = take(mx4 ? rows * e.layers[0].steps * 4 : 0);
   int64_t data[2] = {0, 0}, scales[2] = {0, 0};
   size_t const last = e.layers.size() - 1;
-  for (size_t i = 0; i < last; i++) {
+  for (size_t i = 0; i < last && !whole; i++) {
     data[i % 2] = std::max(data[i % 2], columns * e.layers[i + 1].steps * 64);
     if (mx4) scales[i % 2] = std::max(scales[i % 2], columns * e.layers[i + 1].steps * 4);
   }
@@ -112,14 +131,28 @@ int check_routing_sizes(int32_t experts, int32_t top_k, int64_t batch) {
   return PONNI_OK;
 }
 
-// The layers over `columns` sorted columns of `input` (row source[c], or c itself).
-// (x, if not null: the input itself, [features, input_rows], instead of rows)
-int run_layers(ponni_experts_s const& e, void const* x, int64_t ld_in, Rows input, int64_t input_rows, int32_t const* source, int32_t const* offsets,
-               int64_t columns, void* y, int64_t ld_out, bool rows_out, char* base, Workspace const& w,
-               Rows* result, hipStream_t stream) {
+// The layers over `columns` sorted columns of x [features, input_rows] or of rows made of it (row
+// source[c] of them, or c itself): into y [features, columns], or (y null) rows in `result`.
+int run_layers(ponni_experts_s const& e, void const* x, int64_t ld_in, Rows input, int64_t input_rows,
+               int32_t const* source, int32_t const* offsets, int64_t columns, void* y, int64_t ld_out, char* base,
+               Workspace const& w, Rows* result, hipStream_t stream) {
   bool const mx4 = e.operand == OPERAND_MX4;
   size_t const last = e.layers.size() - 1;
-  for (size_t i = 0; i <= last; i++) {
+  ChainArgs chain;
+  int const chain_tile = chain_of(e, columns, chain);
+  // (rows are the caller's 4-bit ones, or made here where the first kernel does not read x itself)
+  bool const direct = chain_tile > 0 ? y != nullptr : takes_features(columns, e.num_experts, e.layers[0].blocks);
+  if (x != nullptr && !direct) {
+    input.data = base + w.input;
+    input.scales = reinterpret_cast<unsigned char*>(base + w.input_scales);
+    input.stride = int64_t(e.layers[0].steps) * 64;
+    input.scale_stride = 4;
+    input.scale_step = input_rows * 4;
+    hipError_t const err = launch_to_rows(e.operand, e.dtype, x, ld_in, e.layers[0].n_in, input_rows, input, stream);
+    if (err != hipSuccess) return device_error("input rows", err);
+    x = nullptr;
+  }
+  for (size_t i = chain_tile > 0 ? last : 0; i <= last; i++) {
     auto const& l = e.layers[i];
     ContractArgs a{};
     a.weights = l.weights;
@@ -128,7 +161,7 @@ int run_layers(ponni_experts_s const& e, void const* x, int64_t ld_in, Rows inpu
     a.x = input;
     a.features = x;
     a.ldx = ld_in;
-    a.n_in = l.n_in;
+    a.n_in = e.layers[chain_tile > 0 ? 0 : i].n_in;
     a.x_rows = input_rows;
     a.source = source;
     a.offsets = offsets;
@@ -140,7 +173,7 @@ int run_layers(ponni_experts_s const& e, void const* x, int64_t ld_in, Rows inpu
     a.act = l.act;
     a.act_a = l.act_a;
     OutputKind kind = OUT_FEATURES;
-    if (i == last && !rows_out) {
+    if (i == last && y != nullptr) {
       a.y = y;
       a.ldy = ld_out;
     } else {
@@ -154,7 +187,13 @@ int run_layers(ponni_experts_s const& e, void const* x, int64_t ld_in, Rows inpu
       a.row_features = i < last ? next * step_features(e.operand)
                                 : static_cast<int32_t>(a.y_rows.stride / element_bytes(e.dtype));
     }
-    hipError_t const err = launch_contraction(e.operand, e.dtype, kind, a, stream);
+    hipError_t err;
+    if (chain_tile > 0) {
+      chain.io = a;
+      err = launch_chain(e.operand, e.dtype, kind, chain_tile, chain, stream);
+    } else {
+      err = launch_contraction(e.operand, e.dtype, kind, a, stream);
+    }
     if (err != hipSuccess) return device_error("expert layer", err);
     x = nullptr;
     input = a.y_rows;
@@ -197,21 +236,16 @@ int forward_impl(ponni_experts e, const void* x, int64_t ld_in, const void* code
   if (clash || overlap(out, work))
     return fail(PONNI_ERR_INVALID_ARGUMENT, "input, output and workspace must not overlap");
   char* base = static_cast<char*>(workspace);
-  Rows rows;
-  rows.stride = int64_t(first.steps) * 64;
-  rows.scale_stride = mx4_rows ? int64_t(first.steps) * 4 : 4;
-  rows.scale_step = mx4_rows ? 4 : columns * 4;
-  bool const direct = !mx4_rows && takes_features(columns, e->num_experts, first.blocks);
+  Rows rows;  // the caller's 4-bit ones
   if (mx4_rows) {
     rows.data = static_cast<char*>(const_cast<void*>(codes));
     rows.scales = static_cast<unsigned char*>(const_cast<void*>(scales));
-  } else if (!direct) {
-    rows.data = base + w.input;
-    rows.scales = reinterpret_cast<unsigned char*>(base + w.input_scales);
-    hipError_t const err = launch_to_rows(e->operand, e->dtype, x, ld_in, first.n_in, columns, rows, stream);
-    if (err != hipSuccess) return device_error("input rows", err);
+    rows.stride = int64_t(first.steps) * 64;
+    rows.scale_stride = int64_t(first.steps) * 4;
+    rows.scale_step = 4;
   }
-  return run_layers(*e, direct ? x : nullptr, ld_in, rows, columns, nullptr, offsets, columns, y, ld_out, false, base, w, nullptr, stream);
+  return run_layers(*e, mx4_rows ? nullptr : x, ld_in, rows, columns, nullptr, offsets, columns, y, ld_out, base, w,
+                    nullptr, stream);
 }
 
 int mixture_impl(ponni_experts e, const void* x, int64_t ld_in, const ponni_routing* r, void* y, int64_t ld_out,
@@ -239,19 +273,10 @@ int mixture_impl(ponni_experts e, const void* x, int64_t ld_in, const ponni_rout
   if (overlap(in, out) || overlap(in, work) || overlap(out, work))
     return fail(PONNI_ERR_INVALID_ARGUMENT, "input, output and workspace must not overlap");
   char* base = static_cast<char*>(workspace);
-  Rows rows, result;
-  rows.data = base + w.input;
-  rows.scales = reinterpret_cast<unsigned char*>(base + w.input_scales);
-  rows.stride = int64_t(first.steps) * 64;
-  rows.scale_stride = 4;
-  rows.scale_step = r->batch * 4;
-  bool const direct = takes_features(columns, e->num_experts, first.blocks);
-  hipError_t err = hipSuccess;
-  if (!direct) err = launch_to_rows(e->operand, e->dtype, x, ld_in, first.n_in, r->batch, rows, stream);
-  if (err != hipSuccess) return device_error("input rows", err);
-  st = run_layers(*e, direct ? x : nullptr, ld_in, rows, r->batch, r->source, r->offsets, columns, nullptr, 0, true, base, w, &result, stream);
+  Rows result;
+  st = run_layers(*e, x, ld_in, Rows{}, r->batch, r->source, r->offsets, columns, nullptr, 0, base, w, &result, stream);
   if (st != PONNI_OK) return st;
-  err = launch_combine(e->dtype, result, columns, *r, last.n_out, y, ld_out, stream);
+  hipError_t const err = launch_combine(e->dtype, result, columns, *r, last.n_out, y, ld_out, stream);
   return err == hipSuccess ? PONNI_OK : device_error("weighted sum", err);
 }
 

@@ -62,6 +62,36 @@ struct ContractArgs {
   int32_t row_features;
 };
 
+// A whole chain in one kernel, states in LDS (contract_chain).
+constexpr int kChainLayers = 8;
+struct ChainLayer {
+  const char* weights;
+  const unsigned char* w_scales;
+  const float* bias;
+  int32_t steps;
+  int32_t blocks;
+  int32_t n_out;
+  int32_t act;
+  float act_a;
+};
+struct ChainArgs {
+  ContractArgs io;  // input, groups and output (weights, steps and the like unused)
+  ChainLayer layers[kChainLayers];
+  int32_t num_layers;
+  int32_t state_bytes;  // of a column's state: its steps * 64, the widest layer's
+  int32_t waves;        // of a workgroup: 4, or 8 for layers of more than 4 blocks
+};
+// A tile's LDS: the states, and their scales.
+int64_t chain_lds(Operand op, int state_bytes, int columns);
+// Columns of a chain's tile, 0 where the kernel does not take the chain; sets a.waves.
+int chain_columns(Operand op, ChainArgs& a);
+hipError_t launch_chain_f32(OutputKind kind, int columns, ChainArgs const& a, hipStream_t stream);
+hipError_t launch_chain_f16(OutputKind kind, int columns, ChainArgs const& a, hipStream_t stream);
+hipError_t launch_chain_bf16(OutputKind kind, int columns, ChainArgs const& a, hipStream_t stream);
+hipError_t launch_chain_mx4_f16(OutputKind kind, int columns, ChainArgs const& a, hipStream_t stream);
+hipError_t launch_chain_mx4_bf16(OutputKind kind, int columns, ChainArgs const& a, hipStream_t stream);
+hipError_t launch_chain(Operand op, int out_type, OutputKind kind, int columns, ChainArgs const& a, hipStream_t stream);
+
 // Whether a layer of these sizes reads its input as [features, columns] itself.
 bool takes_features(int64_t columns, int32_t experts, int32_t blocks);
 hipError_t launch_contraction(Operand op, int out_type, OutputKind kind, ContractArgs const& a, hipStream_t stream);

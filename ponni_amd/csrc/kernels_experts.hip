@@ -18,178 +18,13 @@
 
 #include <type_traits>
 
-#include "activations.h"
-#include "experts.h"
+#include "contract.h"
 #include "lds_requests.h"
-#include "operand_types.h"
-#include "program.h"
 
 namespace ponni_hip {
 namespace {
 
-typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
-typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) void* lds_void;
-
-// acc += A B for one step's fragments of a 16 x 16 tile.  mx4: a_scale holds the
-// scales of the 4 tiles of a block (TILE picks its byte), b_scale the column's in its first byte.
-template <Operand OP, int TILE>
-__device__ inline f32x4 multiply(i32x4 a, i32x4 b, f32x4 acc, int a_scale, int b_scale) {
-  if constexpr (OP == OPERAND_F16) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), acc, 0, 0, 0);
-  } else if constexpr (OP == OPERAND_BF16) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), acc, 0, 0, 0);
-  } else if constexpr (OP == OPERAND_MX4) {
-    i32x8 const a8 = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, b8 = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, acc, 4, 4, TILE, a_scale, 0, b_scale);
-  } else {
-    f32x4 const af = __builtin_bit_cast(f32x4, a), bf = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-    for (int e = 0; e < 4; e++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(af[e], bf[e], acc, 0, 0, 0);
-    return acc;
-  }
-}
-
-// A pointer that every lane of the wave holds, in scalar registers.
-__device__ inline char const* uniform(char const* p) {
-  uint64_t const v = reinterpret_cast<uint64_t>(p);
-  uint64_t const lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v)) & 0xffffffffu;
-  uint64_t const hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
-  return reinterpret_cast<char const*>(hi << 32 | lo);
-}
-
-// Columns of an expert's group, from offsets that a caller's program wrote:
-// whatever they hold, a group lies within [0, columns).
-struct Group {
-  int32_t first, last;
-};
-__device__ inline Group group_of(int32_t const* offsets, int expert, int32_t columns) {
-  auto clamp = [&](int32_t v) { return v < 0 ? 0 : v > columns ? columns : v; };
-  if (offsets == nullptr) return {0, columns};
-  int32_t const a = clamp(offsets[expert]), b = clamp(offsets[expert + 1]);
-  return {a, b < a ? a : b};
-}
-
-struct Tile {
-  int expert;
-  int32_t first, last;  // columns [first, last), at most the tile's width
-  int block;            // of output features
-  bool none;
-};
-
-// This workgroup's tile.  Every group has ceil(columns / width) column tiles; the
-// grid holds as many as any offsets can give.  Each XCD (workgroups go to the
-// eight in turn) takes a contiguous share of the tiles, output blocks of a column
-// tile first: its rows are read into one L2 only, and an expert's weights by few.
-template <int WIDTH>
-__device__ inline Tile find_tile(ContractArgs const& a, int out_blocks) {
-  int const lane = threadIdx.x & 63;
-  int32_t const columns = static_cast<int32_t>(a.columns);
-  auto tiles = [&](int base) {
-    if (base + lane >= a.experts) return 0;
-    Group const g = group_of(a.offsets, base + lane, columns);
-    return int((int64_t(g.last) - g.first + WIDTH - 1) / WIDTH);
-  };
-  auto scan = [&](int n) {  // inclusive, over the wave
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      int const t = __shfl_up(n, d);
-      n += lane >= d ? t : 0;
-    }
-    return n;
-  };
-  int64_t total = 0;
-  for (int base = 0; base < a.experts; base += 64) total += __shfl(scan(tiles(base)), 63);
-  total *= out_blocks;
-  int64_t const q = total / 8, r = total % 8, xcd = blockIdx.x % 8, at = blockIdx.x / 8;
-  Tile t{};
-  t.none = true;
-  if (at >= q + (xcd < r ? 1 : 0)) return t;
-  int64_t const index = xcd * q + (xcd < r ? xcd : r) + at;
-  int column_tile = static_cast<int>(index / out_blocks);
-  t.block = __builtin_amdgcn_readfirstlane(static_cast<int>(index % out_blocks));
-  for (int base = 0; base < a.experts; base += 64) {
-    int const n = tiles(base), end = scan(n);
-    int const all = __shfl(end, 63);
-    if (column_tile < all) {
-      int const l = __builtin_ctzll(__ballot(column_tile < end));
-      t.expert = __builtin_amdgcn_readfirstlane(base + l);
-      int const within = __builtin_amdgcn_readfirstlane(column_tile - (__shfl(end, l) - __shfl(n, l)));
-      Group const g = group_of(a.offsets, t.expert, columns);
-      t.first = __builtin_amdgcn_readfirstlane(g.first + within * WIDTH);
-      t.last = __builtin_amdgcn_readfirstlane(g.last - t.first < WIDTH ? g.last : t.first + WIDTH);
-      t.none = false;
-      return t;
-    }
-    column_tile -= all;
-  }
-  return t;
-}
-
-template <bool Precise, class Each>
-__device__ inline void activate(int act, float slope, Each&& each) {
-  switch (act) {
-    case ACT_RELU: each([](float v) { return act_relu(v); }); break;
-    case ACT_LEAKY_RELU: each([slope](float v) { return act_leaky_relu(v, slope); }); break;
-    case ACT_TANH: each([](float v) { return Precise ? tanh_f32(v) : tanh_half(v); }); break;
-    case ACT_SIGMOID: each([](float v) { return Precise ? sigmoid_f32(v) : act_sigmoid_fast(v); }); break;
-    case ACT_SILU: each([](float v) { return Precise ? silu_f32(v) : act_silu_fast(v); }); break;
-    case ACT_GELU_TANH: each([](float v) { return Precise ? gelu_tanh_f32(v) : act_gelu_tanh_fast(v); }); break;
-    case ACT_GELU_ERF: each([](float v) { return act_gelu_erf(v); }); break;
-    default: break;
-  }
-}
-
-// 16 consecutive features from feature f0 of row `col` (v: zero past n_out).
-template <OutputKind KIND, class S>
-__device__ inline void store_features(ContractArgs const& a, int64_t col, int f0, f32x4 (&v)[4]) {
-  if constexpr (KIND == OUT_FEATURES) {
-    S* __restrict__ y = static_cast<S*>(a.y) + col;
-#pragma unroll
-    for (int i = 0; i < 4; i++)
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-        if (f0 + 4 * i + e < a.n_out) y[int64_t(f0 + 4 * i + e) * a.ldy] = S(v[i][e]);
-  } else if constexpr (KIND == OUT_ROWS) {
-    typedef S Piece __attribute__((ext_vector_type(16 / sizeof(S))));
-    constexpr int N = 16 / sizeof(S);
-#pragma unroll
-    for (int p = 0; p < 16 / N; p++) {
-      Piece o;
-#pragma unroll
-      for (int e = 0; e < N; e++) o[e] = S(v[(p * N + e) / 4][(p * N + e) % 4]);
-      if (f0 + p * N < a.row_features)
-        *reinterpret_cast<Piece*>(a.y_rows.data + col * a.y_rows.stride + (f0 + p * N) * sizeof(S)) = o;
-    }
-  }
-}
-
-// The same as half a block of 32: lanes 16 apart hold its two halves.
-__device__ inline void store_mx4(ContractArgs const& a, int64_t col, bool valid, int f0, f32x4 (&v)[4]) {
-  float amax = 0.0f;
-  bool finite = true;
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      amax = fmaxf(amax, __builtin_fabsf(v[i][e]));
-      finite = finite && v[i][e] == v[i][e];
-    }
-  if (!finite) amax = __builtin_inff();
-  amax = fmaxf(amax, __shfl_xor(amax, 16));
-  unsigned const scale = mx4_scale(amax);
-  float const scale_value = mx4_scale_value(scale);
-  typedef int i32x2 __attribute__((ext_vector_type(2)));
-  i32x2 codes;
-#pragma unroll
-  for (int w = 0; w < 2; w++) codes[w] = mx4_word(scale_value, [&](int e) { return v[2 * w + e / 4][e % 4]; });
-  if (scale == 255u) codes = {0, 0};
-  if (!valid || f0 >= a.row_features) return;
-  *reinterpret_cast<i32x2*>(a.y_rows.data + col * a.y_rows.stride + f0 / 2) = codes;
-  if (f0 % kMx4Block == 0)
-    a.y_rows.scales[col * a.y_rows.scale_stride + f0 / 128 * a.y_rows.scale_step + f0 / kMx4Block % 4] = static_cast<unsigned char>(scale);
-}
 
 // Steps a turn of the loop: 128 bytes of a row, one whole line of the L2's.
 constexpr int kDepth = 2;
@@ -362,7 +197,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void contract(ContractArgs a) {
 #pragma unroll
       for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f0 + e < a.n_out ? v[e / 4][e % 4] : 0.0f;
       if constexpr (KIND == OUT_MX4) store_mx4(a, col, col < t.last, f0, v);
-      else if (col < t.last) store_features<KIND, S>(a, col, f0, v);
+      else if (col < t.last) store_features<KIND, S>(a, col, f0, v, a.n_out);
     }
   }
 }
@@ -377,7 +212,6 @@ template <Operand OP, class S, OutputKind KIND, bool FEATURES, int NJ, int W>
 __global__ __launch_bounds__(64 * W) void contract_thin(ContractArgs a) {
   constexpr bool MX = OP == OPERAND_MX4;
   constexpr int U = NJ == 1 ? 4 : 2;  // steps under way
-  constexpr int N = OP == OPERAND_F32 ? 4 : MX ? 32 : 8;
   __shared__ f32x4 sums[W][4 * NJ][64];
   int const lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -396,33 +230,7 @@ __global__ __launch_bounds__(64 * W) void contract_thin(ContractArgs a) {
   // This lane's fragment of step s of column j's row, and its scale.
   auto read_row = [&](int s, int j, i32x4& v, int& scale) {
     if constexpr (FEATURES) {
-      S const* x = static_cast<S const*>(a.features) + row[j];
-      S e[N];
-#pragma unroll
-      for (int k = 0; k < N; k++) {
-        int const f = (4 * s + g) * N + k;
-        e[k] = f < a.n_in ? x[f * a.ldx] : S(0.0f);
-      }
-      if constexpr (MX) {
-        float amax = 0.0f;
-        bool finite = true;
-#pragma unroll
-        for (int k = 0; k < N; k++) {
-          amax = fmaxf(amax, __builtin_fabsf(float(e[k])));
-          finite = finite && e[k] == e[k];
-        }
-        scale = finite ? mx4_scale(amax) : 255u;
-        float const scale_value = mx4_scale_value(scale);
-#pragma unroll
-        for (int w = 0; w < 4; w++) v[w] = mx4_word(scale_value, [&](int k) { return e[8 * w + k]; });
-        if (scale == 255) v = {0, 0, 0, 0};
-      } else {
-        typedef S Piece __attribute__((ext_vector_type(N)));
-        Piece p;
-#pragma unroll
-        for (int k = 0; k < N; k++) p[k] = e[k];
-        v = __builtin_bit_cast(i32x4, p);
-      }
+      read_features<OP, S>(a, row[j], 4 * s + g, v, scale);
     } else {
       v = *reinterpret_cast<i32x4 const*>(a.x.data + row[j] * a.x.stride + s * 64 + 16 * g);
       if constexpr (MX) scale = a.x.scales[row[j] * a.x.scale_stride + s * a.x.scale_step + g];
@@ -481,15 +289,146 @@ __global__ __launch_bounds__(64 * W) void contract_thin(ContractArgs a) {
   for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f0 + e < a.n_out ? v[e / 4][e % 4] : 0.0f;
   int64_t const col = int64_t(t.first) + 16 * wave + c;
   if constexpr (KIND == OUT_MX4) store_mx4(a, col, col < t.last, f0, v);
-  else if (col < t.last) store_features<KIND, S>(a, col, f0, v);
+  else if (col < t.last) store_features<KIND, S>(a, col, f0, v, a.n_out);
 }
 
-// The grid of tiles of `width` columns x `out_blocks` blocks, at least as many as any offsets give.
-inline int64_t grid_of(ContractArgs const& a, int64_t width, int64_t out_blocks) {
-  // ceil(n / width) summed over the groups: at most one more than n / width for each that has columns
-  int64_t const partial = a.experts < a.columns ? a.experts : a.columns;
-  // (a share per XCD is rounded up: the grid is whole rounds of the eight)
-  return ((a.columns / width + partial) * out_blocks + 7) / 8 * 8;
+// A whole chain on one tile of C columns: the columns' states stay in LDS, a row of
+// whole steps and 16 bytes of padding a column (16 columns' reads of one
+// fragment then fall into different banks), and a layer's outputs, complete in the
+// accumulators of the eight waves, take the place of its inputs between two
+// barriers.  Weights come from L2 straight into registers, `AHEAD` steps before
+// their MFMAs; each serves 16 NJ columns.  The waves are WM x WN, WM the layer's
+// blocks of 64 features, so that a narrow layer gives every wave fewer columns.
+// FEATURES: the input as the caller holds it.
+template <Operand OP, class S, OutputKind KIND, bool FEATURES, int C>
+__global__ __launch_bounds__(512, 2) void contract_chain(ChainArgs chain) {
+  constexpr bool MX = OP == OPERAND_MX4;
+  constexpr int N = OP == OPERAND_F32 ? 4 : MX ? 32 : 8;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  ContractArgs const& a = chain.io;
+  int const lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Tile const t = find_tile<C>(a, 1);
+  if (t.none) return;
+  int const stride = chain.state_bytes + 16, scale_stride = chain.state_bytes / 16 + 4;
+  char* const states = lds;
+  unsigned char* const scales = reinterpret_cast<unsigned char*>(lds + C * stride);
+  {
+    // The input's pieces of 16 bytes, one lane per column and piece.
+    int const pieces = chain.layers[0].steps * 4;
+    for (int p = threadIdx.x; p < C * pieces; p += 512) {
+      int const local = p % C, piece = p / C;
+      int32_t const col = t.first + local < t.last ? t.first + local : t.last - 1;
+      int64_t row = a.source != nullptr ? a.source[col] : col;
+      row = row < 0 || row >= a.x_rows ? 0 : row;
+      i32x4 v;
+      int scale = 0;
+      if constexpr (FEATURES) {
+        read_features<OP, S>(a, row, piece, v, scale);
+      } else {
+        v = *reinterpret_cast<i32x4 const*>(a.x.data + row * a.x.stride + piece * 16);
+        if constexpr (MX) scale = a.x.scales[row * a.x.scale_stride + piece / 4 * a.x.scale_step + piece % 4];
+      }
+      *reinterpret_cast<i32x4*>(states + local * stride + piece * 16) = v;
+      if constexpr (MX) scales[local * scale_stride + piece] = static_cast<unsigned char>(scale);
+    }
+  }
+  __syncthreads();
+  for (int l = 0; l < chain.num_layers; l++) {
+    ChainLayer const& layer = chain.layers[l];
+    bool const last = l + 1 == chain.num_layers;
+    int const row_features = last ? 0 : chain.layers[l + 1].steps * 4 * N;
+    auto pass = [&]<int NJ>(std::integral_constant<int, NJ>, int wn_bits) {
+      constexpr int AHEAD = NJ >= 8 ? 1 : NJ == 4 ? 2 : 4;
+      int const wm = wave >> wn_bits, wn = wave & ((1 << wn_bits) - 1);
+      bool const busy = wm < layer.blocks && 16 * NJ * wn < C;
+      f32x4 acc[4][NJ];
+      int const steps = layer.steps;
+      if (busy) {
+        int64_t const block = int64_t(t.expert) * layer.blocks + wm;
+        char const* weights = layer.weights + block * steps * 4096 + 16 * lane;
+        int const* w_scales = MX ? reinterpret_cast<int const*>(layer.w_scales + block * steps * 256) + lane : nullptr;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          f32x4 seed = {0, 0, 0, 0};
+          if (layer.bias != nullptr) seed = *reinterpret_cast<f32x4 const*>(layer.bias + block * 64 + 16 * g + 4 * i);
+#pragma unroll
+          for (int j = 0; j < NJ; j++) acc[i][j] = seed;
+        }
+        char const* rows = states + (16 * NJ * wn + c) * stride + 16 * g;
+        unsigned char const* row_scales = scales + (16 * NJ * wn + c) * scale_stride + g;
+        i32x4 av[2][AHEAD][4];
+        int as[2][AHEAD] = {};
+        auto load = [&](int set, int s0) {
+#pragma unroll
+          for (int u = 0; u < AHEAD; u++) {
+            int const s = s0 + u < steps ? s0 + u : steps - 1;
+#pragma unroll
+            for (int i = 0; i < 4; i++) av[set][u][i] = *reinterpret_cast<i32x4 const*>(weights + s * 4096 + i * 1024);
+            if constexpr (MX) as[set][u] = w_scales[s * 64];
+          }
+        };
+        auto multiply_steps = [&](int set, int s0) {
+#pragma unroll
+          for (int u = 0; u < AHEAD; u++) {
+            if (s0 + u >= steps) break;
+            i32x4 bv[NJ];
+            int bs[NJ] = {};
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+              bv[j] = *reinterpret_cast<i32x4 const*>(rows + 16 * j * stride + (s0 + u) * 64);
+              if constexpr (MX) bs[j] = row_scales[16 * j * scale_stride + (s0 + u) * 4];
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+              acc[0][j] = multiply<OP, 0>(av[set][u][0], bv[j], acc[0][j], as[set][u], bs[j]);
+              acc[1][j] = multiply<OP, 1>(av[set][u][1], bv[j], acc[1][j], as[set][u], bs[j]);
+              acc[2][j] = multiply<OP, 2>(av[set][u][2], bv[j], acc[2][j], as[set][u], bs[j]);
+              acc[3][j] = multiply<OP, 3>(av[set][u][3], bv[j], acc[3][j], as[set][u], bs[j]);
+            }
+          }
+        };
+        load(0, 0);
+        for (int s = 0; s < steps; s += 2 * AHEAD) {
+          load(1, s + AHEAD);
+          multiply_steps(0, s);
+          load(0, s + 2 * AHEAD);
+          multiply_steps(1, s + AHEAD);
+        }
+      }
+      if (!last) __syncthreads();  // every wave has read the layer's inputs
+      if (busy) {
+        int const f0 = wm * 64 + 16 * g;
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+          int const local = 16 * (NJ * wn + j) + c;
+          int64_t const col = int64_t(t.first) + local;
+          f32x4 v[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
+          activate<OP == OPERAND_F32>(layer.act, layer.act_a, [&](auto f) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f(v[e / 4][e % 4]);
+          });
+#pragma unroll
+          for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f0 + e < layer.n_out ? v[e / 4][e % 4] : 0.0f;
+          if (last) {
+            if (col < t.last) store_features<KIND, S>(a, col, f0, v, layer.n_out);
+          } else if constexpr (MX) {
+            write_mx4(v, f0 < row_features, reinterpret_cast<i32x2*>(states + local * stride + f0 / 2),
+                      f0 % kMx4Block == 0, scales + local * scale_stride + f0 / kMx4Block);
+          } else {
+            write_pieces<S>(states + local * stride, f0, row_features, v);
+          }
+        }
+      }
+      if (!last) __syncthreads();
+    };
+    // blocks of 64 features -> waves along the columns
+    int const blocks = layer.blocks;
+    if (blocks > 4) pass(std::integral_constant<int, C / 16>{}, 0);
+    else if (blocks > 2) pass(std::integral_constant<int, C / 32>{}, 1);
+    else if (blocks > 1) pass(std::integral_constant<int, C / 64>{}, 2);
+    else pass(std::integral_constant<int, C / 128 < 1 ? 1 : C / 128>{}, 3);
+  }
 }
 
 template <Operand OP, class S, OutputKind KIND, int MI, int NJ, int WM, int WN>
@@ -635,6 +574,39 @@ template <class F> bool with_parameter_dtype(int dtype, F&& f) {
 }
 
 }  // namespace
+
+int64_t chain_lds(Operand op, int state_bytes, int columns) {
+  return int64_t(columns) * (state_bytes + 16) + (op == OPERAND_MX4 ? int64_t(columns) * (state_bytes / 16 + 4) : 0);
+}
+
+int chain_columns(Operand op, ChainArgs& a) {
+  int blocks = 0;
+  for (int l = 0; l < a.num_layers; l++) {
+    blocks = a.layers[l].blocks > blocks ? a.layers[l].blocks : blocks;
+    if (a.layers[l].act == ACT_GELU_ERF) return 0;  // (its code, for every accumulator of every shape of layer)
+  }
+  if (blocks > 8) return 0;
+  a.waves = blocks > 4 ? 8 : 4;
+  static int const force = getenv("CHAINC") ? atoi(getenv("CHAINC")) : 0;
+  int const per_cu = blocks > 4 ? 1 : 2;
+  for (int columns = op == OPERAND_F32 ? 64 : 128; columns >= (blocks > 4 ? 64 : 32); columns /= 2) {
+    if (force && columns > force) continue;
+    if (chain_lds(op, a.state_bytes, columns) > 160 * 1024 / per_cu) continue;
+    if (force || columns == (blocks > 4 ? 64 : 32) || a.io.columns >= int64_t(columns) * 256 * per_cu) return columns;
+  }
+  return 0;
+}
+
+hipError_t launch_chain(Operand op, int out_type, OutputKind kind, int columns, ChainArgs const& a, hipStream_t stream) {
+  switch (op) {
+    case OPERAND_F32: return launch_chain_f32(kind, columns, a, stream);
+    case OPERAND_F16: return launch_chain_f16(kind, columns, a, stream);
+    case OPERAND_BF16: return launch_chain_bf16(kind, columns, a, stream);
+    default:
+      return out_type == PONNI_F16 ? launch_chain_mx4_f16(kind, columns, a, stream)
+                                   : launch_chain_mx4_bf16(kind, columns, a, stream);
+  }
+}
 
 bool takes_features(int64_t columns, int32_t experts, int32_t blocks) { return thin_columns(columns, experts, blocks) > 0; }
 
