@@ -52,8 +52,8 @@ __global__ __launch_bounds__(64 * W, 2) void contract_chain(ChainArgs chain) {
     ChainLayer const& layer = chain.layers[l];
     bool const last = l + 1 == chain.num_layers;
     int const row_features = last ? 0 : chain.layers[l + 1].steps * 4 * N;
-    auto pass = [&]<int NJ>(std::integral_constant<int, NJ>, int wn_bits) {
-      constexpr int SETS = NJ >= 4 ? 2 : 4;  // of weights: the step's, and those of the next ones on their way
+    auto pass = [&]<int NJ>(std::integral_constant<int, NJ>, int wn_bits) __attribute__((always_inline)) {
+      constexpr int AHEAD = NJ >= 4 ? 1 : 3;  // steps that weights are loaded before their MFMAs; rows one
       int const wm = wave >> wn_bits, wn = wave & ((1 << wn_bits) - 1);
       // (new to the compiler in every layer: it would keep the addresses of every tile of
       // every shape of layer in registers, a hundred more than there are)
@@ -79,36 +79,50 @@ __global__ __launch_bounds__(64 * W, 2) void contract_chain(ChainArgs chain) {
         }
         char const* rows = states + (16 * NJ * wn + c) * stride + 16 * g;
         unsigned char const* row_scales = scales + (16 * NJ * wn + c) * scale_stride + g;
-        i32x4 av[SETS][4];
-        int as[SETS] = {};
+        i32x4 av[AHEAD + 1][4], bv[2][NJ];
+        int as[AHEAD + 1] = {}, bs[2][NJ] = {};
         auto load = [&](int set, int s) {
           s = s < steps ? s : steps - 1;
 #pragma unroll
           for (int i = 0; i < 4; i++) av[set][i] = *reinterpret_cast<i32x4 const*>(weights + s * 4096 + i * 1024);
           if constexpr (MX) as[set] = w_scales[s * 64];
         };
+        auto read = [&](int set, int s) {
+          s = s < steps ? s : steps - 1;
 #pragma unroll
-        for (int u = 0; u < SETS - 1; u++) load(u, u);
-        for (int s = 0; s < steps; s += SETS) {
+          for (int j = 0; j < NJ; j++) {
+            bv[set][j] = *reinterpret_cast<i32x4 const*>(rows + 16 * j * stride + s * 64);
+            if constexpr (MX) bs[set][j] = row_scales[16 * j * scale_stride + s * 4];
+          }
+        };
+        auto multiply_step = [&](int aset, int bset) {
 #pragma unroll
-          for (int u = 0; u < SETS; u++) {
-            load((u + SETS - 1) % SETS, s + u + SETS - 1);
-            if (s + u < steps) {
-              i32x4 bv[NJ];
-              int bs[NJ] = {};
+          for (int j = 0; j < NJ; j++) {
+            acc[0][j] = multiply<OP, 0>(av[aset][0], bv[bset][j], acc[0][j], as[aset], bs[bset][j]);
+            acc[1][j] = multiply<OP, 1>(av[aset][1], bv[bset][j], acc[1][j], as[aset], bs[bset][j]);
+            acc[2][j] = multiply<OP, 2>(av[aset][2], bv[bset][j], acc[2][j], as[aset], bs[bset][j]);
+            acc[3][j] = multiply<OP, 3>(av[aset][3], bv[bset][j], acc[3][j], as[aset], bs[bset][j]);
+          }
+        };
 #pragma unroll
-              for (int j = 0; j < NJ; j++) {
-                bv[j] = *reinterpret_cast<i32x4 const*>(rows + 16 * j * stride + (s + u) * 64);
-                if constexpr (MX) bs[j] = row_scales[16 * j * scale_stride + (s + u) * 4];
-              }
+        for (int u = 0; u < AHEAD; u++) load(u, u);
+        read(0, 0);
+        // whole turns of the register sets, then the steps left
+        constexpr int TURN = AHEAD + 1;
+        int s = 0;
+        for (; s + TURN <= steps; s += TURN) {
 #pragma unroll
-              for (int j = 0; j < NJ; j++) {
-                acc[0][j] = multiply<OP, 0>(av[u][0], bv[j], acc[0][j], as[u], bs[j]);
-                acc[1][j] = multiply<OP, 1>(av[u][1], bv[j], acc[1][j], as[u], bs[j]);
-                acc[2][j] = multiply<OP, 2>(av[u][2], bv[j], acc[2][j], as[u], bs[j]);
-                acc[3][j] = multiply<OP, 3>(av[u][3], bv[j], acc[3][j], as[u], bs[j]);
-              }
-            }
+          for (int u = 0; u < TURN; u++) {
+            load((u + AHEAD) % TURN, s + u + AHEAD);
+            read((u + 1) % 2, s + u + 1);
+            multiply_step(u, u % 2);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < TURN - 1; u++) {
+          if (s + u < steps) {
+            if (u > 0) read(u % 2, s + u);
+            multiply_step(u, u % 2);
           }
         }
       }
@@ -120,12 +134,11 @@ __global__ __launch_bounds__(64 * W, 2) void contract_chain(ChainArgs chain) {
           int const local = 16 * (NJ * wn + j) + c;
           int64_t const col = int64_t(t.first) + local;
           f32x4 v[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
-          activate<OP == OPERAND_F32, false>(layer.act, layer.act_a, [&](auto f) {
+          activate<OP == OPERAND_F32, true>(layer.act, layer.act_a, [&](auto f) {
 #pragma unroll
             for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f(v[e / 4][e % 4]);
           });
-#pragma unroll
-          for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f0 + e < layer.n_out ? v[e / 4][e % 4] : 0.0f;
+          clear_past(v, wm * 64, f0, layer.n_out);
           if (last) {
             if (col < t.last) store_features<KIND, S>(a, col, f0, v, layer.n_out);
           } else if constexpr (MX) {
@@ -184,7 +197,7 @@ hipError_t launch_chain_as(OutputKind kind, int columns, ChainArgs const& a, hip
     if (columns == 64)
       return eight ? launch_chain_sized<OP, S, KIND, FEATURES, 64, 8>(a, stream)
                    : launch_chain_sized<OP, S, KIND, FEATURES, 64, 4>(a, stream);
-    return launch_chain_sized<OP, S, KIND, FEATURES, 32, 4>(a, stream);
+    return hipErrorInvalidValue;
   };
   if (kind == OUT_ROWS) return sized.template operator()<OUT_ROWS, false>();
   if (a.io.features != nullptr) return sized.template operator()<OUT_FEATURES, true>();

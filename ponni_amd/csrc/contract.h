@@ -113,21 +113,31 @@ __device__ inline Tile find_tile(ContractArgs const& a, int out_blocks) {
   return t;
 }
 
-// (ERF: with GELU's exact form, the longest.)
-template <bool Precise, bool ERF = true, class Each>
+// CHAIN: without GELU's exact form, the longest, and with tanh's hardware form alone, as the
+// other fused kernels have it (off by an ulp of one near zero).
+template <bool Precise, bool CHAIN = false, class Each>
 __device__ inline void activate(int act, float slope, Each&& each) {
   switch (act) {
     case ACT_RELU: each([](float v) { return act_relu(v); }); break;
     case ACT_LEAKY_RELU: each([slope](float v) { return act_leaky_relu(v, slope); }); break;
-    case ACT_TANH: each([](float v) { return Precise ? tanh_f32(v) : tanh_half(v); }); break;
+    case ACT_TANH: each([](float v) { return Precise ? tanh_f32(v) : CHAIN ? act_tanh_fast(v) : tanh_half(v); }); break;
     case ACT_SIGMOID: each([](float v) { return Precise ? sigmoid_f32(v) : act_sigmoid_fast(v); }); break;
     case ACT_SILU: each([](float v) { return Precise ? silu_f32(v) : act_silu_fast(v); }); break;
     case ACT_GELU_TANH: each([](float v) { return Precise ? gelu_tanh_f32(v) : act_gelu_tanh_fast(v); }); break;
     case ACT_GELU_ERF:
-      if constexpr (ERF) each([](float v) { return act_gelu_erf(v); });
+      if constexpr (!CHAIN) each([](float v) { return act_gelu_erf(v); });
       break;
     default: break;
   }
+}
+
+// Features past the last one are zero: their weights are, but not those times an
+// infinity, nor sigmoid(0).  (16 features from f0 on, of the block of 64 that begins at
+// `block`; whole blocks, which the compiler would check feature by feature, need no check.)
+__device__ inline void clear_past(f32x4 (&v)[4], int block, int f0, int n_out) {
+  if (block + 64 <= n_out) return;
+#pragma unroll
+  for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f0 + e < n_out ? v[e / 4][e % 4] : 0.0f;
 }
 
 // 16 consecutive features from feature f0 on of a row in pieces of 16 bytes (zero past the
@@ -149,10 +159,18 @@ template <OutputKind KIND, class S>
 __device__ inline void store_features(ContractArgs const& a, int64_t col, int f0, f32x4 (&v)[4], int n_out) {
   if constexpr (KIND == OUT_FEATURES) {
     S* y = static_cast<S*>(a.y) + int64_t(f0) * a.ldy + col;
+    if (f0 + 16 <= n_out) {
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
-      if (f0 + e < n_out) *y = S(v[e / 4][e % 4]);
-      y += a.ldy;
+      for (int e = 0; e < 16; e++) {
+        *y = S(v[e / 4][e % 4]);
+        y += a.ldy;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 15; e++) {
+        if (f0 + e < n_out) *y = S(v[e / 4][e % 4]);
+        y += a.ldy;
+      }
     }
   } else {
     write_pieces<S>(a.y_rows.data + col * a.y_rows.stride, f0, a.row_features, v);

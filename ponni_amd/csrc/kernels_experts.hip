@@ -194,8 +194,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void contract(ContractArgs a) {
 #pragma unroll
         for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f(v[e / 4][e % 4]);
       });
-#pragma unroll
-      for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f0 + e < a.n_out ? v[e / 4][e % 4] : 0.0f;
+      clear_past(v, f0 - 16 * g, f0, a.n_out);
       if constexpr (KIND == OUT_MX4) store_mx4(a, col, col < t.last, f0, v);
       else if (col < t.last) store_features<KIND, S>(a, col, f0, v, a.n_out);
     }
@@ -285,8 +284,7 @@ __global__ __launch_bounds__(64 * W) void contract_thin(ContractArgs a) {
 #pragma unroll
     for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f(v[e / 4][e % 4]);
   });
-#pragma unroll
-  for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f0 + e < a.n_out ? v[e / 4][e % 4] : 0.0f;
+  clear_past(v, t.block * 64, f0, a.n_out);
   int64_t const col = int64_t(t.first) + 16 * wave + c;
   if constexpr (KIND == OUT_MX4) store_mx4(a, col, col < t.last, f0, v);
   else if (col < t.last) store_features<KIND, S>(a, col, f0, v, a.n_out);
@@ -588,13 +586,8 @@ int chain_columns(Operand op, ChainArgs& a) {
   if (blocks > 8) return 0;
   a.waves = blocks > 4 ? 8 : 4;
   static int const force = getenv("CHAINC") ? atoi(getenv("CHAINC")) : 0;
-  int const per_cu = blocks > 4 ? 1 : 2;
-  for (int columns = op == OPERAND_F32 ? 64 : 128; columns >= (blocks > 4 ? 64 : 32); columns /= 2) {
-    if (force && columns > force) continue;
-    if (chain_lds(op, a.state_bytes, columns) > 160 * 1024 / per_cu) continue;
-    if (force || columns == (blocks > 4 ? 64 : 32) || a.io.columns >= int64_t(columns) * 256 * per_cu) return columns;
-  }
-  return 0;
+  if (force != 64 && op != OPERAND_F32 && chain_lds(op, a.state_bytes, 128) <= 160 * 1024 / (blocks > 4 ? 1 : 2) && (force || a.io.columns >= 1 << 17)) return 128;
+  return chain_lds(op, a.state_bytes, 64) <= 160 * 1024 ? 64 : 0;
 }
 
 hipError_t launch_chain(Operand op, int out_type, OutputKind kind, int columns, ChainArgs const& a, hipStream_t stream) {
