@@ -15,7 +15,7 @@ namespace {
 // blocks of 64 features, so that a narrow layer gives every wave fewer columns.
 // FEATURES: the input as the caller holds it.
 template <Operand OP, class S, OutputKind KIND, bool FEATURES, int C, int W>
-__global__ __launch_bounds__(64 * W, 2) void contract_chain(ChainArgs chain) {
+__global__ __launch_bounds__(64 * W, W == 4 && (OP == OPERAND_F16 || OP == OPERAND_BF16) ? 4 : 2) void contract_chain(ChainArgs chain) {
   constexpr bool MX = OP == OPERAND_MX4;
   constexpr int N = OP == OPERAND_F32 ? 4 : MX ? 32 : 8;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -188,16 +188,10 @@ hipError_t launch_chain_sized(ChainArgs const& a, hipStream_t stream) {
 template <Operand OP, class S>
 hipError_t launch_chain_as(OutputKind kind, int columns, ChainArgs const& a, hipStream_t stream) {
   auto sized = [&]<OutputKind KIND, bool FEATURES>() {
-    bool const eight = a.waves == 8;
-    if constexpr (OP != OPERAND_F32) {
-      if (columns == 128)
-        return eight ? launch_chain_sized<OP, S, KIND, FEATURES, 128, 8>(a, stream)
-                     : launch_chain_sized<OP, S, KIND, FEATURES, 128, 4>(a, stream);
-    }
-    if (columns == 64)
-      return eight ? launch_chain_sized<OP, S, KIND, FEATURES, 64, 8>(a, stream)
-                   : launch_chain_sized<OP, S, KIND, FEATURES, 64, 4>(a, stream);
-    return hipErrorInvalidValue;
+    if (a.waves == 4) return launch_chain_sized<OP, S, KIND, FEATURES, 64, 4>(a, stream);
+    if constexpr (OP == OPERAND_F32) return hipErrorInvalidValue;
+    else return columns == 128 ? launch_chain_sized<OP, S, KIND, FEATURES, 128, 8>(a, stream)
+                               : launch_chain_sized<OP, S, KIND, FEATURES, 64, 8>(a, stream);
   };
   if (kind == OUT_ROWS) return sized.template operator()<OUT_ROWS, false>();
   if (a.io.features != nullptr) return sized.template operator()<OUT_FEATURES, true>();

@@ -577,16 +577,21 @@ int64_t chain_lds(Operand op, int state_bytes, int columns) {
   return int64_t(columns) * (state_bytes + 16) + (op == OPERAND_MX4 ? int64_t(columns) * (state_bytes / 16 + 4) : 0);
 }
 
+// One kernel takes the chain where the states fit LDS and more columns than a thin tile's
+// share an expert's weights.  Against layer by layer (us): fp16 64-256-256-256-64 tanh,
+// 1,000,000 columns 518 / 1117; bf16 512-512-512, 200,000 360 / 435; 100-200-100, 3,000 13 / 20;
+// 4 bits 256-256, 1,000,000 389 / 411.  Not fp32 layers of more than 256
+// features, whose 64 columns a tile read the weights too often (200-300-100, 20,000: 99 / 79), nor
+// few columns (bf16 500-500-500, 100 columns of 8 experts: 22 / 12).
 int chain_columns(Operand op, ChainArgs& a) {
   int blocks = 0;
   for (int l = 0; l < a.num_layers; l++) {
     blocks = a.layers[l].blocks > blocks ? a.layers[l].blocks : blocks;
     if (a.layers[l].act == ACT_GELU_ERF) return 0;  // (its code, for every accumulator of every shape of layer)
   }
-  if (blocks > 8) return 0;
+  if (blocks > (op == OPERAND_F32 ? 4 : 8) || thin_columns(a.io.columns, a.io.experts, blocks) > 0) return 0;
   a.waves = blocks > 4 ? 8 : 4;
-  static int const force = getenv("CHAINC") ? atoi(getenv("CHAINC")) : 0;
-  if (force != 64 && op != OPERAND_F32 && chain_lds(op, a.state_bytes, 128) <= 160 * 1024 / (blocks > 4 ? 1 : 2) && (force || a.io.columns >= 1 << 17)) return 128;
+  if (blocks > 4 && chain_lds(op, a.state_bytes, 128) <= 160 * 1024 && a.io.columns >= 128 * 512) return 128;
   return chain_lds(op, a.state_bytes, 64) <= 160 * 1024 ? 64 : 0;
 }
 
