@@ -173,7 +173,7 @@ __device__ inline void store_features(ContractArgs const& a, int64_t col, int f0
       }
     }
   } else {
-    write_pieces<S>(a.y_rows.data + col * a.y_rows.stride, f0, a.row_features, v);
+    write_pieces<std::conditional_t<KIND == OUT_FLOATS, float, S>>(a.y_rows.data + col * a.y_rows.stride, f0, a.row_features, v);
   }
 }
 

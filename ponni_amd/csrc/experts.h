@@ -32,7 +32,8 @@ struct Rows {
   int64_t scale_step = 0;           // and to those of the next step
 };
 
-enum OutputKind { OUT_FEATURES = 0, OUT_ROWS = 1, OUT_MX4 = 2 };
+// [features, columns], or rows of the operand's type, of 4 bits, of fp32.
+enum OutputKind { OUT_FEATURES = 0, OUT_ROWS = 1, OUT_MX4 = 2, OUT_FLOATS = 3 };
 
 // One layer over columns grouped by expert:
 // y[f, c] = act(bias_e[f] + sum_k W_e[k][f] x[k, c]) for offsets[e] <= c < offsets[e + 1].
@@ -54,7 +55,7 @@ struct ContractArgs {
   int32_t n_out;
   int32_t act;  // ActCode, 0: none
   float act_a;
-  // OUT_FEATURES: y[f * ldy + c] of `out_type`; OUT_ROWS / OUT_MX4: y_rows,
+  // OUT_FEATURES: y[f * ldy + c] of `out_type`; else y_rows,
   // `row_features` features each (those past n_out zero).
   void* y;
   int64_t ldy;
@@ -99,8 +100,9 @@ hipError_t launch_contraction(Operand op, int out_type, OutputKind kind, Contrac
 // x [features, columns] of `dtype` as rows of `op`, `row_bytes` a row.
 hipError_t launch_to_rows(Operand op, int dtype, const void* x, int64_t ld, int64_t features, int64_t columns,
                           Rows const& rows, hipStream_t stream);
-// y[f, b] = sum_j weights[j, b] rows[slots[j, b]][f] (slots outside [0, num_rows) add nothing).
-hipError_t launch_combine(int dtype, Rows const& rows, int64_t num_rows, const ponni_routing& r, int64_t features,
+// y[f, b] = sum_j weights[j, b] rows[slots[j, b]][f] (slots outside [0, num_rows) add nothing); rows of
+// `dtype`, or floats.
+hipError_t launch_combine(int dtype, bool floats, Rows const& rows, int64_t num_rows, const ponni_routing& r, int64_t features,
                           void* y, int64_t ld, hipStream_t stream);
 // W [experts, n_in, n_out] of `dtype` in fragment order (values past n_in or n_out zero).
 hipError_t launch_pack_weights(Operand op, int dtype, const void* w, int64_t experts, int64_t n_in, int64_t n_out,

@@ -201,24 +201,25 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void contract(ContractArgs a) {
   }
 }
 
-// Few columns: 64 output features x 16 NJ columns a workgroup, whose W waves
-// share the contraction: what bounds these is the weights' way from memory, so each
-// wave has several steps' fragments under way at once, straight into registers, and
-// no wave waits for another before the sums meet in LDS (in the order of the
-// waves).  FEATURES: the input as the caller holds it, without rows made of it
-// first; 4-bit fragments are quantised as they are read.
-template <Operand OP, class S, OutputKind KIND, bool FEATURES, int NJ, int W>
+// Few columns: 16 MT output features (MT tiles of a block of 64) x 16 NJ columns a
+// workgroup, whose W waves share the contraction: what bounds these is the weights' way
+// from memory, so each wave has several steps' fragments under way at once,
+// straight into registers, and no wave waits for another before the sums meet in LDS
+// (in the order of the waves).  FEATURES: the input as the caller holds it, without
+// rows made of it first; 4-bit fragments are quantised as they are read.
+template <Operand OP, class S, OutputKind KIND, bool FEATURES, int MT, int NJ, int W>
 __global__ __launch_bounds__(64 * W) void contract_thin(ContractArgs a) {
+  static_assert(MT == 4 || (MT == 1 && KIND != OUT_MX4), "a lane's 16 features, or 4 of them");
   constexpr bool MX = OP == OPERAND_MX4;
   constexpr int U = NJ == 1 ? 4 : 2;  // steps under way
-  __shared__ f32x4 sums[W][4 * NJ][64];
+  __shared__ f32x4 sums[W][MT * NJ][64];
   int const lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Tile const t = find_tile<16 * NJ>(a, a.blocks);
+  Tile const t = find_tile<16 * NJ>(a, a.blocks * (4 / MT));
   if (t.none) return;
-  int const steps = a.steps;
-  int64_t const block = int64_t(t.expert) * a.blocks + t.block;
-  char const* const weights = a.weights + block * steps * 4096 + 16 * lane;
+  int const steps = a.steps, tile0 = MT == 4 ? 0 : t.block % 4, block_here = MT == 4 ? t.block : t.block / 4;
+  int64_t const block = int64_t(t.expert) * a.blocks + block_here;
+  char const* const weights = a.weights + block * steps * 4096 + tile0 * 1024 + 16 * lane;
   int64_t row[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; j++) {
@@ -235,17 +236,17 @@ __global__ __launch_bounds__(64 * W) void contract_thin(ContractArgs a) {
       if constexpr (MX) scale = a.x.scales[row[j] * a.x.scale_stride + s * a.x.scale_step + g];
     }
   };
-  f32x4 acc[4][NJ] = {};
+  f32x4 acc[MT][NJ] = {};
   for (int s0 = wave; s0 < steps; s0 += U * W) {
-    i32x4 av[U][4], bv[U][NJ];
+    i32x4 av[U][MT], bv[U][NJ];
     int as[U] = {}, bs[U][NJ] = {};
 #pragma unroll
     for (int u = 0; u < U; u++) {
       int const s = s0 + u * W;
       if (s >= steps) continue;
 #pragma unroll
-      for (int i = 0; i < 4; i++) av[u][i] = *reinterpret_cast<i32x4 const*>(weights + int64_t(s) * 4096 + i * 1024);
-      if constexpr (MX) as[u] = reinterpret_cast<int const*>(a.w_scales + (block * steps + s) * 256)[lane];
+      for (int i = 0; i < MT; i++) av[u][i] = *reinterpret_cast<i32x4 const*>(weights + int64_t(s) * 4096 + i * 1024);
+      if constexpr (MX) as[u] = reinterpret_cast<int const*>(a.w_scales + (block * steps + s) * 256)[lane] >> (8 * tile0);
     }
 #pragma unroll
     for (int u = 0; u < U; u++) {
@@ -259,173 +260,48 @@ __global__ __launch_bounds__(64 * W) void contract_thin(ContractArgs a) {
 #pragma unroll
       for (int j = 0; j < NJ; j++) {
         acc[0][j] = multiply<OP, 0>(av[u][0], bv[u][j], acc[0][j], as[u], bs[u][j]);
-        acc[1][j] = multiply<OP, 1>(av[u][1], bv[u][j], acc[1][j], as[u], bs[u][j]);
-        acc[2][j] = multiply<OP, 2>(av[u][2], bv[u][j], acc[2][j], as[u], bs[u][j]);
-        acc[3][j] = multiply<OP, 3>(av[u][3], bv[u][j], acc[3][j], as[u], bs[u][j]);
+        if constexpr (MT == 4) {
+          acc[1][j] = multiply<OP, 1>(av[u][1], bv[u][j], acc[1][j], as[u], bs[u][j]);
+          acc[2][j] = multiply<OP, 2>(av[u][2], bv[u][j], acc[2][j], as[u], bs[u][j]);
+          acc[3][j] = multiply<OP, 3>(av[u][3], bv[u][j], acc[3][j], as[u], bs[u][j]);
+        }
       }
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; i++)
+  for (int i = 0; i < MT; i++)
 #pragma unroll
-    for (int j = 0; j < NJ; j++) sums[wave][4 * j + i][lane] = acc[i][j];
+    for (int j = 0; j < NJ; j++) sums[wave][MT * j + i][lane] = acc[i][j];
   __syncthreads();
   if (wave >= NJ) return;
   // Wave j finishes the columns of tile j.
-  int const f0 = t.block * 64 + 16 * g;
+  int const f0 = block_here * 64 + 16 * g + 4 * tile0;
   f32x4 v[4];
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    v[i] = a.bias != nullptr ? *reinterpret_cast<f32x4 const*>(a.bias + block * 64 + 16 * g + 4 * i) : f32x4{0, 0, 0, 0};
+  for (int i = 0; i < MT; i++) {
+    v[i] = a.bias != nullptr ? *reinterpret_cast<f32x4 const*>(a.bias + block * 64 + 16 * g + 4 * (tile0 + i))
+                             : f32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int w = 0; w < W; w++) v[i] += sums[w][4 * wave + i][lane];
+    for (int w = 0; w < W; w++) v[i] += sums[w][MT * wave + i][lane];
   }
   activate<OP == OPERAND_F32>(a.act, a.act_a, [&](auto f) {
 #pragma unroll
-    for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f(v[e / 4][e % 4]);
+    for (int e = 0; e < 4 * MT; e++) v[e / 4][e % 4] = f(v[e / 4][e % 4]);
   });
-  clear_past(v, t.block * 64, f0, a.n_out);
   int64_t const col = int64_t(t.first) + 16 * wave + c;
-  if constexpr (KIND == OUT_MX4) store_mx4(a, col, col < t.last, f0, v);
-  else if (col < t.last) store_features<KIND, S>(a, col, f0, v, a.n_out);
-}
-
-// A whole chain on one tile of C columns: the columns' states stay in LDS, a row of
-// whole steps and 16 bytes of padding a column (16 columns' reads of one
-// fragment then fall into different banks), and a layer's outputs, complete in the
-// accumulators of the eight waves, take the place of its inputs between two
-// barriers.  Weights come from L2 straight into registers, `AHEAD` steps before
-// their MFMAs; each serves 16 NJ columns.  The waves are WM x WN, WM the layer's
-// blocks of 64 features, so that a narrow layer gives every wave fewer columns.
-// FEATURES: the input as the caller holds it.
-template <Operand OP, class S, OutputKind KIND, bool FEATURES, int C>
-__global__ __launch_bounds__(512, 2) void contract_chain(ChainArgs chain) {
-  constexpr bool MX = OP == OPERAND_MX4;
-  constexpr int N = OP == OPERAND_F32 ? 4 : MX ? 32 : 8;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  ContractArgs const& a = chain.io;
-  int const lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-  int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  Tile const t = find_tile<C>(a, 1);
-  if (t.none) return;
-  int const stride = chain.state_bytes + 16, scale_stride = chain.state_bytes / 16 + 4;
-  char* const states = lds;
-  unsigned char* const scales = reinterpret_cast<unsigned char*>(lds + C * stride);
-  {
-    // The input's pieces of 16 bytes, one lane per column and piece.
-    int const pieces = chain.layers[0].steps * 4;
-    for (int p = threadIdx.x; p < C * pieces; p += 512) {
-      int const local = p % C, piece = p / C;
-      int32_t const col = t.first + local < t.last ? t.first + local : t.last - 1;
-      int64_t row = a.source != nullptr ? a.source[col] : col;
-      row = row < 0 || row >= a.x_rows ? 0 : row;
-      i32x4 v;
-      int scale = 0;
-      if constexpr (FEATURES) {
-        read_features<OP, S>(a, row, piece, v, scale);
-      } else {
-        v = *reinterpret_cast<i32x4 const*>(a.x.data + row * a.x.stride + piece * 16);
-        if constexpr (MX) scale = a.x.scales[row * a.x.scale_stride + piece / 4 * a.x.scale_step + piece % 4];
-      }
-      *reinterpret_cast<i32x4*>(states + local * stride + piece * 16) = v;
-      if constexpr (MX) scales[local * scale_stride + piece] = static_cast<unsigned char>(scale);
+  if constexpr (MT == 4) {
+    clear_past(v, block_here * 64, f0, a.n_out);
+    if constexpr (KIND == OUT_MX4) store_mx4(a, col, col < t.last, f0, v);
+    else if (col < t.last) store_features<KIND, S>(a, col, f0, v, a.n_out);
+  } else if (col < t.last) {
+    using R = std::conditional_t<KIND == OUT_FLOATS, float, S>;
+    R* y = KIND == OUT_FEATURES ? static_cast<R*>(a.y) + int64_t(f0) * a.ldy + col
+                                : reinterpret_cast<R*>(a.y_rows.data + col * a.y_rows.stride) + f0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (KIND == OUT_FEATURES ? f0 + e < a.n_out : f0 + e < a.row_features)
+        y[KIND == OUT_FEATURES ? e * a.ldy : e] = R(f0 + e < a.n_out ? v[0][e] : 0.0f);
     }
-  }
-  __syncthreads();
-  for (int l = 0; l < chain.num_layers; l++) {
-    ChainLayer const& layer = chain.layers[l];
-    bool const last = l + 1 == chain.num_layers;
-    int const row_features = last ? 0 : chain.layers[l + 1].steps * 4 * N;
-    auto pass = [&]<int NJ>(std::integral_constant<int, NJ>, int wn_bits) {
-      constexpr int AHEAD = NJ >= 8 ? 1 : NJ == 4 ? 2 : 4;
-      int const wm = wave >> wn_bits, wn = wave & ((1 << wn_bits) - 1);
-      bool const busy = wm < layer.blocks && 16 * NJ * wn < C;
-      f32x4 acc[4][NJ];
-      int const steps = layer.steps;
-      if (busy) {
-        int64_t const block = int64_t(t.expert) * layer.blocks + wm;
-        char const* weights = layer.weights + block * steps * 4096 + 16 * lane;
-        int const* w_scales = MX ? reinterpret_cast<int const*>(layer.w_scales + block * steps * 256) + lane : nullptr;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          f32x4 seed = {0, 0, 0, 0};
-          if (layer.bias != nullptr) seed = *reinterpret_cast<f32x4 const*>(layer.bias + block * 64 + 16 * g + 4 * i);
-#pragma unroll
-          for (int j = 0; j < NJ; j++) acc[i][j] = seed;
-        }
-        char const* rows = states + (16 * NJ * wn + c) * stride + 16 * g;
-        unsigned char const* row_scales = scales + (16 * NJ * wn + c) * scale_stride + g;
-        i32x4 av[2][AHEAD][4];
-        int as[2][AHEAD] = {};
-        auto load = [&](int set, int s0) {
-#pragma unroll
-          for (int u = 0; u < AHEAD; u++) {
-            int const s = s0 + u < steps ? s0 + u : steps - 1;
-#pragma unroll
-            for (int i = 0; i < 4; i++) av[set][u][i] = *reinterpret_cast<i32x4 const*>(weights + s * 4096 + i * 1024);
-            if constexpr (MX) as[set][u] = w_scales[s * 64];
-          }
-        };
-        auto multiply_steps = [&](int set, int s0) {
-#pragma unroll
-          for (int u = 0; u < AHEAD; u++) {
-            if (s0 + u >= steps) break;
-            i32x4 bv[NJ];
-            int bs[NJ] = {};
-#pragma unroll
-            for (int j = 0; j < NJ; j++) {
-              bv[j] = *reinterpret_cast<i32x4 const*>(rows + 16 * j * stride + (s0 + u) * 64);
-              if constexpr (MX) bs[j] = row_scales[16 * j * scale_stride + (s0 + u) * 4];
-            }
-#pragma unroll
-            for (int j = 0; j < NJ; j++) {
-              acc[0][j] = multiply<OP, 0>(av[set][u][0], bv[j], acc[0][j], as[set][u], bs[j]);
-              acc[1][j] = multiply<OP, 1>(av[set][u][1], bv[j], acc[1][j], as[set][u], bs[j]);
-              acc[2][j] = multiply<OP, 2>(av[set][u][2], bv[j], acc[2][j], as[set][u], bs[j]);
-              acc[3][j] = multiply<OP, 3>(av[set][u][3], bv[j], acc[3][j], as[set][u], bs[j]);
-            }
-          }
-        };
-        load(0, 0);
-        for (int s = 0; s < steps; s += 2 * AHEAD) {
-          load(1, s + AHEAD);
-          multiply_steps(0, s);
-          load(0, s + 2 * AHEAD);
-          multiply_steps(1, s + AHEAD);
-        }
-      }
-      if (!last) __syncthreads();  // every wave has read the layer's inputs
-      if (busy) {
-        int const f0 = wm * 64 + 16 * g;
-#pragma unroll
-        for (int j = 0; j < NJ; j++) {
-          int const local = 16 * (NJ * wn + j) + c;
-          int64_t const col = int64_t(t.first) + local;
-          f32x4 v[4] = {acc[0][j], acc[1][j], acc[2][j], acc[3][j]};
-          activate<OP == OPERAND_F32>(layer.act, layer.act_a, [&](auto f) {
-#pragma unroll
-            for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f(v[e / 4][e % 4]);
-          });
-#pragma unroll
-          for (int e = 0; e < 16; e++) v[e / 4][e % 4] = f0 + e < layer.n_out ? v[e / 4][e % 4] : 0.0f;
-          if (last) {
-            if (col < t.last) store_features<KIND, S>(a, col, f0, v, layer.n_out);
-          } else if constexpr (MX) {
-            write_mx4(v, f0 < row_features, reinterpret_cast<i32x2*>(states + local * stride + f0 / 2),
-                      f0 % kMx4Block == 0, scales + local * scale_stride + f0 / kMx4Block);
-          } else {
-            write_pieces<S>(states + local * stride, f0, row_features, v);
-          }
-        }
-      }
-      if (!last) __syncthreads();
-    };
-    // blocks of 64 features -> waves along the columns
-    int const blocks = layer.blocks;
-    if (blocks > 4) pass(std::integral_constant<int, C / 16>{}, 0);
-    else if (blocks > 2) pass(std::integral_constant<int, C / 32>{}, 1);
-    else if (blocks > 1) pass(std::integral_constant<int, C / 64>{}, 2);
-    else pass(std::integral_constant<int, C / 128 < 1 ? 1 : C / 128>{}, 3);
   }
 }
 
@@ -449,11 +325,18 @@ inline int thin_columns(int64_t columns, int32_t experts, int32_t blocks) {
 template <Operand OP, class S, OutputKind KIND, bool FEATURES, int NJ>
 hipError_t launch_thin(ContractArgs const& a, hipStream_t stream) {
   constexpr int W = 8;
-  int64_t const tiles = grid_of(a, 16 * NJ, a.blocks);
-  if (tiles > INT32_MAX) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((contract_thin<OP, S, KIND, FEATURES, NJ, W>), dim3(static_cast<unsigned>(tiles)), dim3(64 * W), 0,
-                     stream, a);
-  return hipGetLastError();
+  auto launch = [&]<int MT>(std::integral_constant<int, MT>) {
+    int64_t const tiles = grid_of(a, 16 * NJ, int64_t(a.blocks) * (4 / MT));
+    if (tiles > INT32_MAX) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((contract_thin<OP, S, KIND, FEATURES, MT, NJ, W>), dim3(static_cast<unsigned>(tiles)),
+                       dim3(64 * W), 0, stream, a);
+    return hipGetLastError();
+  };
+  // Tiles of 16 features where those of 64 leave CUs without one (a 4-bit output's blocks need 64).
+  if constexpr (KIND != OUT_MX4) {
+    if (grid_of(a, 16 * NJ, a.blocks) <= 256) return launch(std::integral_constant<int, 1>{});
+  }
+  return launch(std::integral_constant<int, 4>{});
 }
 
 template <Operand OP, class S, OutputKind KIND>
@@ -478,6 +361,9 @@ hipError_t launch_kind(OutputKind kind, ContractArgs const& a, hipStream_t strea
   switch (kind) {
     case OUT_FEATURES: return launch_sized<OP, S, OUT_FEATURES>(a, stream);
     case OUT_ROWS: return launch_sized<OP, S, OUT_ROWS>(a, stream);
+    case OUT_FLOATS:
+      if constexpr (OP == OPERAND_F32) return launch_sized<OP, S, OUT_ROWS>(a, stream);
+      else return launch_sized<OP, S, OUT_FLOATS>(a, stream);
     default:
       if constexpr (OP == OPERAND_MX4) return launch_sized<OP, S, OUT_MX4>(a, stream);
       return hipErrorInvalidValue;
@@ -486,7 +372,7 @@ hipError_t launch_kind(OutputKind kind, ContractArgs const& a, hipStream_t strea
 
 // 64 samples x 64 features: a lane sums 8 features of one sample's rows, the
 // tile turns in LDS.
-template <class S>
+template <class R, class S>
 __global__ __launch_bounds__(256) void combine(Rows rows, int64_t num_rows, ponni_routing r, int64_t features,
                                                S* __restrict__ y, int64_t ld) {
   __shared__ float tile[64][65];  // [feature][sample]
@@ -500,7 +386,7 @@ __global__ __launch_bounds__(256) void combine(Rows rows, int64_t num_rows, ponn
         int64_t const slot = r.slots[j * r.batch + b];
         if (slot < 0 || slot >= num_rows) continue;
         float const w = r.weights[j * r.batch + b];
-        S const* row = reinterpret_cast<S const*>(rows.data + slot * rows.stride) + f0 + q;
+        R const* row = reinterpret_cast<R const*>(rows.data + slot * rows.stride) + f0 + q;
 #pragma unroll
         for (int i = 0; i < 8; i++) sum[i] = fmaf(w, float(row[i]), sum[i]);  // (rows are whole 64-byte pieces)
       }
@@ -619,12 +505,16 @@ hipError_t launch_contraction(Operand op, int out_type, OutputKind kind, Contrac
   }
 }
 
-hipError_t launch_combine(int dtype, Rows const& rows, int64_t num_rows, const ponni_routing& r, int64_t features,
+hipError_t launch_combine(int dtype, bool floats, Rows const& rows, int64_t num_rows, const ponni_routing& r, int64_t features,
                           void* y, int64_t ld, hipStream_t stream) {
   dim3 const grid(unsigned((r.batch + 63) / 64), unsigned((features + 63) / 64));
   with_dtype(dtype, [&](auto s) {
     using S = decltype(s);
-    hipLaunchKernelGGL(combine<S>, grid, dim3(256), 0, stream, rows, num_rows, r, features, static_cast<S*>(y), ld);
+    auto launch = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, rows, num_rows, r, features, static_cast<S*>(y), ld);
+    };
+    if (floats) launch(combine<float, S>);
+    else launch(combine<S, S>);
   });
   return hipGetLastError();
 }
