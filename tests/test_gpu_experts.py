@@ -233,3 +233,325 @@ def test_mixture(cuda, E, k, widths, acts, B, dtype, weights):
     close(host(y), want, err, dtype)
     if B > 2:
         assert np.all(host(y)[:, 1] == 0.0)
+
+
+# The kernels that SHAPES leaves out: 256 x 256 tiles, 4-bit states between layers of
+# more features than a chain's kernel takes, its tiles of 128 columns.  A few hundred columns are checked.
+LARGE = [
+    # experts, widths, activations, columns, (dtype, weights)
+    (3, (330, 1100), ("none",), 70_001, ("bf16", "same")),
+    (3, (130, 1100), ("silu",), 70_001, ("f32", "same")),
+    (3, (700, 1030), ("none",), 70_001, ("f16", "mx4")),
+    (4, (129, 700, 600), ("tanh", "none"), 3001, ("bf16", "mx4")),
+    (4, (129, 700, 600), ("gelu_erf", "none"), 3001, ("f16", "same")),
+    (2, (100, 400, 500), ("sigmoid", "none"), 70_003, ("bf16", "same")),
+    (2, (100, 400, 500), ("sigmoid", "none"), 70_003, ("f16", "mx4")),
+    (2, (200, 256, 255), ("tanh", "none"), 40_003, ("f32", "same")),
+    (9, (1000, 200), ("none",), 120, ("f16", "same")),
+    (3, (1000, 200), ("none",), 90, ("bf16", "mx4")),
+]
+
+
+@pytest.mark.parametrize("E,widths,acts,C,types", LARGE)
+def test_grouped_columns_large(cuda, E, widths, acts, C, types):
+    import torch
+
+    dtype, weights = types
+    print(f"experts: E={E} {widths} {acts} C={C} {dtype} {weights}", flush=True)
+    r = np.random.default_rng(C)
+    model, params = networks(r, E, widths, acts, dtype, weights)
+    offsets = group_sizes(r, E, C)
+    x = torch.randn((widths[0], C), device=cuda, generator=torch.Generator(cuda).manual_seed(C)).to(torch_dtype(dtype))
+    y = torch.full((widths[-1], C), 7.0, dtype=x.dtype, device=cuda)
+    model.forward_batch_parallel(x, torch.from_numpy(offsets).to(cuda), y)
+    for e in range(E):
+        a, b = offsets[e], offsets[e + 1]
+        if a < b:
+            # the group's ends and some columns between
+            cols = np.unique(np.concatenate([[a, b - 1], r.integers(a, b, 60)]))
+            at = torch.from_numpy(cols).to(cuda)
+            want, err = N.chain(params[e], host(x[:, at]), dtype, weights)
+            close(host(y[:, at]), want, err, dtype)
+    assert bool((y[:, offsets[-1]:] == 7.0).all())
+
+
+def test_rows_beyond_four_gigabytes(cuda):
+    """Byte offsets past 2^32 in the input, its rows and the output."""
+    import torch
+
+    r = np.random.default_rng(5)
+    C, K, n = 2_200_000, 1024, 1040
+    model, params = networks(r, 2, (K, n), ("none",), "bf16")
+    x = torch.zeros((K, C), dtype=torch.bfloat16, device=cuda)
+    cols = [0, 1, 1_099_999, 1_100_000, 2_097_152, C - 1]
+    for c in cols:
+        x[:, c] = torch.from_numpy(r.standard_normal(K)).to(cuda).to(x.dtype)
+    offsets = torch.tensor([0, 1_100_000, C], dtype=torch.int32, device=cuda)
+    y = model.forward_batch_parallel(x, offsets)
+    for c in cols:
+        want, err = N.chain(params[int(c >= 1_100_000)], host(x[:, c:c + 1]), "bf16")
+        close(host(y[:, c:c + 1]), want, err, "bf16")
+    # a column of zeros gives its expert's biases
+    want, err = N.chain(params[1], np.zeros((K, 1)), "bf16")
+    close(host(y[:, 2_000_000:2_000_001]), want, err, "bf16")
+
+
+@pytest.mark.parametrize("dtype,weights", [("f32", "same"), ("bf16", "same"), ("f16", "mx4")])
+@pytest.mark.parametrize("widths,C", [((37, 50), 20), ((37, 50, 41), 300), ((600, 700), 300)])
+def test_non_finite_columns(cuda, dtype, weights, widths, C):
+    """NaN and infinities stay in their columns, and meet no padding (37 features end inside a step)."""
+    import torch
+
+    r = np.random.default_rng(C)
+    # (Relu, x > 0 ? x : 0, ends a NaN)
+    model, params = networks(r, 2, widths, ("leaky_relu", "none")[-len(widths) + 1:], dtype, weights)
+    x = r.standard_normal((widths[0], C))
+    x[3, 1], x[widths[0] - 1, 2], x[0, C - 1] = np.nan, np.inf, -np.inf
+    offsets = torch.tensor([0, C // 2, C], dtype=torch.int32, device=cuda)
+    xt = tensor(x, dtype, cuda)
+    got = host(model.forward_batch_parallel(xt, offsets))
+    bad = [1, 2, C - 1]
+    assert not np.isfinite(got[:, bad]).all(0).any()
+    if weights == "same" and len(widths) == 2:
+        w = params[0][0][0]
+        assert np.array_equal(got[:, 2], np.where(w[-1] > 0, np.inf, -np.inf))  # inf * w and finite terms
+    good = [c for c in range(C) if c not in bad]
+    for e in range(2):
+        cols = [c for c in good if (c >= C // 2) == bool(e)]
+        want, err = N.chain(params[e], host(xt)[:, cols], dtype, weights)
+        close(got[:, cols], want, err, dtype)
+
+
+def test_empty_groups(cuda):
+    import torch
+
+    r = np.random.default_rng(1)
+    for widths in ((20, 30), (20, 30, 10), (600, 700)):
+        model, params = networks(r, 4, widths, ("none", "none")[-len(widths) + 1:], "f16")
+        for C in (5, 400):
+            x = tensor(r.standard_normal((widths[0], C)), "f16", cuda)
+            y = torch.full((widths[-1], C), 7.0, dtype=torch.float16, device=cuda)
+            model.forward_batch_parallel(x, torch.zeros(5, dtype=torch.int32, device=cuda), y)
+            assert bool((y == 7.0).all())
+            model.forward_batch_parallel(x, torch.tensor([0, 0, 0, C, C], dtype=torch.int32, device=cuda), y)
+            want, err = N.chain(params[2], host(x), "f16")
+            close(host(y), want, err, "f16")
+
+
+def test_parameters_from_host_and_device(cuda):
+    """The same model from numpy and torch arrays of any type, and new parameters after the first."""
+    import torch
+
+    r = np.random.default_rng(3)
+    w, b = r.uniform(-1, 1, (3, 40, 50)).astype(np.float16), r.uniform(-1, 1, (3, 50)).astype(np.float16)
+    x = tensor(r.standard_normal((40, 77)), "f16", cuda)
+    offsets = torch.tensor([0, 30, 30, 77], dtype=torch.int32, device=cuda)
+    want = None
+    for make in (lambda a: a, lambda a: a.astype(np.float32), lambda a: a.astype(np.float64), torch.from_numpy,
+                 lambda a: torch.from_numpy(a).to(cuda), lambda a: torch.from_numpy(a).double().to(cuda)):
+        model = P.create_expert_model(P.ExpertMatvec(make(w)), P.ExpertBias(make(b)), dtype="f16")
+        y = model.forward_batch_parallel(x, offsets)
+        want = y if want is None else want
+        assert torch.equal(y, want)
+    model.set_layer_params(0, -w)
+    model.set_layer_params(1, torch.from_numpy(-b).to(cuda))
+    assert torch.equal(model.forward_batch_parallel(x, offsets), -want)
+
+
+def test_4_bit_rows_as_input(cuda):
+    """4-bit rows made beforehand give what the model makes of x itself."""
+    import torch
+
+    r = np.random.default_rng(8)
+    for widths, C in (((100, 80), 12), ((100, 80, 30), 500), ((900, 700), 700), ((1100, 1100), 40_000)):
+        model, _ = networks(r, 2, widths, ("relu", "none")[-len(widths) + 1:], "bf16", "mx4")
+        x = torch.randn((widths[0], C), device=cuda).bfloat16()
+        offsets = torch.tensor([0, C // 3, C], dtype=torch.int32, device=cuda)
+        assert torch.equal(model.forward_batch_parallel(P.quantize_mx4(x), offsets),
+                           model.forward_batch_parallel(x, offsets))
+
+
+def test_dense_4_bit_layer(cuda):
+    """One expert, no offsets: a plain dense product."""
+    r = np.random.default_rng(9)
+    for C in (1, 33, 200):
+        model, params = networks(r, 1, (150, 90), ("none",), "f16", "mx4")
+        x = tensor(r.standard_normal((150, C)), "f16", cuda)
+        want, err = N.chain(params[0], host(x), "f16", "mx4")
+        close(host(model.forward_batch_parallel(x)), want, err, "f16")
+
+
+def test_own_routing(cuda):
+    """A routing that a program made itself: an expert chosen twice by one sample, unsorted samples, unequal weights."""
+    import torch
+
+    r = np.random.default_rng(11)
+    model, params = networks(r, 3, (30, 20), ("none",), "f32")
+    x = tensor(r.standard_normal((30, 4)), "f32", cuda)
+    i32 = dict(dtype=torch.int32, device=cuda)
+    # expert 0: samples 3, 1, 1; expert 2: samples 0, 3; sample 2 has none
+    routing = P.Routing(torch.tensor([[2, 0, -1, 0], [-1, 0, -1, 2]], **i32),
+                        torch.tensor([[0.5, 2.0, 9.0, -1.0], [9.0, 0.25, 9.0, 3.0]], device=cuda),
+                        torch.tensor([[3, 1, -1, 0], [-1, 2, -1, 4]], **i32),
+                        torch.tensor([3, 1, 1, 0, 3, -1, -1, -1], **i32), torch.tensor([0, 3, 3, 5], **i32))
+    got, xs = host(model.forward_mixture(x, routing)), host(x)
+    f = [lambda c, e=e: N.chain(params[e], xs[:, c:c + 1], "f32")[0][:, 0] for e in range(3)]
+    want = np.stack([0.5 * f[2](0), 2.25 * f[0](1), 0 * f[0](2), -f[0](3) + 3 * f[2](3)], 1)
+    assert np.abs(got - want).max() <= 40 * 2.0 ** -24 * 4 * np.abs(xs).sum(0).max()
+    with pytest.raises(ValueError):
+        model.forward_mixture(x, P.Routing(routing.experts, routing.weights.double(), routing.slots, routing.source,
+                                           routing.offsets))
+    with pytest.raises(ValueError):
+        model.forward_mixture(x, P.Routing(routing.experts, routing.weights, routing.slots, routing.source[:5],
+                                           routing.offsets))
+
+
+def mixture_model(r, dtype="bf16", weights="same"):
+    experts, params = networks(r, 8, (64, 130, 48), ("silu", "none"), dtype, weights)
+    w = r.uniform(-0.5, 0.5, (64, 8))
+    return P.MixtureOfExperts(P.create_inference_model(P.Matvec(w), dtype=dtype), experts, top_k=2), params
+
+
+@pytest.mark.parametrize("B", [1, 50, 3000])
+def test_mixture_of_experts_model(cuda, B):
+    """Router, routing, expert networks and the weighted sum together."""
+    r = np.random.default_rng(B)
+    model, params = mixture_model(r)
+    x = tensor(r.standard_normal((64, B)), "bf16", cuda)
+    y = model.forward_batch_parallel(x)
+    scores = host(model.router.forward_batch_parallel(x))
+    experts, w, *_ = N.route(scores, 2, "chosen")
+    want, err = np.zeros(y.shape), np.zeros(y.shape)
+    for e in range(8):
+        j, b = np.nonzero(experts == e)
+        if len(b):
+            v, d = N.chain(params[e], host(x)[:, b], "bf16")
+            want[:, b] += w[j, b] * v
+            err[:, b] += w[j, b] * (d + 2.0 ** -8 * np.abs(v)) + 2.0 ** -20 * np.abs(v)
+    close(host(y), want, err, "bf16")
+
+
+@pytest.mark.parametrize("weights", ["same", "mx4"])
+@pytest.mark.parametrize("B", [3, 700])
+def test_graph_replays(cuda, B, weights):
+    """Routing and a mixture captured in one graph, replayed with new inputs between
+    the program's own work; two graphs of one model; the eager result each time."""
+    import torch
+
+    r = np.random.default_rng(B)
+    experts, _ = networks(r, 8, (64, 600 if B > 3 else 130, 48), ("silu", "none"), "bf16", weights)
+    x = torch.empty((64, B), dtype=torch.bfloat16, device=cuda)
+    s = torch.empty((8, B), device=cuda)
+
+    def step():
+        return experts.forward_mixture(x, P.route_experts(s, 2, "all"))
+
+    def fill(seed):
+        g = torch.Generator(cuda).manual_seed(seed)
+        x.copy_(torch.randn(x.shape, device=cuda, generator=g))
+        s.copy_(torch.randn(s.shape, device=cuda, generator=g))
+
+    fill(0)
+    step()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step())
+        graphs.append(g)
+    for seed in range(1, 5):
+        fill(seed)
+        for g in graphs:
+            g.replay()
+        want = step()
+        torch.cuda.synchronize()
+        for out in outs:
+            assert torch.equal(out, want)
+
+
+def test_streams_and_dirty_workspaces(cuda):
+    """Calls of one model on two streams at once, and work buffers full of NaN: the same results."""
+    import ctypes
+    import torch
+
+    r = np.random.default_rng(4)
+    for widths, dtype, weights in (((600, 700, 40), "bf16", "same"), ((64, 100, 40), "f16", "mx4"),
+                                   ((700, 600, 64), "f16", "mx4")):
+        model, _ = networks(r, 4, widths, ("tanh", "none"), dtype, weights)
+        L, C = A.lib(), 2000
+        offsets = torch.tensor([0, 300, 301, 1500, C], dtype=torch.int32, device=cuda)
+        xs = [torch.randn((widths[0], C), device=cuda).to(torch_dtype(dtype)) for _ in range(2)]
+        want = [model.forward_batch_parallel(x, offsets) for x in xs]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in xs]
+        for _ in range(5):
+            got = []
+            for x, stream in zip(xs, streams):
+                with torch.cuda.stream(stream):
+                    got.append(model.forward_batch_parallel(x, offsets))
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        need = L.ponni_experts_workspace_bytes(model._experts, C)
+        work = torch.full((need + 64,), 255, dtype=torch.uint8, device=cuda)
+        y = torch.empty_like(want[0])
+        A.check(L.ponni_experts_forward(model._experts, xs[0].data_ptr(), C, offsets.data_ptr(), y.data_ptr(), C, C,
+                                        work.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[0]) and bool((work[need:] == 255).all())
+        routing = P.route_experts(torch.randn((4, C), device=cuda), 2)
+        want = model.forward_mixture(xs[0], routing)
+        need = L.ponni_experts_mixture_workspace_bytes(model._experts, 2, C)
+        work = torch.full((need + 64,), 255, dtype=torch.uint8, device=cuda)
+        arrays = routing.arrays()
+        A.check(L.ponni_experts_forward_mixture(model._experts, xs[0].data_ptr(), C, ctypes.byref(arrays), y.data_ptr(),
+                                                C, work.data_ptr(), need, torch.cuda.current_stream().cuda_stream))
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and bool((work[need:] == 255).all())
+
+
+def test_refusals_of_tensors(cuda):
+    """What the Python calls refuse before anything is launched."""
+    import torch
+
+    r = np.random.default_rng(2)
+    model, _ = networks(r, 3, (20, 30), ("none",), "f16")
+    x = torch.zeros((20, 8), dtype=torch.float16, device=cuda)
+    offsets = torch.tensor([0, 2, 4, 8], dtype=torch.int32, device=cuda)
+    bad = [
+        lambda: model.forward_batch_parallel(x.float(), offsets),
+        lambda: model.forward_batch_parallel(x[:19], offsets),
+        lambda: model.forward_batch_parallel(x.cpu(), offsets),
+        lambda: model.forward_batch_parallel(x.t().contiguous().t(), offsets),
+        lambda: model.forward_batch_parallel(x, offsets.long()),
+        lambda: model.forward_batch_parallel(x, offsets[:3]),
+        lambda: model.forward_batch_parallel(x, offsets.cpu()),
+        lambda: model.forward_batch_parallel(x, offsets, torch.empty((30, 7), dtype=x.dtype, device=cuda)),
+        lambda: model.forward_batch_parallel(x, offsets, torch.empty((30, 8), device=cuda)),
+        lambda: P.route_experts(torch.zeros((4, 4), device=cuda), 1, "some"),
+        lambda: P.quantize_mx4(torch.zeros((4, 4), device=cuda, dtype=torch.int32)),
+        lambda: P.Mx4(torch.zeros((2, 64), dtype=torch.uint8, device=cuda), torch.zeros((2, 3), dtype=torch.uint8,
+                                                                                       device=cuda), 20).dequantize(),
+    ]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    refused = [
+        (A.PONNI_ERR_INVALID_ARGUMENT, lambda: model.forward_batch_parallel(x)),  # three experts, no offsets
+        (A.PONNI_ERR_SHAPE, lambda: model.forward_batch_parallel(x[:, :0], offsets)),
+        (A.PONNI_ERR_UNSUPPORTED, lambda: model.forward_batch_parallel(P.quantize_mx4(x), offsets)),
+        (A.PONNI_ERR_SHAPE, lambda: model.forward_batch_parallel(x[:1, :1].expand(20, 1), offsets)),  # stride 0
+        (A.PONNI_ERR_UNSUPPORTED, lambda: P.route_experts(torch.zeros((4, 4), device=cuda, dtype=torch.float64), 1)),
+        (A.PONNI_ERR_UNSUPPORTED, lambda: P.quantize_mx4(x).dequantize(torch.float64)),
+        (A.PONNI_ERR_INVALID_ARGUMENT, lambda: P.route_experts(torch.zeros((4, 4), device=cuda), 5)),
+        (A.PONNI_ERR_INVALID_ARGUMENT, lambda: P.route_experts(torch.zeros((4, 4), device=cuda), 0)),
+        (A.PONNI_ERR_SHAPE, lambda: model.forward_mixture(x, P.route_experts(torch.zeros((4, 8), device=cuda), 1))),
+    ]
+    for status, call in refused:
+        with pytest.raises(P.PonniError) as e:
+            call()
+        assert e.value.status == status
+    wide = torch.zeros((50, 8), dtype=torch.float16, device=cuda)
+    with pytest.raises(P.PonniError) as e:  # x and y share memory
+        model.forward_batch_parallel(wide[:20], offsets, wide[19:49])
+    assert e.value.status == A.PONNI_ERR_INVALID_ARGUMENT
