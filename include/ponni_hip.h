@@ -532,7 +532,7 @@ int ponni_forward_host(ponni_plan plan, const void* x, int64_t ld_in, void* y, i
 typedef struct ponni_routing {
   int32_t num_experts; /* 1 .. PONNI_MAX_EXPERTS                                       */
   int32_t top_k;       /* 1 .. min(PONNI_MAX_TOP_K, num_experts)                        */
-  int64_t batch;       /* top_k * batch <= INT32_MAX                                    */
+  int64_t batch;       /* top_k * batch <= PONNI_MAX_COLUMNS                            */
   int32_t* experts;    /* [top_k, batch]: the sample's j-th expert, -1 for none         */
   float* weights;      /* [top_k, batch]: its weight, 0 for none                        */
   int32_t* slots;      /* [top_k, batch]: its sorted column, -1 for none                */
@@ -541,6 +541,7 @@ typedef struct ponni_routing {
 } ponni_routing;
 #define PONNI_MAX_EXPERTS 1024
 #define PONNI_MAX_TOP_K 16
+#define PONNI_MAX_COLUMNS 1000000000 /* of one call of these operators */
 
 /* The top_k experts of each sample from scores [num_experts, batch] of `dtype`
  * (F32, F16, BF16) with row stride ld: the largest scores, in descending

@@ -13,6 +13,7 @@ namespace ponni_hip {
 namespace {
 
 constexpr int32_t kMaxWidth = 65536;
+// (PONNI_MAX_COLUMNS: a launch has at most 2^32 threads, and the smallest tiles are 64 columns of 256)
 
 int fail(int status, std::string const& message) { return set_error(status, message); }
 
@@ -138,7 +139,8 @@ int check_routing_sizes(int32_t experts, int32_t top_k, int64_t batch) {
     return fail(PONNI_ERR_INVALID_ARGUMENT,
                 "top_k must be 1 to " + std::to_string(std::min(PONNI_MAX_TOP_K, experts)));
   if (batch <= 0) return fail(PONNI_ERR_SHAPE, "routing requires a nonzero batch size");
-  if (batch > INT32_MAX / top_k) return fail(PONNI_ERR_SHAPE, "top_k * batch exceeds INT_MAX");
+  if (batch > PONNI_MAX_COLUMNS / top_k)
+    return fail(PONNI_ERR_SHAPE, "top_k * batch exceeds " + std::to_string(PONNI_MAX_COLUMNS));
   return PONNI_OK;
 }
 
@@ -221,7 +223,8 @@ int forward_impl(ponni_experts e, const void* x, int64_t ld_in, const void* code
                  int64_t workspace_bytes, hipStream_t stream) {
   if (e == nullptr) return fail(PONNI_ERR_INVALID_ARGUMENT, "experts is null");
   if (columns <= 0) return fail(PONNI_ERR_SHAPE, "expert networks require a nonzero number of columns");
-  if (columns > INT32_MAX) return fail(PONNI_ERR_SHAPE, "columns exceed INT_MAX");
+  if (columns > PONNI_MAX_COLUMNS)
+    return fail(PONNI_ERR_SHAPE, "columns exceed " + std::to_string(PONNI_MAX_COLUMNS));
   if (mx4_rows && e->operand != OPERAND_MX4)
     return fail(PONNI_ERR_UNSUPPORTED, "4-bit rows are the input of networks with 4-bit weights");
   if (y == nullptr || (mx4_rows ? codes == nullptr || scales == nullptr : x == nullptr))
@@ -430,7 +433,8 @@ int check_mx4(const void* codes, const void* scales, const void* values, int64_t
               int64_t columns) {
   if (features < 1 || features > kMaxWidth)
     return fail(PONNI_ERR_SHAPE, "features must be 1 to " + std::to_string(kMaxWidth));
-  if (columns < 1 || columns > INT32_MAX) return fail(PONNI_ERR_SHAPE, "columns must be 1 to INT_MAX");
+  if (columns < 1 || columns > PONNI_MAX_COLUMNS)
+    return fail(PONNI_ERR_SHAPE, "columns must be 1 to " + std::to_string(PONNI_MAX_COLUMNS));
   if (codes == nullptr || scales == nullptr || values == nullptr) return fail(PONNI_ERR_INVALID_ARGUMENT, "null array");
   if (!aligned(codes, 16) || !aligned(scales, 16))
     return fail(PONNI_ERR_INVALID_ARGUMENT, "codes and scales must be at multiples of 16 bytes");
@@ -564,7 +568,8 @@ int64_t ponni_experts_workspace_bytes(ponni_experts e, int64_t columns) {
   int64_t n = -1;
   (void)guarded([&] {
     if (e == nullptr) return fail(PONNI_ERR_INVALID_ARGUMENT, "experts is null");
-    if (columns <= 0 || columns > INT32_MAX) return fail(PONNI_ERR_SHAPE, "columns must be 1 to INT_MAX");
+    if (columns <= 0 || columns > PONNI_MAX_COLUMNS)
+      return fail(PONNI_ERR_SHAPE, "columns must be 1 to " + std::to_string(PONNI_MAX_COLUMNS));
     n = workspace_of(*e, columns, columns, false).total;
     return int(PONNI_OK);
   });

@@ -13,7 +13,7 @@ each call, on the current stream.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 from typing import Sequence
 
 import numpy as np
@@ -88,56 +88,70 @@ def _int_array(t, shape, other, what: str):
 # -- routing ---------------------------------------------------------------------------
 
 
-@dataclass(frozen=True)
 class Routing:
     """Where the samples of a batch go (ponni_routing): experts (int32), weights
     (float32) and slots (int32) [top_k, batch], source [top_k * batch] and offsets
     [num_experts + 1] (int32), on the GPU.  From route_experts, or a program's own."""
 
-    experts: "object"
-    weights: "object"
-    slots: "object"
-    source: "object"
-    offsets: "object"
-    checked: bool = field(default=False, repr=False)
+    __slots__ = ("num_experts", "top_k", "batch", "device", "_arrays", "_tensors", "_buffer")
 
-    @property
-    def num_experts(self) -> int:
-        return self.offsets.shape[0] - 1
+    def __init__(self, experts, weights, slots, source, offsets):
+        import torch
 
-    @property
-    def top_k(self) -> int:
-        return self.slots.shape[0]
+        if slots.dim() != 2 or offsets.dim() != 1 or not slots.is_cuda:
+            raise ValueError("slots must be a GPU tensor [top_k, batch], offsets [num_experts + 1]")
+        self.top_k, self.batch = slots.shape
+        self.num_experts, self.device = offsets.shape[0] - 1, slots.get_device()
+        _int_array(slots, slots.shape, slots, "slots")
+        _int_array(experts, slots.shape, slots, "experts")
+        _int_array(source, (self.top_k * self.batch,), slots, "source")
+        _int_array(offsets, offsets.shape, slots, "offsets")
+        if weights.dtype != torch.float32 or weights.shape != slots.shape or not weights.is_contiguous():
+            raise ValueError(f"weights must be a contiguous float32 tensor of shape {tuple(slots.shape)}")
+        _same_device(weights, slots, "weights")
+        self._tensors = (experts, weights, slots, source, offsets)
+        self._arrays = A.RoutingArrays(self.num_experts, self.top_k, self.batch, *[t.data_ptr() for t in self._tensors])
 
-    @property
-    def batch(self) -> int:
-        return self.slots.shape[1]
+    @classmethod
+    def _made(cls, like, num_experts: int, top_k: int, batch: int, work_bytes: int):
+        """Arrays to be filled, in one allocation with a work buffer behind them; its address."""
+        import torch
 
-    def arrays(self) -> A.RoutingArrays:
-        if not self.checked:
+        r = cls.__new__(cls)
+        r.num_experts, r.top_k, r.batch, r.device, r._tensors = num_experts, top_k, batch, like.get_device(), None
+        n = top_k * batch
+        work = (4 * n + num_experts + 4) // 4 * 4  # (16-byte aligned)
+        r._buffer = torch.empty(work + work_bytes // 4, dtype=torch.int32, device=like.device)
+        at = r._buffer.data_ptr()
+        r._arrays = A.RoutingArrays(num_experts, top_k, batch, at, at + 4 * n, at + 8 * n, at + 12 * n, at + 16 * n)
+        return r, at + 4 * work
+
+    def _tensor(self, i: int):
+        if self._tensors is None:
             import torch
 
-            if self.slots.dim() != 2 or self.offsets.dim() != 1 or not self.slots.is_cuda:
-                raise ValueError("slots must be a GPU tensor [top_k, batch], offsets [num_experts + 1]")
-            _int_array(self.slots, self.slots.shape, self.slots, "slots")
-            _int_array(self.experts, self.slots.shape, self.slots, "experts")
-            _int_array(self.source, (self.top_k * self.batch,), self.slots, "source")
-            _int_array(self.offsets, self.offsets.shape, self.slots, "offsets")
-            if (self.weights.dtype != torch.float32 or self.weights.shape != self.slots.shape
-                    or not self.weights.is_contiguous()):
-                raise ValueError(f"weights must be a contiguous float32 tensor of shape {tuple(self.slots.shape)}")
-            _same_device(self.weights, self.slots, "weights")
-        return A.RoutingArrays(self.num_experts, self.top_k, self.batch, self.experts.data_ptr(),
-                               self.weights.data_ptr(), self.slots.data_ptr(), self.source.data_ptr(),
-                               self.offsets.data_ptr())
+            n = self.top_k * self.batch
+            experts, weights, slots, source, rest = self._buffer.split_with_sizes(
+                (n, n, n, n, self._buffer.shape[0] - 4 * n))
+            shape = (self.top_k, self.batch)
+            self._tensors = (experts.view(shape), weights.view(torch.float32).view(shape), slots.view(shape), source,
+                             rest[:self.num_experts + 1])
+        return self._tensors[i]
+
+    experts = property(lambda self: self._tensor(0))
+    weights = property(lambda self: self._tensor(1))
+    slots = property(lambda self: self._tensor(2))
+    source = property(lambda self: self._tensor(3))
+    offsets = property(lambda self: self._tensor(4))
+
+    def arrays(self) -> A.RoutingArrays:
+        return self._arrays
 
 
 def route_experts(scores, top_k: int, normalize: str = "chosen") -> Routing:
     """The top_k experts of each sample from scores [num_experts, batch] (f32, f16
     or bf16), and the samples sorted by expert (ponni_route).  normalize: the
     weights are softmax values over the sample's "chosen" experts or over "all"."""
-    import torch
-
     codes = _types()[1]
     ld = _rows(scores, "scores")
     if scores.dtype not in codes:
@@ -149,50 +163,44 @@ def route_experts(scores, top_k: int, normalize: str = "chosen") -> Routing:
     need = L.ponni_route_workspace_bytes(e, top_k, b)
     if need < 0:
         raise A.PonniError(A.PONNI_ERR_INVALID_ARGUMENT, L.ponni_last_error().decode())
-    # Two allocations: the [top_k, batch] arrays and the source; offsets, then the work buffer (16-byte aligned).
-    made = torch.empty((4, top_k, b), dtype=torch.int32, device=scores.device)
-    at = (e + 4) // 4 * 4
-    more = torch.empty(at + need // 4, dtype=torch.int32, device=scores.device)
-    experts, weights, slots, source = made.unbind()
-    r = Routing(experts, weights.view(torch.float32), slots, source.view(-1), more[:e + 1], checked=True)
-    arrays, base = r.arrays(), more.data_ptr()
+    r, work = Routing._made(scores, e, top_k, b, need)
     _call(scores, L.ponni_route, scores.data_ptr(), ld, codes[scores.dtype], A.ROUTE_ALL if normalize == "all" else
-          A.ROUTE_CHOSEN, ctypes.byref(arrays), base + 4 * at, need)
+          A.ROUTE_CHOSEN, ctypes.byref(r._arrays), work, need)
     return r
 
 
 # -- 4-bit rows ------------------------------------------------------------------------
 
 
-@dataclass(frozen=True)
+def _mx4_bytes(features: int):
+    """Bytes of a row's codes and of its scales (ponni_mx4_code_bytes, ponni_mx4_scale_bytes)."""
+    steps = -(-features // 128)
+    return 64 * steps, 4 * steps
+
+
 class Mx4:
     """Samples as microscaled 4-bit rows (ponni_mx4_quantize): codes [columns,
     code bytes] and scales [columns, scale bytes], uint8."""
 
-    codes: "object"
-    scales: "object"
-    features: int
-    checked: bool = field(default=False, repr=False)
+    __slots__ = ("codes", "scales", "features", "columns")
 
-    @property
-    def columns(self) -> int:
-        return self.codes.shape[0]
+    def __init__(self, codes, scales, features: int):
+        import torch
 
-    def check(self) -> None:
-        if not self.checked:
-            import torch
+        for t, n, what in zip((codes, scales), _mx4_bytes(features), ("codes", "scales")):
+            if t.dtype != torch.uint8 or tuple(t.shape) != (codes.shape[0], n) or not t.is_contiguous() or not t.is_cuda:
+                raise ValueError(f"{what} must be a contiguous uint8 GPU tensor of shape ({codes.shape[0]}, {n})")
+        _same_device(scales, codes, "scales")
+        self._set(codes, scales, features)
 
-            for t, n, what in ((self.codes, A.lib().ponni_mx4_code_bytes(self.features), "codes"),
-                               (self.scales, A.lib().ponni_mx4_scale_bytes(self.features), "scales")):
-                if t.dtype != torch.uint8 or tuple(t.shape) != (self.columns, n) or not t.is_contiguous() or not t.is_cuda:
-                    raise ValueError(f"{what} must be a contiguous uint8 GPU tensor of shape ({self.columns}, {n})")
-            _same_device(self.scales, self.codes, "scales")
+    def _set(self, codes, scales, features: int):
+        self.codes, self.scales, self.features, self.columns = codes, scales, features, codes.shape[0]
+        return self
 
     def dequantize(self, dtype=None):
         """The values as a [features, columns] tensor (float32, float16 or bfloat16)."""
         import torch
 
-        self.check()
         y = torch.empty((self.features, self.columns), dtype=dtype or torch.float32, device=self.codes.device)
         if y.dtype not in _types()[1]:
             raise ValueError(f"values of type {y.dtype}")
@@ -211,8 +219,9 @@ def quantize_mx4(x) -> Mx4:
         raise ValueError(f"x of type {x.dtype}")
     k, n = x.shape
     L = A.lib()
-    q = Mx4(torch.empty((n, L.ponni_mx4_code_bytes(k)), dtype=torch.uint8, device=x.device),
-            torch.empty((n, L.ponni_mx4_scale_bytes(k)), dtype=torch.uint8, device=x.device), k, checked=True)
+    code_bytes, scale_bytes = _mx4_bytes(k)
+    q = Mx4.__new__(Mx4)._set(torch.empty((n, code_bytes), dtype=torch.uint8, device=x.device),
+                              torch.empty((n, scale_bytes), dtype=torch.uint8, device=x.device), k)
     _call(x, L.ponni_mx4_quantize, x.data_ptr(), ld, _types()[1][x.dtype], k, n, q.codes.data_ptr(), q.scales.data_ptr())
     return q
 
@@ -273,20 +282,16 @@ class ExpertInference:
         A.check(A.lib().ponni_experts_create(descs, len(layers), self.num_experts, _DTYPES[dtype],
                                              A.WEIGHTS_MX4 if weights == "mx4" else A.WEIGHTS_SAME,
                                              ctypes.byref(self._experts)))
-        self._pending = [(i, l.values) for i, l in enumerate(layers) if getattr(l, "values", None) is not None]
-        device = next((v.device for _, v in self._pending if hasattr(v, "data_ptr") and v.is_cuda), None)
+        params = [(i, l.values) for i, l in enumerate(layers) if getattr(l, "values", None) is not None]
         import torch
 
-        if device is not None or torch.cuda.is_available():
-            self._push(device)
-
-    def _push(self, device):
-        import torch
-
-        with torch.cuda.device(device if device is not None else torch.cuda.current_device()):
-            for i, v in self._pending:
+        # On the GPU of the first array that is on one, or the current one.
+        self.device = next((v.get_device() for _, v in params if hasattr(v, "data_ptr") and v.is_cuda), None)
+        if self.device is None and torch.cuda.is_available():
+            self.device = torch.cuda.current_device()
+        if self.device is not None:
+            for i, v in params:
                 self.set_layer_params(i, v)
-        self._pending = []
 
     def __del__(self):
         e = getattr(self, "_experts", None)
@@ -298,16 +303,23 @@ class ExpertInference:
             self._experts = None
 
     def set_layer_params(self, i: int, values) -> None:
-        """All experts' parameters of layer i (numpy or torch, host or GPU)."""
+        """All experts' parameters of layer i (numpy or torch, host or any GPU)."""
+        import torch
+
         if hasattr(values, "data_ptr"):
-            v = values.detach().contiguous()
+            v = values.detach()
+            if v.is_cuda and v.get_device() != self.device:
+                v = v.to(f"cuda:{self.device}")
+            v = v.contiguous() if v.dtype in _types()[1] else v.double().contiguous()
             code, ptr, n, on_device = _types()[1][v.dtype], v.data_ptr(), v.numel(), int(v.is_cuda)
-            stream = _current_stream(v) if on_device else 0
         else:
             v = np.ascontiguousarray(values)
+            v = v if v.dtype in (np.float32, np.float64, np.float16) else v.astype(np.float64)
             code = {np.dtype(np.float32): A.F32, np.dtype(np.float64): A.F64, np.dtype(np.float16): A.F16}[v.dtype]
-            ptr, n, on_device, stream = v.ctypes.data, v.size, 0, 0
-        A.check(A.lib().ponni_experts_set_layer_params(self._experts, i, ptr, code, n, on_device, stream))
+            ptr, n, on_device = v.ctypes.data, v.size, 0
+        with torch.cuda.device(self.device):
+            stream = torch.cuda.current_stream().cuda_stream
+            A.check(A.lib().ponni_experts_set_layer_params(self._experts, i, ptr, code, n, on_device, stream))
 
     def get_num_inputs(self) -> int:
         return self.n_in
@@ -320,7 +332,7 @@ class ExpertInference:
 
         dtype = _types()[0][self.dtype]
         if y is None:
-            y = torch.empty((self.n_out, columns), dtype=dtype, device=like.device)
+            return torch.empty((self.n_out, columns), dtype=dtype, device=like.device), columns
         ld = _rows(y, "y", self.n_out, columns)
         if y.dtype != dtype:
             raise ValueError(f"y is {y.dtype}, the model {dtype}")
@@ -337,7 +349,6 @@ class ExpertInference:
         L = A.lib()
         rows = isinstance(x, Mx4)
         if rows:
-            x.check()
             like, columns = x.codes, x.columns
             if x.features != self.n_in:
                 raise ValueError(f"x has {x.features} features, the model {self.n_in} inputs")
@@ -368,13 +379,13 @@ class ExpertInference:
         ld_in = _rows(x, "x", self.n_in, routing.batch)
         if x.dtype != _types()[0][self.dtype]:
             raise ValueError(f"x is {x.dtype}, the model {_types()[0][self.dtype]}")
-        _same_device(routing.slots, x, "routing")
+        if routing.device != x.get_device():
+            raise ValueError(f"routing is on GPU {routing.device}, the input on {x.device}")
         y, ld = self._buffers(x, routing.batch, y)
         need = L.ponni_experts_mixture_workspace_bytes(self._experts, routing.top_k, routing.batch)
         work = torch.empty(max(need, 1), dtype=torch.uint8, device=x.device)
-        arrays = routing.arrays()
-        _call(x, L.ponni_experts_forward_mixture, self._experts, x.data_ptr(), ld_in, ctypes.byref(arrays), y.data_ptr(),
-              ld, work.data_ptr(), need)
+        _call(x, L.ponni_experts_forward_mixture, self._experts, x.data_ptr(), ld_in, ctypes.byref(routing._arrays),
+              y.data_ptr(), ld, work.data_ptr(), need)
         return y
 
 

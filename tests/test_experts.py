@@ -94,7 +94,7 @@ def test_refused_forward_arguments():
         return L.ponni_experts_forward(e, x, ld, off, y, ldy, n, ws, size, None)
 
     assert fwd(None) == inv
-    assert fwd(e, n=0) == shape and fwd(e, n=-1) == shape and fwd(e, n=1 << 31, ld=1 << 31, ldy=1 << 31) == shape
+    assert fwd(e, n=0) == shape and fwd(e, n=-1) == shape and fwd(e, n=1_000_000_001, ld=1 << 31, ldy=1 << 31) == shape
     assert fwd(e, x=None) == inv and fwd(e, y=None) == inv
     assert fwd(e, off=None) == inv
     assert fwd(e, ld=7) == shape and fwd(e, ldy=7) == shape
@@ -114,7 +114,7 @@ def test_refused_forward_arguments():
 
     assert mix(None) == inv and L.ponni_experts_forward_mixture(e, FAKE, 8, None, FAKE, 8, FAKE, 0, None) == inv
     assert mix(e, k=0) == inv and mix(e, k=4) == inv and mix(e, experts=0) == inv
-    assert mix(e, b=0) == shape and mix(e, b=1 << 30, ld=1 << 30) == shape and mix(e, experts=4) == shape
+    assert mix(e, b=0) == shape and mix(e, b=500_000_001, ld=1 << 30) == shape and mix(e, experts=4) == shape
     assert mix(e, x=None) == inv and mix(e, y=None) == inv and mix(e, ld=7) == shape
     for name in ("weights", "slots", "source", "offsets"):
         assert mix(e, **{name: None}) == inv

@@ -432,14 +432,14 @@ def test_mixture_of_experts_model(cuda, B):
 
 
 @pytest.mark.parametrize("weights", ["same", "mx4"])
-@pytest.mark.parametrize("B", [3, 700])
-def test_graph_replays(cuda, B, weights):
+@pytest.mark.parametrize("B,hidden", [(3, 130), (700, 130), (700, 500), (700, 600)])
+def test_graph_replays(cuda, B, hidden, weights):
     """Routing and a mixture captured in one graph, replayed with new inputs between
     the program's own work; two graphs of one model; the eager result each time."""
     import torch
 
     r = np.random.default_rng(B)
-    experts, _ = networks(r, 8, (64, 600 if B > 3 else 130, 48), ("silu", "none"), "bf16", weights)
+    experts, _ = networks(r, 8, (64, hidden, 48), ("silu", "none"), "bf16", weights)
     x = torch.empty((64, B), dtype=torch.bfloat16, device=cuda)
     s = torch.empty((8, B), device=cuda)
 
