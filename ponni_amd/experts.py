@@ -109,7 +109,7 @@ class Routing:
         if weights.dtype != torch.float32 or weights.shape != slots.shape or not weights.is_contiguous():
             raise ValueError(f"weights must be a contiguous float32 tensor of shape {tuple(slots.shape)}")
         _same_device(weights, slots, "weights")
-        self._tensors = (experts, weights, slots, source, offsets)
+        self._tensors = [experts, weights, slots, source, offsets]
         self._arrays = A.RoutingArrays(self.num_experts, self.top_k, self.batch, *[t.data_ptr() for t in self._tensors])
 
     @classmethod
@@ -118,7 +118,7 @@ class Routing:
         import torch
 
         r = cls.__new__(cls)
-        r.num_experts, r.top_k, r.batch, r.device, r._tensors = num_experts, top_k, batch, like.get_device(), None
+        r.num_experts, r.top_k, r.batch, r.device, r._tensors = num_experts, top_k, batch, like.get_device(), [None] * 5
         n = top_k * batch
         work = (4 * n + num_experts + 4) // 4 * 4  # (16-byte aligned)
         r._buffer = torch.empty(work + work_bytes // 4, dtype=torch.int32, device=like.device)
@@ -127,16 +127,19 @@ class Routing:
         return r, at + 4 * work
 
     def _tensor(self, i: int):
-        if self._tensors is None:
-            import torch
+        t = self._tensors[i]
+        if t is None:  # a view of the buffer, made when it is asked for
+            k, b = self.top_k, self.batch
+            if i < 3:
+                t = self._buffer.as_strided((k, b), (b, 1), i * k * b)
+                if i == 1:
+                    import torch
 
-            n = self.top_k * self.batch
-            experts, weights, slots, source, rest = self._buffer.split_with_sizes(
-                (n, n, n, n, self._buffer.shape[0] - 4 * n))
-            shape = (self.top_k, self.batch)
-            self._tensors = (experts.view(shape), weights.view(torch.float32).view(shape), slots.view(shape), source,
-                             rest[:self.num_experts + 1])
-        return self._tensors[i]
+                    t = t.view(torch.float32)
+            else:
+                t = self._buffer.as_strided((k * b if i == 3 else self.num_experts + 1,), (1,), i * k * b)
+            self._tensors[i] = t
+        return t
 
     experts = property(lambda self: self._tensor(0))
     weights = property(lambda self: self._tensor(1))
