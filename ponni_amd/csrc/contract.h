@@ -66,9 +66,11 @@ struct Tile {
 
 // This workgroup's tile.  Every group has ceil(columns / width) column tiles; the
 // grid holds as many as any offsets can give.  Each XCD (workgroups go to the
-// eight in turn) takes a contiguous share of the tiles, output blocks of a column
-// tile first: its rows are read into one L2 only, and an expert's weights by few.
-template <int WIDTH>
+// eight in turn) takes a contiguous share of the tiles, which go by GROUP column tiles
+// and, within those, by output block: rows are read into one L2 only, an expert's weights by few,
+// and the 32 tiles that an XCD has at a time share both (8 x 4 tiles read 12 parts of
+// a step where 2 x 16 read 18).
+template <int WIDTH, int GROUP = 8>
 __device__ inline Tile find_tile(ContractArgs const& a, int out_blocks) {
   int const lane = threadIdx.x & 63;
   int32_t const columns = static_cast<int32_t>(a.columns);
@@ -87,14 +89,17 @@ __device__ inline Tile find_tile(ContractArgs const& a, int out_blocks) {
   };
   int64_t total = 0;
   for (int base = 0; base < a.experts; base += 64) total += __shfl(scan(tiles(base)), 63);
+  int64_t const column_tiles = total;
   total *= out_blocks;
   int64_t const q = total / 8, r = total % 8, xcd = blockIdx.x % 8, at = blockIdx.x / 8;
   Tile t{};
   t.none = true;
   if (at >= q + (xcd < r ? 1 : 0)) return t;
   int64_t const index = xcd * q + (xcd < r ? xcd : r) + at;
-  int column_tile = static_cast<int>(index / out_blocks);
-  t.block = __builtin_amdgcn_readfirstlane(static_cast<int>(index % out_blocks));
+  int64_t const group = index / (int64_t(GROUP) * out_blocks) * GROUP, rest = column_tiles - group;
+  int const wide = rest < GROUP ? static_cast<int>(rest) : GROUP, within_group = static_cast<int>(index - group * out_blocks);
+  int column_tile = static_cast<int>(group) + within_group % wide;
+  t.block = __builtin_amdgcn_readfirstlane(within_group / wide);
   for (int base = 0; base < a.experts; base += 64) {
     int const n = tiles(base), end = scan(n);
     int const all = __shfl(end, 63);
