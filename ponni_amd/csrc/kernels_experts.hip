@@ -13,7 +13,9 @@
 //
 // A workgroup computes 16 MI WM features x 16 NJ WN columns of one group; two
 // steps' weights and rows, whole 128-byte lines, go from memory straight into
-// LDS a turn and a half ahead, fragments into registers a step ahead.
+// LDS a turn and a half ahead, fragments into registers a step ahead.  Bound by MFMA:
+// bf16 1024-1024, 16 unequal experts, 65,536 columns: 187-200 us, 0.7 PFLOP/s, MFMA busy
+// 43 % of the SIMDs' time; 4-bit 4096-4096, 16,384 columns: 175-195 us, 3 PFLOP/s.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -207,6 +209,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void contract(ContractArgs a) {
 // straight into registers, and no wave waits for another before the sums meet in LDS
 // (in the order of the waves).  FEATURES: the input as the caller holds it, without
 // rows made of it first; 4-bit fragments are quantised as they are read.
+// bf16 1024-2048 and 2048-1024 of up to 6 of 8 experts, 3 samples: 11.4 and 8.0 us (25 MB
+// of weights each at most, 5 us at a copy's rate); 4-bit 2048-2048, 8 columns: 9.0 us,
+// the latency of a launch, one load and the sums.
 template <Operand OP, class S, OutputKind KIND, bool FEATURES, int MT, int NJ, int W>
 __global__ __launch_bounds__(64 * W) void contract_thin(ContractArgs a) {
   static_assert(MT == 4 || (MT == 1 && KIND != OUT_MX4), "a lane's 16 features, or 4 of them");
@@ -370,8 +375,10 @@ hipError_t launch_kind(OutputKind kind, ContractArgs const& a, hipStream_t strea
   }
 }
 
+// y[f, b] = sum_j weight_j[b] row(slot_j[b])[f], in the order of j.
 // 64 samples x 64 features: a lane sums 8 features of one sample's rows, the
-// tile turns in LDS.
+// tile turns in LDS.  Bound by bytes: 512 features, top 4, 65,536 samples (fp16 rows): 78 us
+// for 336 MB, 4.3 TB/s.
 template <class R, class S>
 __global__ __launch_bounds__(256) void combine(Rows rows, int64_t num_rows, ponni_routing r, int64_t features,
                                                S* __restrict__ y, int64_t ld) {

@@ -275,6 +275,35 @@ def test_grouped_columns_large(cuda, E, widths, acts, C, types):
     assert bool((y[:, offsets[-1]:] == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype,weights", [("f16", "same"), ("bf16", "same"), ("f16", "mx4"), ("bf16", "mx4")])
+@pytest.mark.parametrize("E,widths,C", [(3, (130, 1100), 20_001), (11, (600, 650), 1701)])
+@pytest.mark.parametrize("shift", [0, 1, 6])
+def test_grouped_columns_in_aligned_rows(cuda, E, widths, C, shift, dtype, weights):
+    """Rows a multiple of 16 bytes long hold the same bits as others, and the columns around the groups stay."""
+    import torch
+
+    r = np.random.default_rng(C + shift)
+    model, params = networks(r, E, widths, ("none",), dtype, weights)
+    offsets = group_sizes(r, E, C)
+    at = torch.from_numpy(offsets).to(cuda)
+    x = torch.randn((widths[0], C), device=cuda, generator=torch.Generator(cuda).manual_seed(C)).to(torch_dtype(dtype))
+    results = []
+    for pitch in ((C + 15) // 8 * 8, (C + 15) // 8 * 8 + 1):
+        whole = torch.full((widths[-1], pitch), 7.0, dtype=x.dtype, device=cuda)
+        y = whole[:, shift:shift + C]
+        model.forward_batch_parallel(x, at, y)
+        results.append(y.clone())
+        y[:, :offsets[-1]] = 7.0
+        assert bool((whole == 7.0).all())
+    assert torch.equal(*results)
+    for e in range(E):
+        a, b = offsets[e], offsets[e + 1]
+        if a < b:
+            cols = np.unique(np.concatenate([np.arange(a, min(a + 9, b)), np.arange(max(b - 9, a), b), r.integers(a, b, 20)]))
+            want, err = N.chain(params[e], host(x[:, torch.from_numpy(cols).to(cuda)]), dtype, weights)
+            close(host(results[0][:, torch.from_numpy(cols).to(cuda)]), want, err, dtype)
+
+
 def test_rows_beyond_four_gigabytes(cuda):
     """Byte offsets past 2^32 in the input, its rows and the output."""
     import torch
