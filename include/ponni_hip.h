@@ -625,8 +625,8 @@ int64_t ponni_experts_workspace_bytes(ponni_experts experts, int64_t columns);
 
 /* y[:, b] = sum over j, in that order, of weights[j, b] * chain of expert experts[j, b] at x[:, b],
  * x [n_in, batch], y [n_out, batch]; a sample without experts gives zero.
- * Reads routing->weights, slots, source and offsets.  The chains' outputs are
- * held in fp32, or beyond 64 MiB of them in the model's type, their sum in fp32. */
+ * Reads routing->weights, slots, source and offsets.  The chains' outputs and
+ * their sum are held in fp32, rounded to the model's type once, in y. */
 int ponni_experts_forward_mixture(ponni_experts experts, const void* x, int64_t ld_in, const ponni_routing* routing,
                                   void* y, int64_t ld_out, void* workspace, int64_t workspace_bytes,
                                   hipStream_t stream);

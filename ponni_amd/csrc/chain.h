@@ -196,8 +196,7 @@ hipError_t launch_chain_as(OutputKind kind, int columns, ChainArgs const& a, hip
     else return columns == 128 ? launch_chain_sized<OP, S, KIND, FEATURES, 128, 8>(a, stream)
                                : launch_chain_sized<OP, S, KIND, FEATURES, 64, 8>(a, stream);
   };
-  if (kind == OUT_ROWS) return sized.template operator()<OUT_ROWS, false>();
-  if (kind == OUT_FLOATS) return sized.template operator()<OP == OPERAND_F32 ? OUT_ROWS : OUT_FLOATS, false>();
+  if (kind == OUT_FLOATS) return sized.template operator()<OUT_FLOATS, false>();
   if (a.io.features != nullptr) return sized.template operator()<OUT_FEATURES, true>();
   if constexpr (OP == OPERAND_MX4) return sized.template operator()<OUT_FEATURES, false>();
   return hipErrorInvalidValue;

@@ -71,16 +71,11 @@ int chain_of(ponni_experts_s const& e, int64_t columns, ChainArgs& a) {
   return chain_columns(e.operand, a);
 }
 
-// Whether a mixture's chains leave their outputs in fp32 for the weighted sum: where
-// they are few bytes.  More are rounded to the model's type first, which adds a rounding
-// to the result (an error of sqrt(1 + the squared weights) times that of the result's own, 1.41 at
-// most) and halves their way through memory (1024-2048-1024 of 16,384 samples, top 2: 134 MB each way).
-bool float_outputs(ponni_experts_s const& e, int64_t columns) {
-  return e.dtype != PONNI_F32 && columns * e.layers.back().n_out * 4 <= int64_t(64) << 20;
-}
-int64_t output_row_bytes(ponni_experts_s const& e, int64_t columns) {
-  return round_up(e.layers.back().n_out * (float_outputs(e, columns) ? 4 : element_bytes(e.dtype)), 64);
-}
+// A mixture's chains leave their outputs in fp32 for the weighted sum, in batches of every size.
+// Rounded to the model's type first, each would add up to half a step of |weight| |output|: more than the
+// sum itself where outputs cancel, and infinite where fp16 ends.  That would halve their way
+// through memory: fp16 512-1024-512, top 4, 65,536 samples, 537 MB each way, takes 940 us for 810.
+int64_t output_row_bytes(ponni_experts_s const& e) { return int64_t(e.layers.back().blocks) * 256; }
 
 Workspace workspace_of(ponni_experts_s const& e, int64_t rows, int64_t columns, bool mixture) {
   Workspace w;
@@ -102,8 +97,7 @@ Workspace workspace_of(ponni_experts_s const& e, int64_t rows, int64_t columns, 
     data[i % 2] = std::max(data[i % 2], columns * e.layers[i + 1].steps * 64);
     if (mx4) scales[i % 2] = std::max(scales[i % 2], columns * e.layers[i + 1].steps * 4);
   }
-  if (mixture)
-    data[last % 2] = std::max(data[last % 2], columns * output_row_bytes(e, columns));
+  if (mixture) data[last % 2] = std::max(data[last % 2], columns * output_row_bytes(e));
   for (int b = 0; b < 2; b++) {
     w.state[b] = take(data[b]);
     w.state_scales[b] = take(scales[b]);
@@ -190,16 +184,14 @@ int run_layers(ponni_experts_s const& e, void const* x, int64_t ld_in, Rows inpu
       a.y = y;
       a.ldy = ld_out;
     } else {
-      bool const floats = i == last && float_outputs(e, columns);
-      kind = i < last && mx4 ? OUT_MX4 : floats ? OUT_FLOATS : OUT_ROWS;
+      kind = i == last ? OUT_FLOATS : mx4 ? OUT_MX4 : OUT_ROWS;
       int const next = i < last ? e.layers[i + 1].steps : 0;
       a.y_rows.data = base + w.state[i % 2];
       a.y_rows.scales = reinterpret_cast<unsigned char*>(base + w.state_scales[i % 2]);
-      a.y_rows.stride = i < last ? int64_t(next) * 64 : output_row_bytes(e, columns);
+      a.y_rows.stride = i < last ? int64_t(next) * 64 : output_row_bytes(e);
       a.y_rows.scale_stride = 4;
       a.y_rows.scale_step = columns * 4;
-      a.row_features = i < last ? next * step_features(e.operand)
-                                : static_cast<int32_t>(a.y_rows.stride / (floats ? 4 : element_bytes(e.dtype)));
+      a.row_features = i < last ? next * step_features(e.operand) : l.blocks * 64;
     }
     hipError_t err;
     if (chain_tile > 0) {
@@ -291,7 +283,7 @@ int mixture_impl(ponni_experts e, const void* x, int64_t ld_in, const ponni_rout
   Rows result;
   st = run_layers(*e, x, ld_in, Rows{}, r->batch, r->source, r->offsets, columns, nullptr, 0, base, w, &result, stream);
   if (st != PONNI_OK) return st;
-  hipError_t const err = launch_combine(e->dtype, float_outputs(*e, columns), result, columns, *r, last.n_out, y, ld_out, stream);
+  hipError_t const err = launch_combine(e->dtype, result, columns, *r, last.n_out, y, ld_out, stream);
   return err == hipSuccess ? PONNI_OK : device_error("weighted sum", err);
 }
 

@@ -17,6 +17,9 @@ namespace ponni_hip {
 enum Operand { OPERAND_F32 = 0, OPERAND_F16 = 1, OPERAND_BF16 = 2, OPERAND_MX4 = 3 };
 constexpr int kMx4Block = 32;  // features that share a scale
 inline int step_features(Operand o) { return o == OPERAND_F32 ? 16 : o == OPERAND_MX4 ? 128 : 32; }
+// Where the four features 16 g + 4 i .. + 3 of a block of 64 lie in an OUT_FLOATS row: behind those of lane groups
+// below g, so that the four groups' pieces i, stored together, are 64 consecutive bytes.
+__host__ __device__ inline int float_place(int g, int i) { return 16 * i + 4 * g; }
 inline int64_t contraction_steps(Operand o, int64_t features) {
   return (features + step_features(o) - 1) / step_features(o);
 }
@@ -32,7 +35,8 @@ struct Rows {
   int64_t scale_step = 0;           // and to those of the next step
 };
 
-// [features, columns], or rows of the operand's type, of 4 bits, of fp32.
+// [features, columns], or rows: a layer's of the operand's type or of 4 bits for the next one; a
+// mixture's outputs as fp32 of whole blocks of 64 features, in the order of float_place.
 enum OutputKind { OUT_FEATURES = 0, OUT_ROWS = 1, OUT_MX4 = 2, OUT_FLOATS = 3 };
 
 // One layer over columns grouped by expert:
@@ -100,9 +104,8 @@ hipError_t launch_contraction(Operand op, int out_type, OutputKind kind, Contrac
 // x [features, columns] of `dtype` as rows of `op`, `row_bytes` a row.
 hipError_t launch_to_rows(Operand op, int dtype, const void* x, int64_t ld, int64_t features, int64_t columns,
                           Rows const& rows, hipStream_t stream);
-// y[f, b] = sum_j weights[j, b] rows[slots[j, b]][f] (slots outside [0, num_rows) add nothing); rows of
-// `dtype`, or floats.
-hipError_t launch_combine(int dtype, bool floats, Rows const& rows, int64_t num_rows, const ponni_routing& r, int64_t features,
+// y[f, b] = sum_j weights[j, b] rows[slots[j, b]][f] (slots outside [0, num_rows) add nothing); rows of floats.
+hipError_t launch_combine(int dtype, Rows const& rows, int64_t num_rows, const ponni_routing& r, int64_t features,
                           void* y, int64_t ld, hipStream_t stream);
 // W [experts, n_in, n_out] of `dtype` in fragment order (values past n_in or n_out zero).
 hipError_t launch_pack_weights(Operand op, int dtype, const void* w, int64_t experts, int64_t n_in, int64_t n_out,

@@ -300,8 +300,9 @@ __global__ __launch_bounds__(64 * W) void contract_thin(ContractArgs a) {
     else if (col < t.last) store_features<KIND, S>(a, col, f0, v, a.n_out);
   } else if (col < t.last) {
     using R = std::conditional_t<KIND == OUT_FLOATS, float, S>;
-    R* y = KIND == OUT_FEATURES ? static_cast<R*>(a.y) + int64_t(f0) * a.ldy + col
-                                : reinterpret_cast<R*>(a.y_rows.data + col * a.y_rows.stride) + f0;
+    int64_t const at = KIND == OUT_FLOATS ? block_here * 64 + float_place(g, tile0) : f0;
+    R* y = KIND == OUT_FEATURES ? static_cast<R*>(a.y) + at * a.ldy + col
+                                : reinterpret_cast<R*>(a.y_rows.data + col * a.y_rows.stride) + at;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       if (KIND == OUT_FEATURES ? f0 + e < a.n_out : f0 + e < a.row_features)
@@ -365,10 +366,10 @@ template <Operand OP, class S>
 hipError_t launch_kind(OutputKind kind, ContractArgs const& a, hipStream_t stream) {
   switch (kind) {
     case OUT_FEATURES: return launch_sized<OP, S, OUT_FEATURES>(a, stream);
-    case OUT_ROWS: return launch_sized<OP, S, OUT_ROWS>(a, stream);
-    case OUT_FLOATS:
-      if constexpr (OP == OPERAND_F32) return launch_sized<OP, S, OUT_ROWS>(a, stream);
-      else return launch_sized<OP, S, OUT_FLOATS>(a, stream);
+    case OUT_ROWS:
+      if constexpr (OP != OPERAND_MX4) return launch_sized<OP, S, OUT_ROWS>(a, stream);
+      return hipErrorInvalidValue;
+    case OUT_FLOATS: return launch_sized<OP, S, OUT_FLOATS>(a, stream);
     default:
       if constexpr (OP == OPERAND_MX4) return launch_sized<OP, S, OUT_MX4>(a, stream);
       return hipErrorInvalidValue;
@@ -376,29 +377,33 @@ hipError_t launch_kind(OutputKind kind, ContractArgs const& a, hipStream_t strea
 }
 
 // y[f, b] = sum_j weight_j[b] row(slot_j[b])[f], in the order of j.
-// 64 samples x 64 features: a lane sums 8 features of one sample's rows, the
-// tile turns in LDS.  Bound by bytes: 512 features, top 4, 65,536 samples (fp16 rows): 78 us
-// for 336 MB, 4.3 TB/s.
-template <class R, class S>
+// 64 samples x 64 features: a lane sums 8 features of one sample's rows (two neighbouring
+// pieces, of two lane groups: float_place), the tile turns in LDS.  Bound by bytes: 512 features, top 4,
+// 65,536 samples: 130 us for 604 MB, 4.6 TB/s.
+template <class S>
 __global__ __launch_bounds__(256) void combine(Rows rows, int64_t num_rows, ponni_routing r, int64_t features,
                                                S* __restrict__ y, int64_t ld) {
   __shared__ float tile[64][65];  // [feature][sample]
   int64_t const b0 = int64_t(blockIdx.x) * 64, f0 = int64_t(blockIdx.y) * 64;
   for (int p = threadIdx.x; p < 64 * 8; p += 256) {
-    int const s = p >> 3, q = (p & 7) * 8;
+    int const s = p >> 3, q = p & 7, g = 2 * (q & 1), i = q >> 1;
     int64_t const b = b0 + s;
-    float sum[8] = {};
-    if (b < r.batch && f0 + q < features)
+    f32x4 sum[2] = {};
+    if (b < r.batch)
       for (int j = 0; j < r.top_k; j++) {
         int64_t const slot = r.slots[j * r.batch + b];
         if (slot < 0 || slot >= num_rows) continue;
         float const w = r.weights[j * r.batch + b];
-        R const* row = reinterpret_cast<R const*>(rows.data + slot * rows.stride) + f0 + q;
+        f32x4 const* row = reinterpret_cast<f32x4 const*>(rows.data + slot * rows.stride + (f0 + float_place(g, i)) * 4);
 #pragma unroll
-        for (int i = 0; i < 8; i++) sum[i] = fmaf(w, float(row[i]), sum[i]);  // (rows are whole 64-byte pieces)
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) sum[h][e] = fmaf(w, row[h][e], sum[h][e]);
       }
 #pragma unroll
-    for (int i = 0; i < 8; i++) tile[q + i][s] = sum[i];
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) tile[16 * (g + h) + 4 * i + e][s] = sum[h][e];
   }
   __syncthreads();
   int const s = threadIdx.x & 63;
@@ -512,16 +517,12 @@ hipError_t launch_contraction(Operand op, int out_type, OutputKind kind, Contrac
   }
 }
 
-hipError_t launch_combine(int dtype, bool floats, Rows const& rows, int64_t num_rows, const ponni_routing& r, int64_t features,
+hipError_t launch_combine(int dtype, Rows const& rows, int64_t num_rows, const ponni_routing& r, int64_t features,
                           void* y, int64_t ld, hipStream_t stream) {
   dim3 const grid(unsigned((r.batch + 63) / 64), unsigned((features + 63) / 64));
   with_dtype(dtype, [&](auto s) {
     using S = decltype(s);
-    auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, rows, num_rows, r, features, static_cast<S*>(y), ld);
-    };
-    if (floats) launch(combine<float, S>);
-    else launch(combine<S, S>);
+    hipLaunchKernelGGL(combine<S>, grid, dim3(256), 0, stream, rows, num_rows, r, features, static_cast<S*>(y), ld);
   });
   return hipGetLastError();
 }

@@ -584,3 +584,70 @@ def test_refusals_of_tensors(cuda):
     with pytest.raises(P.PonniError) as e:  # x and y share memory
         model.forward_batch_parallel(wide[:20], offsets, wide[19:49])
     assert e.value.status == A.PONNI_ERR_INVALID_ARGUMENT
+
+
+# -- mixtures of many columns ------------------------------------------------------------
+
+# Outputs of more than 64 MiB in 32 bits, held so all the same: no rounding between the chains and the weighted sum.
+MIXTURES = [
+    # experts, top_k, widths, activations, samples
+    (2, 2, (40, 1001), ("none",), 9001),  # tiles of 128 columns
+    (2, 2, (40, 70, 500), ("silu", "none"), 17_001),  # one kernel
+    (5, 3, (130, 1100, 1030), ("tanh", "none"), 9334),  # tiles of 256 columns, gathered and between the layers
+]
+
+
+def check_mixture(model, params, x, routing, y, dtype, weights, samples):
+    """The weighted sums of `samples` from the chains' values in 32 bits: those of N.chain, k products and sums,
+    and the one rounding to dtype."""
+    xs, experts, w = host(x[:, samples]), host(routing.experts[:, samples]).astype(int), host(routing.weights[:, samples])
+    want, err = np.zeros((y.shape[0], len(samples))), np.zeros((y.shape[0], len(samples)))
+    for e, p in enumerate(params):
+        j, b = np.nonzero(experts == e)
+        if len(b):
+            v, d = N.chain(p, xs[:, b], dtype, weights)
+            want[:, b] += w[j, b] * v
+            err[:, b] += w[j, b] * (d + (routing.top_k + 1) * 2.0 ** -24 * (np.abs(v) + d))
+    close(host(y[:, samples]), want, err, dtype)
+
+
+@pytest.mark.parametrize("dtype,weights", [("f32", "same"), ("f16", "same"), ("bf16", "same"), ("f16", "mx4"),
+                                           ("bf16", "mx4")])
+@pytest.mark.parametrize("E,k,widths,acts,B", MIXTURES)
+def test_large_mixture(cuda, E, k, widths, acts, B, dtype, weights):
+    import torch
+
+    print(f"mixture: E={E} k={k} {widths} B={B} {dtype} {weights}", flush=True)
+    r = np.random.default_rng(B)
+    model, params = networks(r, E, widths, acts, dtype, weights)
+    g = torch.Generator(cuda).manual_seed(B)
+    routing = P.route_experts(torch.randn((E, B), device=cuda, generator=g), k)
+    x = torch.randn((widths[0], B), device=cuda, generator=g).to(torch_dtype(dtype))
+    y = model.forward_mixture(x, routing)
+    check_mixture(model, params, x, routing, y, dtype, weights,
+                  torch.from_numpy(np.concatenate([[0, B - 1], r.integers(0, B, 150)])).to(cuda))
+
+
+@pytest.mark.parametrize("dtype,weights", [("f16", "same"), ("bf16", "same"), ("f16", "mx4")])
+@pytest.mark.parametrize("widths,B", [((40, 60), 50), ((40, 1001), 9001), ((40, 500), 17_001)])
+def test_mixture_of_experts_that_cancel(cuda, widths, B, dtype, weights):
+    """Two experts' outputs far above their weighted sum, in fp16 above the type's largest number: in a small batch
+    and in one of more than 64 MiB of them."""
+    import torch
+
+    r = np.random.default_rng(B)
+    size = 1e5 if dtype == "f16" else 100.0
+    model, params = networks(r, 2, widths, ("none",), dtype, weights)
+    bias = np.stack([np.full(widths[1], size), np.full(widths[1], -size)])
+    model.set_layer_params(1, bias)
+    params = [[(p[0][0], bias[e], "none")] for e, p in enumerate(params)]
+    g = torch.Generator(cuda).manual_seed(B)
+    scores = 0.2 * torch.randn((1, B), device=cuda, generator=g)
+    routing = P.route_experts(torch.cat([scores, -scores]), 2)
+    x = torch.randn((widths[0], B), device=cuda, generator=g).to(torch_dtype(dtype))
+    y = model.forward_mixture(x, routing)
+    # (the weights differ by tanh of the score: 0.2 * 4 gives 0.664, and 1e5 times that is beyond fp16's 65504)
+    within = (routing.weights[0] - routing.weights[1]).abs() * size < 65000
+    assert bool(torch.isfinite(y[:, within]).all())
+    samples = torch.from_numpy(r.integers(0, B, 100)).to(cuda)
+    check_mixture(model, params, x, routing, y, dtype, weights, samples[within[samples]])
