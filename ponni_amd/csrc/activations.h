@@ -49,8 +49,9 @@ __device__ inline float tanh_f32(float x) {
 }
 // 16-bit plans: the hardware form, and x itself where that is closer than the
 // type resolves (below 2^-7 tanh(x) is x to 2e-5; the form's error there is an
-// ulp of fp32's one, more than an ulp of a small fp16 result).  fp16
-// 24-1100-200, 40,000 columns: 84 us without, 87 with.
+// ulp of fp32's one, more than an ulp of a small fp16 result, and all of a bf16 one at 1e-8).  fp16
+// 24-1100-200, 40,000 columns: 84 us without, 87 with; a chain of expert layers 64-256-256-256-64,
+// 1,000,000 columns: 489 and 510.
 __device__ inline float tanh_half(float x) { return __builtin_fabsf(x) < 0.0078125f ? x : act_tanh_fast(x); }
 
 }  // namespace ponni_hip

@@ -15,7 +15,7 @@ namespace {
 // blocks of 64 features, so that a narrow layer gives every wave fewer columns.
 // FEATURES: the input as the caller holds it.
 // Bound by the activations' VALU work beside the MFMAs: fp16 64-256-256-256-64 tanh, 1,000,000
-// columns of 8 experts: 485 us, 0.68 PFLOP/s, MFMA busy 33 % and VALU 73 % of the SIMDs'
+// columns of 8 experts: 510 us, 0.64 PFLOP/s, MFMA busy 33 % and VALU 73 % of the SIMDs'
 // time, LDS bank conflicts a third of its accesses' cycles, 65 + 125 MB from and to memory.
 template <Operand OP, class S, OutputKind KIND, bool FEATURES, int C, int W>
 __global__ __launch_bounds__(64 * W, W == 4 && (OP == OPERAND_F16 || OP == OPERAND_BF16) ? 4 : 2) void contract_chain(ChainArgs chain) {

@@ -118,14 +118,13 @@ __device__ inline Tile find_tile(ContractArgs const& a, int out_blocks) {
   return t;
 }
 
-// CHAIN: without GELU's exact form, the longest, and with tanh's hardware form alone, as the
-// other fused kernels have it (off by an ulp of one near zero).
+// CHAIN: without GELU's exact form, the longest.
 template <bool Precise, bool CHAIN = false, class Each>
 __device__ inline void activate(int act, float slope, Each&& each) {
   switch (act) {
     case ACT_RELU: each([](float v) { return act_relu(v); }); break;
     case ACT_LEAKY_RELU: each([slope](float v) { return act_leaky_relu(v, slope); }); break;
-    case ACT_TANH: each([](float v) { return Precise ? tanh_f32(v) : CHAIN ? act_tanh_fast(v) : tanh_half(v); }); break;
+    case ACT_TANH: each([](float v) { return Precise ? tanh_f32(v) : tanh_half(v); }); break;
     case ACT_SIGMOID: each([](float v) { return Precise ? sigmoid_f32(v) : act_sigmoid_fast(v); }); break;
     case ACT_SILU: each([](float v) { return Precise ? silu_f32(v) : act_silu_fast(v); }); break;
     case ACT_GELU_TANH: each([](float v) { return Precise ? gelu_tanh_f32(v) : act_gelu_tanh_fast(v); }); break;

@@ -651,3 +651,46 @@ def test_mixture_of_experts_that_cancel(cuda, widths, B, dtype, weights):
     assert bool(torch.isfinite(y[:, within]).all())
     samples = torch.from_numpy(r.integers(0, B, 100)).to(cuda)
     check_mixture(model, params, x, routing, y, dtype, weights, samples[within[samples]])
+
+
+# -- activations ---------------------------------------------------------------------------
+
+
+def activation_error(act, v, dtype):
+    """How far an activation's fp32 value may be, relative to it near zero and in the tails as elsewhere.
+
+    A power 2^t is off by the rounding of t and an ulp (2^-23) of its own: |t| ln 2 times two roundings of t.
+    fp32 models carry the rounding of t along (tanh: t <= 2.9 |x| only matters while 1 - |tanh| does, a
+    relative 2^-21 at |x| = 0.55, where the form changes), then sum, reciprocal and quotient are a rounding or an ulp
+    each: 2^-21, twice that for tanh.  GELU's argument is four roundings of 2u.  16-bit models round t
+    (|t| ln 2 <= |x|), and tanh is x below 2^-7 (off by x^2 / 3 <= 2^-15), above that off by 2^-21 of one.
+    A reciprocal below the normal range may be zero: 2^-126."""
+    a = np.abs(v)
+    two_u = 2 * np.sqrt(2 / np.pi) * (a + 0.044715 * a ** 3)
+    if dtype == "f32":
+        relative = {"tanh": 2.0 ** -20, "sigmoid": 2.0 ** -21, "silu": 2.0 ** -21,
+                    "gelu": 2.0 ** -21 + two_u * 2.0 ** -22}[act]
+    else:
+        relative = {"tanh": 2.0 ** -14, "sigmoid": (a + 4) * 2.0 ** -23, "silu": (a + 4) * 2.0 ** -23,
+                    "gelu": (two_u + 2) * 2.0 ** -22}[act]
+    return relative * np.abs(N.ACTS[act](v)) + 2.0 ** -126 * (1 + a)
+
+
+@pytest.mark.parametrize("dtype,weights", [("f32", "same"), ("f16", "same"), ("bf16", "same"), ("f16", "mx4"),
+                                           ("bf16", "mx4")])
+@pytest.mark.parametrize("act", ["tanh", "sigmoid", "silu", "gelu"])
+@pytest.mark.parametrize("kernel,n_out,C", [("few columns", 1, 30), ("one kernel", 1, 400), ("tiles", 600, 400)])
+def test_activations_of_every_kernel(cuda, kernel, n_out, C, act, dtype, weights):
+    """Inputs from 1e-8 to 40 through weights of one: every size of batch and layer gives the activation that the
+    type resolves."""
+    import torch
+
+    print(f"activation: {kernel} {act} {dtype} {weights}", flush=True)
+    model = P.create_expert_model(P.ExpertMatvec(np.ones((1, 1, n_out))), ACT[act](n_out), dtype=dtype, weights=weights)
+    v = np.geomspace(1e-8, 40, C // 2)
+    x = tensor(np.concatenate([v, -v])[None], dtype, cuda)
+    got = host(model.forward_batch_parallel(x))
+    v = N.mx4(host(x))[0] if weights == "mx4" else host(x)
+    with np.errstate(over="ignore"):
+        want, err = N.ACTS[act](v), activation_error(act, v, dtype)
+    close(got, np.broadcast_to(want, got.shape), err, dtype)
