@@ -273,6 +273,9 @@ class ExpertInference:
         if weights not in ("same", "mx4"):
             raise ValueError(f"weights must be 'same' or 'mx4', not {weights!r}")
         held = [l for l in layers if getattr(l, "values", None) is not None]
+        if any(l.kind in (A.LAYER_MATVEC, A.LAYER_BIAS) and getattr(l, "values", None) is None for l in layers):
+            # (its parameters would reach no expert)
+            raise A.PonniError(A.PONNI_ERR_INVALID_MODEL, "a Matvec or Bias of one network: use ExpertMatvec or ExpertBias")
         if not held:
             raise A.PonniError(A.PONNI_ERR_INVALID_MODEL, "the chain must begin with a Matvec")
         self.num_experts = int(held[0].values.shape[0])
@@ -394,7 +397,7 @@ class ExpertInference:
 
 def create_expert_model(*layers: Layer, dtype: str = "f32", weights: str = "same") -> ExpertInference:
     """ExpertMatvec, each followed by an optional ExpertBias and an optional
-    activation.  dtype "f32", "f16" or "bf16"; weights "same" (as dtype) or "mx4"
+    activation (no Matvec or Bias of one network).  dtype "f32", "f16" or "bf16"; weights "same" (as dtype) or "mx4"
     (weights and every layer's input in 4 bits)."""
     return ExpertInference(layers, dtype=dtype, weights=weights)
 

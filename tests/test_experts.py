@@ -211,3 +211,14 @@ def test_definition_of_routing():
     assert np.allclose(w[:, 0], np.exp([0, -1]) / (1 + np.exp(-1))) and w[:, 2].tolist() == [0.5, 0.5]
     assert offsets.tolist() == [0, 2, 4, 4] and source.tolist() == [0, 2, 0, 2, -1, -1]
     assert slots.tolist() == [[2, -1, 1], [0, -1, 3]]
+
+
+def test_layers_of_one_network_are_refused():
+    """Their parameters belong to no expert: they would be left out."""
+    w, b = np.ones((2, 3, 4)), np.full(4, 5.0)
+    for layers in ([P.ExpertMatvec(w), P.Bias(b), P.Relu(4)], [P.Matvec(w[0]), P.ExpertBias(np.zeros((2, 4)))],
+                   [P.ExpertMatvec(w), P.Relu(4), P.Matvec(np.zeros((4, 4)))]):
+        with pytest.raises(P.PonniError) as e:
+            P.create_expert_model(*layers)
+        assert e.value.status == A.PONNI_ERR_INVALID_MODEL
+    P.create_expert_model(P.ExpertMatvec(w), P.ExpertBias(np.zeros((2, 4))), P.Relu(4))
