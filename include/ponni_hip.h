@@ -604,7 +604,12 @@ void ponni_experts_destroy(ponni_experts experts);
  * device memory (of the current device, which the object is bound to from the
  * first call on).  Device memory is read on `stream`.  Weights are rounded to
  * the model's operand type.  Synchronous with respect to the host; not for
- * captured streams.  A bias that was never set is zero. */
+ * captured streams.  New parameters in the place of old ones first wait for the
+ * whole device, so that calls made before read the old ones, also on other
+ * streams; graphs read the new ones from their next replay on (a bias that was
+ * first set after their capture is not in them).  Not while another thread makes
+ * a call with the same object or captures a stream of the device.  A bias that
+ * was never set is zero. */
 int ponni_experts_set_layer_params(ponni_experts experts, int32_t layer, const void* values, int32_t dtype,
                                    int64_t count, int32_t on_device, hipStream_t stream);
 int64_t ponni_experts_layer_param_count(ponni_experts experts, int32_t layer);

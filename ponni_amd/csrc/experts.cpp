@@ -397,27 +397,36 @@ int set_params_impl(ponni_experts e, int32_t layer, const void* values, int32_t 
     }
     values = staged;
   }
+  // Calls in flight on any stream, and graphs, read the buffers that are there: they are waited
+  // for, and written in place.  Until that has ended well the layer counts as not set.
+  if (l.weights != nullptr || l.d_bias != nullptr) err = hipDeviceSynchronize();
+  bool const weights_set = l.weights_set;
+  if (err == hipSuccess) l.weights_set = false;
   auto allocate = [&](auto*& p, int64_t n) {
-    return p != nullptr ? hipSuccess : hipMalloc(reinterpret_cast<void**>(&p), n);
+    if (p != nullptr) return hipSuccess;
+    hipError_t const status = hipMalloc(reinterpret_cast<void**>(&p), n);
+    if (status == hipSuccess) e->device = device;
+    return status;
   };
-  if (l.matvec == layer) {
-    int64_t const fragments = int64_t(e->num_experts) * l.blocks * l.steps;
-    err = allocate(l.weights, fragments * 4096);
-    if (err == hipSuccess && e->operand == OPERAND_MX4) err = allocate(l.scales, fragments * 256);
-    if (err == hipSuccess)
-      err = launch_pack_weights(e->operand, dtype, values, e->num_experts, l.n_in, l.n_out, l.blocks, l.weights,
-                                l.scales, stream);
-  } else {
-    int64_t const padded = int64_t(l.blocks) * 64;
-    err = allocate(l.d_bias, e->num_experts * padded * 4);
-    if (err == hipSuccess) err = launch_pack_bias(dtype, values, e->num_experts, l.n_out, padded, l.d_bias, stream);
+  if (err == hipSuccess) {
+    if (l.matvec == layer) {
+      int64_t const fragments = int64_t(e->num_experts) * l.blocks * l.steps;
+      err = allocate(l.weights, fragments * 4096);
+      if (err == hipSuccess && e->operand == OPERAND_MX4) err = allocate(l.scales, fragments * 256);
+      if (err == hipSuccess)
+        err = launch_pack_weights(e->operand, dtype, values, e->num_experts, l.n_in, l.n_out, l.blocks, l.weights,
+                                  l.scales, stream);
+    } else {
+      int64_t const padded = int64_t(l.blocks) * 64;
+      err = allocate(l.d_bias, e->num_experts * padded * 4);
+      if (err == hipSuccess) err = launch_pack_bias(dtype, values, e->num_experts, l.n_out, padded, l.d_bias, stream);
+    }
   }
   hipError_t const done = hipStreamSynchronize(stream);
   if (staged != nullptr) (void)hipFree(staged);
   if (err == hipSuccess) err = done;
   if (err != hipSuccess) return device_error("setting parameters", err);
-  e->device = device;
-  if (l.matvec == layer) l.weights_set = true;
+  l.weights_set = weights_set || l.matvec == layer;
   return PONNI_OK;
 }
 

@@ -309,7 +309,8 @@ class ExpertInference:
             self._experts = None
 
     def set_layer_params(self, i: int, values) -> None:
-        """All experts' parameters of layer i (numpy or torch, host or any GPU)."""
+        """All experts' parameters of layer i (numpy or torch, host or any GPU).  Waits for
+        the device: calls made before, on any stream, read the old ones."""
         import torch
 
         if hasattr(values, "data_ptr"):

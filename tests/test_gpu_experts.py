@@ -694,3 +694,31 @@ def test_activations_of_every_kernel(cuda, kernel, n_out, C, act, dtype, weights
     with np.errstate(over="ignore"):
         want, err = N.ACTS[act](v), activation_error(act, v, dtype)
     close(got, np.broadcast_to(want, got.shape), err, dtype)
+
+
+# -- parameters ----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("on_device", [False, True])
+def test_new_parameters_wait_for_calls_in_flight(cuda, on_device):
+    """A call that another stream has not run yet reads the parameters it was made with."""
+    import torch
+
+    r = np.random.default_rng(6)
+    model, _ = networks(r, 2, (64, 600), ("none",), "f32")
+    x = torch.randn((64, 300), device=cuda)
+    offsets = torch.tensor([0, 100, 300], dtype=torch.int32, device=cuda)
+    want = model.forward_batch_parallel(x, offsets)
+    w = torch.from_numpy(r.standard_normal((2, 64, 600)))
+    w = w.to(cuda) if on_device else w
+    a = torch.randn((8192, 8192), device=cuda)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        for _ in range(20):  # some 100 ms of work before the call
+            a = a @ a
+            a = a / a.abs().amax()
+        got = model.forward_batch_parallel(x, offsets)
+    model.set_layer_params(0, w)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    assert not torch.equal(model.forward_batch_parallel(x, offsets), want)
