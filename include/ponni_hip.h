@@ -551,7 +551,8 @@ typedef struct ponni_routing {
  * (PONNI_ROUTE_CHOSEN) or over all that are not ruled out (PONNI_ROUTE_ALL), in fp32;
  * scores of +inf share the weight equally.  The order of the results does
  * not depend on the order of execution.  `workspace`: device memory of at
- * least ponni_route_workspace_bytes, at a multiple of 16 bytes. */
+ * least ponni_route_workspace_bytes, at a multiple of 16 bytes.  Scores, arrays
+ * and workspace must not overlap. */
 #define PONNI_ROUTE_CHOSEN 0
 #define PONNI_ROUTE_ALL 1
 int ponni_route(const void* scores, int64_t ld, int32_t dtype, int32_t normalize, const ponni_routing* routing,
@@ -618,7 +619,8 @@ int64_t ponni_experts_layer_param_count(ponni_experts experts, int32_t layer);
  * columns] and y [n_out, columns] with row strides ld_in and ld_out, columns
  * sorted by expert.  offsets: device array [num_experts + 1], ascending, of values in
  * 0 .. columns; null with one expert: all columns.  Columns in no group are
- * left as they were.  Groups may be empty.  x, y and the workspace must not overlap. */
+ * left as they were.  Groups may be empty.  y and the workspace must not overlap
+ * each other, x or offsets. */
 int ponni_experts_forward(ponni_experts experts, const void* x, int64_t ld_in, const int32_t* offsets, void* y,
                           int64_t ld_out, int64_t columns, void* workspace, int64_t workspace_bytes,
                           hipStream_t stream);
@@ -631,7 +633,8 @@ int64_t ponni_experts_workspace_bytes(ponni_experts experts, int64_t columns);
 /* y[:, b] = sum over j, in that order, of weights[j, b] * chain of expert experts[j, b] at x[:, b],
  * x [n_in, batch], y [n_out, batch]; a sample without experts gives zero.
  * Reads routing->weights, slots, source and offsets.  The chains' outputs and
- * their sum are held in fp32, rounded to the model's type once, in y. */
+ * their sum are held in fp32, rounded to the model's type once, in y.  y and the
+ * workspace must not overlap each other, x or the arrays that are read. */
 int ponni_experts_forward_mixture(ponni_experts experts, const void* x, int64_t ld_in, const ponni_routing* routing,
                                   void* y, int64_t ld_out, void* workspace, int64_t workspace_bytes,
                                   hipStream_t stream);

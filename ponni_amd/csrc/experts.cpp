@@ -50,6 +50,17 @@ Range bytes(void const* p, int64_t n) {
 }
 bool overlap(Range a, Range b) { return a.begin < b.end && b.begin < a.end; }
 
+// A routing's arrays: weights, slots, source and offsets, which a mixture reads, and experts.
+constexpr int kRoutingArrays = 5;
+void routing_ranges(ponni_routing const& r, Range (&out)[kRoutingArrays]) {
+  int64_t const n = r.top_k * r.batch * 4;
+  out[0] = bytes(r.weights, n);
+  out[1] = bytes(r.slots, n);
+  out[2] = bytes(r.source, n);
+  out[3] = bytes(r.offsets, (int64_t(r.num_experts) + 1) * 4);
+  out[4] = bytes(r.experts, n);
+}
+
 // Work buffers of a call: rows of the input (unless the caller brings them),
 // the layers' outputs in two buffers by turns.
 struct Workspace {
@@ -227,10 +238,9 @@ int forward_impl(ponni_experts e, const void* x, int64_t ld_in, const void* code
     return fail(PONNI_ERR_INVALID_ARGUMENT, "offsets are null with more than one expert");
   if ((!mx4_rows && ld_in < columns) || ld_out < columns)
     return fail(PONNI_ERR_SHAPE, "row strides are smaller than the number of columns");
-  int st = check_ready(*e);
-  if (st != PONNI_OK) return st;
   Workspace const w = workspace_of(*e, mx4_rows ? 0 : columns, columns, false);
-  if ((st = check_workspace(workspace, workspace_bytes, w.total)) != PONNI_OK) return st;
+  int st = check_workspace(workspace, workspace_bytes, w.total);
+  if (st != PONNI_OK) return st;
   auto const& first = e->layers.front();
   int64_t const es = element_bytes(e->dtype);
   Range const out = array(y, e->layers.back().n_out, ld_out, columns, es), work = bytes(workspace, w.total);
@@ -240,8 +250,10 @@ int forward_impl(ponni_experts e, const void* x, int64_t ld_in, const void* code
                                     overlap(work, bytes(scales, columns * first.steps * 4))
                               : overlap(out, array(x, first.n_in, ld_in, columns, es)) ||
                                     overlap(work, array(x, first.n_in, ld_in, columns, es));
-  if (clash || overlap(out, work))
-    return fail(PONNI_ERR_INVALID_ARGUMENT, "input, output and workspace must not overlap");
+  Range const groups = bytes(offsets, offsets != nullptr ? (int64_t(e->num_experts) + 1) * 4 : 0);
+  if (clash || overlap(out, work) || overlap(out, groups) || overlap(work, groups))
+    return fail(PONNI_ERR_INVALID_ARGUMENT, "input, offsets, output and workspace must not overlap");
+  if ((st = check_ready(*e)) != PONNI_OK) return st;
   char* base = static_cast<char*>(workspace);
   Rows rows;  // the caller's 4-bit ones
   if (mx4_rows) {
@@ -269,7 +281,6 @@ int mixture_impl(ponni_experts e, const void* x, int64_t ld_in, const ponni_rout
     return fail(PONNI_ERR_INVALID_ARGUMENT, "a routing array is null");
   if (ld_in < r->batch || ld_out < r->batch)
     return fail(PONNI_ERR_SHAPE, "row strides are smaller than the batch");
-  if ((st = check_ready(*e)) != PONNI_OK) return st;
   int64_t const columns = r->batch * r->top_k, es = element_bytes(e->dtype);
   auto const& first = e->layers.front();
   auto const& last = e->layers.back();
@@ -277,8 +288,13 @@ int mixture_impl(ponni_experts e, const void* x, int64_t ld_in, const ponni_rout
   if ((st = check_workspace(workspace, workspace_bytes, w.total)) != PONNI_OK) return st;
   Range const in = array(x, first.n_in, ld_in, r->batch, es), out = array(y, last.n_out, ld_out, r->batch, es),
               work = bytes(workspace, w.total);
-  if (overlap(in, out) || overlap(in, work) || overlap(out, work))
-    return fail(PONNI_ERR_INVALID_ARGUMENT, "input, output and workspace must not overlap");
+  bool clash = overlap(in, out) || overlap(in, work) || overlap(out, work);
+  Range arrays[kRoutingArrays];
+  routing_ranges(*r, arrays);
+  for (int i = 0; i < 4; i++) clash = clash || overlap(arrays[i], out) || overlap(arrays[i], work);
+  if (clash)
+    return fail(PONNI_ERR_INVALID_ARGUMENT, "input, routing arrays, output and workspace must not overlap");
+  if ((st = check_ready(*e)) != PONNI_OK) return st;
   char* base = static_cast<char*>(workspace);
   Rows result;
   st = run_layers(*e, x, ld_in, Rows{}, r->batch, r->source, r->offsets, columns, nullptr, 0, base, w, &result, stream);
@@ -491,6 +507,17 @@ int ponni_route(const void* scores, int64_t ld, int32_t dtype, int32_t normalize
     if (ld < r->batch) return fail(PONNI_ERR_SHAPE, "row stride is smaller than the batch");
     st = check_workspace(workspace, workspace_bytes, route_workspace_bytes(r->num_experts, r->batch));
     if (st != PONNI_OK) return st;
+    Range arrays[kRoutingArrays];
+    routing_ranges(*r, arrays);
+    Range const in = array(scores, r->num_experts, ld, r->batch, element_bytes(dtype)),
+                work = bytes(workspace, route_workspace_bytes(r->num_experts, r->batch));
+    bool clash = overlap(in, work);
+    for (int i = 0; i < kRoutingArrays; i++) {
+      clash = clash || overlap(arrays[i], in) || overlap(arrays[i], work);
+      for (int j = 0; j < i; j++) clash = clash || overlap(arrays[i], arrays[j]);
+    }
+    if (clash)
+      return fail(PONNI_ERR_INVALID_ARGUMENT, "scores, routing arrays and workspace must not overlap");
     hipError_t const err = launch_route(scores, ld, dtype, normalize, *r, workspace, stream);
     return err == hipSuccess ? int(PONNI_OK) : device_error("routing", err);
   });

@@ -222,3 +222,47 @@ def test_layers_of_one_network_are_refused():
             P.create_expert_model(*layers)
         assert e.value.status == A.PONNI_ERR_INVALID_MODEL
     P.create_expert_model(P.ExpertMatvec(w), P.ExpertBias(np.zeros((2, 4))), P.Relu(4))
+
+
+def test_overlapping_arrays_are_refused():
+    """An output or work buffer on top of what a call reads, or of another output, by their last and first elements."""
+    L = A.lib()
+    names = ("experts", "weights", "slots", "source", "offsets")
+    E, k, b = 8, 2, 1000
+    size = {n: 4 * k * b for n in names} | {"offsets": 4 * (E + 1), "scores": 4 * E * b,
+                                             "work": L.ponni_route_workspace_bytes(E, k, b)}
+
+    def route(at):
+        r = A.RoutingArrays(E, k, b, *[at[n] for n in names])
+        return L.ponni_route(at["scores"], b, A.F32, 0, ctypes.byref(r), at["work"], size["work"], None)
+
+    apart = {n: FAKE * (i + 1) for i, n in enumerate(size)}
+    for one in size:
+        for other in size:
+            at = dict(apart)
+            at[one] = apart[other] + (size[other] - 1) // 16 * 16
+            if one != other:
+                assert route(at) == A.PONNI_ERR_INVALID_ARGUMENT and b"overlap" in L.ponni_last_error(), (one, other)
+
+    _, e = create([matvec(4, 6), P.Relu(6), matvec(6, 5)], 3, A.F16)
+    read = {"x": 2 * 4 * 8, "weights": 64, "slots": 64, "source": 64, "offsets": 16}
+    need = L.ponni_experts_mixture_workspace_bytes(e, 2, 8)
+    assert need > 0
+
+    def mix(at):
+        r = A.RoutingArrays(3, 2, 8, 0, at["weights"], at["slots"], at["source"], at["offsets"])
+        return L.ponni_experts_forward_mixture(e, at["x"], 8, ctypes.byref(r), at["y"], 8, at["work"], need, None)
+
+    apart = {n: FAKE * (i + 1) for i, n in enumerate([*read, "y", "work"])}
+    assert mix(apart) == A.PONNI_ERR_INVALID_ARGUMENT and b"never set" in L.ponni_last_error()
+    for n, bytes_ in [*read.items(), ("y", 80)]:
+        for written in ("y", "work"):
+            if n != written:
+                at = dict(apart)
+                at[written] = apart[n] + (bytes_ - 1) // 16 * 16
+                assert mix(at) == A.PONNI_ERR_INVALID_ARGUMENT and b"overlap" in L.ponni_last_error(), (n, written)
+    need = L.ponni_experts_workspace_bytes(e, 8)
+    for y, work in ((FAKE, 3 * FAKE), (2 * FAKE, FAKE)):
+        status = L.ponni_experts_forward(e, 4 * FAKE, 8, FAKE, y, 8, 8, work, need, None)
+        assert status == A.PONNI_ERR_INVALID_ARGUMENT and b"overlap" in L.ponni_last_error()
+    L.ponni_experts_destroy(e)
