@@ -175,7 +175,7 @@ __global__ __launch_bounds__(64 * W, W == 4 && (OP == OPERAND_F16 || OP == OPERA
 template <Operand OP, class S, OutputKind KIND, bool FEATURES, int C, int W>
 hipError_t launch_chain_sized(ChainArgs const& a, hipStream_t stream) {
   int64_t const tiles = grid_of(a.io, C, 1), bytes = chain_lds(OP, a.state_bytes, C);
-  if (tiles > INT32_MAX) return hipErrorInvalidValue;
+  if (!launchable(tiles, 64 * W)) return hipErrorInvalidConfiguration;
   auto const kernel = contract_chain<OP, S, KIND, FEATURES, C, W>;
   if (bytes > 65536) {
     hipError_t const e = hipFuncSetAttribute(reinterpret_cast<void const*>(kernel),

@@ -13,7 +13,8 @@ namespace ponni_hip {
 namespace {
 
 constexpr int32_t kMaxWidth = 65536;
-// (PONNI_MAX_COLUMNS: a launch has at most 2^32 threads, and the smallest tiles are 64 columns of 256)
+// (PONNI_MAX_COLUMNS: a launch has fewer than 2^32 threads in a dimension, and where the grid is one of columns alone
+// 64 of them have 256 threads at most: 4.0e9.  The layers' tiles, of output features too, are counted when launched.)
 
 int fail(int status, std::string const& message) { return set_error(status, message); }
 

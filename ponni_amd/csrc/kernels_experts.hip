@@ -315,7 +315,7 @@ template <Operand OP, class S, OutputKind KIND, int MI, int NJ, int WM, int WN>
 hipError_t launch_tiled(ContractArgs const& a, hipStream_t stream) {
   constexpr int BM = 16 * MI * WM, BN = 16 * NJ * WN;
   int64_t const tiles = grid_of(a, BN, (int64_t(a.blocks) * 64 + BM - 1) / BM);
-  if (tiles > INT32_MAX) return hipErrorInvalidValue;
+  if (!launchable(tiles, 64 * WM * WN)) return hipErrorInvalidConfiguration;
   dim3 const grid(static_cast<unsigned>(tiles)), block(64 * WM * WN);
   hipLaunchKernelGGL((contract<OP, S, KIND, MI, NJ, WM, WN>), grid, block, 0, stream, a);
   return hipGetLastError();
@@ -333,7 +333,7 @@ hipError_t launch_thin(ContractArgs const& a, hipStream_t stream) {
   constexpr int W = 8;
   auto launch = [&]<int MT>(std::integral_constant<int, MT>) {
     int64_t const tiles = grid_of(a, 16 * NJ, int64_t(a.blocks) * (4 / MT));
-    if (tiles > INT32_MAX) return hipErrorInvalidValue;
+    if (!launchable(tiles, 64 * W)) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((contract_thin<OP, S, KIND, FEATURES, MT, NJ, W>), dim3(static_cast<unsigned>(tiles)),
                        dim3(64 * W), 0, stream, a);
     return hipGetLastError();
@@ -411,15 +411,14 @@ __global__ __launch_bounds__(256) void combine(Rows rows, int64_t num_rows, ponn
   for (int f = threadIdx.x >> 6; f < 64 && f0 + f < features; f += 4) y[(f0 + f) * ld + b0 + s] = S(tile[f][s]);
 }
 
-// One lane per 16-byte piece of the packed weights.
+// One lane per 16-byte piece of the packed weights; the grid's second dimension is the experts.
 template <Operand OP, class T>
-__global__ __launch_bounds__(256) void pack_weights(T const* __restrict__ w, int64_t experts, int64_t n_in,
-                                                    int64_t n_out, int64_t blocks, int64_t steps, char* weights,
+__global__ __launch_bounds__(256) void pack_weights(T const* __restrict__ w, int64_t n_in, int64_t n_out,
+                                                    int64_t blocks, int64_t steps, char* weights,
                                                     unsigned char* scales) {
-  int64_t const piece = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (piece >= experts * blocks * steps * 256) return;
-  int const lane = piece % 64, i = piece / 64 % 4, g = lane >> 4, row = lane & 15;
-  int64_t const step = piece / 256 % steps, block = piece / 256 / steps % blocks, e = piece / 256 / steps / blocks;
+  int const lane = threadIdx.x % 64, i = threadIdx.x / 64, g = lane >> 4, row = lane & 15;
+  int64_t const step = blockIdx.x % steps, block = blockIdx.x / steps, e = blockIdx.y;
+  int64_t const piece = ((e * blocks + block) * steps + step) * 256 + threadIdx.x;
   int64_t const f = block * 64 + 16 * (row >> 2) + 4 * i + (row & 3);
   constexpr int N = OP == OPERAND_F32 ? 4 : OP == OPERAND_MX4 ? 32 : 8;
   int64_t const k0 = step * 4 * N + g * N;
@@ -454,11 +453,10 @@ __global__ __launch_bounds__(256) void pack_weights(T const* __restrict__ w, int
 }
 
 template <class T>
-__global__ __launch_bounds__(256) void pack_bias(T const* __restrict__ b, int64_t experts, int64_t n, int64_t padded,
+__global__ __launch_bounds__(256) void pack_bias(T const* __restrict__ b, int64_t n, int64_t padded,
                                                  float* __restrict__ bias) {
-  int64_t const i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= experts * padded) return;
-  bias[i] = i % padded < n ? float(b[i / padded * n + i % padded]) : 0.0f;
+  int64_t const i = int64_t(blockIdx.x) * 256 + threadIdx.x, e = blockIdx.y;
+  if (i < padded) bias[e * padded + i] = i < n ? float(b[e * n + i]) : 0.0f;
 }
 
 template <class F> bool with_parameter_dtype(int dtype, F&& f) {
@@ -529,13 +527,13 @@ hipError_t launch_combine(int dtype, Rows const& rows, int64_t num_rows, const p
 
 hipError_t launch_pack_weights(Operand op, int dtype, const void* w, int64_t experts, int64_t n_in, int64_t n_out,
                                int64_t blocks, char* weights, unsigned char* scales, hipStream_t stream) {
-  int64_t const steps = contraction_steps(op, n_in), groups = experts * blocks * steps;
-  if (groups > INT32_MAX) return hipErrorInvalidValue;
-  dim3 const grid(static_cast<unsigned>(groups)), block(256);
+  int64_t const steps = contraction_steps(op, n_in);
+  // (65536 features at most: 2^22 workgroups an expert)
+  dim3 const grid(static_cast<unsigned>(blocks * steps), static_cast<unsigned>(experts)), block(256);
   with_parameter_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, grid, block, 0, stream, static_cast<T const*>(w), experts, n_in, n_out, blocks, steps,
+      hipLaunchKernelGGL(kernel, grid, block, 0, stream, static_cast<T const*>(w), n_in, n_out, blocks, steps,
                          weights, scales);
     };
     switch (op) {
@@ -550,12 +548,10 @@ hipError_t launch_pack_weights(Operand op, int dtype, const void* w, int64_t exp
 
 hipError_t launch_pack_bias(int dtype, const void* b, int64_t experts, int64_t n, int64_t padded, float* bias,
                             hipStream_t stream) {
-  int64_t const blocks = (experts * padded + 255) / 256;
-  if (blocks > INT32_MAX) return hipErrorInvalidValue;
+  dim3 const grid(static_cast<unsigned>((padded + 255) / 256), static_cast<unsigned>(experts));
   with_parameter_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    hipLaunchKernelGGL(pack_bias<T>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
-                       static_cast<T const*>(b), experts, n, padded, bias);
+    hipLaunchKernelGGL(pack_bias<T>, grid, dim3(256), 0, stream, static_cast<T const*>(b), n, padded, bias);
   });
   return hipGetLastError();
 }

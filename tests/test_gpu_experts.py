@@ -722,3 +722,24 @@ def test_new_parameters_wait_for_calls_in_flight(cuda, on_device):
     torch.cuda.synchronize()
     assert torch.equal(got, want)
     assert not torch.equal(model.forward_batch_parallel(x, offsets), want)
+
+
+def test_parameters_beyond_a_launch_of_one_dimension(cuda):
+    """More than 2^32 threads' worth of packed pieces: 1024 experts of 4096-4100."""
+    import torch
+
+    if torch.cuda.mem_get_info(cuda)[0] < 120 << 30:
+        pytest.skip("needs 120 GiB of GPU memory")
+    E, K, n = 1024, 4096, 4100
+    w = torch.zeros((E, K, n), dtype=torch.float16, device=cuda)
+    w[0, 0, 0], w[511, 17, 4099], w[E - 1, K - 1, n - 1] = 1.0, 2.0, 3.0
+    model = P.create_expert_model(P.ExpertMatvec(w), dtype="f32")
+    del w
+    torch.cuda.empty_cache()
+    x = torch.ones((K, 3), device=cuda)
+    offsets = torch.zeros(E + 1, dtype=torch.int32, device=cuda)
+    offsets[1:], offsets[512:], offsets[E:] = 1, 2, 3
+    y = model.forward_batch_parallel(x, offsets)
+    want = torch.zeros_like(y)
+    want[0, 0], want[4099, 1], want[n - 1, 2] = 1.0, 2.0, 3.0
+    assert torch.equal(y, want)
