@@ -557,7 +557,7 @@ typedef struct ponni_routing {
 #define PONNI_ROUTE_ALL 1
 int ponni_route(const void* scores, int64_t ld, int32_t dtype, int32_t normalize, const ponni_routing* routing,
                 void* workspace, int64_t workspace_bytes, hipStream_t stream);
-/* (-1 for sizes that ponni_route refuses) */
+/* Enough for `batch` samples and for any fewer (-1 for sizes that ponni_route refuses). */
 int64_t ponni_route_workspace_bytes(int32_t num_experts, int32_t top_k, int64_t batch);
 
 /* Microscaled 4-bit rows (the OCP MXFP4 format): 32 consecutive features of a
@@ -628,6 +628,7 @@ int ponni_experts_forward(ponni_experts experts, const void* x, int64_t ld_in, c
 int ponni_experts_forward_mx4(ponni_experts experts, const void* codes, const void* scales, const int32_t* offsets,
                               void* y, int64_t ld_out, int64_t columns, void* workspace, int64_t workspace_bytes,
                               hipStream_t stream);
+/* Enough for both with `columns` columns, and with any fewer (-1 for sizes that they refuse). */
 int64_t ponni_experts_workspace_bytes(ponni_experts experts, int64_t columns);
 
 /* y[:, b] = sum over j, in that order, of weights[j, b] * chain of expert experts[j, b] at x[:, b],
@@ -638,6 +639,7 @@ int64_t ponni_experts_workspace_bytes(ponni_experts experts, int64_t columns);
 int ponni_experts_forward_mixture(ponni_experts experts, const void* x, int64_t ld_in, const ponni_routing* routing,
                                   void* y, int64_t ld_out, void* workspace, int64_t workspace_bytes,
                                   hipStream_t stream);
+/* Enough for `batch` samples with top_k experts, and for any fewer samples. */
 int64_t ponni_experts_mixture_workspace_bytes(ponni_experts experts, int32_t top_k, int64_t batch);
 
 /* --- synthetic data (bench and tests) ------------------------------------- */

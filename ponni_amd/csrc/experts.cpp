@@ -117,6 +117,22 @@ Workspace workspace_of(ponni_experts_s const& e, int64_t rows, int64_t columns, 
   return w;
 }
 
+// Bytes that any number of columns up to `columns` needs, top_k of them a sample in a mixture (0: none).
+// Where the kernels for few columns end, one kernel may take the whole chain and need fewer; on
+// either side of that the bytes grow with the columns.
+int64_t workspace_bytes_up_to(ponni_experts_s const& e, int32_t top_k, int64_t batch) {
+  int64_t const per = std::max(top_k, 1);
+  int32_t blocks = 0;
+  for (auto const& l : e.layers) blocks = std::max(blocks, l.blocks);
+  auto need = [&](int64_t b) { return b < 1 ? 0 : workspace_of(e, b, b * per, top_k > 0).total; };
+  int64_t few = 0, more = batch + 1;  // the last batch of few columns, the first of more
+  while (few + 1 < more) {
+    int64_t const b = few + (more - few) / 2;
+    (takes_features(b * per, e.num_experts, blocks) ? few : more) = b;
+  }
+  return std::max(need(batch), need(few));
+}
+
 int check_ready(ponni_experts_s const& e) {
   for (size_t i = 0; i < e.layers.size(); i++)
     if (!e.layers[i].weights_set)
@@ -487,7 +503,7 @@ int64_t ponni_route_workspace_bytes(int32_t num_experts, int32_t top_k, int64_t 
   int64_t n = -1;
   (void)guarded([&] {
     int const st = check_routing_sizes(num_experts, top_k, batch);
-    if (st == PONNI_OK) n = route_workspace_bytes(num_experts, batch);
+    if (st == PONNI_OK) n = route_workspace_bytes_up_to(num_experts, batch);
     return st;
   });
   return n;
@@ -599,7 +615,7 @@ int64_t ponni_experts_workspace_bytes(ponni_experts e, int64_t columns) {
     if (e == nullptr) return fail(PONNI_ERR_INVALID_ARGUMENT, "experts is null");
     if (columns <= 0 || columns > PONNI_MAX_COLUMNS)
       return fail(PONNI_ERR_SHAPE, "columns must be 1 to " + std::to_string(PONNI_MAX_COLUMNS));
-    n = workspace_of(*e, columns, columns, false).total;
+    n = workspace_bytes_up_to(*e, 0, columns);
     return int(PONNI_OK);
   });
   return n;
@@ -615,7 +631,7 @@ int64_t ponni_experts_mixture_workspace_bytes(ponni_experts e, int32_t top_k, in
   (void)guarded([&] {
     if (e == nullptr) return fail(PONNI_ERR_INVALID_ARGUMENT, "experts is null");
     int const st = check_routing_sizes(e->num_experts, top_k, batch);
-    if (st == PONNI_OK) n = workspace_of(*e, batch, batch * top_k, true).total;
+    if (st == PONNI_OK) n = workspace_bytes_up_to(*e, top_k, batch);
     return st;
   });
   return n;

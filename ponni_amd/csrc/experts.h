@@ -118,6 +118,7 @@ hipError_t launch_mx4_values(Rows const& rows, int64_t features, int64_t columns
 hipError_t launch_route(const void* scores, int64_t ld, int dtype, int normalize, ponni_routing const& r, void* workspace,
                         hipStream_t stream);
 int64_t route_workspace_bytes(int64_t experts, int64_t batch);
+int64_t route_workspace_bytes_up_to(int64_t experts, int64_t batch);  // that any smaller batch needs too
 
 int set_error(int status, std::string const& message);
 

@@ -287,6 +287,11 @@ int64_t route_workspace_bytes(int64_t experts, int64_t batch) {
   return batch <= 256 ? 0 : (blocks_of(batch) + 1) * experts * int64_t(sizeof(int32_t));
 }
 
+int64_t route_workspace_bytes_up_to(int64_t experts, int64_t batch) {
+  // (larger batches have fewer workgroups at first)
+  return std::max(route_workspace_bytes(experts, batch), route_workspace_bytes(experts, std::min(batch, kSharedBatch)));
+}
+
 hipError_t launch_route(const void* scores, int64_t ld, int dtype, int normalize, ponni_routing const& r, void* workspace,
                         hipStream_t stream) {
   auto* counts = static_cast<int32_t*>(workspace);

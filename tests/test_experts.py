@@ -266,3 +266,28 @@ def test_overlapping_arrays_are_refused():
         status = L.ponni_experts_forward(e, 4 * FAKE, 8, FAKE, y, 8, 8, work, need, None)
         assert status == A.PONNI_ERR_INVALID_ARGUMENT and b"overlap" in L.ponni_last_error()
     L.ponni_experts_destroy(e)
+
+
+def test_a_work_buffer_serves_smaller_batches():
+    """The bytes of the largest batch that a program makes are enough for every smaller one."""
+    L = A.lib()
+    counts = sorted({int(round(1.3 ** i)) for i in range(50)} | {16, 17, 32, 33, 256, 257, 8192, 8193, 131072, 131073})
+
+    for E, widths, weights in ((1, (500, 500), 0), (8, (500, 500, 500), 0), (8, (500, 500, 500), 1), (64, (40, 600), 0),
+                               (64, (40, 2048, 30), 0), (4, (700, 900, 100), 1), (300, (16, 16, 16), 0)):
+        _, e = create([matvec(a, b) for a, b in zip(widths, widths[1:])], E, A.BF16, weights)
+        k = min(2, E)
+        sizes, mixture_sizes = ([f(n) for n in counts] for f in (
+            lambda n: L.ponni_experts_workspace_bytes(e, n), lambda n: L.ponni_experts_mixture_workspace_bytes(e, k, n)))
+        assert sizes == sorted(sizes) and mixture_sizes == sorted(mixture_sizes)
+        for i, n in enumerate(counts):  # the size as this batch's, and as a larger one's
+            for size, mixture_size in ((sizes[i], mixture_sizes[i]), (sizes[-1], mixture_sizes[-1])):
+                assert L.ponni_experts_forward(e, FAKE, n, 2 * FAKE, 3 * FAKE, n, n, 4 * FAKE, size, None) == \
+                    A.PONNI_ERR_INVALID_ARGUMENT and b"never set" in L.ponni_last_error(), (E, widths, n, size)
+                r = A.RoutingArrays(E, k, n, 0, 5 * FAKE, 6 * FAKE, 7 * FAKE, 8 * FAKE)
+                assert L.ponni_experts_forward_mixture(e, FAKE, n, ctypes.byref(r), 3 * FAKE, n, 4 * FAKE, mixture_size,
+                                                       None) == A.PONNI_ERR_INVALID_ARGUMENT
+                assert b"never set" in L.ponni_last_error(), (E, widths, n, mixture_size)
+        L.ponni_experts_destroy(e)
+    sizes = [L.ponni_route_workspace_bytes(64, 2, n) for n in counts]
+    assert sizes == sorted(sizes)
