@@ -256,7 +256,7 @@ inline int64_t grid_of(ContractArgs const& a, int64_t width, int64_t out_blocks)
   // (a share per XCD is rounded up: the grid is whole rounds of the eight)
   return ((a.columns / width + partial) * out_blocks + 7) / 8 * 8;
 }
-// A launch's threads are counted in 32 bits.
+// A launch's threads are counted in 32 bits: a grid of more is cut off, without an error.
 inline bool launchable(int64_t workgroups, int threads) { return workgroups <= int64_t(UINT32_MAX) / threads; }
 
 }  // namespace

@@ -411,6 +411,18 @@ __global__ __launch_bounds__(256) void combine(Rows rows, int64_t num_rows, ponn
   for (int f = threadIdx.x >> 6; f < 64 && f0 + f < features; f += 4) y[(f0 + f) * ld + b0 + s] = S(tile[f][s]);
 }
 
+// A parameter on its way to a type of at most 16 bits.  fp64 is rounded to odd (cut off, the last bit set
+// where something was lost), so that the rounding that follows sees which side of a middle it lay on.
+template <Operand OP, class T> __device__ inline float parameter(T v) {
+  float const f = float(v);
+  if constexpr (std::is_same_v<T, double> && OP != OPERAND_F32) {
+    unsigned const bits = __builtin_bit_cast(unsigned, f);
+    if (double(f) != v && !(bits & 1u) && __builtin_fabsf(f) < __builtin_inff())
+      return __builtin_bit_cast(float, __builtin_fabs(double(f)) < __builtin_fabs(v) ? bits + 1 : bits - 1);
+  }
+  return f;
+}
+
 // One lane per 16-byte piece of the packed weights; the grid's second dimension is the experts.
 template <Operand OP, class T>
 __global__ __launch_bounds__(256) void pack_weights(T const* __restrict__ w, int64_t n_in, int64_t n_out,
@@ -424,7 +436,7 @@ __global__ __launch_bounds__(256) void pack_weights(T const* __restrict__ w, int
   int64_t const k0 = step * 4 * N + g * N;
   float v[N];
 #pragma unroll
-  for (int k = 0; k < N; k++) v[k] = f < n_out && k0 + k < n_in ? float(w[(e * n_in + k0 + k) * n_out + f]) : 0.0f;
+  for (int k = 0; k < N; k++) v[k] = f < n_out && k0 + k < n_in ? parameter<OP>(w[(e * n_in + k0 + k) * n_out + f]) : 0.0f;
   i32x4 out = {0, 0, 0, 0};
   if constexpr (OP == OPERAND_MX4) {
     float amax = 0.0f;

@@ -743,3 +743,26 @@ def test_parameters_beyond_a_launch_of_one_dimension(cuda):
     want = torch.zeros_like(y)
     want[0, 0], want[4099, 1], want[n - 1, 2] = 1.0, 2.0, 3.0
     assert torch.equal(y, want)
+
+
+@pytest.mark.parametrize("on_device", [False, True])
+@pytest.mark.parametrize("dtype,weights", [("f16", "same"), ("bf16", "same"), ("f16", "mx4"), ("f32", "same")])
+def test_fp64_weights_are_rounded_once(cuda, dtype, weights, on_device):
+    """fp64 weights next to the middle of two values of the operands' type, by less than fp32 resolves."""
+    import torch
+
+    # (4 bits: a scale of one from the first row, and values about 1.25)
+    half, base = (0.25, 1.0) if weights == "mx4" else (N.EPS[dtype], 1.0)
+    tiny = 2.0 ** -52
+    w = np.zeros((1, 2, 6))
+    w[0, 0] = 4.0
+    w[0, 1] = [base + half - tiny, base + half, base + half + tiny, base - half / 2, -(base + half + tiny), 0.0]
+    step = 2 * half
+    want = np.array([base, base, base + step, base, -(base + step), 0.0])
+    v = torch.from_numpy(w)
+    model = P.create_expert_model(P.ExpertMatvec(v.to(cuda) if on_device else v), dtype=dtype, weights=weights)
+    x = tensor(np.array([[0.0], [1.0]]), dtype, cuda)
+    assert np.array_equal(host(model.forward_batch_parallel(x))[:, 0], want)
+    if weights == "mx4":  # out of fp32's range: a block of NaN
+        model.set_layer_params(0, w * 1e300)
+        assert np.isnan(host(model.forward_batch_parallel(x))).all()
