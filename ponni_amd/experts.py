@@ -284,6 +284,7 @@ class ExpertInference:
         self.dtype, self.weights = dtype, weights
         self.n_in, self.n_out = layers[0].n_in, layers[-1].n_out
         descs = (A.LayerDesc * len(layers))(*[l.desc() for l in layers])
+        self._shapes = {i: tuple(l.values.shape) for i, l in enumerate(layers) if getattr(l, "values", None) is not None}
         self._experts = ctypes.c_void_p()
         A.check(A.lib().ponni_experts_create(descs, len(layers), self.num_experts, _DTYPES[dtype],
                                              A.WEIGHTS_MX4 if weights == "mx4" else A.WEIGHTS_SAME,
@@ -309,10 +310,14 @@ class ExpertInference:
             self._experts = None
 
     def set_layer_params(self, i: int, values) -> None:
-        """All experts' parameters of layer i (numpy or torch, host or any GPU).  Waits for
-        the device: calls made before, on any stream, read the old ones."""
+        """All experts' parameters of layer i (numpy or torch, host or any GPU), in the
+        layer's shape or as one dimension.  Waits for the device: calls made before, on
+        any stream, read the old ones."""
         import torch
 
+        shape = tuple(values.shape if hasattr(values, "shape") else np.shape(values))
+        if len(shape) > 1 and shape != self._shapes.get(i, shape):
+            raise ValueError(f"layer {i} holds parameters of shape {self._shapes[i]}, got {shape}")
         if hasattr(values, "data_ptr"):
             v = values.detach()
             if v.is_cuda and v.get_device() != self.device:

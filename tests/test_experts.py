@@ -291,3 +291,11 @@ def test_a_work_buffer_serves_smaller_batches():
         L.ponni_experts_destroy(e)
     sizes = [L.ponni_route_workspace_bytes(64, 2, n) for n in counts]
     assert sizes == sorted(sizes)
+
+
+def test_new_parameters_of_another_shape_are_refused():
+    """As many numbers in another order would be taken for weights of the layer's shape."""
+    model = P.create_expert_model(P.ExpertMatvec(np.zeros((2, 3, 4))), P.ExpertBias(np.zeros((2, 4))))
+    for i, shape in ((0, (2, 4, 3)), (0, (4, 3, 2)), (0, (6, 4)), (1, (4, 2)), (1, (2, 2, 2))):
+        with pytest.raises(ValueError):
+            model.set_layer_params(i, np.zeros(shape))

@@ -766,3 +766,17 @@ def test_fp64_weights_are_rounded_once(cuda, dtype, weights, on_device):
     if weights == "mx4":  # out of fp32's range: a block of NaN
         model.set_layer_params(0, w * 1e300)
         assert np.isnan(host(model.forward_batch_parallel(x))).all()
+
+
+def test_new_parameters_in_one_dimension(cuda):
+    r = np.random.default_rng(7)
+    w, b = r.standard_normal((3, 20, 30)), r.standard_normal((3, 30))
+    x = tensor(r.standard_normal((20, 9)), "f32", cuda)
+    import torch
+
+    offsets = torch.tensor([0, 2, 5, 9], dtype=torch.int32, device=cuda)
+    want = P.create_expert_model(P.ExpertMatvec(w), P.ExpertBias(b)).forward_batch_parallel(x, offsets)
+    model = P.create_expert_model(P.ExpertMatvec(np.zeros_like(w)), P.ExpertBias(np.zeros_like(b)))
+    model.set_layer_params(0, w.reshape(-1))
+    model.set_layer_params(1, torch.from_numpy(b).to(cuda).reshape(-1))
+    assert torch.equal(model.forward_batch_parallel(x, offsets), want)
