@@ -780,3 +780,49 @@ def test_new_parameters_in_one_dimension(cuda):
     model.set_layer_params(0, w.reshape(-1))
     model.set_layer_params(1, torch.from_numpy(b).to(cuda).reshape(-1))
     assert torch.equal(model.forward_batch_parallel(x, offsets), want)
+
+
+# Kernels that the shapes above leave out.
+VARIANTS = [
+    # experts, widths, activations, columns
+    (64, (40, 1024), ("none",), 128),  # few columns, whole blocks of features: read in place
+    (64, (40, 1024, 1030), ("tanh", "none"), 128),  # and rows between the layers
+    (16, (300, 200, 130), ("silu", "none"), 400),  # few columns, tiles of 32 of them
+    (40, (300, 900, 500), ("relu", "none"), 1000),  # both
+]
+
+
+@pytest.mark.parametrize("dtype,weights", [("f32", "same"), ("f16", "same"), ("bf16", "same"), ("f16", "mx4"),
+                                           ("bf16", "mx4")])
+@pytest.mark.parametrize("E,widths,acts,C", VARIANTS)
+def test_grouped_few_columns(cuda, E, widths, acts, C, dtype, weights):
+    test_grouped_columns(cuda, E, widths, acts, C, dtype, weights)
+
+
+@pytest.mark.parametrize("dtype,weights", [("f32", "same"), ("f16", "same"), ("bf16", "same"), ("f16", "mx4"),
+                                           ("bf16", "mx4")])
+@pytest.mark.parametrize("E,k,widths,acts,B", [(64, 2, (40, 1024, 1030), ("tanh", "none"), 64),
+                                               (40, 2, (300, 900, 500), ("relu", "none"), 500),
+                                               (16, 2, (300, 200, 130), ("silu", "none"), 200)])
+def test_mixture_of_few_columns(cuda, E, k, widths, acts, B, dtype, weights):
+    import torch
+
+    print(f"mixture: E={E} k={k} {widths} B={B} {dtype} {weights}", flush=True)
+    r = np.random.default_rng(B)
+    model, params = networks(r, E, widths, acts, dtype, weights)
+    g = torch.Generator(cuda).manual_seed(B)
+    routing = P.route_experts(torch.randn((E, B), device=cuda, generator=g), k)
+    x = torch.randn((widths[0], B), device=cuda, generator=g).to(torch_dtype(dtype))
+    check_mixture(model, params, x, routing, model.forward_mixture(x, routing), dtype, weights,
+                  torch.arange(B, device=cuda))
+
+
+@pytest.mark.parametrize("E,widths,acts,C,types", [
+    (3, (330, 1100, 1030), ("relu", "none"), 70_001, ("bf16", "same")),  # 256 x 256 tiles, rows between the layers
+    (3, (330, 1100, 1030), ("relu", "none"), 70_001, ("f16", "same")),
+    (3, (130, 1100, 1030), ("silu", "none"), 70_001, ("f32", "same")),
+    (3, (700, 1100, 1030), ("silu", "none"), 70_001, ("f16", "mx4")),  # and 4-bit ones
+    (3, (700, 1100, 1030), ("silu", "none"), 70_001, ("bf16", "mx4")),
+])
+def test_grouped_columns_large_states(cuda, E, widths, acts, C, types):
+    test_grouped_columns_large(cuda, E, widths, acts, C, types)
