@@ -134,7 +134,7 @@ struct ponni_experts_s {
     char* weights = nullptr;
     unsigned char* scales = nullptr;
     float* d_bias = nullptr;
-    bool weights_set = false, bias_set = false;
+    bool weights_set = false;
   };
   std::vector<ponni_layer_desc> descs;
   std::vector<Layer> layers;

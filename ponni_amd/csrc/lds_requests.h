@@ -19,9 +19,6 @@ __device__ inline void dma16(void const* g, unsigned lds) {
 __device__ inline void dma16(void const* base, unsigned offset, unsigned lds) {
   asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "{m0}"(lds) : "memory");
 }
-__device__ inline void dma4(void const* base, unsigned offset, unsigned lds) {
-  asm volatile("s_nop 4\n\tglobal_load_lds_dword %0, %1" ::"v"(offset), "s"(base), "{m0}"(lds) : "memory");
-}
 __device__ inline void dma4(void const* g, unsigned lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "{m0}"(lds) : "memory");
 }
