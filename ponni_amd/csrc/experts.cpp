@@ -93,7 +93,7 @@ Workspace workspace_of(ponni_experts_s const& e, int64_t rows, int64_t columns, 
   Workspace w;
   ChainArgs chain;
   bool const whole = chain_of(e, columns, chain) > 0;
-  bool const direct = whole ? !mixture : takes_features(columns, e.num_experts, e.layers[0].blocks);
+  bool const direct = whole ? !mixture : takes_features(e.operand, columns, e.num_experts, e.layers[0].blocks);
   if (direct) rows = 0;
   auto take = [&](int64_t n) {
     int64_t const at = w.total;
@@ -128,7 +128,7 @@ int64_t workspace_bytes_up_to(ponni_experts_s const& e, int32_t top_k, int64_t b
   int64_t few = 0, more = batch + 1;  // the last batch of few columns, the first of more
   while (few + 1 < more) {
     int64_t const b = few + (more - few) / 2;
-    (takes_features(b * per, e.num_experts, blocks) ? few : more) = b;
+    (takes_features(e.operand, b * per, e.num_experts, blocks) ? few : more) = b;
   }
   return std::max(need(batch), need(few));
 }
@@ -176,7 +176,7 @@ int run_layers(ponni_experts_s const& e, void const* x, int64_t ld_in, Rows inpu
   ChainArgs chain;
   int const chain_tile = chain_of(e, columns, chain);
   // (rows are the caller's 4-bit ones, or made here where the first kernel does not read x itself)
-  bool const direct = chain_tile > 0 ? y != nullptr : takes_features(columns, e.num_experts, e.layers[0].blocks);
+  bool const direct = chain_tile > 0 ? y != nullptr : takes_features(e.operand, columns, e.num_experts, e.layers[0].blocks);
   if (x != nullptr && !direct) {
     input.data = base + w.input;
     input.scales = reinterpret_cast<unsigned char*>(base + w.input_scales);

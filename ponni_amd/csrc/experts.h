@@ -98,7 +98,7 @@ hipError_t launch_chain_mx4_bf16(OutputKind kind, int columns, ChainArgs const& 
 hipError_t launch_chain(Operand op, int out_type, OutputKind kind, int columns, ChainArgs const& a, hipStream_t stream);
 
 // Whether a layer of these sizes reads its input as [features, columns] itself.
-bool takes_features(int64_t columns, int32_t experts, int32_t blocks);
+bool takes_features(Operand op, int64_t columns, int32_t experts, int32_t blocks);
 hipError_t launch_contraction(Operand op, int out_type, OutputKind kind, ContractArgs const& a, hipStream_t stream);
 
 // x [features, columns] of `dtype` as rows of `op`, `row_bytes` a row.

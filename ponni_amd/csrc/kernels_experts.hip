@@ -321,10 +321,20 @@ hipError_t launch_tiled(ContractArgs const& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Columns of a thin tile, 0 where the other kernels' tiles serve better.
-inline int thin_columns(int64_t columns, int32_t experts, int32_t blocks) {
+// Columns of a thin tile, 0 where the other kernels' tiles serve better: with more than 32 columns per expert,
+// or more tiles than read their weights, and quantise their input, at the pace of the others' MFMAs.  Times in
+// us, thin / 128 x 128 tiles: 16 bits, 2048-2048: 8 experts, 32 columns 17 / 29, 256 columns 22 / 31, 512
+// columns 29 / 32; 64 experts, 128 columns 90 / 102, 512 columns 125 / 119; 1024-4096, 16 experts, 256 columns
+// 33 / 28. 4 bits, 2048-2048, 8 experts: 32 columns 9.7 / 16, 128 columns 13 to 17 / 16, 256 columns 24 / 16;
+// 1024-4096, 16 experts, 64 columns 23 / 16, 512 columns 49 / 17. fp32, whose tiles take as long half empty as
+// full, 2048-2048: 64 experts, 128 columns 171 / 482, 2048 columns 378 / 498. (One expert alone is also faster
+// in thin tiles above 32 columns: 16 bits 2048-2048, 64 columns 9 / 28, 512 columns 19 / 32, 1024 columns 33 /
+// 34; fp32 64 columns 14 / 137.  That is not used.)
+inline int thin_columns(Operand op, int64_t columns, int32_t experts, int32_t blocks) {
   int64_t const groups = experts < columns ? experts : columns;
-  if (columns > 32 * groups || (columns / 128 + groups) * ((blocks + 1) / 2) >= 1024) return 0;
+  if (columns > 32 * groups) return 0;
+  if (op == OPERAND_MX4 && (columns / 32 + groups) * blocks > 320) return 0;
+  if ((op == OPERAND_F16 || op == OPERAND_BF16) && (columns / 128 + groups) * ((blocks + 1) / 2) >= 1024) return 0;
   return columns <= 16 * groups ? 16 : 32;
 }
 
@@ -338,9 +348,13 @@ hipError_t launch_thin(ContractArgs const& a, hipStream_t stream) {
                        dim3(64 * W), 0, stream, a);
     return hipGetLastError();
   };
-  // Tiles of 16 features where those of 64 leave CUs without one (a 4-bit output's blocks need 64).
+  // Tiles of 16 features where those of 64 leave CUs without one (a 4-bit output's blocks need 64); fewer of
+  // them with 16 and 4 bits, where four read the same input as one.  Times in us, 16 / 64 features, 8 columns:
+  // 16 bits 2048-2048 7.8 / 9.4 (32 tiles of 64), of 4 experts 10.2 / 9.5 (128), 512-512 of 8, 64 columns 5.3 /
+  // 5.8 (96); 4 bits 8.5 / 9.3, 11.6 / 9.3, 5.9 / 6.5; fp32 10.5 / 19.6, 17.7 / 21.0, 8 experts 17.8 / 22.2
+  // (256), 32 columns 30.8 / 26.8 (288).
   if constexpr (KIND != OUT_MX4) {
-    if (grid_of(a, 16 * NJ, a.blocks) <= 256) return launch(std::integral_constant<int, 1>{});
+    if (grid_of(a, 16 * NJ, a.blocks) <= (OP == OPERAND_F32 ? 256 : 96)) return launch(std::integral_constant<int, 1>{});
   }
   return launch(std::integral_constant<int, 4>{});
 }
@@ -348,17 +362,21 @@ hipError_t launch_thin(ContractArgs const& a, hipStream_t stream) {
 template <Operand OP, class S, OutputKind KIND>
 hipError_t launch_sized(ContractArgs const& a, hipStream_t stream) {
   bool const features = a.features != nullptr;
-  switch (thin_columns(a.columns, a.experts, a.blocks)) {
+  switch (thin_columns(OP, a.columns, a.experts, a.blocks)) {
     case 16: return features ? launch_thin<OP, S, KIND, true, 1>(a, stream) : launch_thin<OP, S, KIND, false, 1>(a, stream);
     case 32: return features ? launch_thin<OP, S, KIND, true, 2>(a, stream) : launch_thin<OP, S, KIND, false, 2>(a, stream);
     default: break;
   }
   if (features) return hipErrorInvalidValue;  // (takes_features)
-  // 256 x 256 tiles, which read half as much from L2 per multiply-add, where two
-  // rounds of the 256 CUs have one each; else 128 x 128.  bf16 1024-1024, 16 experts,
-  // 65,536 columns: 195 us against 241.
-  int64_t const large = a.columns / 256 * ((a.blocks + 3) / 4);
-  if (a.blocks >= 4 && large >= 512) return launch_tiled<OP, S, KIND, 8, 4, 2, 4>(a, stream);
+  // 256 x 256 tiles, which read half as much from L2 per multiply-add, where two rounds of the 256 CUs have one
+  // each; else 128 x 128, and always in fp32, whose MFMAs take so long that two workgroups a CU matter more.
+  // Times in us, 256 / 128: bf16 1024-1024, 65,536 columns, one expert 207 / 236, 16 226 / 264, 128 253 / 291,
+  // 131,072 columns of 512 657 / 715; 16,384 columns (256 tiles) 53 / 56; 4 bits 113 / 123, 128 / 130, 145 /
+  // 157, 367 / 434; fp32 1122 / 1110, 1356 / 1173, 1378 / 1235.
+  if constexpr (OP != OPERAND_F32) {
+    int64_t const large = a.columns / 256 * ((a.blocks + 3) / 4);
+    if (a.blocks >= 4 && large >= 512) return launch_tiled<OP, S, KIND, 8, 4, 2, 4>(a, stream);
+  }
   return launch_tiled<OP, S, KIND, 4, 4, 2, 2>(a, stream);
 }
 
@@ -485,23 +503,27 @@ int64_t chain_lds(Operand op, int state_bytes, int columns) {
   return int64_t(columns) * (state_bytes + 16) + (op == OPERAND_MX4 ? int64_t(columns) * (state_bytes / 16 + 4) : 0);
 }
 
-// One kernel takes the chain where the states fit LDS and more columns than a thin tile's
-// share an expert's weights.  Against layer by layer (us): fp16 64-256-256-256-64 tanh,
-// 1,000,000 columns 518 / 1117; bf16 512-512-512, 200,000 360 / 435; 100-200-100, 3,000 13 / 20;
-// 4 bits 256-256, 1,000,000 389 / 411.  Not fp32 layers of more than 256
-// features, whose 64 columns a tile read the weights too often (200-300-100, 20,000: 99 / 79), nor
-// few columns (bf16 500-500-500, 100 columns of 8 experts: 22 / 12).
+// One kernel takes the chain where there are more columns than a thin tile's to share an expert's weights,
+// layers have at most 8 blocks of 64 outputs (fp32: 4), and states 2 KB a column (512 fp32 or 1024 16-bit
+// features; 4 bits 1024 features): its tiles of 64 columns read all weights once each.  Against layer by layer
+// (us): fp16 64-256-256-256-64 tanh, 1,000,000 columns 518 / 1117; bf16 512-512-512, 300,000 506 / 613, 5,000
+// 25 / 32; 800-500-500, 40,000 105 / 120; 100-200-100, 3,000 13 / 20; 4 bits 256-256, 1,000,000 389 / 411;
+// 1024-512-512, 300,000 471 / 550; fp32 300-200-17, 40,000 102 / 123.  Wider inputs: bf16 1200-256-64, 40,000
+// 122 / 84, 5,000 33 / 38; 4 bits 2048-256, 5,000 40 / 22 (300,000 483 / 532); 4608-64, 40,000 242 / 127; fp32
+// 600-256, 40,000 188 / 159; 200-300-100 (5 blocks), 20,000 99 / 79.  Few columns: bf16 500-500-500, 100 of 8
+// experts 21 / 11.
 int chain_columns(Operand op, ChainArgs& a) {
   int blocks = 0;
   for (int l = 0; l < a.num_layers; l++) {
     blocks = a.layers[l].blocks > blocks ? a.layers[l].blocks : blocks;
     if (a.layers[l].act == ACT_GELU_ERF) return 0;  // (its code, for every accumulator of every shape of layer)
   }
-  if (blocks > (op == OPERAND_F32 ? 4 : 8) || thin_columns(a.io.columns, a.io.experts, blocks) > 0) return 0;
+  if (blocks > (op == OPERAND_F32 ? 4 : 8) || a.state_bytes > (op == OPERAND_MX4 ? 512 : 2048)) return 0;
+  if (thin_columns(op, a.io.columns, a.io.experts, blocks) > 0) return 0;
   a.waves = blocks > 4 ? 8 : 4;
-  if (blocks > 4 && chain_lds(op, a.state_bytes, 128) <= 160 * 1024 && a.io.columns >= 128 * 512) return 128;
-  return chain_lds(op, a.state_bytes, 64) <= 160 * 1024 ? 64 : 0;
+  return blocks > 4 && chain_lds(op, a.state_bytes, 128) <= 160 * 1024 && a.io.columns >= 128 * 512 ? 128 : 64;
 }
+static_assert(64 * (2048 + 16) <= 160 * 1024, "a tile of 64 columns fits LDS");
 
 hipError_t launch_chain(Operand op, int out_type, OutputKind kind, int columns, ChainArgs const& a, hipStream_t stream) {
   switch (op) {
@@ -514,7 +536,9 @@ hipError_t launch_chain(Operand op, int out_type, OutputKind kind, int columns, 
   }
 }
 
-bool takes_features(int64_t columns, int32_t experts, int32_t blocks) { return thin_columns(columns, experts, blocks) > 0; }
+bool takes_features(Operand op, int64_t columns, int32_t experts, int32_t blocks) {
+  return thin_columns(op, columns, experts, blocks) > 0;
+}
 
 hipError_t launch_contraction(Operand op, int out_type, OutputKind kind, ContractArgs const& a, hipStream_t stream) {
   switch (op) {

@@ -789,6 +789,8 @@ VARIANTS = [
     (64, (40, 1024, 1030), ("tanh", "none"), 128),  # and rows between the layers
     (16, (300, 200, 130), ("silu", "none"), 400),  # few columns, tiles of 32 of them
     (40, (300, 900, 500), ("relu", "none"), 1000),  # both
+    (8, (200, 500, 450), ("gelu", "none"), 100),  # few columns, whole blocks, of every type
+    (3, (1100, 250, 60), ("silu", "none"), 1500),  # more input than one kernel takes for a chain
 ]
 
 
@@ -803,7 +805,8 @@ def test_grouped_few_columns(cuda, E, widths, acts, C, dtype, weights):
                                            ("bf16", "mx4")])
 @pytest.mark.parametrize("E,k,widths,acts,B", [(64, 2, (40, 1024, 1030), ("tanh", "none"), 64),
                                                (40, 2, (300, 900, 500), ("relu", "none"), 500),
-                                               (16, 2, (300, 200, 130), ("silu", "none"), 200)])
+                                               (16, 2, (300, 200, 130), ("silu", "none"), 200),
+                                               (8, 2, (200, 500, 450), ("gelu", "none"), 50)])
 def test_mixture_of_few_columns(cuda, E, k, widths, acts, B, dtype, weights):
     import torch
 
