@@ -177,10 +177,11 @@ __device__ inline void store_features(ContractArgs const& a, int64_t col, int f0
       }
     }
   } else if constexpr (KIND == OUT_FLOATS) {
-    float* row = reinterpret_cast<float*>(a.y_rows.data + col * a.y_rows.stride) + f0 / 64 * 64;
+    int const block = f0 / 64 * 64, groups = float_groups(block, a.row_features);
+    float* row = reinterpret_cast<float*>(a.y_rows.data + col * a.y_rows.stride) + block;
     if (f0 < a.row_features)
 #pragma unroll
-      for (int i = 0; i < 4; i++) *reinterpret_cast<f32x4*>(row + float_place(f0 % 64 / 16, i)) = v[i];
+      for (int i = 0; i < 4; i++) *reinterpret_cast<f32x4*>(row + float_place(f0 % 64 / 16, i, groups)) = v[i];
   } else {
     write_pieces<S>(a.y_rows.data + col * a.y_rows.stride, f0, a.row_features, v);
   }

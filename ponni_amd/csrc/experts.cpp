@@ -87,7 +87,7 @@ int chain_of(ponni_experts_s const& e, int64_t columns, ChainArgs& a) {
 // Rounded to the model's type first, each would add up to half a step of |weight| |output|: more than the
 // sum itself where outputs cancel, and infinite where fp16 ends.  That would halve their way
 // through memory: fp16 512-1024-512, top 4, 65,536 samples, 537 MB each way, takes 940 us for 810.
-int64_t output_row_bytes(ponni_experts_s const& e) { return int64_t(e.layers.back().blocks) * 256; }
+int64_t output_row_bytes(ponni_experts_s const& e) { return round_up(e.layers.back().n_out, 16) * 4; }
 
 Workspace workspace_of(ponni_experts_s const& e, int64_t rows, int64_t columns, bool mixture) {
   Workspace w;
@@ -219,7 +219,7 @@ int run_layers(ponni_experts_s const& e, void const* x, int64_t ld_in, Rows inpu
       a.y_rows.stride = i < last ? int64_t(next) * 64 : output_row_bytes(e);
       a.y_rows.scale_stride = 4;
       a.y_rows.scale_step = columns * 4;
-      a.row_features = i < last ? next * step_features(e.operand) : l.blocks * 64;
+      a.row_features = i < last ? next * step_features(e.operand) : static_cast<int32_t>(output_row_bytes(e) / 4);
     }
     hipError_t err;
     if (chain_tile > 0) {

@@ -17,9 +17,13 @@ namespace ponni_hip {
 enum Operand { OPERAND_F32 = 0, OPERAND_F16 = 1, OPERAND_BF16 = 2, OPERAND_MX4 = 3 };
 constexpr int kMx4Block = 32;  // features that share a scale
 inline int step_features(Operand o) { return o == OPERAND_F32 ? 16 : o == OPERAND_MX4 ? 128 : 32; }
-// Where the four features 16 g + 4 i .. + 3 of a block of 64 lie in an OUT_FLOATS row: behind those of lane groups
-// below g, so that the four groups' pieces i, stored together, are 64 consecutive bytes.
-__host__ __device__ inline int float_place(int g, int i) { return 16 * i + 4 * g; }
+// Where the four features 16 g + 4 i .. + 3 of a block of 64 lie in an OUT_FLOATS row, `groups` (1 to 4) of 16 features
+// in the block: so that what the groups' lanes store together, their pieces i, is consecutive.
+__host__ __device__ inline int float_place(int g, int i, int groups) { return 4 * (i * groups + g); }
+// Groups of 16 features in the block of 64 that begins at `block`, of a row of row_features.
+__host__ __device__ inline int float_groups(int block, int row_features) {
+  return row_features - block < 64 ? (row_features - block) / 16 : 4;
+}
 inline int64_t contraction_steps(Operand o, int64_t features) {
   return (features + step_features(o) - 1) / step_features(o);
 }
@@ -36,7 +40,7 @@ struct Rows {
 };
 
 // [features, columns], or rows: a layer's of the operand's type or of 4 bits for the next one; a
-// mixture's outputs as fp32 of whole blocks of 64 features, in the order of float_place.
+// mixture's outputs as fp32, whole groups of 16 features in the order of float_place.
 enum OutputKind { OUT_FEATURES = 0, OUT_ROWS = 1, OUT_MX4 = 2, OUT_FLOATS = 3 };
 
 // One layer over columns grouped by expert:

@@ -300,7 +300,8 @@ __global__ __launch_bounds__(64 * W) void contract_thin(ContractArgs a) {
     else if (col < t.last) store_features<KIND, S>(a, col, f0, v, a.n_out);
   } else if (col < t.last) {
     using R = std::conditional_t<KIND == OUT_FLOATS, float, S>;
-    int64_t const at = KIND == OUT_FLOATS ? block_here * 64 + float_place(g, tile0) : f0;
+    int const block0 = block_here * 64;
+    int64_t const at = KIND == OUT_FLOATS ? block0 + float_place(g, tile0, float_groups(block0, a.row_features)) : f0;
     R* y = KIND == OUT_FEATURES ? static_cast<R*>(a.y) + at * a.ldy + col
                                 : reinterpret_cast<R*>(a.y_rows.data + col * a.y_rows.stride) + at;
 #pragma unroll
@@ -395,33 +396,38 @@ hipError_t launch_kind(OutputKind kind, ContractArgs const& a, hipStream_t strea
 }
 
 // y[f, b] = sum_j weight_j[b] row(slot_j[b])[f], in the order of j.
-// 64 samples x 64 features: a lane sums 8 features of one sample's rows (two neighbouring
-// pieces, of two lane groups: float_place), the tile turns in LDS.  Bound by bytes: 512 features, top 4,
+// 64 samples x 64 features: a lane sums two neighbouring pieces of four features of one
+// sample's rows (float_place), the tile turns in LDS.  Bound by bytes: 512 features, top 4,
 // 65,536 samples: 130 us for 604 MB, 4.6 TB/s.
 template <class S>
 __global__ __launch_bounds__(256) void combine(Rows rows, int64_t num_rows, ponni_routing r, int64_t features,
                                                S* __restrict__ y, int64_t ld) {
   __shared__ float tile[64][65];  // [feature][sample]
   int64_t const b0 = int64_t(blockIdx.x) * 64, f0 = int64_t(blockIdx.y) * 64;
+  int const groups = float_groups(static_cast<int>(f0), static_cast<int>(rows.stride / 4));
+  int const over = groups == 4 ? 8 : groups == 3 ? 11 : groups == 2 ? 16 : 32;  // n / groups is n * over / 32
   for (int p = threadIdx.x; p < 64 * 8; p += 256) {
-    int const s = p >> 3, q = p & 7, g = 2 * (q & 1), i = q >> 1;
+    int const s = p >> 3, q = 2 * (p & 7);  // pieces q and q + 1 of the block's 4 * groups
     int64_t const b = b0 + s;
     f32x4 sum[2] = {};
+    if (q >= 4 * groups) continue;
     if (b < r.batch)
       for (int j = 0; j < r.top_k; j++) {
         int64_t const slot = r.slots[j * r.batch + b];
         if (slot < 0 || slot >= num_rows) continue;
         float const w = r.weights[j * r.batch + b];
-        f32x4 const* row = reinterpret_cast<f32x4 const*>(rows.data + slot * rows.stride + (f0 + float_place(g, i)) * 4);
+        f32x4 const* row = reinterpret_cast<f32x4 const*>(rows.data + slot * rows.stride + f0 * 4) + q;
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
           for (int e = 0; e < 4; e++) sum[h][e] = fmaf(w, row[h][e], sum[h][e]);
       }
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+    for (int h = 0; h < 2; h++) {
+      int const i = (q + h) * over >> 5, g = q + h - i * groups;
 #pragma unroll
-      for (int e = 0; e < 4; e++) tile[16 * (g + h) + 4 * i + e][s] = sum[h][e];
+      for (int e = 0; e < 4; e++) tile[16 * g + 4 * i + e][s] = sum[h][e];
+    }
   }
   __syncthreads();
   int const s = threadIdx.x & 63;
