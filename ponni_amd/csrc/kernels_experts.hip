@@ -518,6 +518,9 @@ int64_t chain_lds(Operand op, int state_bytes, int columns) {
 // 122 / 84, 5,000 33 / 38; 4 bits 2048-256, 5,000 40 / 22 (300,000 483 / 532); 4608-64, 40,000 242 / 127; fp32
 // 600-256, 40,000 188 / 159; 200-300-100 (5 blocks), 20,000 99 / 79.  Few columns: bf16 500-500-500, 100 of 8
 // experts 21 / 11.
+// Layers of more than 4 blocks take tiles of 128 columns where there are 2048 of them: 64 / 128 columns bf16
+// 512-512-512, 65,536 133 / 137, 500,000 891 / 797; 64-512-64, 65,536 40 / 48, 500,000 233 / 247; 4 bits
+// 512-512-512, 65,536 97 / 109, 500,000 608 / 597; 64-512-64, 65,536 55 / 50, 500,000 322 / 251.
 int chain_columns(Operand op, ChainArgs& a) {
   int blocks = 0;
   for (int l = 0; l < a.num_layers; l++) {
@@ -527,7 +530,7 @@ int chain_columns(Operand op, ChainArgs& a) {
   if (blocks > (op == OPERAND_F32 ? 4 : 8) || a.state_bytes > (op == OPERAND_MX4 ? 512 : 2048)) return 0;
   if (thin_columns(op, a.io.columns, a.io.experts, blocks) > 0) return 0;
   a.waves = blocks > 4 ? 8 : 4;
-  return blocks > 4 && chain_lds(op, a.state_bytes, 128) <= 160 * 1024 && a.io.columns >= 128 * 512 ? 128 : 64;
+  return blocks > 4 && chain_lds(op, a.state_bytes, 128) <= 160 * 1024 && a.io.columns >= 128 * 2048 ? 128 : 64;
 }
 static_assert(64 * (2048 + 16) <= 160 * 1024, "a tile of 64 columns fits LDS");
 

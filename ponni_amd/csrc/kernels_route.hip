@@ -10,7 +10,7 @@
 //
 // Places come from one bit per sample and expert of a workgroup's samples: a
 // group's count is a population count, a sample's rank in it the count of the bits
-// below.  Up to 256 samples are one launch; more are three: choices and counts, the
+// below.  Few samples are one launch; more are three: choices and counts, the
 // counts' sums over the workgroups before, places.  Top 4 of 64 experts,
 // 1,000,003 bf16 samples: 81 us (chosen) and 96 us (all) where the bytes take 34; bound by
 // VALU issue.  8 experts, 96 samples: 5 us, the launch and one pass of dependent steps.
@@ -262,10 +262,16 @@ __global__ __launch_bounds__(SAMPLES) void route_place(ponni_routing r, int32_t 
   }
 }
 
-// Lanes per sample: 16, or 4, for batches that would leave most of the chip without
-// a wave, each lane's loads one after the other.  Top 8 of 512 bf16 scores, 65,000 samples:
-// 59 us with 4 lanes, 85 with one; top 8 of 256 fp32 scores, 16,384: 32 with 4, 37 with 16.
-constexpr int64_t kSixteenLanes = 4096, kSharedBatch = 131072;
+// One launch: up to 64 samples with 16 lanes each, up to 256 with 4 where the experts are few enough for
+// one workgroup.  Times in us, one launch / three: 8 experts, top 2, 16 samples 5.2 / 8.8, 256 samples 5.8 / 9.5; 64 experts,
+// top 4, 256 samples 9.3 / 11.8; 256 experts, top 8, 64 samples 26 / 32, 256 samples 42 / 34; 1000 experts 59 / 38.
+// Three launches: 4 lanes a sample for batches that would leave most of the chip without a wave, each lane's
+// loads one after the other.  Top 8 of 512 bf16 scores, 65,000 samples: 59 us with 4 lanes, 85 with one; with
+// 16 no fewer (256 fp32 scores, 1,000 samples: 30 with 4, 36 with 16; 64 bf16 scores, top 4, 4096: 11.5 and 12.7).
+constexpr int64_t kOneLaunch = 64, kOneLaunchFewExperts = 256, kFewExperts = 128, kSharedBatch = 131072;
+bool one_launch(int64_t experts, int64_t batch) {
+  return batch <= kOneLaunch || (batch <= kOneLaunchFewExperts && experts <= kFewExperts);
+}
 int64_t blocks_of(int64_t batch) { return batch <= kSharedBatch ? (batch + 63) / 64 : (batch + 255) / 256; }
 
 template <class S, int K>
@@ -274,9 +280,8 @@ void choose(S const* scores, int64_t ld, int normalize, ponni_routing const& r, 
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(blocks)), dim3(threads), size_t(r.num_experts) * samples / 8,
                        stream, scores, ld, normalize, r, counts);
   };
-  if (r.batch <= 64) launch(route_choose<S, K, 16, 64, true>, 1, 1024, 64);
-  else if (r.batch <= 256) launch(route_choose<S, K, 4, 256, true>, 1, 1024, 256);
-  else if (r.batch <= kSixteenLanes) launch(route_choose<S, K, 16, 64, false>, blocks_of(r.batch), 1024, 64);
+  if (r.batch <= kOneLaunch) launch(route_choose<S, K, 16, 64, true>, 1, 1024, 64);
+  else if (one_launch(r.num_experts, r.batch)) launch(route_choose<S, K, 4, 256, true>, 1, 1024, 256);
   else if (r.batch <= kSharedBatch) launch(route_choose<S, K, 4, 64, false>, blocks_of(r.batch), 256, 64);
   else launch(route_choose<S, K, 1, 256, false>, blocks_of(r.batch), 256, 256);
 }
@@ -284,7 +289,7 @@ void choose(S const* scores, int64_t ld, int normalize, ponni_routing const& r, 
 }  // namespace
 
 int64_t route_workspace_bytes(int64_t experts, int64_t batch) {
-  return batch <= 256 ? 0 : (blocks_of(batch) + 1) * experts * int64_t(sizeof(int32_t));
+  return one_launch(experts, batch) ? 0 : (blocks_of(batch) + 1) * experts * int64_t(sizeof(int32_t));
 }
 
 int64_t route_workspace_bytes_up_to(int64_t experts, int64_t batch) {
@@ -304,7 +309,7 @@ hipError_t launch_route(const void* scores, int64_t ld, int dtype, int normalize
     else if (r.top_k <= 8) choose<S, 8>(in, ld, normalize, r, counts, stream);
     else choose<S, 16>(in, ld, normalize, r, counts, stream);
   });
-  if (r.batch <= 256) return hipGetLastError();
+  if (one_launch(r.num_experts, r.batch)) return hipGetLastError();
   int const blocks = static_cast<int>(blocks_of(r.batch));
   int32_t* totals = counts + int64_t(blocks) * r.num_experts;
   hipLaunchKernelGGL(route_sums, dim3(r.num_experts), dim3(256), 0, stream, counts, blocks, totals);

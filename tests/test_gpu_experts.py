@@ -829,3 +829,20 @@ def test_mixture_of_few_columns(cuda, E, k, widths, acts, B, dtype, weights):
 ])
 def test_grouped_columns_large_states(cuda, E, widths, acts, C, types):
     test_grouped_columns_large(cuda, E, widths, acts, C, types)
+
+
+# -- borders of the rules that choose kernels --------------------------------------------------
+
+
+@pytest.mark.parametrize("normalize", ["chosen", "all"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("E,k,B", [(128, 8, 64), (128, 8, 65), (128, 16, 256), (129, 8, 64), (129, 8, 65), (1024, 16, 256),
+                                   (64, 4, 4096), (9, 2, 131_072)])
+def test_routing_at_the_borders(cuda, E, k, B, dtype, normalize):
+    test_routing(cuda, E, k, B, dtype, normalize)
+
+
+@pytest.mark.parametrize("types", [("f16", "same"), ("bf16", "same"), ("f16", "mx4"), ("bf16", "mx4")])
+def test_grouped_columns_in_wide_chain_tiles(cuda, types):
+    """Tiles of 128 columns."""
+    test_grouped_columns_large(cuda, 2, (100, 400, 500), ("tanh", "none"), 262_147, types)
