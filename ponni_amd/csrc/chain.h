@@ -14,9 +14,10 @@ namespace {
 // their MFMAs; each serves 16 NJ columns.  The waves are WM x WN, WM the layer's
 // blocks of 64 features, so that a narrow layer gives every wave fewer columns.
 // FEATURES: the input as the caller holds it.
-// Bound by the activations' VALU work beside the MFMAs: fp16 64-256-256-256-64 tanh, 1,000,000
-// columns of 8 experts: 510 us, 0.64 PFLOP/s, MFMA busy 33 % and VALU 73 % of the SIMDs'
-// time, LDS bank conflicts a third of its accesses' cycles, 65 + 125 MB from and to memory.
+// fp16 64-256-256-256-64 tanh, 1,000,000 columns of 8 experts: 511 us, 0.64 PFLOP/s: the
+// activations' VALU work (78 % of the SIMDs' time) and the MFMAs (31 %) follow one another, where a kernel
+// that overlaps them takes 356; LDS bank conflicts a third of its accesses' cycles, 65 + 125 MB
+// from and to memory.
 template <Operand OP, class S, OutputKind KIND, bool FEATURES, int C, int W>
 __global__ __launch_bounds__(64 * W, W == 4 && (OP == OPERAND_F16 || OP == OPERAND_BF16) ? 4 : 2) void contract_chain(ChainArgs chain) {
   constexpr bool MX = OP == OPERAND_MX4;

@@ -330,7 +330,8 @@ hipError_t launch_tiled(ContractArgs const& a, hipStream_t stream) {
 // 1024-4096, 16 experts, 64 columns 23 / 16, 512 columns 49 / 17. fp32, whose tiles take as long half empty as
 // full, 2048-2048: 64 experts, 128 columns 171 / 482, 2048 columns 378 / 498. (One expert alone is also faster
 // in thin tiles above 32 columns: 16 bits 2048-2048, 64 columns 9 / 28, 512 columns 19 / 32, 1024 columns 33 /
-// 34; fp32 64 columns 14 / 137.  That is not used.)
+// 34; fp32 64 columns 14 / 137.  That is not used.)  Tiles of 16 / 32 columns: 16 bits 2048-2048, one expert, 8
+// columns 7.8 / 9.0; 64 experts, 512 columns 126 / 135, 1024 columns 136 / 138, 2048 columns 178 / 159.
 inline int thin_columns(Operand op, int64_t columns, int32_t experts, int32_t blocks) {
   int64_t const groups = experts < columns ? experts : columns;
   if (columns > 32 * groups) return 0;
