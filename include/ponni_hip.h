@@ -642,6 +642,147 @@ int ponni_experts_forward_mixture(ponni_experts experts, const void* x, int64_t 
 /* Enough for `batch` samples with top_k experts, and for any fewer samples. */
 int64_t ponni_experts_mixture_workspace_bytes(ponni_experts experts, int32_t top_k, int64_t batch);
 
+/* Operators between and behind dense layers, with their gradients: blocks of two
+ * projections whose product feeds a third, what stands between such blocks,
+ * and the log probabilities of given classes.  Arrays are device memory of
+ * F32, F16 or BF16 with rows of contiguous columns, read where the caller
+ * holds them: nothing is packed or kept, so a program that trains changes its
+ * parameters in place between two calls.  Sums, statistics and
+ * activations are fp32.  Work buffers are the caller's, at multiples of 16
+ * bytes; calls on different streams and captured graphs need only have buffers
+ * of their own.  Every call is asynchronous on `stream`, can be captured and
+ * gives the same bits every time.  Outputs and the workspace must overlap neither each other nor
+ * what a call reads (column ranges of one array do not overlap). */
+
+/* A gated feed-forward block over columns:
+ *   g = G^T x + g0, u = U^T x + u0, h = act(g) * u, y = D^T h + d0
+ * with h rounded to `dtype`, the type of every array.  act: a pointwise layer of
+ * n_hidden features (RELU, LEAKY_RELU, GELU, SILU, SIGMOID, TANH). */
+typedef struct ponni_gated {
+  int32_t n_in, n_hidden, n_out; /* 1 .. 65536                                     */
+  int32_t dtype;                 /* F32, F16 or BF16                               */
+  ponni_layer_desc act;
+  const void *gate, *up, *down;  /* G, U [n_in, n_hidden], D [n_hidden, n_out]     */
+  int64_t ld_gate, ld_up, ld_down;
+  const void *gate_bias, *up_bias, *down_bias; /* g0, u0 [n_hidden], d0 [n_out]; null: none */
+} ponni_gated;
+/* Most columns, and the largest row stride, of a gated block's arrays. */
+#define PONNI_GATED_MAX_COLUMNS 16777216
+
+/* y [n_out, columns] of x [n_in, columns].  states [3 n_hidden, columns], or null:
+ * g and u, rounded to the type, and h, which the backward pass reads. */
+int ponni_gated_forward(const ponni_gated* block, const void* x, int64_t ld_x, void* y, int64_t ld_y, void* states,
+                        int64_t ld_states, int64_t columns, void* workspace, int64_t workspace_bytes,
+                        hipStream_t stream);
+/* Enough for `columns` columns and for any fewer (-1 for blocks and sizes that are refused). */
+int64_t ponni_gated_workspace_bytes(const ponni_gated* block, int64_t columns);
+
+/* Gradients of a gated block, each of the type and shape of what it belongs to; a
+ * null one is not computed. */
+typedef struct ponni_gated_gradients {
+  void* x; /* [n_in, columns] */
+  int64_t ld_x;
+  void *gate, *up, *down;
+  int64_t ld_gate, ld_up, ld_down;
+  void *gate_bias, *up_bias, *down_bias; /* also of a block that has no such bias */
+} ponni_gated_gradients;
+/* From x, the states that the forward pass left, and dy [n_out, columns]:
+ *   dh = D dy, du = dh * act(g), dg = dh * u * act'(g), the latter two rounded to the type;
+ *   dx = G dg + U du, dG = x dg^T, dU = x du^T, dD = h dy^T; dg0, du0 and dd0 the sums of dg, du and dy over
+ *   the columns.
+ * act'(0) of RELU is 0, of LEAKY_RELU its slope. */
+int ponni_gated_backward(const ponni_gated* block, const void* x, int64_t ld_x, const void* states, int64_t ld_states,
+                         const void* dy, int64_t ld_dy, int64_t columns, const ponni_gated_gradients* gradients,
+                         void* workspace, int64_t workspace_bytes, hipStream_t stream);
+int64_t ponni_gated_backward_workspace_bytes(const ponni_gated* block, int64_t columns);
+
+/* What stands between two blocks, over columns of n features:
+ *   state = residual + scale * gate * after(x),  normed = before(state)
+ * after and before: norms of each column's features, in fp32 (normed is that of the
+ * state before it is rounded). */
+#define PONNI_NORM_NONE 0  /* v                                                      */
+#define PONNI_NORM_RMS 1   /* v / sqrt(mean(v^2) + eps) * weight + bias              */
+#define PONNI_NORM_LAYER 2 /* the same of v - mean(v)                                */
+typedef struct ponni_norm {
+  int32_t kind;
+  float eps;           /* >= 0                                                       */
+  const float* weight; /* [n], null: ones                                            */
+  const float* bias;   /* [n], null: zeros                                           */
+} ponni_norm;
+typedef struct ponni_residual_norm {
+  int32_t n;     /* 1 .. 65536                                                       */
+  int32_t dtype; /* of x, residual, gate, state and normed                           */
+  int64_t columns;
+  ponni_norm after, before;
+  float scale;
+  const void* x; /* [n, columns]                                                     */
+  int64_t ld_x;
+  const void* residual; /* [n, columns], null: zeros                                 */
+  int64_t ld_residual;
+  const float* feature_gate; /* [n], or                                              */
+  const void* gate;          /* [n, columns]; both null: ones                        */
+  int64_t ld_gate;
+  void* state; /* [n, columns], null: not written (nor read by the backward pass)    */
+  int64_t ld_state;
+  void* normed; /* [n, columns], null without a norm before the next block            */
+  int64_t ld_normed;
+  float* statistics; /* [4, columns]: mean and 1 / sqrt(..) of both norms, read by the
+                        backward pass; null: not written                             */
+} ponni_residual_norm;
+int ponni_residual_norm_forward(const ponni_residual_norm* r, hipStream_t stream);
+
+/* d_state and d_normed [n, columns] are read (null: zeros), the others written (null: not). */
+typedef struct ponni_residual_norm_gradients {
+  const void* d_state;
+  int64_t ld_d_state;
+  const void* d_normed;
+  int64_t ld_d_normed;
+  void* d_x;
+  int64_t ld_d_x;
+  void* d_residual;
+  int64_t ld_d_residual;
+  void* d_gate;          /* of a gate [n, columns]                                    */
+  int64_t ld_d_gate;
+  float* d_feature_gate; /* [n], and                                                  */
+  float *d_after_weight, *d_after_bias, *d_before_weight, *d_before_bias; /* [n]       */
+} ponni_residual_norm_gradients;
+/* Reads x, residual, gate and statistics of r again. */
+int ponni_residual_norm_backward(const ponni_residual_norm* r, const ponni_residual_norm_gradients* gradients,
+                                 void* workspace, int64_t workspace_bytes, hipStream_t stream);
+/* Enough for `columns` columns and for any fewer (-1 for sizes that are refused). */
+int64_t ponni_residual_norm_workspace_bytes(int32_t n, int32_t dtype, int64_t columns);
+
+/* Log probabilities of classes from logits [classes, columns] of `dtype`, each column a distribution
+ * p = exp(logits - log_normalizer), log_normalizer = log sum exp(logits):
+ * logits of -inf rule their class out, with probability 0.  A column that holds NaN
+ * or +inf gives NaN, except for its top classes and a target that is ruled out; one whose
+ * classes are all ruled out gives log_normalizer -inf, entropy 0 and zero gradients. */
+typedef struct ponni_log_probs {
+  int64_t classes, columns; /* 1 .. PONNI_MAX_COLUMNS                                  */
+  const void* logits;
+  int64_t ld;
+  int32_t dtype;
+  int32_t top_k;          /* 0 .. min(PONNI_MAX_TOP_K, classes)                        */
+  const int32_t* targets; /* [columns], null: none.  A column whose target is not in
+                             0 .. classes - 1 has log probability 0, and no gradient of it */
+  float* log_probs;       /* [columns]: logits[target] - log_normalizer (-inf of one
+                             that is ruled out); null without targets                  */
+  float* entropy;         /* [columns]: -sum p log p                                   */
+  float* log_normalizer;  /* [columns]                                                 */
+  int32_t* top_classes;   /* [top_k, columns]: the classes of the largest logits, of
+                             equal ones the lower first; NaN and -inf are none; -1 past the last */
+  float* top_log_probs;   /* [top_k, columns], -inf past the last                      */
+} ponni_log_probs;
+int ponni_log_probs_forward(const ponni_log_probs* p, void* workspace, int64_t workspace_bytes, hipStream_t stream);
+/* Enough for `columns` columns and for any fewer (-1 for sizes that are refused). */
+int64_t ponni_log_probs_workspace_bytes(int64_t classes, int64_t columns, int32_t top_k);
+/* d_logits [classes, columns] of `dtype` from the gradients [columns] of log_probs, entropy and
+ * log_normalizer (null: zeros):
+ *   p (d_log_normalizer - d_log_probs) - d_entropy p (log p + entropy), and d_log_probs at the target.
+ * Reads logits, targets, entropy and log_normalizer of p again.  d_logits may be the logits' own array. */
+int ponni_log_probs_backward(const ponni_log_probs* p, const float* d_log_probs, const float* d_entropy,
+                             const float* d_log_normalizer, void* d_logits, int64_t ld_d_logits, hipStream_t stream);
+
 /* --- synthetic data (bench and tests) ------------------------------------- */
 
 /* Fill n elements of a device buffer of `dtype` with the counter-based

@@ -17,5 +17,9 @@ from .experts import (  # noqa: F401
     ExpertBias, ExpertInference, ExpertMatvec, MixtureOfExperts, Mx4, Routing, create_expert_model, quantize_mx4,
     route_experts,
 )
+from .blocks import (  # noqa: F401
+    BlockNorm, GatedGradients, GatedInference, LogProbabilities, ResidualNorm, ResidualNormGradients, create_gated_model,
+    create_residual_norm, log_probabilities,
+)
 
 __all__ = [n for n in dir() if not n.startswith("_")] + ["_abi"]

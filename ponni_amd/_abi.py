@@ -151,6 +151,56 @@ class RoutingArrays(ctypes.Structure):
                 ("source", ctypes.c_void_p), ("offsets", ctypes.c_void_p)]
 
 
+MAX_COLUMNS, GATED_MAX_COLUMNS = 1_000_000_000, 16_777_216
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+
+
+class Gated(ctypes.Structure):
+    """ponni_gated (include/ponni_hip.h)."""
+    _fields_ = [*((n, ctypes.c_int32) for n in ("n_in", "n_hidden", "n_out", "dtype")), ("act", LayerDesc),
+                *((n, ctypes.c_void_p) for n in ("gate", "up", "down")),
+                *((n, ctypes.c_int64) for n in ("ld_gate", "ld_up", "ld_down")),
+                *((n, ctypes.c_void_p) for n in ("gate_bias", "up_bias", "down_bias"))]
+
+
+class GatedGradientArrays(ctypes.Structure):
+    """ponni_gated_gradients."""
+    _fields_ = [("x", ctypes.c_void_p), ("ld_x", ctypes.c_int64), *((n, ctypes.c_void_p) for n in ("gate", "up", "down")),
+                *((n, ctypes.c_int64) for n in ("ld_gate", "ld_up", "ld_down")),
+                *((n, ctypes.c_void_p) for n in ("gate_bias", "up_bias", "down_bias"))]
+
+
+class Norm(ctypes.Structure):
+    """ponni_norm."""
+    _fields_ = [("kind", ctypes.c_int32), ("eps", ctypes.c_float), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p)]
+
+
+class ResidualNormArrays(ctypes.Structure):
+    """ponni_residual_norm."""
+    _fields_ = [("n", ctypes.c_int32), ("dtype", ctypes.c_int32), ("columns", ctypes.c_int64), ("after", Norm),
+                ("before", Norm), ("scale", ctypes.c_float), ("x", ctypes.c_void_p), ("ld_x", ctypes.c_int64),
+                ("residual", ctypes.c_void_p), ("ld_residual", ctypes.c_int64), ("feature_gate", ctypes.c_void_p),
+                ("gate", ctypes.c_void_p), ("ld_gate", ctypes.c_int64), ("state", ctypes.c_void_p),
+                ("ld_state", ctypes.c_int64), ("normed", ctypes.c_void_p), ("ld_normed", ctypes.c_int64),
+                ("statistics", ctypes.c_void_p)]
+
+
+class ResidualNormGradientArrays(ctypes.Structure):
+    """ponni_residual_norm_gradients."""
+    _fields_ = [(n, t) for a in ("d_state", "d_normed", "d_x", "d_residual", "d_gate")
+                for n, t in ((a, ctypes.c_void_p), ("ld_" + a, ctypes.c_int64))] + [
+                    (n, ctypes.c_void_p) for n in ("d_feature_gate", "d_after_weight", "d_after_bias", "d_before_weight",
+                                                   "d_before_bias")]
+
+
+class LogProbsArrays(ctypes.Structure):
+    """ponni_log_probs."""
+    _fields_ = [("classes", ctypes.c_int64), ("columns", ctypes.c_int64), ("logits", ctypes.c_void_p),
+                ("ld", ctypes.c_int64), ("dtype", ctypes.c_int32), ("top_k", ctypes.c_int32),
+                *((n, ctypes.c_void_p) for n in ("targets", "log_probs", "entropy", "log_normalizer", "top_classes",
+                                                 "top_log_probs"))]
+
+
 def lib() -> ctypes.CDLL:
     """Load the in-tree libponni_hip.so; fail loudly when it is missing."""
     global _lib
@@ -262,6 +312,28 @@ def lib() -> ctypes.CDLL:
     L.ponni_experts_forward_mixture.argtypes = [vp, vp, i64, routing, vp, i64, vp, i64, vp]
     L.ponni_experts_mixture_workspace_bytes.restype = i64
     L.ponni_experts_mixture_workspace_bytes.argtypes = [vp, i32, i64]
+    gated, norm = ctypes.POINTER(Gated), ctypes.POINTER(ResidualNormArrays)
+    L.ponni_gated_forward.restype = ctypes.c_int
+    L.ponni_gated_forward.argtypes = [gated, vp, i64, vp, i64, vp, i64, i64, vp, i64, vp]
+    L.ponni_gated_workspace_bytes.restype = i64
+    L.ponni_gated_workspace_bytes.argtypes = [gated, i64]
+    L.ponni_gated_backward.restype = ctypes.c_int
+    L.ponni_gated_backward.argtypes = [gated, vp, i64, vp, i64, vp, i64, i64, ctypes.POINTER(GatedGradientArrays), vp, i64, vp]
+    L.ponni_gated_backward_workspace_bytes.restype = i64
+    L.ponni_gated_backward_workspace_bytes.argtypes = [gated, i64]
+    L.ponni_residual_norm_forward.restype = ctypes.c_int
+    L.ponni_residual_norm_forward.argtypes = [norm, vp]
+    L.ponni_residual_norm_backward.restype = ctypes.c_int
+    L.ponni_residual_norm_backward.argtypes = [norm, ctypes.POINTER(ResidualNormGradientArrays), vp, i64, vp]
+    L.ponni_residual_norm_workspace_bytes.restype = i64
+    L.ponni_residual_norm_workspace_bytes.argtypes = [i32, i32, i64]
+    log_probs = ctypes.POINTER(LogProbsArrays)
+    L.ponni_log_probs_forward.restype = ctypes.c_int
+    L.ponni_log_probs_forward.argtypes = [log_probs, vp, i64, vp]
+    L.ponni_log_probs_workspace_bytes.restype = i64
+    L.ponni_log_probs_workspace_bytes.argtypes = [i64, i64, i32]
+    L.ponni_log_probs_backward.restype = ctypes.c_int
+    L.ponni_log_probs_backward.argtypes = [log_probs, vp, vp, vp, vp, i64, vp]
     _lib = L
     return L
 

@@ -43,6 +43,13 @@ SOURCES = [
     "kernels_chain_mx4_bf16.hip",
     "kernels_route.hip",
     "kernels_mx4.hip",
+    "blocks.cpp",
+    "kernels_gated.hip",
+    "kernels_norm.hip",
+    "kernels_norm_f32.hip",
+    "kernels_norm_f16.hip",
+    "kernels_norm_bf16.hip",
+    "kernels_logp.hip",
 ]
 
 # Headers embedded in the library for the run-time (hipRTC) compiler.

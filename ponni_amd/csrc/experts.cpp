@@ -4,52 +4,16 @@
 
 #include <algorithm>
 #include <memory>
-#include <new>
 #include <string>
 
+#include "abi_checks.h"
 #include "program.h"
 
 namespace ponni_hip {
 namespace {
 
-constexpr int32_t kMaxWidth = 65536;
 // (PONNI_MAX_COLUMNS: a launch has fewer than 2^32 threads in a dimension, and where the grid is one of columns alone
 // 64 of them have 256 threads at most: 4.0e9.  The layers' tiles, of output features too, are counted when launched.)
-
-int fail(int status, std::string const& message) { return set_error(status, message); }
-
-// Runs a C entry point's body; nothing is thrown across the ABI.
-template <class F> int guarded(F&& f) {
-  try {
-    return f();
-  } catch (std::bad_alloc const&) {
-    return fail(PONNI_ERR_INVALID_ARGUMENT, "out of host memory");
-  } catch (std::exception const& e) {
-    return fail(PONNI_ERR_INVALID_ARGUMENT, e.what());
-  }
-}
-
-int device_error(char const* what, hipError_t e) {
-  return fail(PONNI_ERR_DEVICE, std::string(what) + ": " + hipGetErrorString(e));
-}
-
-int64_t element_bytes(int32_t dtype) { return dtype == PONNI_F64 ? 8 : dtype == PONNI_F32 ? 4 : 2; }
-bool data_type(int32_t dtype) { return dtype == PONNI_F32 || dtype == PONNI_F16 || dtype == PONNI_BF16; }
-bool aligned(void const* p, uint64_t bytes) { return reinterpret_cast<uint64_t>(p) % bytes == 0; }
-int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
-
-struct Range {
-  uint64_t begin, end;
-};
-Range array(void const* p, int64_t rows, int64_t ld, int64_t columns, int64_t es) {
-  auto const b = reinterpret_cast<uint64_t>(p);
-  return {b, b + uint64_t(((rows - 1) * ld + columns) * es)};
-}
-Range bytes(void const* p, int64_t n) {
-  auto const b = reinterpret_cast<uint64_t>(p);
-  return {b, b + uint64_t(n)};
-}
-bool overlap(Range a, Range b) { return a.begin < b.end && b.begin < a.end; }
 
 // A routing's arrays: weights, slots, source and offsets, which a mixture reads, and experts.
 constexpr int kRoutingArrays = 5;
@@ -142,15 +106,6 @@ int check_ready(ponni_experts_s const& e) {
   hipError_t const err = hipGetDevice(&device);
   if (err != hipSuccess) return device_error("hipGetDevice", err);
   if (device != e.device) return fail(PONNI_ERR_DEVICE, "the expert networks' parameters are on another device");
-  return PONNI_OK;
-}
-
-int check_workspace(void const* workspace, int64_t bytes, int64_t need) {
-  if (need > 0 && workspace == nullptr) return fail(PONNI_ERR_INVALID_ARGUMENT, "workspace is null");
-  if (!aligned(workspace, 16)) return fail(PONNI_ERR_INVALID_ARGUMENT, "workspace is not at a multiple of 16 bytes");
-  if (bytes < need)
-    return fail(PONNI_ERR_SHAPE, "workspace holds " + std::to_string(bytes) + " bytes, " + std::to_string(need) +
-                                     " are needed");
   return PONNI_OK;
 }
 
@@ -318,19 +273,6 @@ int mixture_impl(ponni_experts e, const void* x, int64_t ld_in, const ponni_rout
   if (st != PONNI_OK) return st;
   hipError_t const err = launch_combine(e->dtype, result, columns, *r, last.n_out, y, ld_out, stream);
   return err == hipSuccess ? PONNI_OK : device_error("weighted sum", err);
-}
-
-// ActCode of an activation layer, -1 for one the expert kernels do not have.
-int activation_of(ponni_layer_desc const& d) {
-  switch (d.kind) {
-    case PONNI_LAYER_RELU: return ACT_RELU;
-    case PONNI_LAYER_LEAKY_RELU: return ACT_LEAKY_RELU;
-    case PONNI_LAYER_GELU: return (d.flags & PONNI_FLAG_GELU_APPROXIMATE) ? ACT_GELU_TANH : ACT_GELU_ERF;
-    case PONNI_LAYER_SILU: return ACT_SILU;
-    case PONNI_LAYER_SIGMOID: return ACT_SIGMOID;
-    case PONNI_LAYER_TANH: return ACT_TANH;
-    default: return -1;
-  }
 }
 
 int create_impl(const ponni_layer_desc* descs, int32_t n, int32_t num_experts, int32_t dtype, int32_t weights,

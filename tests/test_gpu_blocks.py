@@ -1,0 +1,506 @@
+"""Gated blocks, norms between blocks and log probabilities on the GPU against numpy in 64 bits
+(numpy_blocks.py, which bounds every element's distance), and their gradients against differences."""
+import numpy as np
+import pytest
+
+import ponni_amd as P
+from ponni_amd import _abi as A
+from tests import numpy_blocks as N
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = ["f32", "f16", "bf16"]
+
+
+def torch_dtype(name):
+    import torch
+
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+def tensor(a, dtype, device, pad=0, shift=0):
+    """a [rows, columns] on the GPU in a wider array, `shift` columns in."""
+    import torch
+
+    t = torch.full((a.shape[0], a.shape[1] + pad + shift), 7.0, dtype=torch_dtype(dtype), device=device)
+    v = t[:, shift:shift + a.shape[1]]
+    v.copy_(torch.from_numpy(np.ascontiguousarray(a)).to(device))
+    return v
+
+
+def vector(a, device, dtype="f32"):
+    import torch
+
+    return None if a is None else torch.from_numpy(np.ascontiguousarray(a)).to(device).to(torch_dtype(dtype))
+
+
+def host(t):
+    return None if t is None else t.double().cpu().numpy()
+
+
+def close(got, want, bound, what):
+    got = host(got) if not isinstance(got, np.ndarray) else got
+    assert got.shape == want.shape, what
+    same = (got == want) | (np.isnan(got) & np.isnan(want))
+    with np.errstate(invalid="ignore"):
+        off = np.where(same, 0.0, np.abs(got - want))
+    worst = np.nanmax(np.where(same, 0.0, off / bound)) if off.size else 0.0
+    assert np.all(same | (off <= bound)), f"{what}: {worst:.3g} of its bound"
+
+
+# -- log probabilities ---------------------------------------------------------------------
+
+
+def logits_of(r, c, b, masked, dtype):
+    x = r.standard_normal((c, b)) * 3
+    if dtype == "bf16":
+        x = np.round(x * 4) / 4  # (many ties)
+    if masked:
+        x[r.random((c, b)) < masked] = -np.inf
+        if b > 2:
+            x[:, r.integers(0, b, 2)] = -np.inf  # columns without a class
+    return x
+
+
+def check_logp(cuda, c, b, k, dtype, masked=0.3, pad=0, shift=0, seed=0, targets=True):
+    r = np.random.default_rng(seed + c * 31 + b)
+    x = tensor(logits_of(r, c, b, masked, dtype), dtype, cuda, pad, shift)
+    t = r.integers(-1, c + 1, b) if targets else None
+    got = P.log_probabilities(x, None if t is None else vector(t, cuda).int(), top_k=k)
+    want = N.log_probs(host(x), t, k)
+    for name in ("log_normalizer", "entropy", "log_probs", "top_log_probs"):
+        if getattr(got, name) is not None:
+            close(getattr(got, name), *want[name], name)
+    if k:
+        assert np.array_equal(got.top_classes.cpu().numpy(), want["top_classes"])
+    assert (got.log_probs is None) == (t is None) and (got.top_classes is None) == (k == 0)
+    g = [r.standard_normal(b).astype(np.float32) for _ in range(3)]
+    for use in ((1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1)):
+        if t is None and use[0]:
+            continue
+        gs = [v if u else None for u, v in zip(use, g)]
+        d = got.backward(*(vector(v, cuda) for v in gs))
+        close(d, *N.log_probs_backward(want, *(None if v is None else v.astype(float) for v in gs), dtype), f"d_logits {use}")
+    return got, x
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c,b,k", [(1, 1, 1), (1, 9, 0), (2, 3, 2), (10, 5000, 3), (64, 1030, 4), (65, 1, 16), (100, 7, 0),
+                                   (257, 33, 5), (1000, 64, 8), (1263, 516, 3), (5003, 3, 16), (5003, 1, 8), (20_011, 70, 0),
+                                   (300, 70_003, 0), (33, 100_001, 16), (130_001, 2, 4)])
+def test_log_probabilities(cuda, c, b, k, dtype):
+    print(f"log probabilities: {c} classes {b} columns top {k} {dtype}", flush=True)
+    check_logp(cuda, c, b, k, dtype, pad=b % 3, shift=b % 2)
+
+
+def test_log_probabilities_without_targets_or_masks(cuda):
+    check_logp(cuda, 1000, 130, 0, "bf16", masked=0.0, targets=False)
+    check_logp(cuda, 100, 1, 2, "f32", masked=0.0, targets=False)
+
+
+def test_equal_logits(cuda):
+    """Ties go to the lower class across lanes, waves and workgroups."""
+    import torch
+
+    for c, b in ((40_000, 1), (40_000, 3), (3000, 40), (50, 300)):
+        x = torch.zeros((c, b), device=cuda)
+        r = P.log_probabilities(x, None, 16)
+        assert torch.equal(r.top_classes.cpu(), torch.arange(16, dtype=torch.int32)[:, None].expand(16, b))
+        x[c // 2:] = 1.0
+        r = P.log_probabilities(x.bfloat16(), None, 5)
+        assert torch.equal(r.top_classes.cpu(), (c // 2 + torch.arange(5, dtype=torch.int32))[:, None].expand(5, b))
+        # an early class is overtaken and stays before its equals
+        x[7] = 1.0
+        r = P.log_probabilities(x, None, 4)
+        assert r.top_classes[:, 0].tolist() == [7, c // 2, c // 2 + 1, c // 2 + 2]
+        x[c - 1] = 2.0
+        r = P.log_probabilities(x, None, 4)
+        assert r.top_classes[:, 0].tolist() == [c - 1, 7, c // 2, c // 2 + 1]
+
+
+@pytest.mark.parametrize("c,b", [(50, 300), (5000, 4), (3000, 70)])
+def test_non_finite_logits(cuda, c, b):
+    """NaN and +inf stay in their column; the lowest finite value is no mask."""
+    import torch
+
+    r = np.random.default_rng(c)
+    x = r.standard_normal((c, b))
+    x[3, 0], x[c - 1, 1] = np.nan, np.inf
+    x[:, 2] = -np.finfo(np.float32).max
+    x[5, 2] = -np.inf
+    t = torch.full((b,), 4, dtype=torch.int32, device=cuda)
+    got = P.log_probabilities(tensor(x, "f32", cuda), t, 2)
+    assert torch.isnan(got.log_normalizer[:2]).all() and torch.isnan(got.entropy[:2]).all()
+    assert torch.isnan(got.log_probs[:2]).all() and torch.isnan(got.top_log_probs[:, :2]).all()
+    assert int(got.top_classes[0, 1]) == c - 1 and int(got.top_classes[0, 0]) not in (3, -1)
+    # equal classes of the lowest value: c - 1 of them
+    assert abs(float(got.entropy[2]) - np.log(c - 1)) < 1e-5 * np.log(c)
+    assert got.top_classes[:, 2].tolist() == [0, 1]
+    want = N.log_probs(x[:, 3:].astype(np.float32).astype(float), np.full(b - 3, 4), 2)
+    for name in ("log_normalizer", "entropy", "log_probs", "top_log_probs"):
+        close(getattr(got, name)[..., 3:].contiguous(), *want[name], name)
+    ones = torch.ones(b, device=cuda)
+    d = got.backward(ones, ones, ones)
+    assert torch.isnan(d[:, :2]).all() and not torch.isnan(d[:, 2:]).any()
+    # the lowest float as a mask: its classes have no probability, whatever is left
+    y = torch.full((c, 2), torch.finfo(torch.float32).min, device=cuda)
+    y[9] = 0.0
+    got = P.log_probabilities(y, t[:2], 1)
+    assert torch.equal(got.log_normalizer, torch.zeros(2, device=cuda)) and torch.equal(got.entropy, torch.zeros(2, device=cuda))
+    assert got.top_classes[0].tolist() == [9, 9]
+    assert not torch.isnan(got.backward(ones[:2], ones[:2], ones[:2])).any()
+
+
+def test_gradient_of_log_probabilities_in_place(cuda):
+    """Into the logits' own array, into a column range of a wider one, which keeps its other columns."""
+    import torch
+
+    for dtype in DTYPES:
+        got, x = check_logp(cuda, 700, 83, 0, dtype, seed=5)
+        g = torch.randn(83, device=cuda)
+        want = got.backward(g)
+        wide = torch.full((700, 99), 7.0, dtype=x.dtype, device=cuda)
+        got.backward(g, out=wide[:, 5:88])
+        assert torch.equal(wide[:, 5:88], want)
+        assert bool((wide[:, :5] == 7).all()) and bool((wide[:, 88:] == 7).all())
+        assert got.backward(g, out=x) is x
+        assert torch.equal(x, want)
+
+
+def test_gradient_of_log_probabilities_by_differences(cuda):
+    import torch
+
+    r = np.random.default_rng(2)
+    x = r.standard_normal((30, 6))
+    t = vector(np.array([3, 0, 29, -1, 7, 8]), cuda).int()
+    g = [r.standard_normal(6) for _ in range(3)]
+
+    def value(v):
+        want = N.log_probs(v, t.cpu().numpy(), 0)
+        return sum((a * want[n][0]).sum() for a, n in zip(g, ("log_probs", "entropy", "log_normalizer")))
+
+    got = host(P.log_probabilities(vector(x, cuda), t).backward(*(vector(v, cuda) for v in g)))
+    for i, c in ((0, 0), (3, 0), (29, 2), (5, 3), (7, 4), (1, 5)):
+        e = np.zeros_like(x)
+        e[i, c] = 1e-5
+        # (differences of second order: 1e-10 of third derivatives; fp32's roundings beside them)
+        assert abs((value(x + e) - value(x - e)) / 2e-5 - got[i, c]) < 1e-5
+
+
+# -- norms between blocks ----------------------------------------------------------------------
+
+
+def check_norm(cuda, n, b, after, before, gate, residual, dtype, scale=0.7, eps=1e-5, pad=0, shift=0, seed=0, bias=True,
+               weight=True):
+    r = np.random.default_rng(seed + 7 * n + b)
+    x = tensor(r.standard_normal((n, b)) * np.exp(0.5 * r.standard_normal((n, 1))) + 0.3, dtype, cuda, pad, shift)
+    res = tensor(2 * r.standard_normal((n, b)) + 0.5, dtype, cuda, shift, pad) if residual else None
+    gt = vector(r.standard_normal(n), cuda) if gate == "feature" else tensor(r.standard_normal((n, b)), dtype, cuda, pad) \
+        if gate == "full" else None
+    specs, norms = [], []
+    for kind in (after, before):
+        w = (1 + 0.3 * r.standard_normal(n)).astype(np.float32) if weight else None
+        c = (0.2 * r.standard_normal(n)).astype(np.float32) if bias else None
+        norms.append(None if kind is None else (kind, None if w is None else w.astype(float), None if c is None else c.astype(float)))
+        specs.append(None if kind is None else P.BlockNorm(kind, vector(w, cuda), vector(c, cuda), eps))
+    model = P.create_residual_norm(n, after=specs[0], before=specs[1], scale=scale, dtype=dtype)
+    f = np.float32(scale).astype(float)
+    want, s = N.norm_forward(host(x), host(res), host(gt), norms[0], norms[1], f, float(np.float32(eps)), dtype)
+    state, normed, statistics = model.forward_with_statistics(x, res, gt)
+    close(state, *want["state"], "state")
+    assert (normed is None) == (before is None)
+    if before is not None:
+        close(normed, *want["normed"], "normed")
+    again = model.forward_batch_parallel(x, res, gt)
+    import torch
+
+    assert torch.equal(again[0], state) and (normed is None or torch.equal(again[1], normed))
+    ds, dn = tensor(r.standard_normal((n, b)), dtype, cuda, pad), tensor(r.standard_normal((n, b)), dtype, cuda, pad, shift)
+    for d_state, d_normed in ((ds, dn), (None, dn), (ds, None)):
+        if before is None and d_normed is not None:
+            if d_state is None:
+                continue
+            d_normed = None
+        d = model.backward(x, res, gt, statistics, d_state, d_normed)
+        wanted = N.norm_backward(s, norms[0], norms[1], host(d_state), host(d_normed), f, host(gt), dtype)
+        for name in ("x", "residual", "gate", "after_weight", "after_bias", "before_weight", "before_bias"):
+            got = getattr(d, name)
+            if got is None:
+                continue
+            if name not in wanted:  # no gradient comes this way
+                assert not got.any()
+                continue
+            close(got, *wanted[name], f"d_{name} {d_state is not None} {d_normed is not None}")
+    return model
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,b,after,before,gate,residual", [
+    (1, 1, "rms", "rms", None, True), (1, 300, None, "rms", "feature", True), (5, 3, "layer", "layer", "full", True),
+    (64, 1000, "rms", "rms", "feature", True), (100, 33, "layer", "rms", None, False), (333, 515, "layer", "layer", "full", True),
+    (511, 8, None, "layer", "full", False), (1024, 2051, "rms", None, "feature", True), (1000, 9000, "rms", "layer", None, True),
+    (4096, 1, "rms", "rms", None, True), (4096, 37, None, "rms", None, True), (4097, 19, "layer", "rms", "full", True),
+    (20_000, 2, "rms", "layer", "feature", True), (9000, 40, "layer", "layer", None, True), (700, 4, None, None, "full", True),
+    (2048, 20, "rms", "rms", "full", False)])
+def test_norms(cuda, n, b, after, before, gate, residual, dtype):
+    print(f"norms: n={n} b={b} {after} {before} {gate} {residual} {dtype}", flush=True)
+    check_norm(cuda, n, b, after, before, gate, residual, dtype, pad=b % 3, shift=b % 2)
+
+
+def test_norms_without_weights(cuda):
+    check_norm(cuda, 120, 50, "rms", "layer", None, True, "f16", weight=False, bias=False)
+    check_norm(cuda, 120, 50, "layer", "rms", "full", False, "f32", weight=True, bias=False, scale=-1.0)
+
+
+def test_norm_of_constant_columns(cuda):
+    """Nothing is left to normalise: a layer norm gives its bias, zeros under eps."""
+    import torch
+
+    n, b = 96, 11
+    x = torch.full((n, b), 3.0, device=cuda)
+    bias = torch.randn(n, device=cuda)
+    model = P.create_residual_norm(n, before=P.BlockNorm("layer", None, bias))
+    _, normed, statistics = model.forward_with_statistics(x)
+    assert torch.equal(normed, bias[:, None].expand(n, b))
+    zero = P.create_residual_norm(n, before=P.BlockNorm("rms")).forward_batch_parallel(torch.zeros_like(x))[1]
+    assert not zero.any()
+    d = model.backward(x, None, None, statistics, None, torch.randn_like(x))
+    assert torch.isfinite(d.x).all()
+
+
+def test_non_finite_columns_of_norms(cuda):
+    import torch
+
+    for n, b in ((64, 40), (5000, 24), (300, 3)):
+        x = torch.randn((n, b), device=cuda)
+        model = P.create_residual_norm(n, after=P.BlockNorm("rms"), before=P.BlockNorm("layer"))
+        want = model.forward_batch_parallel(x, x)
+        x2 = x.clone()
+        x2[1, 1], x2[2, 2] = float("nan"), float("inf")
+        got = model.forward_batch_parallel(x2, x)
+        for g, w in zip(got, want):
+            assert torch.equal(g[:, [0, *range(3, b)]], w[:, [0, *range(3, b)]])
+        assert torch.isnan(got[1][:, 1]).all() and torch.isnan(got[1][:, 2]).any()
+
+
+def test_norm_rows_beyond_four_gigabytes(cuda):
+    """Byte offsets past 2^32."""
+    import torch
+
+    n, b = 1100, 2_200_000
+    x = torch.zeros((n, b), dtype=torch.bfloat16, device=cuda)
+    cols = [0, 1_500_000, b - 1]
+    x[:, cols] = torch.randn((n, 3), device=cuda).bfloat16()
+    model = P.create_residual_norm(n, before=P.BlockNorm("rms"), dtype="bf16")
+    state, normed = model.forward_batch_parallel(x)
+    want = model.forward_batch_parallel(x[:, cols].contiguous())
+    assert torch.equal(state[:, cols], want[0]) and torch.equal(normed[:, cols], want[1])
+
+
+# -- gated blocks -------------------------------------------------------------------------
+
+
+def act_layer(name, n):
+    return {"relu": P.Relu, "leaky_relu": lambda n: P.LeakyRelu(n, 0.1), "silu": P.Silu, "gelu": lambda n: P.Gelu(n, True),
+            "gelu_erf": P.Gelu, "tanh": P.Tanh, "sigmoid": P.Sigmoid}[name](n)
+
+
+def check_gated(cuda, sizes, b, act, dtype, bias=False, pad=0, shift=0, seed=0, backward=True, wpad=0):
+    i, h, o = sizes
+    r = np.random.default_rng(seed + i + h + o + b)
+    ws = [tensor(r.uniform(-1, 1, s) * np.sqrt(6 / sum(s)), dtype, cuda, wpad, wpad % 2) for s in ((i, h), (i, h), (h, o))]
+    bs = [vector(0.3 * r.standard_normal(n), cuda, dtype) if bias else None for n in (h, h, o)]
+    x = tensor(r.standard_normal((i, b)), dtype, cuda, pad, shift)
+    model = P.create_gated_model(*ws, act_layer(act, h), *bs)
+    w, hb = [host(t) for t in ws], [host(t) for t in bs]
+    want = N.gated(w, host(x), act, dtype, hb)
+    y = model.forward_batch_parallel(x)
+    close(y, *want[3], "y")
+    if not backward:
+        return model, x, y
+    y2, states = model.forward_with_states(x)
+    close(y2, *want[3], "y with states")
+    kept = np.split(host(states), 3)
+    for name, got, (v, e) in zip("guh", kept, want):
+        close(got, v, e, name)
+    dy = tensor(r.standard_normal((o, b)), dtype, cuda, shift, pad)
+    d = model.backward(x, states, dy)
+    wanted = N.gated_backward(w, host(x), kept, host(dy), act, dtype)
+    for name, (v, e) in wanted.items():
+        got = getattr(d, name)
+        if got is not None:
+            close(got, v, e, f"d_{name}")
+    assert bias == (d.gate_bias is not None)
+    return model, x, y
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes,b", [((1, 1, 1), 1), ((3, 5, 2), 4), ((16, 16, 16), 16), ((64, 256, 64), 1), ((64, 256, 64), 20),
+                                     ((130, 70, 33), 65), ((333, 101, 77), 503), ((256, 300, 200), 1025), ((40, 640, 40), 3),
+                                     ((200, 513, 129), 33), ((96, 128, 64), 3000), ((520, 264, 136), 257)])
+def test_gated(cuda, sizes, b, dtype):
+    print(f"gated: {sizes} b={b} {dtype}", flush=True)
+    check_gated(cuda, sizes, b, "silu", dtype, bias=b % 2 == 1, pad=b % 5, shift=b % 2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", N.ACTS)
+def test_gated_activations(cuda, act, dtype):
+    for b in (2, 40, 300):
+        check_gated(cuda, (48, 80, 56), b, act, dtype, bias=True)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_strides(cuda, dtype):
+    """Weights, inputs and gradients as column ranges of wider arrays, at odd and even places."""
+    for pad, shift, wpad in ((8, 0, 8), (3, 1, 0), (16, 8, 3), (0, 0, 1), (64, 2, 2)):
+        for b in (1, 24, 190):
+            check_gated(cuda, (72, 136, 88), b, "silu", dtype, bias=True, pad=pad, shift=shift, wpad=wpad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_non_finite_columns(cuda, dtype):
+    """NaN and infinities stay in their columns, and meet no padding."""
+    import torch
+
+    for b in (7, 90, 300):
+        r = np.random.default_rng(b)
+        i, h, o = 37, 70, 41
+        ws = [tensor(r.uniform(-1, 1, s) * 0.3, dtype, cuda) for s in ((i, h), (i, h), (h, o))]
+        model = P.create_gated_model(*ws, P.LeakyRelu(h, 0.1))
+        x = tensor(r.standard_normal((i, b)), dtype, cuda)
+        want = model.forward_batch_parallel(x)
+        x2 = x.clone()
+        x2[3, 1], x2[i - 1, 2], x2[0, b - 1] = float("nan"), float("inf"), -float("inf")
+        got, states = model.forward_with_states(x2)
+        good = [c for c in range(b) if c not in (1, 2, b - 1)]
+        assert torch.equal(got[:, good], want[:, good])
+        assert not torch.isfinite(got[:, [1, 2, b - 1]]).any()
+
+
+def test_gated_gradient_by_differences(cuda):
+    r = np.random.default_rng(9)
+    i, h, o, b = 6, 9, 5, 4
+    w = [r.standard_normal(s) for s in ((i, h), (i, h), (h, o))]
+    bs = [r.standard_normal(n) for n in (h, h, o)]
+    x, dy = r.standard_normal((i, b)), r.standard_normal((o, b))
+    for act in ("silu", "gelu", "gelu_erf", "tanh", "sigmoid"):
+        model = P.create_gated_model(*(vector(v, cuda) for v in w), act_layer(act, h), *(vector(v, cuda) for v in bs))
+        _, states = model.forward_with_states(vector(x, cuda))
+        d = model.backward(vector(x, cuda), states, vector(dy, cuda))
+
+        def value(w, bs, x):
+            a = N.activation(act, w[0].T @ x + bs[0][:, None])[0]
+            return (dy * (w[2].T @ (a * (w[1].T @ x + bs[1][:, None])) + bs[2][:, None])).sum()
+
+        leaves = [*w, *bs, x]
+        grads = [d.gate, d.up, d.down, d.gate_bias, d.up_bias, d.down_bias, d.x]
+        for k, g in enumerate(grads):
+            direction = r.standard_normal(leaves[k].shape)
+
+            def at(e):
+                v = [a + e * direction if j == k else a for j, a in enumerate(leaves)]
+                return value(v[:3], v[3:6], v[6])
+
+            # fp32's roundings of some 300 terms of size up to 10, and the differences' third order
+            want = (at(1e-4) - at(-1e-4)) / 2e-4
+            assert abs((host(g) * direction).sum() - want) < 2e-4 * max(1.0, abs(want))
+
+
+# -- together ---------------------------------------------------------------------------------
+
+
+def test_a_block_with_its_head(cuda):
+    """norm -> gated block -> residual, gate and norms -> head -> log probabilities and back, in fp32 against torch's
+    gradients in 64 bits."""
+    import torch
+
+    torch.manual_seed(3)
+    n, h, c, b = 48, 120, 211, 77
+    w = {k: torch.randn(s, dtype=torch.float64) / s[0] ** 0.5 for k, s in
+         (("G", (n, h)), ("U", (n, h)), ("D", (h, n)), ("R", (n, c)))}
+    v = {k: 1 + 0.2 * torch.randn(n, dtype=torch.float64) for k in ("w1", "w2", "w3", "gate")}
+    x = torch.randn((n, b), dtype=torch.float64)
+    t = torch.randint(0, c, (b,))
+    leaves = {k: p.to(torch.float32).double().requires_grad_() for k, p in {**w, **v, "x": x}.items()}
+
+    def rms(y, weight):
+        return y * (y.pow(2).mean(0, keepdim=True) + 1e-5).rsqrt() * weight[:, None]
+
+    L = leaves
+    hidden = rms(L["x"], L["w1"])
+    y = L["D"].T @ (torch.nn.functional.silu(L["G"].T @ hidden) * (L["U"].T @ hidden))
+    state = L["x"] + 0.5 * L["gate"][:, None] * rms(y, L["w2"])
+    lp = torch.log_softmax(L["R"].T @ rms(state, L["w3"]), 0)
+    entropy = -(lp.exp() * lp).sum(0)
+    loss = -lp[t, torch.arange(b)].mean() + 0.1 * entropy.mean()
+    loss.backward()
+
+    g = {k: p.detach().float().to(cuda) for k, p in leaves.items()}
+    first = P.create_residual_norm(n, before=P.BlockNorm("rms", g["w1"]))
+    block = P.create_gated_model(g["G"], g["U"], g["D"], P.Silu(h))
+    last = P.create_residual_norm(n, after=P.BlockNorm("rms", g["w2"]), before=P.BlockNorm("rms", g["w3"]), scale=0.5)
+    head = P.create_inference_model(P.Matvec(g["R"].cpu().numpy()))
+    back = P.create_inference_model(P.Matvec(g["R"].T.contiguous().cpu().numpy()))
+    _, normed, s1 = first.forward_with_statistics(g["x"])
+    out, states = block.forward_with_states(normed)
+    new, final, s2 = last.forward_with_statistics(out, g["x"], g["gate"])
+    r = P.log_probabilities(head.forward_batch_parallel(final), t.int().to(cuda), 3)
+    got = -r.log_probs.mean() + 0.1 * r.entropy.mean()
+    assert abs(float(got) - float(loss)) < 1e-5
+    d_logits = r.backward(torch.full((b,), -1.0 / b, device=cuda), torch.full((b,), 0.1 / b, device=cuda))
+    d_final = back.forward_batch_parallel(d_logits)
+    d2 = last.backward(out, g["x"], g["gate"], s2, None, d_final)
+    db = block.backward(normed, states, d2.x)
+    d1 = first.backward(g["x"], None, None, s1, d2.residual, db.x)
+    for name, value in (("G", db.gate), ("U", db.up), ("D", db.down), ("w1", d1.before_weight), ("w2", d2.after_weight),
+                        ("w3", d2.before_weight), ("gate", d2.gate), ("x", d1.x)):
+        want = leaves[name].grad
+        # some 500 roundings of 2^-24 along the way
+        assert float((value.double().cpu() - want).norm() / want.norm()) < 500 * 2.0 ** -24, name
+
+
+def test_block_operators_on_streams_and_in_graphs(cuda):
+    """Captured once, replayed with new inputs between eager calls; the same bits every time."""
+    import torch
+
+    n, h, c = 72, 200, 300
+    for dtype, b in (("bf16", 3), ("f16", 200), ("f32", 70)):
+        t = torch_dtype(dtype)
+        ws = [(torch.randn(s, device=cuda) / 8).to(t) for s in ((n, h), (n, h), (h, c))]
+        block = P.create_gated_model(*ws, P.Gelu(h, True))
+        norm = P.create_residual_norm(n, after=P.BlockNorm("rms", torch.randn(n, device=cuda)),
+                                      before=P.BlockNorm("layer", torch.randn(n, device=cuda), torch.randn(n, device=cuda)),
+                                      dtype=dtype)
+        x, res = torch.randn((n, b), device=cuda).to(t), torch.randn((n, b), device=cuda).to(t)
+        gate = torch.randn(n, device=cuda)
+        targets = torch.randint(0, c, (b,), dtype=torch.int32, device=cuda)
+        g = torch.randn(b, device=cuda)
+
+        def step():
+            state, normed, s = norm.forward_with_statistics(x, res, gate)
+            y, states = block.forward_with_states(normed)
+            r = P.log_probabilities(y, targets, 2)
+            dy = r.backward(g, g)
+            d = block.backward(normed, states, dy)
+            e = norm.backward(x, res, gate, s, state, d.x)
+            return [state, normed, y, r.log_probs, r.entropy, r.top_classes, r.top_log_probs, dy, d.x, d.gate, d.up, d.down,
+                    e.x, e.residual, e.gate, e.after_weight, e.before_weight, e.before_bias]
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            warm = step()
+        torch.cuda.current_stream().wait_stream(side)
+        assert all(torch.equal(a, e) for a, e in zip(warm, step()))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        for seed in range(3):
+            torch.manual_seed(seed)
+            x.copy_(torch.randn((n, b), device=cuda))
+            ws[0].copy_(torch.randn((n, h), device=cuda) / 8)
+            graph.replay()
+            want = step()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, e) for a, e in zip(outs, want))
