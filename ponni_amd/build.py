@@ -45,6 +45,9 @@ SOURCES = [
     "kernels_mx4.hip",
     "blocks.cpp",
     "kernels_gated.hip",
+    "kernels_gated_f32.hip",
+    "kernels_gated_f16.hip",
+    "kernels_gated_bf16.hip",
     "kernels_norm.hip",
     "kernels_norm_f32.hip",
     "kernels_norm_f16.hip",

@@ -1,0 +1,55 @@
+// Products of gated blocks: what kernels_gated.hip asks of the kernels of gated_product.h.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace ponni_hip {
+
+// An operand: rows `ld` bytes apart, of `rows` rows, `bytes` from the first element to the end of the last row (up to a
+// multiple of 16).  p and ld are multiples of 16 bytes.
+struct Side {
+  char const* p;
+  int64_t ld, bytes, rows;
+};
+
+enum Output {
+  OUT_PLAIN,   // y = C (+ bias)
+  OUT_PAIR,    // rows of two products: y = act(C) * C2, and both of them as states
+  OUT_STATES,  // from C and the states: y[0] = C u act'(g), y[1] = C act(g)
+  OUT_PARTS    // fp32 sums of a part of k
+};
+enum Form {
+  FORM_PAIR,     // k outside in both; a: two arrays
+  FORM_FORWARD,  // k outside in both
+  FORM_STATES,   // k inside in a
+  FORM_INPUT,    // k inside in a
+  FORM_WEIGHTS   // k inside in both
+};
+
+struct ProductArgs {
+  Side a[2], b[2];
+  int64_t k, rows, columns;  // C [rows, columns]
+  int terms;                 // 2: the sum of a[0] b[0] and a[1] b[1]
+  int problems;              // 2: a[0] b[0] and a[0] b[1], into y[0] and y[1]
+  int parts;                 // workgroups that share a tile's k
+  void* y[2];
+  int64_t ld[2];
+  void const* bias[2];
+  int act;
+  float slope;
+  void* states;  // [2 rows, columns]: OUT_PAIR writes them (null: not), OUT_STATES reads them
+  int64_t ld_states;
+  float* sums;   // OUT_PARTS: [parts, problems, rows, ld_sums]
+  int64_t ld_sums;
+  // the grid, filled in by the launch
+  int m_tiles, n_tiles, split_n, steps;
+};
+
+// large: tiles of 256 x 256 (16 bits), else of 128 x 128.
+hipError_t launch_product_f32(Form form, bool large, ProductArgs const& p, hipStream_t stream);
+hipError_t launch_product_f16(Form form, bool large, ProductArgs const& p, hipStream_t stream);
+hipError_t launch_product_bf16(Form form, bool large, ProductArgs const& p, hipStream_t stream);
+
+}  // namespace ponni_hip

@@ -1,155 +1,188 @@
-// Gated feed-forward blocks: y = D^T (act(G^T x + g0) * (U^T x + u0)) + d0 and the
-// gradients.  64 x 64 tiles of a product, operands of any strides through LDS as
-// floats, 4 x 4 sums a lane.
+// Gated feed-forward blocks: their products one after the other (gated_product.h), in
+// the caller's arrays and work buffer.
+//   forward   h = act(G^T x + g0) * (U^T x + u0) (and g, u), then y = D^T h + d0
+//   backward  dg, du from D dy and the states; dx = G dg + U du; dG, dU = x dg^T, x du^T; dD = h dy^T;
+//             biases' gradients are sums of rows
+// Operands go into LDS by 16-byte pieces, so an array whose rows do not begin at
+// multiples of 16 bytes is first copied to one whose rows do.
 #include <algorithm>
 
-#include "activations.h"
 #include "blocks.h"
+#include "column_rows.h"
+#include "gated.h"
 #include "operand_types.h"
 
 namespace ponni_hip {
 namespace {
 
-constexpr int kTile = 64, kDepth = 16;
-
-// One operand: element (i, k) at p[i * row + k * step].
-struct Operand {
-  void const* p;
-  int64_t row, step;
-};
-// Sum over the terms t and k of a[t](m, k) b[t](n, k); with `pair` a second sum of a2 and b[0].
-struct Product {
-  Operand a[2], b[2], a2;
-  int64_t k;
-  int terms;
-  int64_t rows, columns;
-};
-enum Output { OUT_PLAIN, OUT_PAIR, OUT_STATES };
-struct Outputs {
-  void* y;
-  int64_t ld;
-  void const *bias, *bias2;
-  int act;
-  float slope;
-  void *g, *u;          // states: written by OUT_PAIR (null: not), read by OUT_STATES
-  int64_t ld_states;
-  void *dg, *du;        // OUT_STATES
-  int64_t ld_gradients;
-};
-
-// act(v) and act'(v)
-__device__ inline void activation(int act, float slope, float v, float& a, float& d) {
-  switch (act) {
-    case ACT_RELU: a = act_relu(v), d = v > 0.0f ? 1.0f : 0.0f; break;
-    case ACT_LEAKY_RELU: a = act_leaky_relu(v, slope), d = v > 0.0f ? 1.0f : slope; break;
-    case ACT_TANH: a = tanh_f32(v), d = 1.0f - a * a; break;
-    case ACT_SIGMOID: a = sigmoid_f32(v), d = a * sigmoid_f32(-v); break;
-    case ACT_SILU: {
-      float const p = sigmoid_f32(v);
-      a = silu_f32(v), d = p * fmaf(v, sigmoid_f32(-v), 1.0f);
-      break;
-    }
-    case ACT_GELU_TANH: {
-      constexpr float c = 0.79788456080286535588f;
-      float const p = sigmoid_f32(2.0f * c * v * fmaf(0.044715f * v, v, 1.0f));
-      a = gelu_tanh_f32(v);
-      d = p * fmaf(2.0f * c * v * fmaf(3.0f * 0.044715f * v, v, 1.0f), 1.0f - p, 1.0f);
-      break;
-    }
-    default: {
-      float const p = 0.5f * erfcf(-0.70710678118654752440f * v);
-      a = act_gelu_erf(v), d = fmaf(v * 0.39894228040143267794f, exp_f32(-0.5f * v * v), p);
-    }
-  }
-}
-
-template <class T, Output OUT> __global__ __launch_bounds__(256) void product(Product p, Outputs o) {
-  constexpr bool PAIR = OUT == OUT_PAIR;
-  __shared__ float as[PAIR ? 2 : 1][kDepth][kTile + 4], bs[kDepth][kTile + 4];
-  int64_t const m0 = int64_t(blockIdx.y) * kTile, n0 = int64_t(blockIdx.x) * kTile;
-  int const ty = threadIdx.x / 16, tx = threadIdx.x % 16;
-  float acc[PAIR ? 2 : 1][4][4] = {};
-  for (int term = 0; term < p.terms; term++) {
-    for (int64_t k0 = 0; k0 < p.k; k0 += kDepth) {
-      auto stage = [&](Operand const& from, int64_t first, int64_t end, float (&to)[kDepth][kTile + 4]) {
-        for (int e = threadIdx.x; e < kTile * kDepth; e += 256) {
-          // (neighbouring lanes along the contiguous dimension)
-          int const i = from.row == 1 ? e % kTile : e / kDepth, k = from.row == 1 ? e / kTile : e % kDepth;
-          bool const in = first + i < end && k0 + k < p.k;
-          to[k][i] = in ? float(static_cast<T const*>(from.p)[(first + i) * from.row + (k0 + k) * from.step]) : 0.0f;
-        }
-      };
-      stage(p.a[term], m0, p.rows, as[0]);
-      if constexpr (PAIR) stage(p.a2, m0, p.rows, as[1]);
-      stage(p.b[term], n0, p.columns, bs);
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < kDepth; k++)
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            acc[0][i][j] = fmaf(as[0][k][ty * 4 + i], bs[k][tx * 4 + j], acc[0][i][j]);
-            if constexpr (PAIR) acc[1][i][j] = fmaf(as[1][k][ty * 4 + i], bs[k][tx * 4 + j], acc[1][i][j]);
-          }
-      __syncthreads();
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      int64_t const m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (m >= p.rows || n >= p.columns) continue;
-      float v = acc[0][i][j], a, d;
-      if constexpr (OUT != OUT_STATES)
-        if (o.bias != nullptr) v += float(static_cast<T const*>(o.bias)[m]);
-      if constexpr (OUT == OUT_PAIR) {
-        float u = acc[1][i][j];
-        if (o.bias2 != nullptr) u += float(static_cast<T const*>(o.bias2)[m]);
-        activation(o.act, o.slope, v, a, d);
-        if (o.g != nullptr) {
-          static_cast<T*>(o.g)[m * o.ld_states + n] = T(v);
-          static_cast<T*>(o.u)[m * o.ld_states + n] = T(u);
-        }
-        v = a * u;
-      }
-      if constexpr (OUT == OUT_STATES) {
-        activation(o.act, o.slope, float(static_cast<T const*>(o.g)[m * o.ld_states + n]), a, d);
-        static_cast<T*>(o.dg)[m * o.ld_gradients + n] = T(v * float(static_cast<T const*>(o.u)[m * o.ld_states + n]) * d);
-        static_cast<T*>(o.du)[m * o.ld_gradients + n] = T(v * a);
-      } else {
-        static_cast<T*>(o.y)[m * o.ld + n] = T(v);
-      }
-    }
+// Rows of a strided array at strides of whole pieces.
+template <class T> __global__ __launch_bounds__(256) void align_rows(T const* from, int64_t ld, int64_t columns, T* to, int64_t ld_to) {
+  constexpr int N = 16 / sizeof(T);
+  int64_t const c = (int64_t(blockIdx.x) * 256 + threadIdx.x) * N, row = blockIdx.y;
+  if (c >= columns) return;
+  Pack<T, N> v;
+  v.load(from + row * ld + c, columns - c < N ? int(columns - c) : N, 0.0f);
+  v.store(to + row * ld_to + c, N);
 }
 
 // y[row] = the sum of a row.
 template <class T> __global__ __launch_bounds__(256) void row_sums(T const* x, int64_t ld, int64_t columns, T* y) {
+  constexpr int N = 16 / sizeof(T);
   __shared__ float lds[4];
   T const* row = x + int64_t(blockIdx.x) * ld;
-  float s = 0.0f;
-  for (int64_t c = threadIdx.x; c < columns; c += 256) s += float(row[c]);
-  for (int d = 1; d < 64; d *= 2) s += __shfl_xor(s, d);
-  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = s;
+  float s[N] = {};
+  for (int64_t c = threadIdx.x * N; c < columns; c += 256 * N) {
+    Pack<T, N> v;
+    v.load(row + c, columns - c < N ? int(columns - c) : N, 0.0f);
+#pragma unroll
+    for (int e = 0; e < N; e++) s[e] += v[e];
+  }
+  float t = 0.0f;
+#pragma unroll
+  for (int e = 0; e < N; e++) t += s[e];
+  for (int d = 1; d < 64; d *= 2) t += __shfl_xor(t, d);
+  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = t;
   __syncthreads();
   if (threadIdx.x == 0) y[blockIdx.x] = T((lds[0] + lds[1]) + (lds[2] + lds[3]));
 }
 
-template <class T, Output OUT> hipError_t launch_product(Product const& p, Outputs const& o, hipStream_t stream) {
-  int64_t const x = (p.columns + kTile - 1) / kTile, y = (p.rows + kTile - 1) / kTile;
-  if (x > int64_t(UINT32_MAX) / 256 / y || y > 65535) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL((product<T, OUT>), dim3(unsigned(x), unsigned(y)), dim3(256), 0, stream, p, o);
-  return hipGetLastError();
+int64_t round_to(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+int64_t element(ponni_gated const& b) { return b.dtype == PONNI_F32 ? 4 : 2; }
+// Row strides of the library's own arrays: whole lines of 128 bytes.
+int64_t own_stride(int64_t columns, int64_t es) { return round_to(columns, 128 / es); }
+
+// Tiles and parts of k of a product C [rows, columns] x problems over `steps` steps.  Times in us a step of a tile,
+// and to begin and end one.
+struct Choice {
+  bool large;
+  int parts;
+};
+constexpr int kMostParts = 16, kLeastSteps = 8;
+constexpr int64_t kMostSums = int64_t(256) * 256 * 256 * 4;  // bytes: of as many tiles as run at once
+
+Choice choose(int64_t es, int64_t rows, int64_t columns, int problems, int64_t steps, bool pair, bool may_split) {
+  Choice best{false, 1};
+  double least = 1e300;
+  for (int large = 0; large <= (es == 2 ? 1 : 0); large++) {
+    int64_t const bm = (large ? 256 : 128) / (pair ? 2 : 1), bn = large || (pair && es == 4) ? 256 : 128,
+                  at_once = large || (pair && es == 4) ? 256 : 512;
+    int64_t const tiles = (rows + bm - 1) / bm * ((columns + bn - 1) / bn) * problems;
+    for (int parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      if (parts > 1 && (!may_split || steps / parts < kLeastSteps || tiles * parts > at_once)) break;
+      int64_t const groups = tiles * parts, rounds = (groups + at_once - 1) / at_once;
+      double const step = large ? 1.0 : groups <= 256 ? 0.4 : 0.62;
+      double time = double(rounds) * (double((steps + parts - 1) / parts) * step + 5.0);
+      if (parts > 1) time += 4.0 + double(parts + 1) * double(rows * columns * problems) * 4.0 / 3e6;
+      if (time < least) least = time, best = {large != 0, parts};
+    }
+  }
+  return best;
 }
 
-int64_t padded(int64_t columns) { return (columns + 63) / 64 * 64; }
-int64_t element(ponni_gated const& b) { return b.dtype == PONNI_F32 ? 4 : 2; }
+// The caller's work buffer, taken piece by piece (base null: counted only).
+struct Taker {
+  char* base;
+  int64_t used = 0;
+  char* take(int64_t bytes) {
+    char* const p = base + used;
+    used += round_to(bytes, 256);
+    return p;
+  }
+};
+
+struct Matrix {
+  void const* p;
+  int64_t rows, columns, ld;
+};
+
+int64_t aligned_bytes(int64_t rows, int64_t columns, int64_t es) { return rows * own_stride(columns, es) * es; }
+// At most, for any number of columns up to the one given.
+int64_t sums_bytes(int64_t rows, int64_t columns, int problems, int64_t steps) {
+  int64_t const parts = std::min<int64_t>(kMostParts, steps / kLeastSteps);
+  return parts < 2 ? 0 : std::min(kMostSums, parts * problems * rows * round_to(columns, 4) * 4);
+}
+
+// One call's products.
+template <class T> struct Run {
+  Taker work;
+  hipStream_t stream;
+  hipError_t err = hipSuccess;
+
+  static bool in_place(Matrix const& m) {
+    return reinterpret_cast<uint64_t>(m.p) % 16 == 0 && (m.rows == 1 || m.ld * int64_t(sizeof(T)) % 16 == 0);
+  }
+  Side side(Matrix const& m) {
+    if (!in_place(m)) return copied(m);
+    constexpr int64_t ES = sizeof(T);
+    int64_t const ld = m.rows == 1 ? round_to(m.columns, 16 / ES) : m.ld;
+    return {static_cast<char const*>(m.p), ld * ES, round_to(((m.rows - 1) * ld + m.columns) * ES, 16), m.rows};
+  }
+  // Two arrays of one shape, of one stride.
+  void sides(Matrix const& a, Matrix const& b, Side (&out)[2]) {
+    bool const both = in_place(a) && in_place(b) && (a.rows == 1 || a.ld == b.ld);
+    out[0] = both ? side(a) : copied(a), out[1] = both ? side(b) : copied(b);
+  }
+  Side copied(Matrix const& m) {
+    constexpr int64_t ES = sizeof(T);
+    int64_t const ld = own_stride(m.columns, ES);
+    T* const to = reinterpret_cast<T*>(work.take(m.rows * ld * ES));
+    constexpr int64_t ROWS = 65535;
+    for (int64_t row = 0; row < m.rows && err == hipSuccess; row += ROWS) {
+      dim3 const grid(unsigned((m.columns * ES + 4095) / 4096), unsigned(std::min(ROWS, m.rows - row)));
+      hipLaunchKernelGGL(align_rows<T>, grid, dim3(256), 0, stream, static_cast<T const*>(m.p) + row * m.ld, m.ld, m.columns,
+                         to + row * ld, ld);
+      err = hipGetLastError();
+    }
+    return {reinterpret_cast<char const*>(to), ld * ES, round_to(((m.rows - 1) * ld + m.columns) * ES, 16), m.rows};
+  }
+  void product(Form form, ProductArgs p) {
+    if (err != hipSuccess) return;
+    constexpr int64_t ES = sizeof(T), STEP = 64 / ES;
+    bool const pair = form == FORM_PAIR, plain = !pair && form != FORM_STATES;
+    if (p.terms == 0) p.terms = 1;
+    if (p.problems == 0) p.problems = 1;
+    Choice const c = choose(ES, p.rows, p.columns, p.problems, p.terms * ((p.k + STEP - 1) / STEP), pair, plain);
+    p.parts = c.parts;
+    Taker const before = work;  // (the sums are read before the next product begins)
+    if (c.parts > 1) {
+      p.ld_sums = round_to(p.columns, 4);
+      p.sums = reinterpret_cast<float*>(work.take(c.parts * p.problems * p.rows * p.ld_sums * 4));
+    }
+    err = (std::is_same_v<T, float>      ? launch_product_f32
+           : std::is_same_v<T, _Float16> ? launch_product_f16
+                                         : launch_product_bf16)(form, c.large, p, stream);
+    work = before;
+  }
+  void sums(void* y, void const* x, int64_t rows, int64_t ld, int64_t columns) {
+    if (y == nullptr || err != hipSuccess) return;
+    hipLaunchKernelGGL(row_sums<T>, dim3(unsigned(rows)), dim3(256), 0, stream, static_cast<T const*>(x), ld, columns,
+                       static_cast<T*>(y));
+    err = hipGetLastError();
+  }
+};
+
+int64_t steps_of(int64_t k, int64_t es) { return (k + 64 / es - 1) / (64 / es); }
 
 }  // namespace
 
 int64_t gated_workspace_bytes(ponni_gated const& b, int64_t columns, bool backward) {
-  return padded(columns) * b.n_hidden * element(b) * (backward ? 2 : 1);
+  int64_t const es = element(b), i = b.n_in, h = b.n_hidden, o = b.n_out;
+  Taker t{nullptr};
+  // Copies of operands, for the arrays that need them.
+  t.take(aligned_bytes(i, h, es));
+  t.take(aligned_bytes(i, h, es));
+  t.take(aligned_bytes(h, o, es));
+  t.take(aligned_bytes(i, columns, es));
+  t.take(aligned_bytes(h, columns, es));  // h itself, or a copy of the states'
+  if (!backward) {
+    t.take(sums_bytes(o, columns, 1, steps_of(h, es)));
+    return t.used;
+  }
+  t.take(aligned_bytes(o, columns, es));
+  t.take(aligned_bytes(2 * h, columns, es));  // dg, du
+  t.take(std::max({sums_bytes(i, columns, 1, 2 * steps_of(h, es)), sums_bytes(i, h, 2, steps_of(columns, es)),
+                   sums_bytes(h, o, 1, steps_of(columns, es))}));
+  return t.used;
 }
 
 hipError_t launch_gated(ponni_gated const& b, int act, void const* x, int64_t ld_x, void* y, int64_t ld_y, void* states,
@@ -157,19 +190,24 @@ hipError_t launch_gated(ponni_gated const& b, int act, void const* x, int64_t ld
   hipError_t err = hipSuccess;
   with_dtype(b.dtype, [&](auto e) {
     using T = decltype(e);
+    Run<T> run{{static_cast<char*>(workspace)}, stream};
+    int64_t const hidden = b.n_hidden, es = sizeof(T);
     T* const s = static_cast<T*>(states);
-    int64_t const ld_h = s != nullptr ? ld_states : padded(columns);
-    T* const h = s != nullptr ? s + 2 * b.n_hidden * ld_states : static_cast<T*>(workspace);
-    Outputs o{};
-    o.y = h, o.ld = ld_h, o.bias = b.gate_bias, o.bias2 = b.up_bias, o.act = act, o.slope = float(b.act.attr[0]);
-    if (s != nullptr) o.g = s, o.u = s + b.n_hidden * ld_states, o.ld_states = ld_states;
-    err = launch_product<T, OUT_PAIR>({{{b.gate, 1, b.ld_gate}}, {{x, 1, ld_x}}, {b.up, 1, b.ld_up}, b.n_in, 1, b.n_hidden,
-                                       columns}, o, stream);
-    if (err != hipSuccess) return;
-    Outputs last{};
-    last.y = y, last.ld = ld_y, last.bias = b.down_bias;
-    err = launch_product<T, OUT_PLAIN>({{{b.down, 1, b.ld_down}}, {{h, 1, ld_h}}, {}, b.n_hidden, 1, b.n_out, columns}, last,
-                                       stream);
+    int64_t const ld_h = s != nullptr ? ld_states : own_stride(columns, es);
+    T* const h = s != nullptr ? s + 2 * hidden * ld_states : reinterpret_cast<T*>(run.work.take(hidden * ld_h * es));
+    ProductArgs p{};
+    run.sides({b.gate, b.n_in, hidden, b.ld_gate}, {b.up, b.n_in, hidden, b.ld_up}, p.a);
+    p.b[0] = run.side({x, b.n_in, columns, ld_x});
+    p.k = b.n_in, p.rows = hidden, p.columns = columns;
+    p.y[0] = h, p.ld[0] = ld_h, p.bias[0] = b.gate_bias, p.bias[1] = b.up_bias;
+    p.act = act, p.slope = float(b.act.attr[0]), p.states = s, p.ld_states = ld_states;
+    run.product(FORM_PAIR, p);
+    ProductArgs q{};
+    q.a[0] = run.side({b.down, hidden, b.n_out, b.ld_down});
+    q.b[0] = run.side({h, hidden, columns, ld_h});
+    q.k = hidden, q.rows = b.n_out, q.columns = columns, q.y[0] = y, q.ld[0] = ld_y, q.bias[0] = b.down_bias;
+    run.product(FORM_FORWARD, q);
+    err = run.err;
   });
   return err;
 }
@@ -180,34 +218,47 @@ hipError_t launch_gated_backward(ponni_gated const& b, int act, void const* x, i
   hipError_t err = hipSuccess;
   with_dtype(b.dtype, [&](auto e) {
     using T = decltype(e);
-    T* const s = static_cast<T*>(const_cast<void*>(states));
-    int64_t const ld = padded(columns), hidden = b.n_hidden;
-    T *const dg = static_cast<T*>(workspace), *const du = dg + hidden * ld;
-    auto run = [&](auto out, Product const& p, Outputs const& o) {
-      if (err == hipSuccess) err = launch_product<T, decltype(out)::value>(p, o, stream);
-    };
-    auto plain = [&](void* y, int64_t ld_y, Product const& p) {
-      Outputs o{};
-      o.y = y, o.ld = ld_y;
-      if (y != nullptr) run(std::integral_constant<Output, OUT_PLAIN>{}, p, o);
-    };
-    auto sums = [&](void* y, T const* from, int64_t rows, int64_t ld_from) {
-      if (y == nullptr || err != hipSuccess) return;
-      hipLaunchKernelGGL(row_sums<T>, dim3(unsigned(rows)), dim3(256), 0, stream, from, ld_from, columns, static_cast<T*>(y));
-      err = hipGetLastError();
-    };
-    Outputs o{};
-    o.act = act, o.slope = float(b.act.attr[0]), o.g = s, o.u = s + hidden * ld_states, o.ld_states = ld_states;
-    o.dg = dg, o.du = du, o.ld_gradients = ld;
-    run(std::integral_constant<Output, OUT_STATES>{},
-        {{{b.down, b.ld_down, 1}}, {{dy, 1, ld_dy}}, {}, b.n_out, 1, hidden, columns}, o);
-    plain(d.x, d.ld_x, {{{b.gate, b.ld_gate, 1}, {b.up, b.ld_up, 1}}, {{dg, 1, ld}, {du, 1, ld}}, {}, hidden, 2, b.n_in, columns});
-    plain(d.gate, d.ld_gate, {{{x, ld_x, 1}}, {{dg, ld, 1}}, {}, columns, 1, b.n_in, hidden});
-    plain(d.up, d.ld_up, {{{x, ld_x, 1}}, {{du, ld, 1}}, {}, columns, 1, b.n_in, hidden});
-    plain(d.down, d.ld_down, {{{s + 2 * hidden * ld_states, ld_states, 1}}, {{dy, ld_dy, 1}}, {}, columns, 1, hidden, b.n_out});
-    sums(d.gate_bias, dg, hidden, ld);
-    sums(d.up_bias, du, hidden, ld);
-    sums(d.down_bias, static_cast<T const*>(dy), b.n_out, ld_dy);
+    Run<T> run{{static_cast<char*>(workspace)}, stream};
+    int64_t const hidden = b.n_hidden, es = sizeof(T), ld = own_stride(columns, es);
+    T const* const s = static_cast<T const*>(states);
+    T *const dg = reinterpret_cast<T*>(run.work.take(2 * hidden * ld * es)), *const du = dg + hidden * ld;
+    Matrix const m_dy{dy, b.n_out, columns, ld_dy};
+    Side const s_dy = run.side(m_dy);
+    ProductArgs p{};
+    p.a[0] = run.side({b.down, hidden, b.n_out, b.ld_down});
+    p.b[0] = s_dy;
+    p.k = b.n_out, p.rows = hidden, p.columns = columns, p.y[0] = dg, p.y[1] = du, p.ld[0] = ld;
+    p.act = act, p.slope = float(b.act.attr[0]), p.states = const_cast<T*>(s), p.ld_states = ld_states;
+    run.product(FORM_STATES, p);
+    Side const s_dg = run.side({dg, hidden, columns, ld}), s_du = run.side({du, hidden, columns, ld});
+    if (d.x != nullptr) {
+      ProductArgs q{};
+      run.sides({b.gate, b.n_in, hidden, b.ld_gate}, {b.up, b.n_in, hidden, b.ld_up}, q.a);
+      q.b[0] = s_dg, q.b[1] = s_du, q.terms = 2, q.k = hidden, q.rows = b.n_in, q.columns = columns;
+      q.y[0] = d.x, q.ld[0] = d.ld_x;
+      run.product(FORM_INPUT, q);
+    }
+    if (d.gate != nullptr || d.up != nullptr) {
+      ProductArgs q{};
+      q.a[0] = run.side({x, b.n_in, columns, ld_x});
+      q.k = columns, q.rows = b.n_in, q.columns = hidden;
+      int n = 0;
+      if (d.gate != nullptr) q.b[n] = s_dg, q.y[n] = d.gate, q.ld[n] = d.ld_gate, n++;
+      if (d.up != nullptr) q.b[n] = s_du, q.y[n] = d.up, q.ld[n] = d.ld_up, n++;
+      q.problems = n;
+      run.product(FORM_WEIGHTS, q);
+    }
+    if (d.down != nullptr) {
+      ProductArgs q{};
+      q.a[0] = run.side({s + 2 * hidden * ld_states, hidden, columns, ld_states});
+      q.b[0] = s_dy;
+      q.k = columns, q.rows = hidden, q.columns = b.n_out, q.y[0] = d.down, q.ld[0] = d.ld_down;
+      run.product(FORM_WEIGHTS, q);
+    }
+    run.sums(d.gate_bias, dg, hidden, ld, columns);
+    run.sums(d.up_bias, du, hidden, ld, columns);
+    run.sums(d.down_bias, dy, b.n_out, ld_dy, columns);
+    err = run.err;
   });
   return err;
 }

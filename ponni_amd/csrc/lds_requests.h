@@ -25,8 +25,8 @@ __device__ inline void dma4(void const* g, unsigned lds) {
 // At most N requests of this wave outstanding, and its LDS accesses done.
 template <int N>
 __device__ inline void wait_requests() {
-  static_assert(N >= 0 && N < 16, "vmcnt field");
-  __builtin_amdgcn_s_waitcnt(0x0070 | N);
+  static_assert(N >= 0 && N < 64, "vmcnt field");
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
 }
 // This wave's LDS reads have their data.
 __device__ inline void wait_lds() {
