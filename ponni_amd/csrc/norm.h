@@ -41,20 +41,49 @@ struct NormArgs {
 // One float per feature, `otherwise` where there is no array.
 __device__ inline float feature(float const* p, int row, float otherwise) { return p != nullptr ? p[row] : otherwise; }
 
-// The workgroup's sums of NC values per lane over the lanes that share columns.
+__device__ inline float swap_add32(float a, float b) {  // lanes 0-31: the sum of a over lanes 32 apart, others: of b
+  auto const r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ inline float swap_add16(float a, float b) {  // the same of even and odd rows of 16
+  auto const r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The workgroup's sums of NC values per lane over the lanes that share columns.  Within a wave each exchange halves
+// the columns that a lane holds (8: 15 instructions, where every lane's sum of each would be 24 exchanges through LDS).
 template <int NC> struct Reducer {
   float (*lds)[kWaves][8 * NC];  // [4]: a sum's area is written again four sums later
   int across, tx, next;
   __device__ void sum(float (&v)[NC]) {
-    for (int d = across; d < 64; d *= 2)
-#pragma unroll
-      for (int j = 0; j < NC; j++) v[j] += __shfl_xor(v[j], d);
     int const lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float t;
+    int column = 0, d = 32;
+    if constexpr (NC == 1) {
+      t = v[0];
+    } else {
+      float h[NC / 2];
+#pragma unroll
+      for (int j = 0; j < NC / 2; j++) h[j] = swap_add32(v[j], v[j + NC / 2]);
+      float q[NC / 4];
+#pragma unroll
+      for (int j = 0; j < NC / 4; j++) q[j] = swap_add16(h[j], h[j + NC / 4]);
+      column = (lane >> 5) * (NC / 2) + (lane >> 4 & 1) * (NC / 4);
+      t = q[0];
+      d = 8;
+      if constexpr (NC == 8) {
+        bool const upper = lane & 8;
+        float const mine = upper ? q[1] : q[0], other = upper ? q[0] : q[1];
+        t = mine + __shfl_xor(other, 8);
+        column += lane >> 3 & 1;
+        d = 4;
+      }
+    }
+    for (; d >= across; d /= 2) t += __shfl_xor(t, d);
     auto& area = lds[next];
     next = (next + 1) & 3;
-    if (lane < across)
-#pragma unroll
-      for (int j = 0; j < NC; j++) area[wave][tx * NC + j] = v[j];
+    constexpr int SHARED = NC == 8 ? 8 : NC == 4 ? 16 : 64;  // lanes from here on hold other columns
+    if ((lane & (SHARED - 1)) < across) area[wave][tx * NC + column] = t;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < NC; j++) {
@@ -66,62 +95,84 @@ template <int NC> struct Reducer {
   }
 };
 
-template <class T, int NC, int STEPS, bool HELD, bool GATE>
-__global__ __launch_bounds__(kThreads) void residual_norm(NormArgs a) {
+// Workgroup b of n: those of an XCD (they go to the eight in turn) are consecutive, since tiles side by side
+// share the lines of their rows.
+__device__ inline int64_t by_xcd(int64_t b, int64_t n) {
+  int64_t const q = n / 8, rest = n % 8, xcd = b % 8;
+  return xcd * q + (xcd < rest ? xcd : rest) + b / 8;
+}
+
+// A lane's rows of one array: row ty + i * down at at(i).
+template <class T> struct Rows {
+  T* p;
+  int64_t stride;
+  __device__ Rows(void const* base, int64_t ld, int ty, int down, int64_t c0)
+      : p(static_cast<T*>(const_cast<void*>(base)) + ty * ld + c0), stride(down * ld) {}
+  __device__ T* at(int i) const { return p + i * stride; }
+};
+
+// LAYER: one of the norms is a layer norm (else the means are zero).
+template <class T, int NC, int STEPS, bool HELD, bool GATE, bool LAYER>
+__global__ __launch_bounds__(kThreads, (HELD && STEPS > 4) || GATE ? 2 : 4) void residual_norm(NormArgs a) {
   auto const& r = a.r;
   __shared__ float lds[4][kWaves][8 * NC];
   int const across = 1 << a.lane_columns, tx = threadIdx.x & (across - 1), ty = threadIdx.x >> a.lane_columns;
   int const down = kThreads >> a.lane_columns, n = r.n;
   Reducer<NC> reduce{lds, across, tx, 0};
-  int64_t const c0 = (int64_t(blockIdx.x) * across + tx) * NC, left = r.columns - c0;
+  int64_t const c0 = (by_xcd(blockIdx.x, gridDim.x) * across + tx) * NC, left = r.columns - c0;
   int const count = left < 1 ? 0 : left < NC ? int(left) : NC;
   float const inv_n = 1.0f / float(n);
+  Rows<T> const rows_x(r.x, r.ld_x, ty, down, c0), rows_r(r.residual, r.ld_residual, ty, down, c0),
+      rows_g(r.gate, r.ld_gate, ty, down, c0);
   Pack<T, NC> x[STEPS], res[STEPS], gate[GATE ? STEPS : 1];
   auto load = [&](int chunk, bool all) {
 #pragma unroll
     for (int s = 0; s < STEPS; s++) {
-      int64_t const row = (chunk * STEPS + s) * down + ty;
+      int const i = chunk * STEPS + s;
       res[s].fill(0.0f);
-      if (row >= n || count == 0) continue;
-      x[s].load(static_cast<T const*>(r.x) + row * r.ld_x + c0, count, 0.0f);
-      if (all && r.residual != nullptr)
-        res[s].load(static_cast<T const*>(r.residual) + row * r.ld_residual + c0, count, 0.0f);
+      if (i * down + ty >= n || count == 0) continue;
+      x[s].load(rows_x.at(i), count, 0.0f);
+      if (all && r.residual != nullptr) res[s].load(rows_r.at(i), count, 0.0f);
       if constexpr (GATE)
-        if (all) gate[s].load(static_cast<T const*>(r.gate) + row * r.ld_gate + c0, count, 0.0f);
+        if (all) gate[s].load(rows_g.at(i), count, 0.0f);
     }
   };
-  // f(step, row) for this lane's rows, whose data is in registers.
+  // f(step, row's index) for this lane's rows, whose data is in registers.
   auto each = [&](bool all, auto&& f) {
     for (int chunk = 0; chunk < a.chunks; chunk++) {
       if (!HELD) load(chunk, all);
 #pragma unroll
       for (int s = 0; s < STEPS; s++) {
-        int const row = (chunk * STEPS + s) * down + ty;
+        int const i = chunk * STEPS + s;
         x[s].pin();
         res[s].pin();
-        if (row < n && count > 0) f(s, row);
+        if (i * down + ty < n && count > 0) f(s, i);
       }
     }
   };
   if (HELD) load(0, true);
-  float m1[NC], r1[NC], m2[NC], r2[NC];
+  float m1[LAYER ? NC : 1] = {}, m2[LAYER ? NC : 1] = {}, r1[NC], r2[NC];
+  auto mean1 = [&](int j) { return LAYER ? m1[j] : 0.0f; };
+  auto mean2 = [&](int j) { return LAYER ? m2[j] : 0.0f; };
 #pragma unroll
-  for (int j = 0; j < NC; j++) m1[j] = m2[j] = 0.0f, r1[j] = r2[j] = 1.0f;
-  if (r.after.kind == PONNI_NORM_LAYER) {
-    each(false, [&](int s, int) {
+  for (int j = 0; j < NC; j++) r1[j] = r2[j] = 1.0f;
+  if constexpr (LAYER) {
+    if (r.after.kind == PONNI_NORM_LAYER) {
+      each(false, [&](int s, int) {
 #pragma unroll
-      for (int j = 0; j < NC; j++) m1[j] += x[s][j];
-    });
-    reduce.sum(m1);
+        for (int j = 0; j < NC; j++) m1[j] += x[s][j];
+      });
+      reduce.sum(m1);
 #pragma unroll
-    for (int j = 0; j < NC; j++) m1[j] *= inv_n;
+      for (int j = 0; j < NC; j++) m1[j] *= inv_n;
+    }
   }
   if (r.after.kind != PONNI_NORM_NONE) {
     float v[NC] = {};
     each(false, [&](int s, int) {
 #pragma unroll
       for (int j = 0; j < NC; j++) {
-        float const d = x[s][j] - m1[j];
+        float const d = x[s][j] - mean1(j);
         v[j] = fmaf(d, d, v[j]);
       }
     });
@@ -129,35 +180,38 @@ __global__ __launch_bounds__(kThreads) void residual_norm(NormArgs a) {
 #pragma unroll
     for (int j = 0; j < NC; j++) r1[j] = 1.0f / sqrtf(fmaf(v[j], inv_n, r.after.eps));
   }
-  auto state = [&](int s, int row, float (&v)[NC]) {
+  auto state = [&](int s, int i, float (&v)[NC]) {
+    int const row = i * down + ty;
     float const w = feature(r.after.weight, row, 1.0f), b = feature(r.after.bias, row, 0.0f);
     float const g = r.scale * feature(r.feature_gate, row, 1.0f);
 #pragma unroll
     for (int j = 0; j < NC; j++) {
-      float const branch = fmaf((x[s][j] - m1[j]) * r1[j], w, b);
+      float const branch = fmaf((x[s][j] - mean1(j)) * r1[j], w, b);
       if constexpr (GATE) v[j] = fmaf(g * gate[s][j], branch, res[s][j]);
       else v[j] = fmaf(g, branch, res[s][j]);
     }
   };
-  if (r.before.kind == PONNI_NORM_LAYER) {
-    each(true, [&](int s, int row) {
-      float v[NC];
-      state(s, row, v);
+  if constexpr (LAYER) {
+    if (r.before.kind == PONNI_NORM_LAYER) {
+      each(true, [&](int s, int i) {
+        float v[NC];
+        state(s, i, v);
 #pragma unroll
-      for (int j = 0; j < NC; j++) m2[j] += v[j];
-    });
-    reduce.sum(m2);
+        for (int j = 0; j < NC; j++) m2[j] += v[j];
+      });
+      reduce.sum(m2);
 #pragma unroll
-    for (int j = 0; j < NC; j++) m2[j] *= inv_n;
+      for (int j = 0; j < NC; j++) m2[j] *= inv_n;
+    }
   }
   if (r.before.kind != PONNI_NORM_NONE) {
     float q[NC] = {};
-    each(true, [&](int s, int row) {
+    each(true, [&](int s, int i) {
       float v[NC];
-      state(s, row, v);
+      state(s, i, v);
 #pragma unroll
       for (int j = 0; j < NC; j++) {
-        float const d = v[j] - m2[j];
+        float const d = v[j] - mean2(j);
         q[j] = fmaf(d, d, q[j]);
       }
     });
@@ -165,20 +219,22 @@ __global__ __launch_bounds__(kThreads) void residual_norm(NormArgs a) {
 #pragma unroll
     for (int j = 0; j < NC; j++) r2[j] = 1.0f / sqrtf(fmaf(q[j], inv_n, r.before.eps));
   }
-  each(true, [&](int s, int row) {
+  Rows<T> const rows_s(r.state, r.ld_state, ty, down, c0), rows_n(r.normed, r.ld_normed, ty, down, c0);
+  each(true, [&](int s, int i) {
     float v[NC];
-    state(s, row, v);
+    state(s, i, v);
     Pack<T, NC> o;
     if (r.state != nullptr) {
 #pragma unroll
       for (int j = 0; j < NC; j++) o.set(j, v[j]);
-      o.store(static_cast<T*>(r.state) + row * r.ld_state + c0, count);
+      o.store(rows_s.at(i), count);
     }
     if (r.normed != nullptr) {
+      int const row = i * down + ty;
       float const w = feature(r.before.weight, row, 1.0f), b = feature(r.before.bias, row, 0.0f);
 #pragma unroll
-      for (int j = 0; j < NC; j++) o.set(j, fmaf((v[j] - m2[j]) * r2[j], w, b));
-      o.store(static_cast<T*>(r.normed) + row * r.ld_normed + c0, count);
+      for (int j = 0; j < NC; j++) o.set(j, fmaf((v[j] - mean2(j)) * r2[j], w, b));
+      o.store(rows_n.at(i), count);
     }
   });
   if (r.statistics != nullptr && ty == 0)
@@ -186,11 +242,12 @@ __global__ __launch_bounds__(kThreads) void residual_norm(NormArgs a) {
     for (int j = 0; j < NC; j++)
       if (j < count) {
         float* at = r.statistics + c0 + j;
-        at[0] = m1[j], at[r.columns] = r1[j], at[2 * r.columns] = m2[j], at[3 * r.columns] = r2[j];
+        at[0] = mean1(j), at[r.columns] = r1[j], at[2 * r.columns] = mean2(j), at[3 * r.columns] = r2[j];
       }
 }
 
-template <class T, int NC, int STEPS, bool HELD, bool GATE>
+// AFTER: there is a norm after the block.
+template <class T, int NC, int STEPS, bool HELD, bool GATE, bool LAYER, bool AFTER>
 __global__ __launch_bounds__(kThreads) void residual_norm_backward(NormArgs a) {
   auto const& r = a.r;
   auto const& g = a.g;
@@ -199,7 +256,8 @@ __global__ __launch_bounds__(kThreads) void residual_norm_backward(NormArgs a) {
   int const down = kThreads >> a.lane_columns, n = r.n;
   Reducer<NC> reduce{lds, across, tx, 0};
   float const inv_n = 1.0f / float(n);
-  bool const after = r.after.kind != PONNI_NORM_NONE, before = r.before.kind != PONNI_NORM_NONE && g.d_normed != nullptr;
+  bool const before = r.before.kind != PONNI_NORM_NONE && g.d_normed != nullptr;
+  constexpr int FIRST = AFTER ? 0 : NORM_SUM_GATE;  // of the sums
   float sums[STEPS][NORM_SUMS] = {};
   // This workgroup's sums of a chunk's rows, from FROM to TO.
   auto flush = [&](int chunk, int from, int to, bool first) {
@@ -207,7 +265,7 @@ __global__ __launch_bounds__(kThreads) void residual_norm_backward(NormArgs a) {
     for (int s = 0; s < STEPS; s++) {
       int const row = (chunk * STEPS + s) * down + ty;
 #pragma unroll
-      for (int q = 0; q < NORM_SUMS; q++) {
+      for (int q = FIRST; q < NORM_SUMS; q++) {
         if (q < from || q >= to) continue;
         float v = sums[s][q];
         for (int d = 1; d < across; d *= 2) v += __shfl_xor(v, d);
@@ -219,152 +277,168 @@ __global__ __launch_bounds__(kThreads) void residual_norm_backward(NormArgs a) {
       }
     }
   };
-  for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-    bool const first = tile == blockIdx.x;
+  int64_t const begin = by_xcd(blockIdx.x, gridDim.x);
+  for (int64_t tile = begin; tile < a.tiles; tile += gridDim.x) {
+    bool const first = tile == begin;
     int64_t const c0 = (tile * across + tx) * NC, left = r.columns - c0;
     int const count = left < 1 ? 0 : left < NC ? int(left) : NC;
+    Rows<T> const rows_x(r.x, r.ld_x, ty, down, c0), rows_r(r.residual, r.ld_residual, ty, down, c0),
+        rows_g(r.gate, r.ld_gate, ty, down, c0), rows_n(g.d_normed, g.ld_d_normed, ty, down, c0),
+        rows_s(g.d_state, g.ld_d_state, ty, down, c0);
     Pack<T, NC> x[STEPS], res[STEPS], dn[STEPS], gate[GATE ? STEPS : 1];
     auto load = [&](int chunk) {
 #pragma unroll
       for (int s = 0; s < STEPS; s++) {
-        int64_t const row = (chunk * STEPS + s) * down + ty;
+        int const i = chunk * STEPS + s;
         dn[s].fill(0.0f);
         res[s].fill(0.0f);
         x[s].fill(0.0f);
-        if (row >= n || count == 0) continue;
-        x[s].load(static_cast<T const*>(r.x) + row * r.ld_x + c0, count, 0.0f);
+        if (i * down + ty >= n || count == 0) continue;
+        x[s].load(rows_x.at(i), count, 0.0f);
         if (before) {
-          dn[s].load(static_cast<T const*>(g.d_normed) + row * g.ld_d_normed + c0, count, 0.0f);
-          if (r.residual != nullptr)
-            res[s].load(static_cast<T const*>(r.residual) + row * r.ld_residual + c0, count, 0.0f);
+          dn[s].load(rows_n.at(i), count, 0.0f);
+          if (r.residual != nullptr) res[s].load(rows_r.at(i), count, 0.0f);
         }
-        if constexpr (GATE) gate[s].load(static_cast<T const*>(r.gate) + row * r.ld_gate + c0, count, 0.0f);
+        if constexpr (GATE) gate[s].load(rows_g.at(i), count, 0.0f);
       }
     };
-    float m1[NC], r1[NC], m2[NC], r2[NC];
-#pragma unroll
-    for (int j = 0; j < NC; j++) {
-      bool const in = j < count;
-      m1[j] = in ? r.statistics[c0 + j] : 0.0f;
-      r1[j] = in ? r.statistics[r.columns + c0 + j] : 0.0f;
-      m2[j] = in ? r.statistics[2 * r.columns + c0 + j] : 0.0f;
-      r2[j] = in ? r.statistics[3 * r.columns + c0 + j] : 0.0f;
-    }
-    if (HELD) load(0);
-    auto unit = [&](int s, int j) { return (x[s][j] - m1[j]) * r1[j]; };
-    auto factor = [&](int s, int j, float f) {
-      if constexpr (GATE) return f * gate[s][j];
-      else return f;
-    };
-    float e2[NC] = {}, eu2[NC] = {};
-    if (before) {
+    // f(step, row's index, row) for this lane's rows, whose data is in registers; done(chunk) behind each chunk.
+    auto each = [&](auto&& f, auto&& done) {
       for (int chunk = 0; chunk < a.chunks; chunk++) {
         if (!HELD) load(chunk);
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
-          int const row = (chunk * STEPS + s) * down + ty;
-          if (row >= n || count == 0) continue;
-          float const w1 = feature(r.after.weight, row, 1.0f), b1 = feature(r.after.bias, row, 0.0f),
-                      w2 = feature(r.before.weight, row, 1.0f), f = r.scale * feature(r.feature_gate, row, 1.0f);
-#pragma unroll
-          for (int j = 0; j < NC; j++) {
-            float const st = fmaf(factor(s, j, f), fmaf(unit(s, j), w1, b1), res[s][j]);
-            float const u = (st - m2[j]) * r2[j], d = dn[s][j], e = d * w2;
-            e2[j] += e;
-            eu2[j] = fmaf(e, u, eu2[j]);
-            sums[s][NORM_SUM_W2] = fmaf(d, u, sums[s][NORM_SUM_W2]);
-            sums[s][NORM_SUM_B2] += d;
-          }
+          int const i = chunk * STEPS + s;
+          x[s].pin();
+          res[s].pin();
+          dn[s].pin();
+          if (i * down + ty < n && count > 0) f(s, i, i * down + ty);
         }
-        if (!HELD) flush(chunk, NORM_SUM_W2, NORM_SUMS, first);
+        if (!HELD) done(chunk);
       }
-      if (r.before.kind == PONNI_NORM_LAYER) reduce.sum(e2);
+    };
+    constexpr int MEANS = LAYER ? NC : 1, FIRSTS = AFTER ? NC : 1;
+    float m1[LAYER && AFTER ? NC : 1] = {}, m2[MEANS] = {}, r1[FIRSTS], r2[NC];
+#pragma unroll
+    for (int j = 0; j < NC; j++) {
+      bool const in = j < count;
+      if constexpr (LAYER && AFTER) m1[j] = in ? r.statistics[c0 + j] : 0.0f;
+      if constexpr (AFTER) r1[j] = in ? r.statistics[r.columns + c0 + j] : 0.0f;
+      if constexpr (LAYER) m2[j] = in ? r.statistics[2 * r.columns + c0 + j] : 0.0f;
+      r2[j] = in ? r.statistics[3 * r.columns + c0 + j] : 0.0f;
+    }
+    if (HELD) load(0);
+    auto unit = [&](int s, int j) {
+      if constexpr (AFTER) return (x[s][j] - (LAYER ? m1[j] : 0.0f)) * r1[j];
+      else return x[s][j];
+    };
+    auto factor = [&](int s, int j, float f) {
+      if constexpr (GATE) return f * gate[s][j];
+      else return f;
+    };
+    // What a row multiplies with.
+    struct Feature {
+      float w1, b1, w2, f;
+    };
+    auto feature_of = [&](int row) {
+      return Feature{AFTER ? feature(r.after.weight, row, 1.0f) : 1.0f, AFTER ? feature(r.after.bias, row, 0.0f) : 0.0f,
+                     feature(r.before.weight, row, 1.0f), r.scale * feature(r.feature_gate, row, 1.0f)};
+    };
+    auto branch = [&](int s, int j, Feature const& w) { return AFTER ? fmaf(unit(s, j), w.w1, w.b1) : x[s][j]; };
+    auto unit2 = [&](int s, int j, Feature const& w, float v) {
+      return (fmaf(factor(s, j, w.f), v, res[s][j]) - (LAYER ? m2[j] : 0.0f)) * r2[j];
+    };
+    float e2[MEANS] = {}, eu2[NC] = {};
+    if (before) {
+      each(
+          [&](int s, int, int row) {
+            Feature const w = feature_of(row);
+#pragma unroll
+            for (int j = 0; j < NC; j++) {
+              float const u = unit2(s, j, w, branch(s, j, w)), d = dn[s][j], e = d * w.w2;
+              if constexpr (LAYER) e2[j] += e;
+              eu2[j] = fmaf(e, u, eu2[j]);
+              sums[s][NORM_SUM_W2] = fmaf(d, u, sums[s][NORM_SUM_W2]);
+              sums[s][NORM_SUM_B2] += d;
+            }
+          },
+          [&](int chunk) { flush(chunk, NORM_SUM_W2, NORM_SUMS, first); });
+      if constexpr (LAYER) {
+        if (r.before.kind == PONNI_NORM_LAYER) reduce.sum(e2);
+#pragma unroll
+        for (int j = 0; j < NC; j++) e2[j] = r.before.kind == PONNI_NORM_LAYER ? e2[j] * inv_n : 0.0f;
+      }
       reduce.sum(eu2);
 #pragma unroll
-      for (int j = 0; j < NC; j++) {
-        e2[j] = r.before.kind == PONNI_NORM_LAYER ? e2[j] * inv_n : 0.0f;
-        eu2[j] *= inv_n;
-      }
+      for (int j = 0; j < NC; j++) eu2[j] *= inv_n;
     } else if (!HELD) {
       for (int chunk = 0; chunk < a.chunks; chunk++) flush(chunk, NORM_SUM_W2, NORM_SUMS, first);
     }
-    // D of an element, and v
-    auto gradient = [&](int s, int j, float w1, float b1, float w2, float f, float ds, float& v) {
-      v = fmaf(unit(s, j), w1, b1);
+    // D of an element from v.
+    auto gradient = [&](int s, int j, Feature const& w, float ds, float v) {
       if (!before) return ds;
-      float const u = (fmaf(factor(s, j, f), v, res[s][j]) - m2[j]) * r2[j];
-      return fmaf(r2[j], fmaf(dn[s][j], w2, -e2[j]) - u * eu2[j], ds);
+      return fmaf(r2[j], fmaf(dn[s][j], w.w2, LAYER ? -e2[j] : 0.0f) - unit2(s, j, w, v) * eu2[j], ds);
     };
-    auto load_state = [&](int64_t row) {
+    auto load_state = [&](int i) {
       Pack<T, NC> ds;
       ds.fill(0.0f);
-      if (g.d_state != nullptr) ds.load(static_cast<T const*>(g.d_state) + row * g.ld_d_state + c0, count, 0.0f);
+      if (g.d_state != nullptr) ds.load(rows_s.at(i), count, 0.0f);
       return ds;
     };
-    float e1[NC] = {}, eu1[NC] = {};
-    for (int chunk = 0; chunk < a.chunks; chunk++) {
-      if (!HELD) load(chunk);
+    Rows<T> const out_r(g.d_residual, g.ld_d_residual, ty, down, c0), out_g(g.d_gate, g.ld_d_gate, ty, down, c0),
+        out_x(g.d_x, g.ld_d_x, ty, down, c0);
+    float e1[LAYER && AFTER ? NC : 1] = {}, eu1[FIRSTS] = {};
+    each(
+        [&](int s, int i, int row) {
+          Feature const w = feature_of(row);
+          Pack<T, NC> const ds = load_state(i);
+          Pack<T, NC> o, og, ox;
 #pragma unroll
-      for (int s = 0; s < STEPS; s++) {
-        int64_t const row = (chunk * STEPS + s) * down + ty;
-        x[s].pin();
-        res[s].pin();
-        dn[s].pin();
-        if (row >= n || count == 0) continue;
-        float const w1 = feature(r.after.weight, row, 1.0f), b1 = feature(r.after.bias, row, 0.0f),
-                    w2 = feature(r.before.weight, row, 1.0f), f = r.scale * feature(r.feature_gate, row, 1.0f);
-        Pack<T, NC> const ds = load_state(row);
-        Pack<T, NC> o, og, ox;
+          for (int j = 0; j < NC; j++) {
+            float const v = branch(s, j, w), d = gradient(s, j, w, ds[j], v), dv = factor(s, j, w.f) * d;
+            o.set(j, d);
+            if constexpr (GATE) og.set(j, r.scale * d * v);
+            else sums[s][NORM_SUM_GATE] = fmaf(r.scale * d, v, sums[s][NORM_SUM_GATE]);
+            if constexpr (AFTER) {
+              float const u = unit(s, j), e = dv * w.w1;
+              if constexpr (LAYER) e1[j] += e;
+              eu1[j] = fmaf(e, u, eu1[j]);
+              sums[s][NORM_SUM_W1] = fmaf(dv, u, sums[s][NORM_SUM_W1]);
+              sums[s][NORM_SUM_B1] += dv;
+            } else {
+              ox.set(j, dv);
+            }
+          }
+          if (g.d_residual != nullptr) o.store(out_r.at(i), count);
+          if constexpr (GATE)
+            if (g.d_gate != nullptr) og.store(out_g.at(i), count);
+          if constexpr (!AFTER)
+            if (g.d_x != nullptr) ox.store(out_x.at(i), count);
+        },
+        [&](int chunk) { flush(chunk, FIRST, NORM_SUM_W2, first); });
+    if constexpr (AFTER) {
+      if (g.d_x == nullptr) continue;
+      if constexpr (LAYER) {
+        if (r.after.kind == PONNI_NORM_LAYER) reduce.sum(e1);
 #pragma unroll
-        for (int j = 0; j < NC; j++) {
-          float v;
-          float const d = gradient(s, j, w1, b1, w2, f, ds[j], v);
-          o.set(j, d);
-          float const dv = factor(s, j, f) * d, u = unit(s, j), e = dv * w1;
-          og.set(j, r.scale * d * v);
-          ox.set(j, dv);
-          e1[j] += e;
-          eu1[j] = fmaf(e, u, eu1[j]);
-          sums[s][NORM_SUM_W1] = fmaf(dv, u, sums[s][NORM_SUM_W1]);
-          sums[s][NORM_SUM_B1] += dv;
-          sums[s][NORM_SUM_GATE] = fmaf(r.scale * d, v, sums[s][NORM_SUM_GATE]);
-        }
-        if (g.d_residual != nullptr) o.store(static_cast<T*>(g.d_residual) + row * g.ld_d_residual + c0, count);
-        if constexpr (GATE)
-          if (g.d_gate != nullptr) og.store(static_cast<T*>(g.d_gate) + row * g.ld_d_gate + c0, count);
-        if (!after && g.d_x != nullptr) ox.store(static_cast<T*>(g.d_x) + row * g.ld_d_x + c0, count);
+        for (int j = 0; j < NC; j++) e1[j] = r.after.kind == PONNI_NORM_LAYER ? e1[j] * inv_n : 0.0f;
       }
-      if (!HELD) flush(chunk, NORM_SUM_W1, NORM_SUM_W2, first);
-    }
-    if (!after || g.d_x == nullptr) continue;
-    if (r.after.kind == PONNI_NORM_LAYER) reduce.sum(e1);
-    reduce.sum(eu1);
+      reduce.sum(eu1);
 #pragma unroll
-    for (int j = 0; j < NC; j++) {
-      e1[j] = r.after.kind == PONNI_NORM_LAYER ? e1[j] * inv_n : 0.0f;
-      eu1[j] *= inv_n;
-    }
-    for (int chunk = 0; chunk < a.chunks; chunk++) {
-      if (!HELD) load(chunk);
+      for (int j = 0; j < NC; j++) eu1[j] *= inv_n;
+      each(
+          [&](int s, int i, int row) {
+            Feature const w = feature_of(row);
+            Pack<T, NC> const ds = load_state(i);
+            Pack<T, NC> o;
 #pragma unroll
-      for (int s = 0; s < STEPS; s++) {
-        int64_t const row = (chunk * STEPS + s) * down + ty;
-        x[s].pin();
-        res[s].pin();
-        dn[s].pin();
-        if (row >= n || count == 0) continue;
-        float const w1 = feature(r.after.weight, row, 1.0f), b1 = feature(r.after.bias, row, 0.0f),
-                    w2 = feature(r.before.weight, row, 1.0f), f = r.scale * feature(r.feature_gate, row, 1.0f);
-        Pack<T, NC> const ds = load_state(row);
-        Pack<T, NC> o;
-#pragma unroll
-        for (int j = 0; j < NC; j++) {
-          float v;
-          float const d = gradient(s, j, w1, b1, w2, f, ds[j], v);
-          o.set(j, r1[j] * (factor(s, j, f) * d * w1 - e1[j] - unit(s, j) * eu1[j]));
-        }
-        o.store(static_cast<T*>(g.d_x) + row * g.ld_d_x + c0, count);
-      }
+            for (int j = 0; j < NC; j++) {
+              float const v = branch(s, j, w), d = gradient(s, j, w, ds[j], v);
+              o.set(j, r1[j] * (fmaf(factor(s, j, w.f) * d, w.w1, LAYER ? -e1[j] : 0.0f) - unit(s, j) * eu1[j]));
+            }
+            o.store(out_x.at(i), count);
+          },
+          [](int) {});
     }
   }
   if (HELD) flush(0, 0, NORM_SUMS, true);
@@ -380,7 +454,7 @@ struct Shape {
   int64_t tiles;
 };
 
-inline Shape shape_of(int32_t n, int64_t columns, int32_t dtype, int max_steps) {
+inline Shape shape_of(int32_t n, int64_t columns, int32_t dtype, int max_steps, int narrowest) {
   int const wide = dtype == PONNI_F32 ? 4 : 8;
   Shape s{};
   s.columns = columns < wide ? 1 : wide;
@@ -388,33 +462,45 @@ inline Shape shape_of(int32_t n, int64_t columns, int32_t dtype, int max_steps) 
   while (s.lane_columns < 3 && (1 << s.lane_columns) < lanes) s.lane_columns++;
   auto steps_at = [&](int l) { return (n + (kThreads >> l) - 1) / (kThreads >> l); };
   auto tiles_at = [&](int l) { return (lanes + (1 << l) - 1) >> l; };
-  while (s.lane_columns > 0 && (steps_at(s.lane_columns) > max_steps || tiles_at(s.lane_columns) < 256)) s.lane_columns--;
+  while (s.lane_columns > 0 && tiles_at(s.lane_columns) < 256) s.lane_columns--;
+  // In registers at 128 bytes of a row, in the forward pass down to 64; narrower pieces are slower than to read whole lines
+  // again.  us in registers / read again, bf16, 67 M elements, rms norms, forward: n = 1024 (128 bytes) 151 / 170,
+  // 2048 (64) 168 / 178, 4096 (32 bytes) 285 / 191; before only, backward: 1024 (64) 243 / 216, 4096 (16) 418 / 230.
+  if (steps_at(s.lane_columns) > max_steps && (s.lane_columns < 3 || steps_at(narrowest) <= max_steps))
+    while (s.lane_columns > 0 && steps_at(s.lane_columns) > max_steps) s.lane_columns--;
   int const steps = steps_at(s.lane_columns);
   s.tiles = tiles_at(s.lane_columns);
-  s.steps = steps <= 4 ? 4 : 8;
+  s.steps = steps <= 4 ? 4 : steps <= 8 ? 8 : 16;
   s.chunks = (steps + s.steps - 1) / s.steps;
   if (steps > max_steps) {
     s.steps = 4;
-    s.chunks = (steps + 3) / 4;
+    s.chunks = (steps + 3) / 4;  // (read again)
   }
   return s;
 }
 
 // Rows a lane can hold without spilling.
-inline int most_steps(bool backward, bool gate) { return backward && gate ? 4 : 8; }
+inline int most_steps(bool backward, bool gate) { return backward ? (gate ? 4 : 8) : gate ? 8 : 16; }
 
-template <class F> void with_steps(Shape const& s, bool gate, F&& f) {
-  auto steps = [&](auto g) {
-    if (s.chunks > 1) f(std::integral_constant<int, 4>{}, std::false_type{}, g);
-    else if (s.steps == 4) f(std::integral_constant<int, 4>{}, std::true_type{}, g);
-    else f(std::integral_constant<int, 8>{}, std::true_type{}, g);
+// f(steps, held, gate, layer) as constants.
+template <class F> void with_variant(Shape const& s, bool gate, bool layer, F&& f) {
+  auto pick = [&](auto g, auto l) {
+    if (s.chunks > 1) f(std::integral_constant<int, 4>{}, std::false_type{}, g, l);
+    else if (s.steps == 4) f(std::integral_constant<int, 4>{}, std::true_type{}, g, l);
+    else if (s.steps == 8) f(std::integral_constant<int, 8>{}, std::true_type{}, g, l);
+    else f(std::integral_constant<int, 16>{}, std::true_type{}, g, l);
   };
-  if (gate) steps(std::true_type{});
-  else steps(std::false_type{});
+  if (gate && layer) pick(std::true_type{}, std::true_type{});
+  else if (gate) pick(std::true_type{}, std::false_type{});
+  else if (layer) pick(std::false_type{}, std::true_type{});
+  else pick(std::false_type{}, std::false_type{});
+}
+inline bool has_layer(ponni_residual_norm const& r) {
+  return r.after.kind == PONNI_NORM_LAYER || r.before.kind == PONNI_NORM_LAYER;
 }
 
 template <class T> hipError_t launch_norm(ponni_residual_norm const& r, hipStream_t stream) {
-  Shape const s = shape_of(r.n, r.columns, r.dtype, most_steps(false, r.gate != nullptr));
+  Shape const s = shape_of(r.n, r.columns, r.dtype, most_steps(false, r.gate != nullptr), 2);
   NormArgs a{};
   a.r = r;
   a.lane_columns = s.lane_columns;
@@ -422,11 +508,11 @@ template <class T> hipError_t launch_norm(ponni_residual_norm const& r, hipStrea
   a.tiles = s.tiles;
   if (s.tiles > int64_t(UINT32_MAX) / kThreads) return hipErrorInvalidConfiguration;
   dim3 const grid(static_cast<unsigned>(s.tiles));
-  with_steps(s, r.gate != nullptr, [&](auto steps, auto held, auto gate) {
+  with_variant(s, r.gate != nullptr, has_layer(r), [&](auto steps, auto held, auto gate, auto layer) {
     constexpr int S = decltype(steps)::value, NC = 16 / sizeof(T);
-    constexpr bool H = decltype(held)::value, G = decltype(gate)::value;
-    if (s.columns == 1) hipLaunchKernelGGL((residual_norm<T, 1, S, H, G>), grid, dim3(kThreads), 0, stream, a);
-    else hipLaunchKernelGGL((residual_norm<T, NC, S, H, G>), grid, dim3(kThreads), 0, stream, a);
+    constexpr bool H = decltype(held)::value, G = decltype(gate)::value, L = decltype(layer)::value;
+    if (s.columns == 1) hipLaunchKernelGGL((residual_norm<T, 1, S, H, G, true>), grid, dim3(kThreads), 0, stream, a);
+    else hipLaunchKernelGGL((residual_norm<T, NC, S, H, G, L>), grid, dim3(kThreads), 0, stream, a);
   });
   return hipGetLastError();
 }
@@ -434,7 +520,7 @@ template <class T> hipError_t launch_norm(ponni_residual_norm const& r, hipStrea
 template <class T>
 hipError_t launch_norm_backward(ponni_residual_norm const& r, ponni_residual_norm_gradients const& g, void* workspace,
                                 int& groups, hipStream_t stream) {
-  Shape const s = shape_of(r.n, r.columns, r.dtype, most_steps(true, r.gate != nullptr));
+  Shape const s = shape_of(r.n, r.columns, r.dtype, most_steps(true, r.gate != nullptr), 3);
   NormArgs a{};
   a.r = r;
   a.g = g;
@@ -443,12 +529,18 @@ hipError_t launch_norm_backward(ponni_residual_norm const& r, ponni_residual_nor
   a.tiles = s.tiles;
   a.parts = static_cast<float*>(workspace);
   groups = static_cast<int>(std::min<int64_t>(s.tiles, kNormWorkgroups));
-  with_steps(s, r.gate != nullptr, [&](auto steps, auto held, auto gate) {
+  with_variant(s, r.gate != nullptr, has_layer(r), [&](auto steps, auto held, auto gate, auto layer) {
     constexpr int S = decltype(steps)::value, NC = 16 / sizeof(T);
-    constexpr bool H = decltype(held)::value, G = decltype(gate)::value;
-    if constexpr (!(G && S == 8)) {
-      if (s.columns == 1) hipLaunchKernelGGL((residual_norm_backward<T, 1, S, H, G>), dim3(groups), dim3(kThreads), 0, stream, a);
-      else hipLaunchKernelGGL((residual_norm_backward<T, NC, S, H, G>), dim3(groups), dim3(kThreads), 0, stream, a);
+    constexpr bool H = decltype(held)::value, G = decltype(gate)::value, L = decltype(layer)::value;
+    dim3 const grid(groups), block(kThreads);
+    if constexpr (!(G && S == 8) && S < 16) {
+      if (r.after.kind == PONNI_NORM_NONE) {
+        if (s.columns == 1) hipLaunchKernelGGL((residual_norm_backward<T, 1, S, H, G, true, false>), grid, block, 0, stream, a);
+        else hipLaunchKernelGGL((residual_norm_backward<T, NC, S, H, G, L, false>), grid, block, 0, stream, a);
+      } else {
+        if (s.columns == 1) hipLaunchKernelGGL((residual_norm_backward<T, 1, S, H, G, true, true>), grid, block, 0, stream, a);
+        else hipLaunchKernelGGL((residual_norm_backward<T, NC, S, H, G, L, true>), grid, block, 0, stream, a);
+      }
     }
   });
   return hipGetLastError();
