@@ -17,6 +17,8 @@ template <class T, int N> struct Pack {
   Vector v;
   __device__ float operator[](int j) const { return float(v[j]); }
   __device__ void set(int j, float x) { v[j] = T(x); }
+  __device__ void put(int j, T x) { v[j] = x; }
+  __device__ T raw(int j) const { return v[j]; }
   __device__ void fill(float x) {
 #pragma unroll
     for (int j = 0; j < N; j++) v[j] = T(x);
@@ -46,6 +48,8 @@ template <class T> struct Pack<T, 1> {
   T v;
   __device__ float operator[](int) const { return float(v); }
   __device__ void set(int, float x) { v = T(x); }
+  __device__ void put(int, T x) { v = x; }
+  __device__ T raw(int) const { return v; }
   __device__ void fill(float x) { v = T(x); }
   __device__ void load(T const* p, int, float) { v = *p; }
   __device__ void store(T* p, int) const { *p = v; }

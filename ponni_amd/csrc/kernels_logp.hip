@@ -4,7 +4,8 @@
 // One pass over x.  With m the largest x so far and t = (x - m) log2(e) a column keeps
 //   z = sum 2^t,  q = sum 2^t t,
 // which a larger m' turns into z s, (q + d z) s with d = (m - m') log2(e), s = 2^d, and
-//   log_normalizer = m + ln2 log2 z,  entropy = ln2 (log2 z - q / z).
+//   log_normalizer = m + ln2 log2 z,  entropy = ln2 (log2 z - q / z);
+// any m near the largest x serves as well.
 // (x log2(e) by itself, an operation less, has no room for the lowest floats.)
 // A lane holds NC consecutive columns (16 bytes of a row) and takes every R-th row;
 // lanes, waves and workgroups that share columns join their (m, z, q) in a fixed
@@ -34,6 +35,11 @@ struct LogpArgs {
   float* part_values;     // [splits, K, columns]
   int32_t* part_classes;  // [splits, K, columns]
 };
+
+// Rows of a turn.
+constexpr int rows_under_way(int columns, int k) { return columns == 1 && k == 0 ? 8 : 4; }
+// A column's m is its largest logit up to kSlack: few turns have to move it, and no power passes 2^6.
+constexpr float kSlack = 4.0f;
 
 // Sums of one column, and its K largest logits.
 template <int K> struct Column {
@@ -100,32 +106,82 @@ template <int K> struct Column {
   }
 };
 
-template <class T, int K> __device__ void finish(ponni_log_probs const& p, int64_t c, Column<K> const& s) {
-  float const lz = __log2f(s.z);
-  float const normalizer = fmaf(kLn2, lz, s.m);
-  p.log_normalizer[c] = normalizer;
-  p.entropy[c] = s.z == 0.0f ? 0.0f : kLn2 * (lz - s.q / s.z);
+// The results of `count` of NC columns, whole rows of them at a time.
+template <class T, int NC, int K> __device__ void finish(ponni_log_probs const& p, int64_t c, int count, Column<K> const (&s)[NC]) {
+  Pack<float, NC> normalizer, entropy, log_prob;
+#pragma unroll
+  for (int j = 0; j < NC; j++) {
+    float const lz = __log2f(s[j].z);
+    normalizer.set(j, fmaf(kLn2, lz, s[j].m));
+    entropy.set(j, s[j].z == 0.0f ? 0.0f : kLn2 * (lz - s[j].q / s[j].z));
+  }
+  normalizer.store(p.log_normalizer + c, count);
+  entropy.store(p.entropy + c, count);
   if (p.targets != nullptr) {
-    int64_t const t = p.targets[c];
-    float l = 0.0f;
-    if (t >= 0 && t < p.classes) {
-      l = static_cast<T const*>(p.logits)[t * p.ld + c];
-      if (l != -kInf) l -= normalizer;
+#pragma unroll
+    for (int j = 0; j < NC; j++) {
+      int64_t const t = p.targets[c + (j < count ? j : 0)];
+      float l = 0.0f;
+      if (t >= 0 && t < p.classes) {
+        l = static_cast<T const*>(p.logits)[t * p.ld + c + (j < count ? j : 0)];
+        if (l != -kInf) l -= normalizer[j];
+      }
+      log_prob.set(j, l);
     }
-    p.log_probs[c] = l;
+    log_prob.store(p.log_probs + c, count);
   }
   if constexpr (K > 0)
 #pragma unroll
     for (int k = 0; k < K; k++) {
       if (k >= p.top_k) continue;
-      bool const none = s.value[k] == -kInf;
-      p.top_classes[k * p.columns + c] = none ? -1 : s.index[k];
-      p.top_log_probs[k * p.columns + c] = none ? -kInf : s.value[k] - normalizer;
+      Pack<float, NC> value;
+      Pack<int32_t, NC> index;
+#pragma unroll
+      for (int j = 0; j < NC; j++) {
+        bool const none = s[j].value[k] == -kInf;
+        index.put(j, none ? -1 : s[j].index[k]);
+        value.set(j, none ? -kInf : s[j].value[k] - normalizer[j]);
+      }
+      index.store(p.top_classes + k * p.columns + c, count);
+      value.store(p.top_log_probs + k * p.columns + c, count);
     }
 }
 
+// The K largest of a lane's 16-bit logits: a logit's bits in ascending order above the complement of its turn, so
+// that a place takes a maximum and a minimum (a value and its class apart take six operations).
+template <class T, int K> struct Keys {
+  unsigned key[K];
+  __device__ void clear() {
+#pragma unroll
+    for (int k = 0; k < K; k++) key[k] = 0;
+  }
+  static __device__ unsigned make(T v, unsigned turn) {
+    int w;  // (of NaN those of -inf, of -0 those of 0)
+    if constexpr (std::is_same_v<T, _Float16>) {
+      _Float16 const x = __builtin_fmaxf16(v + _Float16(0.0f), _Float16(-kInf));
+      w = int(__builtin_bit_cast(unsigned short, x)) << 16;
+    } else {
+      w = __float_as_int(fmaxf(float(v) + 0.0f, -kInf));
+    }
+    return (unsigned(w ^ (w >> 31 | int(0x80000000))) & 0xffff0000u) | (0xffffu - turn);
+  }
+  __device__ void insert(unsigned x) {
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+      unsigned const more = x > key[k] ? x : key[k], less = x > key[k] ? key[k] : x;
+      key[k] = more, x = less;
+    }
+  }
+  // Place k's logit (-inf: none), and its turn.
+  __device__ float value(int k, int& turn) const {
+    turn = 0xffff - int(key[k] & 0xffffu);
+    unsigned const w = key[k] >> 16, bits = w & 0x8000u ? w ^ 0x8000u : w ^ 0xffffu;
+    return key[k] == 0 ? -kInf : float(__builtin_bit_cast(T, static_cast<unsigned short>(bits)));
+  }
+};
+
 template <class T, int NC, int K> __global__ __launch_bounds__(kThreads) void logp(LogpArgs a) {
-  constexpr int U = NC >= 4 ? 4 : 8;  // rows under way
+  constexpr int U = rows_under_way(NC, K);
   constexpr int WAVES = kThreads / 64;
   int const across = 1 << a.lane_columns, tx = threadIdx.x & (across - 1), ty = threadIdx.x >> a.lane_columns;
   int const down = kThreads >> a.lane_columns;
@@ -134,40 +190,80 @@ template <class T, int NC, int K> __global__ __launch_bounds__(kThreads) void lo
   int64_t const c0 = (tile * across + tx) * NC, left = a.p.columns - c0;
   int const count = left < 1 ? 0 : left < NC ? int(left) : NC;
   int64_t const first = split * a.rows, end = first + a.rows < a.p.classes ? first + a.rows : a.p.classes;
+  constexpr bool KEYS = K > 0 && sizeof(T) == 2;
   Column<K> s[NC];
+  Keys<T, KEYS ? K : 1> keys[KEYS ? NC : 1];
 #pragma unroll
-  for (int j = 0; j < NC; j++) s[j].clear();
-  T const* x = static_cast<T const*>(a.p.logits) + c0;
-  if (count > 0)
-    for (int64_t row = first + ty; row < end; row += int64_t(down) * U) {
+  for (int j = 0; j < NC; j++) {
+    s[j].clear();
+    if constexpr (KEYS) keys[j].clear();
+  }
+  if (count > 0) {
+    unsigned at = 0;  // rows of this lane so far
+    int64_t const stride = down * a.p.ld;
+    T const* x = static_cast<T const*>(a.p.logits) + (first + ty) * a.p.ld + c0;
+    for (int64_t row = first + ty; row < end; row += int64_t(down) * U, x += U * stride) {
       Pack<T, NC> v[U];
+      if (row + (U - 1) * down < end) {
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        if (row + u * down < end) v[u].load(x + (row + u * down) * a.p.ld, count, -kInf);
-        else v[u].fill(-kInf);
+        for (int u = 0; u < U; u++) v[u].load(x + u * stride, count, -kInf);
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+          if (row + u * down < end) v[u].load(x + u * stride, count, -kInf);
+          else v[u].fill(-kInf);
+        }
+      }
+      float top[NC];
+      bool beyond = false;
+#pragma unroll
+      for (int j = 0; j < NC; j++) {
+        top[j] = v[0][j];
+#pragma unroll
+        for (int u = 1; u < U; u++) top[j] = fmaxf(top[j], v[u][j]);
+        beyond = beyond || top[j] > s[j].m + kSlack;
+      }
+      if (__any(beyond)) {
+#pragma unroll
+        for (int j = 0; j < NC; j++) s[j].move_to(top[j] > s[j].m + kSlack ? top[j] : s[j].m);
       }
 #pragma unroll
       for (int j = 0; j < NC; j++) {
-        float top = v[0][j];
-#pragma unroll
-        for (int u = 1; u < U; u++) top = fmaxf(top, v[u][j]);
-        float const m = fmaxf(s[j].m, top);
-        s[j].move_to(m);
-        float const shift = m == -kInf ? 0.0f : m;
+        float const shift = s[j].m == -kInf ? 0.0f : s[j].m;
 #pragma unroll
         for (int u = 0; u < U; u++) {
           float const t = (v[u][j] - shift) * kLog2e, e = __builtin_amdgcn_exp2f(t);
           s[j].z += e;
           s[j].q = fmaf(e, fmaxf(t, kFar), s[j].q);
         }
-        if constexpr (K > 0) {
-          if (__any(top > s[j].value[K - 1])) {
+        if constexpr (KEYS) {
+          unsigned x[U], most = 0;
+#pragma unroll
+          for (int u = 0; u < U; u++) x[u] = keys[j].make(v[u].raw(j), at + u), most = x[u] > most ? x[u] : most;
+          if (K <= 4 || __any(most > keys[j].key[K - 1])) {
+#pragma unroll
+            for (int u = 0; u < U; u++) keys[j].insert(x[u]);
+          }
+        } else if constexpr (K > 0) {
+          if (__any(top[j] > s[j].value[K - 1])) {
 #pragma unroll
             for (int u = 0; u < U; u++) s[j].insert(v[u][j], int32_t(row + u * down));
           }
         }
       }
+      at += U;
     }
+  }
+  if constexpr (KEYS) {
+#pragma unroll
+    for (int j = 0; j < NC; j++)
+#pragma unroll
+      for (int k = 0; k < K; k++) {
+        int turn;
+        s[j].value[k] = keys[j].value(k, turn);
+        s[j].index[k] = s[j].value[k] == -kInf ? INT32_MAX : int32_t(first + ty + int64_t(turn) * down);
+      }
+  }
   // Lanes of a wave that share columns, then the waves.
   if (down > 1) {
     for (int d = across; d < 64; d *= 2) {
@@ -199,14 +295,15 @@ template <class T, int NC, int K> __global__ __launch_bounds__(kThreads) void lo
     if (c >= across * NC || column >= a.p.columns) return;
     Column<K> r;
     r.clear();
-#pragma unroll
+#pragma unroll 1  // (code that runs once comes from memory: the shorter the better)
     for (int w = 0; w < WAVES; w++) {
       r.join(lds[w][0][c], lds[w][1][c], lds[w][2][c]);
       if constexpr (K > 0)
         r.join_list([&](int k, float& v, int32_t& i) { v = lds[w][3 + k][c], i = __float_as_int(lds[w][3 + K + k][c]); });
     }
     if (a.splits == 1) {
-      finish<T, K>(a.p, column, r);
+      Column<K> const one[1] = {r};
+      finish<T, 1, K>(a.p, column, 1, one);
     } else {
       float* part = a.parts + split * 3 * a.p.columns + column;
       part[0] = r.m, part[a.p.columns] = r.z, part[2 * a.p.columns] = r.q;
@@ -217,9 +314,7 @@ template <class T, int NC, int K> __global__ __launch_bounds__(kThreads) void lo
       }
     }
   } else {
-#pragma unroll
-    for (int j = 0; j < NC; j++)
-      if (j < count) finish<T, K>(a.p, c0 + j, s[j]);
+    if (count > 0) finish<T, NC, K>(a.p, c0, count, s);
   }
 }
 
@@ -248,7 +343,10 @@ template <class T, int K> __global__ __launch_bounds__(kThreads) void logp_join(
       r.join_list([&](int k, float& v, int32_t& i) { v = o.value[k], i = o.index[k]; });
     }
   }
-  if (l == 0 && column < a.p.columns) finish<T, K>(a.p, column, r);
+  if (l == 0 && column < a.p.columns) {
+    Column<K> const one[1] = {r};
+    finish<T, 1, K>(a.p, column, 1, one);
+  }
 }
 
 struct LogpBackwardArgs {
@@ -273,27 +371,32 @@ template <class T, int NC> __global__ __launch_bounds__(kThreads) void logp_back
   int64_t const first = blockIdx.x / a.tiles * a.rows, end = first + a.rows < a.p.classes ? first + a.rows : a.p.classes;
   float normalizer[NC], base[NC], entropy_weight[NC], at_target[NC];
   int32_t target[NC];
+  Pack<float, NC> l, h, gp, gh, gn;
+  Pack<int32_t, NC> t;
+  l.load(a.p.log_normalizer + c0, count, 0.0f);
+  gp.fill(0.0f), gh.fill(0.0f), gn.fill(0.0f), h.fill(0.0f);
+  if (a.d_log_probs != nullptr) gp.load(a.d_log_probs + c0, count, 0.0f), t.load(a.p.targets + c0, count, -1.0f);
+  if (a.d_entropy != nullptr) gh.load(a.d_entropy + c0, count, 0.0f), h.load(a.p.entropy + c0, count, 0.0f);
+  if (a.d_log_normalizer != nullptr) gn.load(a.d_log_normalizer + c0, count, 0.0f);
 #pragma unroll
   for (int j = 0; j < NC; j++) {
-    int64_t const c = c0 + (j < count ? j : 0);
-    float const l = a.p.log_normalizer[c];
-    bool const none = l == -kInf;
-    normalizer[j] = none ? kInf : l;  // (every p is 0)
-    target[j] = a.p.targets != nullptr ? a.p.targets[c] : -1;
-    bool const given = !none && target[j] >= 0 && int64_t(target[j]) < a.p.classes && a.d_log_probs != nullptr;
-    at_target[j] = given ? a.d_log_probs[c] : 0.0f;
-    entropy_weight[j] = a.d_entropy != nullptr ? a.d_entropy[c] : 0.0f;
-    base[j] = (a.d_log_normalizer != nullptr ? a.d_log_normalizer[c] : 0.0f) - at_target[j];
-    if (a.d_entropy != nullptr) base[j] -= entropy_weight[j] * a.p.entropy[c];
-    if (!given) target[j] = -1;
+    bool const none = l[j] == -kInf;
+    normalizer[j] = none ? kInf : l[j];  // (every p is 0)
+    target[j] = a.d_log_probs != nullptr ? t.raw(j) : -1;
+    if (none || int64_t(target[j]) >= a.p.classes) target[j] = -1;
+    at_target[j] = target[j] >= 0 ? gp[j] : 0.0f;
+    entropy_weight[j] = gh[j];
+    base[j] = gn[j] - at_target[j];
+    if (a.d_entropy != nullptr) base[j] -= gh[j] * h[j];
   }
-  T const* x = static_cast<T const*>(a.p.logits) + c0;
-  T* d = static_cast<T*>(a.d_logits) + c0;
-  for (int64_t row = first + ty; row < end; row += int64_t(down) * U) {
+  int64_t const stride = down * a.p.ld, stride_d = down * a.ld_d;
+  T const* x = static_cast<T const*>(a.p.logits) + (first + ty) * a.p.ld + c0;
+  T* d = static_cast<T*>(a.d_logits) + (first + ty) * a.ld_d + c0;
+  for (int64_t row = first + ty; row < end; row += int64_t(down) * U, x += U * stride, d += U * stride_d) {
     Pack<T, NC> v[U];
 #pragma unroll
     for (int u = 0; u < U; u++)
-      if (row + u * down < end) v[u].load(x + (row + u * down) * a.p.ld, count, 0.0f);
+      if (row + u * down < end) v[u].load(x + u * stride, count, 0.0f);
 #pragma unroll
     for (int u = 0; u < U; u++) {
       int64_t const r = row + u * down;
@@ -306,7 +409,7 @@ template <class T, int NC> __global__ __launch_bounds__(kThreads) void logp_back
         float const g = p * (base[j] - entropy_weight[j] * (lp < -200.0f ? -200.0f : lp));
         o.set(j, int32_t(r) == target[j] ? g + at_target[j] : g);
       }
-      o.store(d + r * a.ld_d, count);
+      o.store(d + u * stride_d, count);
     }
   }
 }
@@ -327,18 +430,21 @@ Shape shape_of(int64_t classes, int64_t columns, int32_t dtype, int32_t top_k) {
   Shape s{};
   s.columns = columns < wide ? 1 : k == 0 ? wide : k <= 8 ? 4 : 2;
   int64_t const lanes = (columns + s.columns - 1) / s.columns;
-  // Few classes: every lane takes all rows of its columns.  Else at most 8 lanes across.
+  // Few classes: every lane takes all rows of its columns.  Else 128 bytes of a row across.
+  int const line = s.columns == 1 || s.columns == wide ? 3 : s.columns * 2 == wide ? 4 : 5;
   if (classes <= 64 && lanes > 64) {
     s.lane_columns = 8;
   } else {
-    while (s.lane_columns < 3 && (1 << s.lane_columns) < lanes) s.lane_columns++;
+    while (s.lane_columns < line && (1 << s.lane_columns) < lanes) s.lane_columns++;
     while (s.lane_columns < 5 && (1 << s.lane_columns) < lanes && (kThreads >> s.lane_columns) > classes) s.lane_columns++;
   }
   int64_t const across = int64_t(s.columns) << s.lane_columns, down = kThreads >> s.lane_columns;
   s.tiles = (columns + across - 1) / across;
-  int64_t const turn = down * (s.columns >= 4 ? 4 : 8), turns = (classes + turn - 1) / turn;
-  int64_t const want = down == 1 ? 1 : std::max<int64_t>(1, std::min(turns, kMostGroups / s.tiles));
-  s.rows = (turns + want - 1) / want * turn;
+  int64_t const turn = down * rows_under_way(s.columns, k), turns = (classes + turn - 1) / turn;
+  // (lists are worth joining from a few turns on; a lane's rows are counted in 16 bits)
+  int64_t const most = k == 0 ? turns : (turns + 3) / 4;
+  int64_t const want = down == 1 ? 1 : std::max<int64_t>(1, std::min(most, kMostGroups / s.tiles));
+  s.rows = std::min((turns + want - 1) / want * turn, down * int64_t(65536));
   s.splits = static_cast<int>((classes + s.rows - 1) / s.rows);
   return s;
 }
@@ -361,11 +467,14 @@ int64_t logp_workspace_bytes(int64_t classes, int64_t columns, int32_t dtype, in
   return s.splits == 1 ? 0 : int64_t(s.splits) * (3 + 2 * list_size(top_k)) * columns * 4;
 }
 
-// A turn is at least 128 rows; more than one workgroup shares a tile of at most 64 columns, 1024 / tiles of them.
+// A turn is at least 32 rows; more than one workgroup shares a tile of at most 64 columns, 1024 / tiles of them (or as
+// many as count their rows in 16 bits).
 int64_t logp_workspace_bytes_up_to(int64_t classes, int64_t columns, int32_t top_k) {
-  int64_t const turns = (classes + 127) / 128;
+  int64_t const turns = (classes + 31) / 32;
   if (turns == 1) return 0;
-  int64_t const parts = columns < kMostParts / turns ? columns * turns : kMostParts;
+  int64_t parts = columns < kMostParts / turns ? columns * turns : kMostParts;
+  constexpr int64_t COUNTED = 65536 * (kThreads >> 5);  // rows at least of a workgroup before its lanes' counts end
+  if (classes > COUNTED) parts += columns * ((classes + COUNTED - 1) / COUNTED);
   return parts * (3 + 2 * list_size(top_k)) * 4;
 }
 
@@ -411,8 +520,8 @@ hipError_t launch_logp_backward(ponni_log_probs const& p, float const* d_log_pro
   int const wide = p.dtype == PONNI_F32 ? 4 : 8, nc = p.columns < wide ? 1 : wide;
   LogpBackwardArgs a{p, d_log_probs, d_entropy, d_log_normalizer, d_logits, ld_d_logits};
   int64_t const lanes = (p.columns + nc - 1) / nc;
+  if (p.classes <= 64 && lanes > 64) a.lane_columns = 8;  // (every lane takes all rows of its columns)
   while (a.lane_columns < 3 && (1 << a.lane_columns) < lanes) a.lane_columns++;
-  while (a.lane_columns < 8 && (1 << a.lane_columns) < lanes && (kThreads >> a.lane_columns) > p.classes) a.lane_columns++;
   int64_t const across = int64_t(nc) << a.lane_columns, turn = (kThreads >> a.lane_columns) * (nc >= 4 ? 4 : 8);
   a.tiles = (p.columns + across - 1) / across;
   int64_t const turns = (p.classes + turn - 1) / turn;

@@ -480,7 +480,9 @@ inline Shape shape_of(int32_t n, int64_t columns, int32_t dtype, int max_steps, 
 }
 
 // Rows a lane can hold without spilling.
-inline int most_steps(bool backward, bool gate) { return backward ? (gate ? 4 : 8) : gate ? 8 : 16; }
+inline int most_steps(int32_t dtype, bool backward, bool gate) {
+  return backward ? (gate && dtype != PONNI_F32 ? 4 : 8) : gate ? 8 : 16;
+}
 
 // f(steps, held, gate, layer) as constants.
 template <class F> void with_variant(Shape const& s, bool gate, bool layer, F&& f) {
@@ -500,7 +502,7 @@ inline bool has_layer(ponni_residual_norm const& r) {
 }
 
 template <class T> hipError_t launch_norm(ponni_residual_norm const& r, hipStream_t stream) {
-  Shape const s = shape_of(r.n, r.columns, r.dtype, most_steps(false, r.gate != nullptr), 2);
+  Shape const s = shape_of(r.n, r.columns, r.dtype, most_steps(r.dtype, false, r.gate != nullptr), 2);
   NormArgs a{};
   a.r = r;
   a.lane_columns = s.lane_columns;
@@ -520,7 +522,7 @@ template <class T> hipError_t launch_norm(ponni_residual_norm const& r, hipStrea
 template <class T>
 hipError_t launch_norm_backward(ponni_residual_norm const& r, ponni_residual_norm_gradients const& g, void* workspace,
                                 int& groups, hipStream_t stream) {
-  Shape const s = shape_of(r.n, r.columns, r.dtype, most_steps(true, r.gate != nullptr), 3);
+  Shape const s = shape_of(r.n, r.columns, r.dtype, most_steps(r.dtype, true, r.gate != nullptr), 3);
   NormArgs a{};
   a.r = r;
   a.g = g;
@@ -533,7 +535,7 @@ hipError_t launch_norm_backward(ponni_residual_norm const& r, ponni_residual_nor
     constexpr int S = decltype(steps)::value, NC = 16 / sizeof(T);
     constexpr bool H = decltype(held)::value, G = decltype(gate)::value, L = decltype(layer)::value;
     dim3 const grid(groups), block(kThreads);
-    if constexpr (!(G && S == 8) && S < 16) {
+    if constexpr (!(G && S == 8 && sizeof(T) == 2) && S < 16) {
       if (r.after.kind == PONNI_NORM_NONE) {
         if (s.columns == 1) hipLaunchKernelGGL((residual_norm_backward<T, 1, S, H, G, true, false>), grid, block, 0, stream, a);
         else hipLaunchKernelGGL((residual_norm_backward<T, NC, S, H, G, L, false>), grid, block, 0, stream, a);
