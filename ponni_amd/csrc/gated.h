@@ -7,8 +7,8 @@
 
 namespace ponni_hip {
 
-// An operand: rows `ld` bytes apart, of `rows` rows, `bytes` from the first element to the end of the last row (up to a
-// multiple of 16).  p and ld are multiples of 16 bytes.
+// An operand: rows `ld` bytes apart, of `rows` rows, `bytes` from the first element to the end of the last row, up to a
+// multiple of 4 as p and ld are.
 struct Side {
   char const* p;
   int64_t ld, bytes, rows;
@@ -24,14 +24,13 @@ enum Form {
   FORM_PAIR,     // k outside in both; a: two arrays
   FORM_FORWARD,  // k outside in both
   FORM_STATES,   // k inside in a
-  FORM_INPUT,    // k inside in a
+  FORM_INPUT,    // k inside in a: the sum of a[0] b[0] and a[1] b[1], pairs of one shape and stride
   FORM_WEIGHTS   // k inside in both
 };
 
 struct ProductArgs {
   Side a[2], b[2];
   int64_t k, rows, columns;  // C [rows, columns]
-  int terms;                 // 2: the sum of a[0] b[0] and a[1] b[1]
   int problems;              // 2: a[0] b[0] and a[0] b[1], into y[0] and y[1]
   int parts;                 // workgroups that share a tile's k
   void* y[2];
@@ -51,5 +50,30 @@ struct ProductArgs {
 hipError_t launch_product_f32(Form form, bool large, ProductArgs const& p, hipStream_t stream);
 hipError_t launch_product_f16(Form form, bool large, ProductArgs const& p, hipStream_t stream);
 hipError_t launch_product_bf16(Form form, bool large, ProductArgs const& p, hipStream_t stream);
+
+// A product of few columns (gated_thin.h): parts [slices, problems, columns, stride] of fp32.
+constexpr int kThinColumns = 32;
+enum ThinInput { THIN_COLUMNS, THIN_PARTS, THIN_ROWS };
+struct ThinArgs {
+  void const* w[2];  // [k, outputs]
+  int64_t ld[2];
+  int k, outputs, columns;
+  int slices, slice_k;  // slice_k a multiple of the waves' steps
+  float* parts;
+  int stride;  // outputs rounded up to whole tiles
+  // the columns: x [k, columns], or h of the parts of g and u, or h [columns, stride_in]
+  void const* x;
+  int64_t ld_x;
+  void* h;
+  float const* parts_in;
+  int slices_in, stride_in, act;
+  float slope;
+  void const* bias[3];  // of g, u and y
+  void* y;
+  int64_t ld_y;
+};
+hipError_t launch_thin_f32(ThinArgs const& hidden, ThinArgs const& last, hipStream_t stream);
+hipError_t launch_thin_f16(ThinArgs const& hidden, ThinArgs const& last, hipStream_t stream);
+hipError_t launch_thin_bf16(ThinArgs const& hidden, ThinArgs const& last, hipStream_t stream);
 
 }  // namespace ponni_hip

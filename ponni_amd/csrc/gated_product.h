@@ -94,12 +94,11 @@ __device__ inline i32x4 resource_of(uint64_t p, uint64_t bytes) {
                __builtin_amdgcn_readfirstlane(int(n)), 0x00027000};
 }
 
-template <class T> __device__ inline f32x4 mfma_step(i32x4 a, i32x4 b, f32x4 c) {
+// A step's product of two fragments, in fp32 of its part e of four (16 bits: of one).
+template <class T> constexpr int kMfmaParts = sizeof(T) == 4 ? 4 : 1;
+template <class T> __device__ inline f32x4 mfma_part(i32x4 a, i32x4 b, f32x4 c, int e) {
   if constexpr (std::is_same_v<T, float>) {
-    f32x4 const x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
-#pragma unroll
-    for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
-    return c;
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, a)[e], __builtin_bit_cast(f32x4, b)[e], c, 0, 0, 0);
   } else if constexpr (std::is_same_v<T, _Float16>) {
     typedef _Float16 h8 __attribute__((ext_vector_type(8)));
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
@@ -136,7 +135,7 @@ template <class T, bool INNER, int SIZE, int PANELS, int W> struct Loader {
   static constexpr int PLACES = ROW / 16;            // pieces of it
   static constexpr int PER_PANEL = PANEL * 64 / 1024;  // requests
   static constexpr int BASES = INNER ? REQUESTS : PANELS;
-  static_assert(BYTES % (1024 * W) == 0 && 64 % PLACES == 0 && (PANELS == 1 || PER_PANEL == W), "whole requests, of one panel each");
+  static_assert(BYTES % (1024 * W) == 0 && 64 % PLACES == 0 && (PANELS == 1 || PER_PANEL % W == 0), "whole requests, of one panel each");
   unsigned offset[REQUESTS];  // of the lane's piece from the request's base
   int k[REQUESTS];            // INNER: the first k of the piece, within a step
   // Of the step that is asked for next, uniform: where each base lies, the bytes from there to the array's end, k's left.
@@ -186,10 +185,17 @@ template <class T, bool INNER, int SIZE, int PANELS, int W> struct Loader {
     for (int b = 0; b < BASES; b++) at[b] = uniform64(at[b] + stride), left[b] = uniform64(left[b] - stride);
     k_left = __builtin_amdgcn_readfirstlane(k_left - STEP);
   }
+  // From behind the last step of one array to the first of another `distance` bytes on, of the same shape.
+  __device__ void jump(bool now, uint64_t distance, int steps, int64_t last) {
+    uint64_t const back = now ? steps * stride : 0, on = now ? distance : 0;
+#pragma unroll
+    for (int b = 0; b < BASES; b++) at[b] = uniform64(at[b] + on - back), left[b] = uniform64(left[b] + back);
+    k_left = __builtin_amdgcn_readfirstlane(now ? int(last) : k_left);
+  }
   __device__ void request(int r, int wave, unsigned lds) const {
-    constexpr bool EACH = INNER || PANELS > 1;
+    int const base = INNER ? r : W * r / PER_PANEL;
     unsigned const o = INNER && k[r] >= k_left ? 0xfffffff0u : offset[r];
-    dma16_in_range(resource_of(at[EACH ? r : 0], left[EACH ? r : 0]), o, lds + (wave + W * r) * 1024);
+    dma16_in_range(resource_of(at[base], left[base]), o, lds + (wave + W * r) * 1024);
   }
 
   // Reads.  The lane's place for fragment 0 of the wave's fragments, which begin at row `first` of a panel.
@@ -261,7 +267,8 @@ template <class T> __device__ inline void load16(T const* x, int64_t left, float
   }
 }
 
-template <class T, bool A_INNER, bool B_INNER, Output OUT, int MI, int NJ, int WM, int WN>
+// TWO: a sum of two products, of operands of the same shapes and strides.
+template <class T, bool A_INNER, bool B_INNER, Output OUT, bool TWO, int MI, int NJ, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, 2) void product(ProductArgs p) {
   constexpr int W = WM * WN, BM = 16 * MI * WM, BN = 16 * NJ * WN, ES = sizeof(T), STEP = 64 / ES;
   constexpr bool PAIR = OUT == OUT_PAIR;
@@ -287,7 +294,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void product(ProductArgs p) {
   int const second = p.split_n > 0 && nt >= p.split_n ? 1 : 0;
   constexpr int FEATURES = PAIR ? BM / 2 : BM;  // rows of C of a tile
   int64_t const m0 = int64_t(mt) * FEATURES, n0 = int64_t(nt - (second ? p.split_n : 0)) * BN;
-  int const steps_each = p.steps, all_steps = p.terms * steps_each;
+  int const steps_each = p.steps, all_steps = (TWO ? 2 : 1) * steps_each;
   int const first_step = int(int64_t(all_steps) * part / p.parts), end = int(int64_t(all_steps) * (part + 1) / p.parts);
   unsigned const lds0 = static_cast<unsigned>(reinterpret_cast<uint64_t>((lds_void)lds));
 
@@ -295,14 +302,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void product(ProductArgs p) {
   LB lb;
   la.init(wave, lane, p.a[0], m0);
   lb.init(wave, lane, p.b[second], n0);
-  // The next step that is asked for: `to` its slot.
+  // The next step that is asked for.
   int next = first_step;
-  auto seek = [&](int term) __attribute__((always_inline)) {
-    int64_t const k0 = int64_t(next - term * steps_each) * STEP;
-    la.seek(wave, p.a + term, m0, k0, p.k);
-    lb.seek(wave, p.b + (second | term), n0, k0, p.k);
-  };
-  seek(next >= steps_each ? 1 : 0);
+  int const term = TWO && next >= steps_each ? 1 : 0;
+  int64_t const k0 = int64_t(next - term * steps_each) * STEP;
+  la.seek(wave, p.a + term, m0, k0, p.k);
+  lb.seek(wave, p.b + (second | term), n0, k0, p.k);
+  uint64_t const on_a = TWO ? uniform64(uint64_t(p.a[1].p) - uint64_t(p.a[0].p)) : 0,
+                 on_b = TWO ? uniform64(uint64_t(p.b[1].p) - uint64_t(p.b[0].p)) : 0;
   auto request = [&](int r) __attribute__((always_inline)) {
     unsigned const slot = lds0 + unsigned(next - first_step) % kSlots * SLOT;
     if (r < LA::REQUESTS) la.request(r, wave, slot);
@@ -311,10 +318,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void product(ProductArgs p) {
       next++;
       la.advance();
       lb.advance();
-      if (p.terms == 2 && next == steps_each) {
-        int term = 1;
-        asm volatile("" : "+s"(term));  // (nothing of it is computed before, and kept)
-        seek(term);
+      if constexpr (TWO) {
+        bool const now = next == steps_each;
+        la.jump(now, on_a, steps_each, p.k);
+        lb.jump(now, on_b, steps_each, p.k);
       }
     }
   };
@@ -339,7 +346,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void product(ProductArgs p) {
     constexpr int set = decltype(at_set)::value;
     constexpr bool WHOLE = decltype(whole)::value;  // a step kSlots on
     if constexpr (A_INNER || B_INNER) {
-      int64_t const left = p.k - int64_t(step >= steps_each ? step - steps_each : step) * STEP;
+      int64_t const left = p.k - int64_t(TWO && step >= steps_each ? step - steps_each : step) * STEP;
       if (left < STEP && left % (16 / ES) != 0) {
 #pragma unroll
         for (int i = 0; i < MI; i++) clear_past<T, A_INNER>(av[set][i], lane, left);
@@ -358,7 +365,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void product(ProductArgs p) {
         for (int r = j * READS / NJ; r < (j + 1) * READS / NJ; r++) read(step + 1, std::integral_constant<int, 1 - set>{}, r);
       }
 #pragma unroll
-      for (int i = 0; i < MI; i++) acc[i][j] = mfma_step<T>(bv[set][j], av[set][i], acc[i][j]);
+      for (int e = 0; e < kMfmaParts<T>; e++)
+#pragma unroll
+        for (int i = 0; i < MI; i++) acc[i][j] = mfma_part<T>(bv[set][j], av[set][i], acc[i][j], e);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -483,7 +492,7 @@ template <class T> __global__ __launch_bounds__(256) void join_parts(ProductArgs
   o.store(static_cast<T*>(p.y[second]) + m * p.ld[second] + n, p.columns - n < 4 ? int(p.columns - n) : 4);
 }
 
-template <class T, bool A_INNER, bool B_INNER, Output OUT, int MI, int NJ, int WM, int WN>
+template <class T, bool A_INNER, bool B_INNER, Output OUT, bool TWO, int MI, int NJ, int WM, int WN>
 hipError_t launch_tiles(ProductArgs p, hipStream_t stream) {
   constexpr int BM = 16 * MI * WM / (OUT == OUT_PAIR ? 2 : 1), BN = 16 * NJ * WN, STEP = 64 / sizeof(T);
   int64_t const m_tiles = (p.rows + BM - 1) / BM, n_tiles = (p.columns + BN - 1) / BN * p.problems;
@@ -492,20 +501,20 @@ hipError_t launch_tiles(ProductArgs p, hipStream_t stream) {
   p.steps = int((p.k + STEP - 1) / STEP);
   int64_t const groups = (m_tiles * n_tiles * p.parts + 7) / 8 * 8;
   if (groups > int64_t(UINT32_MAX) / (64 * WM * WN)) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL((product<T, A_INNER, B_INNER, OUT, MI, NJ, WM, WN>), dim3(unsigned(groups)), dim3(64 * WM * WN), 0, stream, p);
+  hipLaunchKernelGGL((product<T, A_INNER, B_INNER, OUT, TWO, MI, NJ, WM, WN>), dim3(unsigned(groups)), dim3(64 * WM * WN), 0, stream, p);
   return hipGetLastError();
 }
 
-template <class T, bool A_INNER, bool B_INNER, Output OUT> hipError_t launch_sized(bool large, ProductArgs const& p, hipStream_t stream) {
+template <class T, bool A_INNER, bool B_INNER, Output OUT, bool TWO = false> hipError_t launch_sized(bool large, ProductArgs const& p, hipStream_t stream) {
   if constexpr (sizeof(T) == 2)
-    if (large) return launch_tiles<T, A_INNER, B_INNER, OUT, 8, 4, 2, 4>(p, stream);
-  if constexpr (sizeof(T) == 4 && OUT == OUT_PAIR) return launch_tiles<T, A_INNER, B_INNER, OUT, 8, 4, 1, 4>(p, stream);
-  else return launch_tiles<T, A_INNER, B_INNER, OUT, 4, 4, 2, 2>(p, stream);
+    if (large) return launch_tiles<T, A_INNER, B_INNER, OUT, TWO, 8, 4, 2, 4>(p, stream);
+  if constexpr (sizeof(T) == 4 && OUT == OUT_PAIR) return launch_tiles<T, A_INNER, B_INNER, OUT, TWO, 8, 4, 1, 2>(p, stream);
+  else return launch_tiles<T, A_INNER, B_INNER, OUT, TWO, 4, 4, 2, 2>(p, stream);
 }
 
-template <class T, bool A_INNER, bool B_INNER> hipError_t launch_plain(bool large, ProductArgs const& p, hipStream_t stream) {
-  if (p.parts == 1) return launch_sized<T, A_INNER, B_INNER, OUT_PLAIN>(large, p, stream);
-  hipError_t const err = launch_sized<T, A_INNER, B_INNER, OUT_PARTS>(large, p, stream);
+template <class T, bool A_INNER, bool B_INNER, bool TWO = false> hipError_t launch_plain(bool large, ProductArgs const& p, hipStream_t stream) {
+  if (p.parts == 1) return launch_sized<T, A_INNER, B_INNER, OUT_PLAIN, TWO>(large, p, stream);
+  hipError_t const err = launch_sized<T, A_INNER, B_INNER, OUT_PARTS, TWO>(large, p, stream);
   if (err != hipSuccess) return err;
   hipLaunchKernelGGL(join_parts<T>, dim3(unsigned(p.rows), unsigned((p.columns + 1023) / 1024), unsigned(p.problems)), dim3(256),
                      0, stream, p);
@@ -517,7 +526,7 @@ template <class T> hipError_t launch_product_as(Form form, bool large, ProductAr
     case FORM_PAIR: return launch_sized<T, false, false, OUT_PAIR>(large, p, stream);
     case FORM_STATES: return launch_sized<T, true, false, OUT_STATES>(large, p, stream);
     case FORM_FORWARD: return launch_plain<T, false, false>(large, p, stream);
-    case FORM_INPUT: return launch_plain<T, true, false>(large, p, stream);
+    case FORM_INPUT: return launch_plain<T, true, false, true>(large, p, stream);
     default: return launch_plain<T, true, true>(large, p, stream);
   }
 }

@@ -3,8 +3,8 @@
 //   forward   h = act(G^T x + g0) * (U^T x + u0) (and g, u), then y = D^T h + d0
 //   backward  dg, du from D dy and the states; dx = G dg + U du; dG, dU = x dg^T, x du^T; dD = h dy^T;
 //             biases' gradients are sums of rows
-// Operands go into LDS by 16-byte pieces, so an array whose rows do not begin at
-// multiples of 16 bytes is first copied to one whose rows do.
+// Operands go into LDS by 16-byte pieces from multiples of 4 bytes, so a 16-bit array
+// whose rows do not all begin at such is first copied to one whose rows do.
 #include <algorithm>
 
 #include "blocks.h"
@@ -64,8 +64,7 @@ Choice choose(int64_t es, int64_t rows, int64_t columns, int problems, int64_t s
   Choice best{false, 1};
   double least = 1e300;
   for (int large = 0; large <= (es == 2 ? 1 : 0); large++) {
-    int64_t const bm = (large ? 256 : 128) / (pair ? 2 : 1), bn = large || (pair && es == 4) ? 256 : 128,
-                  at_once = large || (pair && es == 4) ? 256 : 512;
+    int64_t const bm = (large ? 256 : 128) / (pair ? 2 : 1), bn = large ? 256 : 128, at_once = large ? 256 : 512;
     int64_t const tiles = (rows + bm - 1) / bm * ((columns + bn - 1) / bn) * problems;
     for (int parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
       if (parts > 1 && (!may_split || steps / parts < kLeastSteps || tiles * parts > at_once)) break;
@@ -109,13 +108,13 @@ template <class T> struct Run {
   hipError_t err = hipSuccess;
 
   static bool in_place(Matrix const& m) {
-    return reinterpret_cast<uint64_t>(m.p) % 16 == 0 && (m.rows == 1 || m.ld * int64_t(sizeof(T)) % 16 == 0);
+    return reinterpret_cast<uint64_t>(m.p) % 4 == 0 && (m.rows == 1 || m.ld * int64_t(sizeof(T)) % 4 == 0);
   }
   Side side(Matrix const& m) {
     if (!in_place(m)) return copied(m);
     constexpr int64_t ES = sizeof(T);
-    int64_t const ld = m.rows == 1 ? round_to(m.columns, 16 / ES) : m.ld;
-    return {static_cast<char const*>(m.p), ld * ES, round_to(((m.rows - 1) * ld + m.columns) * ES, 16), m.rows};
+    int64_t const ld = m.rows == 1 ? round_to(m.columns, 4 / ES) : m.ld;
+    return {static_cast<char const*>(m.p), ld * ES, round_to(((m.rows - 1) * ld + m.columns) * ES, 4), m.rows};
   }
   // Two arrays of one shape, of one stride.
   void sides(Matrix const& a, Matrix const& b, Side (&out)[2]) {
@@ -133,15 +132,14 @@ template <class T> struct Run {
                          to + row * ld, ld);
       err = hipGetLastError();
     }
-    return {reinterpret_cast<char const*>(to), ld * ES, round_to(((m.rows - 1) * ld + m.columns) * ES, 16), m.rows};
+    return {reinterpret_cast<char const*>(to), ld * ES, round_to(((m.rows - 1) * ld + m.columns) * ES, 4), m.rows};
   }
   void product(Form form, ProductArgs p) {
     if (err != hipSuccess) return;
     constexpr int64_t ES = sizeof(T), STEP = 64 / ES;
     bool const pair = form == FORM_PAIR, plain = !pair && form != FORM_STATES;
-    if (p.terms == 0) p.terms = 1;
     if (p.problems == 0) p.problems = 1;
-    Choice const c = choose(ES, p.rows, p.columns, p.problems, p.terms * ((p.k + STEP - 1) / STEP), pair, plain);
+    Choice const c = choose(ES, p.rows, p.columns, p.problems, (form == FORM_INPUT ? 2 : 1) * ((p.k + STEP - 1) / STEP), pair, plain);
     p.parts = c.parts;
     Taker const before = work;  // (the sums are read before the next product begins)
     if (c.parts > 1) {
@@ -161,6 +159,36 @@ template <class T> struct Run {
   }
 };
 
+// Slices of k of a product of few columns: about `groups` workgroups, each with at least a step for each of its four
+// waves.
+struct Slices {
+  int count, k;
+};
+Slices slices_of(int64_t es, int64_t k, int64_t outputs, int problems, int64_t groups) {
+  int64_t const step = 4 * (64 / es), tile = 256 / es, tiles = (outputs + tile - 1) / tile * problems;
+  int64_t const want = std::max<int64_t>(1, groups / tiles);
+  int64_t const most = std::min((k + step - 1) / step, want), each = round_to((k + most - 1) / most, step);
+  // (its columns, and the waves' sums, in 64 KB of LDS)
+  int64_t const held = std::min<int64_t>(each, 1024 / es);
+  return {int((k + held - 1) / held), int(held)};
+}
+struct ThinPlan {
+  Slices hidden, last;
+  int64_t stride_hidden, stride_last, parts_hidden, parts_last, rows;  // strides in elements, the others in bytes
+  int64_t bytes() const { return parts_hidden + parts_last + rows; }
+};
+ThinPlan thin_plan(ponni_gated const& b, int64_t columns) {
+  int64_t const es = element(b), tile = 256 / es, hidden = round_to(b.n_hidden, tile), last = round_to(b.n_out, tile);
+  ThinPlan p{slices_of(es, b.n_in, b.n_hidden, 2, columns <= 8 ? 512 : 256), slices_of(es, b.n_hidden, b.n_out, 1, 512), hidden, last, 0, 0, 0};
+  p.parts_hidden = round_to(p.hidden.count * 2 * columns * hidden * 4, 256);
+  p.parts_last = round_to(p.last.count * columns * last * 4, 256);
+  // Every tile of the last product reads all parts of its slice again, unless h is made of them once: us with / without
+  // that launch, 2048-4096-2048 fp16, 20 columns: 14 / 16; where few parts are read, as 2 MB at 1024-4096-1024 and one
+  // column, it would add its 4.
+  if (last / tile * p.parts_hidden > hidden * b.n_out * es) p.rows = round_to(columns * hidden * es, 256);
+  return p;
+}
+
 int64_t steps_of(int64_t k, int64_t es) { return (k + 64 / es - 1) / (64 / es); }
 
 }  // namespace
@@ -176,7 +204,9 @@ int64_t gated_workspace_bytes(ponni_gated const& b, int64_t columns, bool backwa
   t.take(aligned_bytes(h, columns, es));  // h itself, or a copy of the states'
   if (!backward) {
     t.take(sums_bytes(o, columns, 1, steps_of(h, es)));
-    return t.used;
+    // (the slices become fewer past 8 columns)
+    return std::max({t.used, thin_plan(b, std::min<int64_t>(columns, 8)).bytes(),
+                     thin_plan(b, std::min<int64_t>(columns, kThinColumns)).bytes()});
   }
   t.take(aligned_bytes(o, columns, es));
   t.take(aligned_bytes(2 * h, columns, es));  // dg, du
@@ -192,6 +222,28 @@ hipError_t launch_gated(ponni_gated const& b, int act, void const* x, int64_t ld
     using T = decltype(e);
     Run<T> run{{static_cast<char*>(workspace)}, stream};
     int64_t const hidden = b.n_hidden, es = sizeof(T);
+    if (states == nullptr && columns <= kThinColumns) {
+      ThinPlan const plan = thin_plan(b, columns);
+      ThinArgs first{}, last{};
+      first.w[0] = b.gate, first.w[1] = b.up, first.ld[0] = b.ld_gate, first.ld[1] = b.ld_up;
+      first.k = b.n_in, first.outputs = b.n_hidden, first.columns = int(columns);
+      first.slices = plan.hidden.count, first.slice_k = plan.hidden.k, first.stride = int(plan.stride_hidden);
+      first.x = x, first.ld_x = ld_x;
+      first.parts = reinterpret_cast<float*>(run.work.take(plan.parts_hidden));
+      last.w[0] = b.down, last.ld[0] = b.ld_down;
+      last.k = b.n_hidden, last.outputs = b.n_out, last.columns = int(columns);
+      last.slices = plan.last.count, last.slice_k = plan.last.k, last.stride = int(plan.stride_last);
+      last.parts = reinterpret_cast<float*>(run.work.take(plan.parts_last));
+      if (plan.rows > 0) last.h = run.work.take(plan.rows);
+      last.parts_in = first.parts, last.slices_in = first.slices, last.stride_in = first.stride;
+      last.act = act, last.slope = float(b.act.attr[0]);
+      last.bias[0] = b.gate_bias, last.bias[1] = b.up_bias, last.bias[2] = b.down_bias;
+      last.y = y, last.ld_y = ld_y;
+      err = (std::is_same_v<T, float>      ? launch_thin_f32
+             : std::is_same_v<T, _Float16> ? launch_thin_f16
+                                           : launch_thin_bf16)(first, last, stream);
+      return;
+    }
     T* const s = static_cast<T*>(states);
     int64_t const ld_h = s != nullptr ? ld_states : own_stride(columns, es);
     T* const h = s != nullptr ? s + 2 * hidden * ld_states : reinterpret_cast<T*>(run.work.take(hidden * ld_h * es));
@@ -234,7 +286,7 @@ hipError_t launch_gated_backward(ponni_gated const& b, int act, void const* x, i
     if (d.x != nullptr) {
       ProductArgs q{};
       run.sides({b.gate, b.n_in, hidden, b.ld_gate}, {b.up, b.n_in, hidden, b.ld_up}, q.a);
-      q.b[0] = s_dg, q.b[1] = s_du, q.terms = 2, q.k = hidden, q.rows = b.n_in, q.columns = columns;
+      q.b[0] = s_dg, q.b[1] = s_du, q.k = hidden, q.rows = b.n_in, q.columns = columns;
       q.y[0] = d.x, q.ld[0] = d.ld_x;
       run.product(FORM_INPUT, q);
     }
