@@ -66,10 +66,11 @@ Choice choose(int64_t es, int64_t rows, int64_t columns, int problems, int64_t s
   for (int large = 0; large <= (es == 2 ? 1 : 0); large++) {
     int64_t const bm = (large ? 256 : 128) / (pair ? 2 : 1), bn = large ? 256 : 128, at_once = large ? 256 : 512;
     int64_t const tiles = (rows + bm - 1) / bm * ((columns + bn - 1) / bn) * problems;
-    for (int parts : {1, 2, 3, 4, 6, 8, 12, 16}) {
+    for (int parts = 1; parts <= kMostParts; parts++) {
       if (parts > 1 && (!may_split || steps / parts < kLeastSteps || tiles * parts > at_once)) break;
       int64_t const groups = tiles * parts, rounds = (groups + at_once - 1) / at_once;
-      double const step = large ? 1.0 : groups <= 256 ? 0.4 : 0.62;
+      double const alone = es == 4 ? 1.3 : large ? 1.0 : 0.4, two = es == 4 ? 2.3 : 0.62;
+      double const step = large || groups <= 256 ? alone : two;
       double time = double(rounds) * (double((steps + parts - 1) / parts) * step + 5.0);
       if (parts > 1) time += 4.0 + double(parts + 1) * double(rows * columns * problems) * 4.0 / 3e6;
       if (time < least) least = time, best = {large != 0, parts};
