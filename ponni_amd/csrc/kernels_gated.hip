@@ -51,8 +51,15 @@ int64_t element(ponni_gated const& b) { return b.dtype == PONNI_F32 ? 4 : 2; }
 // Row strides of the library's own arrays: whole lines of 128 bytes.
 int64_t own_stride(int64_t columns, int64_t es) { return round_to(columns, 128 / es); }
 
-// Tiles and parts of k of a product C [rows, columns] x problems over `steps` steps.  Times in us a step of a tile,
-// and to begin and end one.
+// Tiles and parts of k of a product C [rows, columns] x problems over `steps` steps, by the time that each choice
+// takes: us for a step of a tile (alone on its CU, or with another) and to begin and end one.  Small
+// products lack tiles, so their k is cut; large ones take the tile that reads less.  Forward with states + backward,
+// bf16 1024-4096-1024, us:
+//                       128 x 128 whole   in 8 parts   256 x 256 whole   in 8 parts   chosen
+//   200 columns         53 + 149          32 + 71      105 + 260         54 + 116     34 + 71
+//   1000 columns        62 + 174          59 + 116     108 + 295         68 + 161     51 + 119
+//   16,000 columns      476 + 1114        462 + 1118   376 + 1183        377 + 835    384 + 839
+// and fp32 (128 x 128) 333-1001-77, 5000 columns: whole 178 + 818, chosen 140 + 233.
 struct Choice {
   bool large;
   int parts;

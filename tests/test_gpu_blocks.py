@@ -167,6 +167,28 @@ def test_gradient_of_log_probabilities_in_place(cuda):
         assert torch.equal(x, want)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_log_probabilities_of_column_ranges(cuda, dtype):
+    """Logits and their gradients in wider arrays, at odd and even places: neighbours neither enter nor change."""
+    import torch
+
+    t = torch_dtype(dtype)
+    for c, b, left, right in ((50, 300, 1, 6), (5000, 4, 3, 2), (700, 131, 8, 5)):
+        a = torch.full((c, left + b + right), float("inf"), dtype=t, device=cuda)
+        x = a[:, left:left + b]
+        x.copy_(torch.randn((c, b), device=cuda) * 2)
+        near = x.contiguous()
+        targets = torch.randint(0, c, (b,), dtype=torch.int32, device=cuda)
+        got, want = P.log_probabilities(x, targets, 3), P.log_probabilities(near, targets, 3)
+        for name in ("log_probs", "entropy", "log_normalizer", "top_classes", "top_log_probs"):
+            assert torch.equal(getattr(got, name), getattr(want, name)), name
+        g = torch.randn(b, device=cuda)
+        d = want.backward(g, g, g)
+        assert got.backward(g, g, g, out=x) is x
+        assert torch.equal(x, d)
+        assert bool(torch.isinf(a[:, :left]).all()) and bool(torch.isinf(a[:, left + b:]).all())
+
+
 def test_gradient_of_log_probabilities_by_differences(cuda):
     import torch
 
@@ -297,6 +319,57 @@ def test_norm_rows_beyond_four_gigabytes(cuda):
     assert torch.equal(state[:, cols], want[0]) and torch.equal(normed[:, cols], want[1])
 
 
+def test_norm_results_leave_their_neighbours(cuda):
+    """Column ranges of wider arrays for every result."""
+    import ctypes
+
+    import torch
+
+    for dtype in DTYPES:
+        t = torch_dtype(dtype)
+        for n, b, left, right in ((33, 5, 3, 4), (70, 131, 8, 3), (5000, 41, 1, 7)):
+            w = [1 + torch.randn(n, device=cuda) / 4 for _ in range(2)]
+            model = P.create_residual_norm(n, after=P.BlockNorm("rms", w[0]), before=P.BlockNorm("layer", w[1]), scale=0.5,
+                                           dtype=dtype)
+            x, res, gate, ds, dn = (torch.randn((n, b), device=cuda).to(t) for _ in range(5))
+            want = model.forward_with_statistics(x, res, gate)
+            wanted = model.backward(x, res, gate, want[2], ds, dn)
+
+            def wide():
+                a = torch.full((n + 1, left + b + right), 7.0, dtype=t, device=cuda)
+                return a, a[:n, left:left + b]
+
+            def same(a, v, want):
+                rest = torch.ones_like(a, dtype=torch.bool)
+                rest[:n, left:left + b] = False
+                return torch.equal(v, want) and bool((a[rest] == 7.0).all())
+
+            r = model._arrays(x, res, gate)
+            (sa, sv), (na, nv) = wide(), wide()
+            statistics = torch.empty((4, b), device=cuda)
+            r.state, r.normed, r.statistics = sv.data_ptr(), nv.data_ptr(), statistics.data_ptr()
+            r.ld_state = r.ld_normed = left + b + right
+            stream = torch.cuda.current_stream().cuda_stream
+            L = A.lib()
+            assert L.ponni_residual_norm_forward(ctypes.byref(r), stream) == 0
+            assert same(sa, sv, want[0]) and same(na, nv, want[1]) and torch.equal(statistics, want[2])
+            r = model._arrays(x, res, gate)
+            r.statistics = statistics.data_ptr()
+            g = A.ResidualNormGradientArrays()
+            g.d_state, g.ld_d_state, g.d_normed, g.ld_d_normed = ds.data_ptr(), b, dn.data_ptr(), b
+            out = [wide() for _ in range(3)]
+            for name, (a, v) in zip(("d_x", "d_residual", "d_gate"), out):
+                setattr(g, name, v.data_ptr())
+                setattr(g, "ld_" + name, a.stride(0))
+            need = L.ponni_residual_norm_workspace_bytes(n, r.dtype, b)
+            work = torch.empty(need + 64, dtype=torch.uint8, device=cuda)
+            work[need:] = 7
+            assert L.ponni_residual_norm_backward(ctypes.byref(r), ctypes.byref(g), work.data_ptr(), need, stream) == 0
+            for (a, v), v2 in zip(out, (wanted.x, wanted.residual, wanted.gate)):
+                assert same(a, v, v2)
+            assert bool((work[need:] == 7).all())
+
+
 # -- gated blocks -------------------------------------------------------------------------
 
 
@@ -376,6 +449,163 @@ def test_gated_non_finite_columns(cuda, dtype):
             want, got = forward(x), forward(x2)
             assert torch.equal(got[:, good], want[:, good])
             assert not torch.isfinite(got[:, [1, 2, b - 1]]).any()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("sizes,b", [((103, 30, 1186), 6774), ((2205, 31, 35), 3647), ((37, 997, 36), 8387),
+                                     ((1959, 2170, 121), 310), ((134, 1717, 177), 8561), ((2157, 387, 193), 4897)])
+def test_gated_large_tiles(cuda, sizes, b, dtype):
+    """Products large enough for the wider tiles, whole and cut along k, with ragged edges on every side."""
+    print(f"gated: {sizes} b={b} {dtype}", flush=True)
+    check_gated(cuda, sizes, b, "silu", dtype, bias=b % 2 == 1, pad=b % 5, shift=b % 2)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes", [(64, 256, 64), (1000, 600, 700), (130, 70, 33), (7, 1031, 5)])
+def test_gated_few_columns(cuda, sizes, dtype):
+    """Either side of the numbers of columns where kernels change; a column's result is that of the column alone, but
+    for the order of sums."""
+    for b in (1, 7, 8, 9, 15, 16, 17, 31, 32, 33):
+        check_gated(cuda, sizes, b, "gelu", dtype, bias=b % 2 == 0, pad=b % 3, backward=False, seed=b, wpad=b % 4)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_results_leave_their_neighbours(cuda, dtype):
+    """Results that are column ranges of wider arrays: what lies beside them stays, with and without states, and of
+    every gradient."""
+    import ctypes
+
+    import torch
+
+    t = torch_dtype(dtype)
+    r = np.random.default_rng(5)
+    for (i, h, o), b, left, right in (((37, 70, 41), 5, 3, 4), ((37, 70, 41), 61, 8, 3), ((300, 300, 290), 517, 1, 7)):
+        ws = [tensor(r.uniform(-1, 1, s) * 0.3, dtype, cuda) for s in ((i, h), (i, h), (h, o))]
+        bs = [vector(r.standard_normal(n), cuda, dtype) for n in (h, h, o)]
+        model = P.create_gated_model(*ws, P.Tanh(h), *bs)
+        x, dy = tensor(r.standard_normal((i, b)), dtype, cuda), tensor(r.standard_normal((o, b)), dtype, cuda)
+
+        def wide(rows, columns):
+            a = torch.full((rows + 1, left + columns + right), 7.0, dtype=t, device=cuda)
+            return a, a[:rows, left:left + columns]
+
+        def untouched(a, v):
+            rest = torch.ones_like(a, dtype=torch.bool)
+            rest[:v.shape[0], left:left + v.shape[1]] = False
+            return bool((a[rest] == 7.0).all())
+
+        a, y = wide(o, b)
+        assert model.forward_batch_parallel(x, y) is y
+        assert untouched(a, y) and torch.equal(y, model.forward_batch_parallel(x))
+        y2, states = model.forward_with_states(x)
+        a, y = wide(o, b)
+        sa, sv = wide(3 * h, b)
+        L = A.lib()
+        need = L.ponni_gated_backward_workspace_bytes(model._ref, b)
+        work = torch.empty(need, dtype=torch.uint8, device=cuda)
+        stream = torch.cuda.current_stream().cuda_stream
+        assert L.ponni_gated_forward(model._ref, x.data_ptr(), b, y.data_ptr(), a.stride(0), sv.data_ptr(), sa.stride(0), b,
+                                     work.data_ptr(), L.ponni_gated_workspace_bytes(model._ref, b), stream) == 0
+        assert untouched(a, y) and untouched(sa, sv) and torch.equal(y, y2) and torch.equal(sv, states)
+        want = model.backward(x, states, dy)
+        got = [wide(*s) for s in ((i, b), (i, h), (i, h), (h, o))]
+        biases = [torch.empty(n, dtype=t, device=cuda) for n in (h, h, o)]
+        g = A.GatedGradientArrays(got[0][1].data_ptr(), got[0][0].stride(0), *(v.data_ptr() for _, v in got[1:]),
+                                  *(w.stride(0) for w, _ in got[1:]), *(v.data_ptr() for v in biases))
+        assert L.ponni_gated_backward(model._ref, x.data_ptr(), b, sv.data_ptr(), sa.stride(0), dy.data_ptr(), b, b,
+                                      ctypes.byref(g), work.data_ptr(), need, stream) == 0
+        for (a, v), w in zip(got, (want.x, want.gate, want.up, want.down)):
+            assert untouched(a, v) and torch.equal(v, w)
+        for v, w in zip(biases, (want.gate_bias, want.up_bias, want.down_bias)):
+            assert torch.equal(v, w)
+
+
+def test_gated_gradients_that_are_asked_for(cuda):
+    """Each gradient by itself has the bits that it has among all."""
+    import ctypes
+
+    import torch
+
+    i, h, o, b = 70, 150, 90, 333
+    for dtype in DTYPES:
+        t = torch_dtype(dtype)
+        ws = [(torch.randn(s, device=cuda) / 8).to(t) for s in ((i, h), (i, h), (h, o))]
+        bs = [torch.randn(n, device=cuda).to(t) for n in (h, h, o)]
+        model = P.create_gated_model(*ws, P.Sigmoid(h), *bs)
+        x, dy = torch.randn((i, b), device=cuda).to(t), torch.randn((o, b), device=cuda).to(t)
+        _, states = model.forward_with_states(x)
+        want = model.backward(x, states, dy)
+        only = model.backward(x, states, dy, need_parameters=False)
+        assert torch.equal(only.x, want.x) and only.gate is None and only.down_bias is None
+        rest = model.backward(x, states, dy, need_x=False)
+        assert rest.x is None and torch.equal(rest.up, want.up) and torch.equal(rest.gate_bias, want.gate_bias)
+        L = A.lib()
+        need = L.ponni_gated_backward_workspace_bytes(model._ref, b)
+        work = torch.empty(need, dtype=torch.uint8, device=cuda)
+        for name, ld in (("gate", h), ("up", h), ("down", o), ("gate_bias", 0), ("up_bias", 0), ("down_bias", 0)):
+            v = torch.empty_like(getattr(want, name))
+            g = A.GatedGradientArrays()
+            setattr(g, name, v.data_ptr())
+            if ld:
+                setattr(g, "ld_" + name, ld)
+            assert L.ponni_gated_backward(model._ref, x.data_ptr(), b, states.data_ptr(), states.stride(0), dy.data_ptr(), b, b,
+                                          ctypes.byref(g), work.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == 0
+            if name not in ("gate", "up"):
+                assert torch.equal(v, getattr(want, name)), name
+                continue
+            # One of the two products of x may be cut along k otherwise than both: b terms in another order, and a
+            # rounding to either side.
+            gv, uv = states[:h].double(), states[h:2 * h].double()
+            p, dh = torch.sigmoid(gv), ws[2].double() @ dy.double()
+            dv = dh * uv * p * (1 - p) if name == "gate" else dh * p
+            bound = 1.1 * (2 * b * 2.0 ** -24 * (x.double().abs() @ dv.abs().T)
+                           + torch.finfo(t).eps * getattr(want, name).double().abs())
+            assert bool(((v.double() - getattr(want, name).double()).abs() <= bound).all()), name
+
+
+def test_gated_inputs_beyond_four_gigabytes(cuda):
+    """Columns of an array whose rows lie 4 MB apart: byte offsets past 2^32 in every operand with columns."""
+    import torch
+
+    i, ld, b = 1100, 2_000_000, 150
+    wide = torch.zeros((i, ld), dtype=torch.bfloat16, device=cuda)
+    x = wide[:, ld - b:]
+    x.copy_(torch.randn((i, b), device=cuda))
+    ws = [(torch.randn(s, device=cuda) / 16).bfloat16() for s in ((i, 96), (i, 96), (96, i))]
+    model = P.create_gated_model(*ws, P.Silu(96))
+    near = x.contiguous()
+    for n in (b, 20):
+        want = model.forward_batch_parallel(near[:, :n])
+        assert torch.equal(model.forward_batch_parallel(x[:, :n]), want)
+    y, states = model.forward_with_states(near)
+    want = model.backward(near, states, near)
+    got = model.backward(x, states, x)
+    for name in ("x", "gate", "up", "down"):
+        assert torch.equal(getattr(got, name), getattr(want, name)), name
+    assert torch.equal(model.forward_batch_parallel(near, x), y) and torch.equal(x, y)
+    assert not wide[:, :ld - b].any()
+
+
+def test_gated_work_buffer_of_more_columns(cuda):
+    """One buffer, of the most columns, for calls of fewer."""
+    import torch
+
+    i, h, o, most = 200, 900, 150, 3000
+    for dtype in DTYPES:
+        t = torch_dtype(dtype)
+        ws = [(torch.randn(s, device=cuda) / 16).to(t) for s in ((i, h), (i, h), (h, o))]
+        model = P.create_gated_model(*ws, P.Silu(h))
+        L = A.lib()
+        need = L.ponni_gated_workspace_bytes(model._ref, most)
+        work = torch.empty(need + 64, dtype=torch.uint8, device=cuda)
+        work[need:] = 7
+        for b in (1, 8, 9, 32, 33, 200, 1000, most):
+            x = torch.randn((i, b), device=cuda).to(t)
+            y = torch.empty((o, b), dtype=t, device=cuda)
+            assert L.ponni_gated_forward(model._ref, x.data_ptr(), b, y.data_ptr(), b, None, 0, b, work.data_ptr(), need,
+                                         torch.cuda.current_stream().cuda_stream) == 0
+            assert torch.equal(y, model.forward_batch_parallel(x))
+        assert bool((work[need:] == 7).all())
 
 
 def test_gated_gradient_by_differences(cuda):
@@ -501,6 +731,46 @@ def test_block_operators_on_streams_and_in_graphs(cuda):
             x.copy_(torch.randn((n, b), device=cuda))
             ws[0].copy_(torch.randn((n, h), device=cuda) / 8)
             graph.replay()
+            want = step()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, e) for a, e in zip(outs, want))
+
+
+def test_graphs_of_block_operators_side_by_side(cuda):
+    """Two captured programs, of other sizes, replayed in turn: neither disturbs the other's buffers."""
+    import torch
+
+    programs = []
+    for n, h, c, b in ((72, 900, 300, 3), (160, 700, 1200, 90)):
+        ws = [(torch.randn(s, device=cuda) / 16).bfloat16() for s in ((n, h), (n, h), (h, c))]
+        block = P.create_gated_model(*ws, P.Silu(h))
+        x = torch.randn((n, b), device=cuda).bfloat16()
+        targets = torch.randint(0, c, (b,), dtype=torch.int32, device=cuda)
+        g = torch.randn(b, device=cuda)
+
+        def step(block=block, x=x, targets=targets, g=g):
+            y = block.forward_batch_parallel(x)
+            y2, states = block.forward_with_states(x)
+            r = P.log_probabilities(y, targets, 4)
+            d = block.backward(x, states, r.backward(g))
+            return [y, y2, r.log_probs, r.top_classes, r.top_log_probs, d.x, d.gate, d.up, d.down]
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+        programs.append((graph, outs, step, x))
+    for seed in range(3):
+        torch.manual_seed(seed)
+        for _, _, _, x in programs:
+            x.copy_(torch.randn(x.shape, device=cuda))
+        for graph, _, _, _ in programs:
+            graph.replay()
+        for graph, outs, step, _ in programs[::-1]:
             want = step()
             torch.cuda.synchronize()
             assert all(torch.equal(a, e) for a, e in zip(outs, want))
