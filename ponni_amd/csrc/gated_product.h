@@ -276,7 +276,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 2 ? 2 : 1) void product(Pro
   using LA = Loader<T, A_INNER, BM, PAIR ? 2 : 1, W>;
   using LB = Loader<T, B_INNER, BN, 1, W>;
   constexpr int SLOT = LA::BYTES + LB::BYTES, REQ = LA::REQUESTS + LB::REQUESTS;
-  static_assert(NJ % 4 == 0 && MI % (PAIR && ES == 4 ? 8 : 4) == 0 && !(PAIR && A_INNER), "blocks of 64");
+  static_assert(NJ % 4 == 0 && (ES == 2 || NJ == 4) && MI % (PAIR && ES == 4 ? 8 : 4) == 0 && !(PAIR && A_INNER), "blocks of 64");
   __shared__ __attribute__((aligned(1024))) char lds[kSlots * SLOT];
   int const lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -358,11 +358,12 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 2 ? 2 : 1) void product(Pro
     // Requests and reads stand between the products of 16 bits; where one side has k inside, before them.  bf16
     // 1024 x 4096 x 16,384: 108 us between, 118 before; with k inside 258 and 253, in fp32 no difference.
     constexpr bool BETWEEN = ES == 2 && !A_INNER;
+    // fp32: a sum's four products stand all others apart.
     constexpr int SLOTS = kMfmaParts<T> * MI;
 #pragma unroll
-    for (int j = 0; j < NJ; j++) {
-      int const r0 = j * REQ / NJ, requests = (j + 1) * REQ / NJ - r0;
-      int const f0 = j * READS / NJ, events = requests + (j + 1) * READS / NJ - f0;
+    for (int q = 0; q < NJ; q++) {
+      int const r0 = q * REQ / NJ, requests = (q + 1) * REQ / NJ - r0;
+      int const f0 = q * READS / NJ, events = requests + (q + 1) * READS / NJ - f0;
 #pragma unroll
       for (int t = 0; t < SLOTS; t++) {
 #pragma unroll
@@ -374,8 +375,8 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 2 ? 2 : 1) void product(Pro
             if (WHOLE || step + 1 < end) read(step + 1, std::integral_constant<int, 1 - set>{}, f0 + n - requests);
           }
         }
-        acc[t % MI][j] = mfma_part<T>(fragment<T, B_INNER>(bv[set], j, t / MI), fragment<T, A_INNER>(av[set], t % MI, t / MI),
-                                       acc[t % MI][j], t / MI);
+        int const i = t % MI, j = ES == 4 ? t / MI : q, e = ES == 4 ? q : 0;
+        acc[i][j] = mfma_part<T>(fragment<T, B_INNER>(bv[set], j, e), fragment<T, A_INNER>(av[set], i, e), acc[i][j], e);
         if (BETWEEN || t == SLOTS - 1) __builtin_amdgcn_sched_barrier(0);
       }
     }

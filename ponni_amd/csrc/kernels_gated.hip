@@ -25,15 +25,23 @@ template <class T> __global__ __launch_bounds__(256) void align_rows(T const* fr
   v.store(to + row * ld_to + c, N);
 }
 
-// y[row] = the sum of a row.
-template <class T> __global__ __launch_bounds__(256) void row_sums(T const* x, int64_t ld, int64_t columns, T* y) {
+// y[row] = the sum of a row, of up to three arrays: a launch for all of a block's biases.
+struct RowSums {
+  void const* x[3];
+  int64_t ld[3], rows[3];
+  void* y[3];
+};
+template <class T> __global__ __launch_bounds__(256) void row_sums(RowSums a, int64_t columns) {
   constexpr int N = 16 / sizeof(T);
   __shared__ float lds[4];
-  T const* row = x + int64_t(blockIdx.x) * ld;
+  int64_t row = blockIdx.x;
+  int const which = row < a.rows[0] ? 0 : row < a.rows[0] + a.rows[1] ? 1 : 2;
+  row -= which == 0 ? 0 : which == 1 ? a.rows[0] : a.rows[0] + a.rows[1];
+  T const* const x = static_cast<T const*>(a.x[which]) + row * a.ld[which];
   float s[N] = {};
   for (int64_t c = threadIdx.x * N; c < columns; c += 256 * N) {
     Pack<T, N> v;
-    v.load(row + c, columns - c < N ? int(columns - c) : N, 0.0f);
+    v.load(x + c, columns - c < N ? int(columns - c) : N, 0.0f);
 #pragma unroll
     for (int e = 0; e < N; e++) s[e] += v[e];
   }
@@ -43,7 +51,7 @@ template <class T> __global__ __launch_bounds__(256) void row_sums(T const* x, i
   for (int d = 1; d < 64; d *= 2) t += __shfl_xor(t, d);
   if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = t;
   __syncthreads();
-  if (threadIdx.x == 0) y[blockIdx.x] = T((lds[0] + lds[1]) + (lds[2] + lds[3]));
+  if (threadIdx.x == 0) static_cast<T*>(a.y[which])[row] = T((lds[0] + lds[1]) + (lds[2] + lds[3]));
 }
 
 int64_t round_to(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
@@ -159,10 +167,10 @@ template <class T> struct Run {
                                          : launch_product_bf16)(form, c.large, p, stream);
     work = before;
   }
-  void sums(void* y, void const* x, int64_t rows, int64_t ld, int64_t columns) {
-    if (y == nullptr || err != hipSuccess) return;
-    hipLaunchKernelGGL(row_sums<T>, dim3(unsigned(rows)), dim3(256), 0, stream, static_cast<T const*>(x), ld, columns,
-                       static_cast<T*>(y));
+  void sums(RowSums const& a, int64_t columns) {
+    int64_t const rows = a.rows[0] + a.rows[1] + a.rows[2];
+    if (err != hipSuccess || rows == 0) return;
+    hipLaunchKernelGGL(row_sums<T>, dim3(unsigned(rows)), dim3(256), 0, stream, a, columns);
     err = hipGetLastError();
   }
 };
@@ -315,9 +323,9 @@ hipError_t launch_gated_backward(ponni_gated const& b, int act, void const* x, i
       q.k = columns, q.rows = hidden, q.columns = b.n_out, q.y[0] = d.down, q.ld[0] = d.ld_down;
       run.product(FORM_WEIGHTS, q);
     }
-    run.sums(d.gate_bias, dg, hidden, ld, columns);
-    run.sums(d.up_bias, du, hidden, ld, columns);
-    run.sums(d.down_bias, dy, b.n_out, ld_dy, columns);
+    run.sums({{dg, du, dy}, {ld, ld, ld_dy},
+              {d.gate_bias ? hidden : 0, d.up_bias ? hidden : 0, d.down_bias ? b.n_out : 0},
+              {d.gate_bias, d.up_bias, d.down_bias}}, columns);
     err = run.err;
   });
   return err;
