@@ -14,7 +14,12 @@
 //   d_x = r1 (e1 - mean(e1) - u1 mean(e1 u1));
 // weights' gradients are sums over columns: a workgroup adds those of its tiles in
 // registers, a second kernel the workgroups' in their order.
-// Columns of more features than the registers hold are read again for each sum.
+// Columns of more features than the registers hold (shape_of) are read again for each sum, 128 bytes of a row at a time.
+//
+// Bound by bytes: what a tile reads waits for its sums, which workgroups of the same CU fill up to where registers end.
+// bf16, 1024 features x 65,536, rms norms after and before, a gate for each feature: 170 us, 3.2 TB/s; its gradients 432.
+// fp32, 333 x 40,003 (rows at any 4 bytes), all inputs: 98 us, 2.7 TB/s; gradients 174 + 13.  fp16, 4096 x 16,384 (read
+// again): 170 us; gradients 280 + 9.  One column of 4096: 6.6 us.
 #pragma once
 
 #include <algorithm>
@@ -151,6 +156,25 @@ __global__ __launch_bounds__(kThreads, (HELD && STEPS > 4) || GATE ? 2 : 4) void
     }
   };
   if (HELD) load(0, true);
+  // With one column a lane the features' own are under way with the columns, not behind the sums: bf16, one column of 4096,
+  // 8.2 us without.
+  constexpr bool EARLY = HELD && NC == 1;
+  float early[EARLY ? 5 : 1][EARLY ? STEPS : 1];
+  float const* const own[5] = {r.after.weight, r.after.bias, r.feature_gate, r.before.weight, r.before.bias};
+  if constexpr (EARLY) {
+#pragma unroll
+    for (int k = 0; k < 5; k++)
+#pragma unroll
+      for (int s = 0; s < STEPS; s++) {
+        int const row = s * down + ty;
+        early[k][s] = feature(own[k], row < n ? row : 0, k == 1 || k == 4 ? 0.0f : 1.0f);
+      }
+  }
+  // Of row s of the lane's, `row` of all: 0, 1 weight and bias after, 2 gate, 3, 4 weight and bias before.
+  auto of_feature = [&](int k, int s, int row) {
+    if constexpr (EARLY) return early[k][s];
+    else return feature(own[k], row, k == 1 || k == 4 ? 0.0f : 1.0f);
+  };
   float m1[LAYER ? NC : 1] = {}, m2[LAYER ? NC : 1] = {}, r1[NC], r2[NC];
   auto mean1 = [&](int j) { return LAYER ? m1[j] : 0.0f; };
   auto mean2 = [&](int j) { return LAYER ? m2[j] : 0.0f; };
@@ -182,8 +206,7 @@ __global__ __launch_bounds__(kThreads, (HELD && STEPS > 4) || GATE ? 2 : 4) void
   }
   auto state = [&](int s, int i, float (&v)[NC]) {
     int const row = i * down + ty;
-    float const w = feature(r.after.weight, row, 1.0f), b = feature(r.after.bias, row, 0.0f);
-    float const g = r.scale * feature(r.feature_gate, row, 1.0f);
+    float const w = of_feature(0, s, row), b = of_feature(1, s, row), g = r.scale * of_feature(2, s, row);
 #pragma unroll
     for (int j = 0; j < NC; j++) {
       float const branch = fmaf((x[s][j] - mean1(j)) * r1[j], w, b);
@@ -231,7 +254,7 @@ __global__ __launch_bounds__(kThreads, (HELD && STEPS > 4) || GATE ? 2 : 4) void
     }
     if (r.normed != nullptr) {
       int const row = i * down + ty;
-      float const w = feature(r.before.weight, row, 1.0f), b = feature(r.before.bias, row, 0.0f);
+      float const w = of_feature(3, s, row), b = of_feature(4, s, row);
 #pragma unroll
       for (int j = 0; j < NC; j++) o.set(j, fmaf((v[j] - mean2(j)) * r2[j], w, b));
       o.store(rows_n.at(i), count);
@@ -463,9 +486,12 @@ inline Shape shape_of(int32_t n, int64_t columns, int32_t dtype, int max_steps, 
   auto steps_at = [&](int l) { return (n + (kThreads >> l) - 1) / (kThreads >> l); };
   auto tiles_at = [&](int l) { return (lanes + (1 << l) - 1) >> l; };
   while (s.lane_columns > 0 && tiles_at(s.lane_columns) < 256) s.lane_columns--;
-  // In registers at 128 bytes of a row, in the forward pass down to 64; narrower pieces are slower than to read whole lines
-  // again.  us in registers / read again, bf16, 67 M elements, rms norms, forward: n = 1024 (128 bytes) 151 / 170,
-  // 2048 (64) 168 / 178, 4096 (32 bytes) 285 / 191; before only, backward: 1024 (64) 243 / 216, 4096 (16) 418 / 230.
+  // In registers at 128 bytes of a row or down to `narrowest` (3: 128, 1: 32): the kernel that reads whole lines again reads
+  // more, narrower pieces come slower.  us in registers / read again, 67 M elements: forward bf16, rms norms, n = 1024
+  // (128 bytes) 151 / 170, 2048 (64) 162 / 179, 4096 (32) 285 / 191, with a gate layer norms 2048 (32) 274 / 322;
+  // backward fp32 rms norms 1024 (64) 561 / 833, 2048 (32) 771 / 865, a norm before alone 1024 (64) 552 / 542, 2048 (32)
+  // 673 / 589; backward bf16 rms norms 2048 (32) 498 / 413, layer norms 700 (64) 588 / 453, a norm before alone 4096 (16
+  // bytes) 418 / 230.
   if (steps_at(s.lane_columns) > max_steps && (s.lane_columns < 3 || steps_at(narrowest) <= max_steps))
     while (s.lane_columns > 0 && steps_at(s.lane_columns) > max_steps) s.lane_columns--;
   int const steps = steps_at(s.lane_columns);
@@ -479,9 +505,21 @@ inline Shape shape_of(int32_t n, int64_t columns, int32_t dtype, int max_steps, 
   return s;
 }
 
-// Rows a lane can hold without spilling.
-inline int most_steps(int32_t dtype, bool backward, bool gate) {
-  return backward ? (gate && dtype != PONNI_F32 ? 4 : 8) : gate ? 8 : 16;
+inline bool has_layer(ponni_residual_norm const& r) {
+  return r.after.kind == PONNI_NORM_LAYER || r.before.kind == PONNI_NORM_LAYER;
+}
+
+// Rows that a lane holds at most.  A few spilled registers cost less than to read again (backward, fp32 rms norms, n = 512
+// 455 / 811 us), but not those of two layer norms of 16 bits (bf16, n = 512: 525 / 461).
+inline int most_steps(ponni_residual_norm const& r, bool backward) {
+  bool const gate = r.gate != nullptr, half = r.dtype != PONNI_F32;
+  if (!backward) return gate ? 8 : 16;
+  return half && (gate || (has_layer(r) && r.after.kind != PONNI_NORM_NONE)) ? 4 : 8;
+}
+// log2 of the lanes across, at least.
+inline int narrowest(ponni_residual_norm const& r, bool backward) {
+  if (!backward) return r.gate != nullptr ? 1 : 2;
+  return r.dtype != PONNI_F32 ? 3 : r.after.kind != PONNI_NORM_NONE ? 1 : 2;
 }
 
 // f(steps, held, gate, layer) as constants.
@@ -497,12 +535,9 @@ template <class F> void with_variant(Shape const& s, bool gate, bool layer, F&& 
   else if (layer) pick(std::false_type{}, std::true_type{});
   else pick(std::false_type{}, std::false_type{});
 }
-inline bool has_layer(ponni_residual_norm const& r) {
-  return r.after.kind == PONNI_NORM_LAYER || r.before.kind == PONNI_NORM_LAYER;
-}
 
 template <class T> hipError_t launch_norm(ponni_residual_norm const& r, hipStream_t stream) {
-  Shape const s = shape_of(r.n, r.columns, r.dtype, most_steps(r.dtype, false, r.gate != nullptr), 2);
+  Shape const s = shape_of(r.n, r.columns, r.dtype, most_steps(r, false), narrowest(r, false));
   NormArgs a{};
   a.r = r;
   a.lane_columns = s.lane_columns;
@@ -513,8 +548,10 @@ template <class T> hipError_t launch_norm(ponni_residual_norm const& r, hipStrea
   with_variant(s, r.gate != nullptr, has_layer(r), [&](auto steps, auto held, auto gate, auto layer) {
     constexpr int S = decltype(steps)::value, NC = 16 / sizeof(T);
     constexpr bool H = decltype(held)::value, G = decltype(gate)::value, L = decltype(layer)::value;
-    if (s.columns == 1) hipLaunchKernelGGL((residual_norm<T, 1, S, H, G, true>), grid, dim3(kThreads), 0, stream, a);
-    else hipLaunchKernelGGL((residual_norm<T, NC, S, H, G, L>), grid, dim3(kThreads), 0, stream, a);
+    if constexpr (!(G && S == 16)) {  // (most_steps)
+      if (s.columns == 1) hipLaunchKernelGGL((residual_norm<T, 1, S, H, G, true>), grid, dim3(kThreads), 0, stream, a);
+      else hipLaunchKernelGGL((residual_norm<T, NC, S, H, G, L>), grid, dim3(kThreads), 0, stream, a);
+    }
   });
   return hipGetLastError();
 }
@@ -522,7 +559,7 @@ template <class T> hipError_t launch_norm(ponni_residual_norm const& r, hipStrea
 template <class T>
 hipError_t launch_norm_backward(ponni_residual_norm const& r, ponni_residual_norm_gradients const& g, void* workspace,
                                 int& groups, hipStream_t stream) {
-  Shape const s = shape_of(r.n, r.columns, r.dtype, most_steps(r.dtype, true, r.gate != nullptr), 3);
+  Shape const s = shape_of(r.n, r.columns, r.dtype, most_steps(r, true), narrowest(r, true));
   NormArgs a{};
   a.r = r;
   a.g = g;
@@ -535,13 +572,14 @@ hipError_t launch_norm_backward(ponni_residual_norm const& r, ponni_residual_nor
     constexpr int S = decltype(steps)::value, NC = 16 / sizeof(T);
     constexpr bool H = decltype(held)::value, G = decltype(gate)::value, L = decltype(layer)::value;
     dim3 const grid(groups), block(kThreads);
-    if constexpr (!(G && S == 8 && sizeof(T) == 2) && S < 16) {
+    if constexpr (!(G && S == 8 && sizeof(T) == 2) && S < 16) {  // (most_steps)
       if (r.after.kind == PONNI_NORM_NONE) {
         if (s.columns == 1) hipLaunchKernelGGL((residual_norm_backward<T, 1, S, H, G, true, false>), grid, block, 0, stream, a);
         else hipLaunchKernelGGL((residual_norm_backward<T, NC, S, H, G, L, false>), grid, block, 0, stream, a);
       } else {
         if (s.columns == 1) hipLaunchKernelGGL((residual_norm_backward<T, 1, S, H, G, true, true>), grid, block, 0, stream, a);
-        else hipLaunchKernelGGL((residual_norm_backward<T, NC, S, H, G, L, true>), grid, block, 0, stream, a);
+        else if constexpr (!(L && H && S == 8 && sizeof(T) == 2))
+          hipLaunchKernelGGL((residual_norm_backward<T, NC, S, H, G, L, true>), grid, block, 0, stream, a);
       }
     }
   });
