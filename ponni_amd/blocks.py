@@ -25,9 +25,7 @@ from .model import _DTYPES, Layer
 
 
 def _empty(like, *shape, dtype=None):
-    import torch
-
-    return torch.empty(shape, dtype=dtype or like.dtype, device=like.device)
+    return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
 
 
 def _work(like, need: int):
