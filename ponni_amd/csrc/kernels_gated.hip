@@ -222,7 +222,7 @@ int64_t gated_workspace_bytes(ponni_gated const& b, int64_t columns, bool backwa
     t.take(sums_bytes(o, columns, 1, steps_of(h, es)));
     // (the slices become fewer past 8 columns)
     return std::max({t.used, thin_plan(b, std::min<int64_t>(columns, 8)).bytes(),
-                     thin_plan(b, std::min<int64_t>(columns, kThinColumns)).bytes()});
+                     thin_plan(b, std::min<int64_t>(columns, thin_columns(es))).bytes()});
   }
   t.take(aligned_bytes(o, columns, es));
   t.take(aligned_bytes(2 * h, columns, es));  // dg, du
@@ -238,7 +238,7 @@ hipError_t launch_gated(ponni_gated const& b, int act, void const* x, int64_t ld
     using T = decltype(e);
     Run<T> run{{static_cast<char*>(workspace)}, stream};
     int64_t const hidden = b.n_hidden, es = sizeof(T);
-    if (states == nullptr && columns <= kThinColumns) {
+    if (states == nullptr && columns <= thin_columns(es)) {
       ThinPlan const plan = thin_plan(b, columns);
       ThinArgs first{}, last{};
       first.w[0] = b.gate, first.w[1] = b.up, first.ld[0] = b.ld_gate, first.ld[1] = b.ld_up;
