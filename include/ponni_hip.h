@@ -670,7 +670,8 @@ typedef struct ponni_gated {
 #define PONNI_GATED_MAX_COLUMNS 16777216
 
 /* y [n_out, columns] of x [n_in, columns].  states [3 n_hidden, columns], or null:
- * g and u, rounded to the type, and h, which the backward pass reads. */
+ * g and u, rounded to the type, and h, which the backward pass reads.  Batches of
+ * other sizes, and calls with and without states, add in other orders: a column's y may differ in its last bits. */
 int ponni_gated_forward(const ponni_gated* block, const void* x, int64_t ld_x, void* y, int64_t ld_y, void* states,
                         int64_t ld_states, int64_t columns, void* workspace, int64_t workspace_bytes,
                         hipStream_t stream);

@@ -52,10 +52,6 @@ hipError_t launch_product_f16(Form form, bool large, ProductArgs const& p, hipSt
 hipError_t launch_product_bf16(Form form, bool large, ProductArgs const& p, hipStream_t stream);
 
 // A product of few columns (gated_thin.h): parts [slices, problems, columns, stride] of fp32.
-// At most so many, by the elements' bytes.  us so / in tiles, 1024-4096-1024: bf16 1 column 18 / 31, 32 columns 26 / 28; fp32 32 columns
-// 33 / 161, 128 82 / 163, 256 139 / 168, 384 198 / 177 (whose tiles of 128 columns leave CUs idle); fp16 256-700-256, 32
-// columns 20 / 20; fp32 333-1001-77, 256 columns 30 / 68.
-constexpr int thin_columns(int64_t es) { return es == 4 ? 256 : 32; }
 enum ThinInput { THIN_COLUMNS, THIN_PARTS, THIN_ROWS };
 struct ThinArgs {
   void const* w[2];  // [k, outputs]

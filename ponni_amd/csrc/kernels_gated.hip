@@ -188,6 +188,15 @@ Slices slices_of(int64_t es, int64_t k, int64_t outputs, int problems, int64_t g
   int64_t const held = std::min<int64_t>(each, 1024 / es);
   return {int((k + held - 1) / held), int(held)};
 }
+// Columns that they take at most.  fp32: up to 512 while tiles of the first products would leave half of the CUs idle.  us
+// so / in tiles, 1024-4096-1024: bf16 1 column 18 / 31, 32 columns 26 / 28; fp32 32 columns 33 / 161, 128 82 / 163, 256 (128
+// tiles) 139 / 168, 384 198 / 177; fp32 333-1001-77, 512 columns 40 / 69, 64-4096-64, 256 32 / 45, 4096-1024-4096, 512
+// 271 / 553.
+int64_t most_thin(ponni_gated const& b) {
+  constexpr int64_t kThin = 32, kMostThin = 512, kTiles = 128;
+  if (element(b) == 2) return kThin;
+  return std::clamp(kTiles / ((b.n_hidden + 63) / 64) * 128, kThin, kMostThin);
+}
 struct ThinPlan {
   Slices hidden, last;
   int64_t stride_hidden, stride_last, parts_hidden, parts_last, rows;  // strides in elements, the others in bytes
@@ -222,7 +231,7 @@ int64_t gated_workspace_bytes(ponni_gated const& b, int64_t columns, bool backwa
     t.take(sums_bytes(o, columns, 1, steps_of(h, es)));
     // (the slices become fewer past 8 columns)
     return std::max({t.used, thin_plan(b, std::min<int64_t>(columns, 8)).bytes(),
-                     thin_plan(b, std::min<int64_t>(columns, thin_columns(es))).bytes()});
+                     thin_plan(b, std::min(columns, most_thin(b))).bytes()});
   }
   t.take(aligned_bytes(o, columns, es));
   t.take(aligned_bytes(2 * h, columns, es));  // dg, du
@@ -238,7 +247,7 @@ hipError_t launch_gated(ponni_gated const& b, int act, void const* x, int64_t ld
     using T = decltype(e);
     Run<T> run{{static_cast<char*>(workspace)}, stream};
     int64_t const hidden = b.n_hidden, es = sizeof(T);
-    if (states == nullptr && columns <= thin_columns(es)) {
+    if (states == nullptr && columns <= most_thin(b)) {
       ThinPlan const plan = thin_plan(b, columns);
       ThinArgs first{}, last{};
       first.w[0] = b.gate, first.w[1] = b.up, first.ld[0] = b.ld_gate, first.ld[1] = b.ld_up;

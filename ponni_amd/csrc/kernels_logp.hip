@@ -12,7 +12,7 @@
 // order.  The largest logits are lists in descending order, of equal values by
 // class; two lists are joined by a bitonic step.
 // Bound by the logits' way from memory; 11 VALU operations an element beside it.  bf16 65,536 classes x 4096: 150 + 5 us, 3.5
-// TB/s, the gradient 212, 5.1 TB/s read and written; fp32 10 x 4,194,304 with the 3 largest: 100, 3.1 TB/s of logits and
+// TB/s, the gradient 212, 5.1 TB/s read and written; fp32 10 x 4,194,304 with the 3 largest: 100, 3.4 TB/s of logits and
 // results; one bf16 column of 131,072 with the 8 largest: 15 + 7, latency.
 #include <cmath>
 
