@@ -79,6 +79,8 @@ class GatedInference:
     pointwise layer: Relu, LeakyRelu, Gelu, Silu, Sigmoid or Tanh of n_hidden features."""
 
     def __init__(self, gate, up, down, act: Layer, gate_bias=None, up_bias=None, down_bias=None):
+        if not isinstance(act, Layer):
+            raise ValueError(f"act must be a pointwise layer such as Silu(n_hidden), not {act!r}")
         _rows(gate, "gate")
         self.n_in, self.n_hidden = gate.shape
         _array(up, "up", gate, self.n_in, self.n_hidden)

@@ -206,6 +206,8 @@ def test_python_refusals():
         P.log_probabilities(torch.zeros(3, 4))  # not on a GPU
     with pytest.raises(ValueError):
         P.create_gated_model(torch.zeros(3, 4), torch.zeros(3, 4), torch.zeros(4, 2), P.Silu(4))
+    with pytest.raises(ValueError, match="act must be"):
+        P.create_gated_model(torch.zeros(3, 4), torch.zeros(3, 4), torch.zeros(4, 2), "silu")
 
 
 # -- the oracle's formulas by differences ---------------------------------------------------------

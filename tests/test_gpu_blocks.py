@@ -274,6 +274,12 @@ def test_norms_without_weights(cuda):
     check_norm(cuda, 120, 50, "layer", "rms", "full", False, "f32", weight=True, bias=False, scale=-1.0)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_norms_of_the_most_features(cuda, dtype):
+    for b in (1, 3, 20):
+        check_norm(cuda, 65536, b, "layer", "rms", "full", True, dtype)
+
+
 def test_norm_of_constant_columns(cuda):
     """Nothing is left to normalise: a layer norm gives its bias, zeros under eps."""
     import torch
@@ -467,6 +473,16 @@ def test_gated_few_columns(cuda, sizes, dtype):
     for the order of sums."""
     for b in (1, 7, 8, 9, 15, 16, 17, 31, 32, 33, *((64, 65, 257, 511, 512, 513) if dtype == "f32" else ())):
         check_gated(cuda, sizes, b, "gelu", dtype, bias=b % 2 == 0, pad=b % 3, backward=False, seed=b, wpad=b % 4)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_widest(cuda, dtype):
+    """The largest widths, one at a time, and (16 bits) the most columns."""
+    for sizes in ((2, 65536, 1), (65536, 3, 2), (5, 2, 65536)):
+        for b in (1, 40):
+            check_gated(cuda, sizes, b, "relu", dtype, bias=True)
+    if dtype == "bf16":
+        check_gated(cuda, (2, 3, 1), A.GATED_MAX_COLUMNS, "relu", dtype)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
