@@ -6,8 +6,8 @@
 // ([i, k]: transposed weights, and both operands of a weight's gradient).
 //
 // A step is 64 bytes of k of every row: 32 features of a 16-bit type, 16 of fp32.  Its
-// tiles go from memory straight into one of kSlots slots of LDS, up to kSlots - 1 steps
-// ahead, a request's 64 pieces of 16 bytes in a row; a step's fragments are
+// tiles go from memory straight into one of four slots of LDS, up to three steps
+// ahead (fp32 with k outside: three slots), a request's 64 pieces of 16 bytes in a row; a step's fragments are
 // read while the one before is multiplied.  Rows of k outside are
 // turned on their way out of LDS (ds_read_b64_tr_b16: four rows of four elements to four
 // lanes); pieces lie at places that depend on their row, so that a
@@ -24,7 +24,7 @@
 // beside them where it is short: all workgroups come to their outputs together.  bf16 1024-4096-1024, 16,384 columns, us (PFLOP/s):
 // g, u and h 315 (0.87), y 114 (1.21), dg and du 279 (0.49), dx 270 (1.02), dG and dU 256 + 12 (1.03),
 // dD 147 + 14 (0.85); a library's product of 8192 x 8192 x 8192 1.12.  fp16 2048-8192-2048,
-// 32,768: h 1961 (1.12), y 860 (1.28).  fp32 1024-4096-1024, 16,384: 116 to 142 TFLOP/s of 154; 333-1001-77, 5,003: 55 to
+// 32,768: h 1961 (1.12), y 860 (1.28).  fp32 1024-4096-1024, 16,384: 136 to 142 TFLOP/s of 154; 333-1001-77, 5,003: 66 to
 // 83, few tiles and short sums.
 #pragma once
 
@@ -43,7 +43,6 @@ namespace {
 
 typedef __attribute__((address_space(3))) void* lds_void;
 
-constexpr int kSlots = 4;
 constexpr int kGroup = 8;  // columns of tiles that workgroups of an XCD share
 
 __device__ inline uint64_t uniform64(uint64_t p) {
@@ -277,12 +276,15 @@ template <class T> __device__ inline void load16(T const* x, int64_t left, float
 
 // TWO: a sum of two products, of operands of the same shapes and strides.
 template <class T, bool A_INNER, bool B_INNER, Output OUT, bool TWO, int MI, int NJ, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, WM * WN > 2 ? 2 : 1) void product(ProductArgs p) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void product(ProductArgs p) {
   constexpr int W = WM * WN, BM = 16 * MI * WM, BN = 16 * NJ * WN, ES = sizeof(T), STEP = 64 / ES;
   constexpr bool PAIR = OUT == OUT_PAIR;
   using LA = Loader<T, A_INNER, BM, PAIR ? 2 : 1, W>;
   using LB = Loader<T, B_INNER, BN, 1, W>;
-  constexpr int SLOT = LA::BYTES + LB::BYTES, REQ = LA::REQUESTS + LB::REQUESTS;
+  // fp32, k outside: a quarter of k is done with behind its products, so that the next step's takes its registers and two
+  // waves of both products fit a SIMD: 1024-4096-1024 x 16,384 2025 us for 2279, 333-1001 x 5,003 101 for 118.
+  constexpr bool SINGLE = ES == 4 && !A_INNER && !B_INNER;
+  constexpr int kSlots = SINGLE ? 3 : 4, SLOT = LA::BYTES + LB::BYTES, REQ = LA::REQUESTS + LB::REQUESTS;
   static_assert(NJ % 4 == 0 && (ES == 2 || NJ == 4) && MI % (PAIR && ES == 4 ? 8 : 4) == 0 && !(PAIR && A_INNER), "blocks of 64");
   __shared__ __attribute__((aligned(1024))) char lds[kSlots * SLOT];
   int const lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
@@ -336,9 +338,9 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 2 ? 2 : 1) void product(Pro
   constexpr int HALF = PAIR ? MI / 2 : MI;  // fragments of a panel
   unsigned const read_a = LA::read_base(wm * 16 * HALF, lane), read_b = LB::read_base(wn * 16 * NJ, lane);
   f32x4 acc[MI][NJ] = {};
-  i32x4 av[2][MI], bv[2][NJ];
+  i32x4 av[SINGLE ? 1 : 2][MI], bv[SINGLE ? 1 : 2][NJ];
   auto read = [&](int step, auto at_set, int r) __attribute__((always_inline)) {
-    constexpr int set = decltype(at_set)::value;
+    constexpr int set = SINGLE ? 0 : decltype(at_set)::value;
     char const* slot = lds + unsigned(step - first_step) % kSlots * SLOT;
     if (r < MI) {
       int const panel = r / HALF;
@@ -351,7 +353,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 2 ? 2 : 1) void product(Pro
   using First = std::integral_constant<int, 0>;
   using Second = std::integral_constant<int, 1>;
   auto multiply = [&](int step, auto at_set, auto whole) __attribute__((always_inline)) {
-    constexpr int set = decltype(at_set)::value;
+    constexpr int set = SINGLE ? 0 : decltype(at_set)::value;
     constexpr bool WHOLE = decltype(whole)::value;  // a step kSlots on
     if constexpr (A_INNER || B_INNER) {
       int64_t const left = p.k - int64_t(TWO && step >= steps_each ? step - steps_each : step) * STEP;
@@ -370,7 +372,7 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 2 ? 2 : 1) void product(Pro
 #pragma unroll
     for (int q = 0; q < NJ; q++) {
       int const r0 = q * REQ / NJ, requests = (q + 1) * REQ / NJ - r0;
-      int const f0 = q * READS / NJ, events = requests + (q + 1) * READS / NJ - f0;
+      int const f0 = q * READS / NJ, events = requests + (SINGLE ? 0 : (q + 1) * READS / NJ - f0);
 #pragma unroll
       for (int t = 0; t < SLOTS; t++) {
 #pragma unroll
@@ -385,6 +387,10 @@ __global__ __launch_bounds__(64 * WM * WN, WM * WN > 2 ? 2 : 1) void product(Pro
         int const i = t % MI, j = ES == 4 ? t / MI : q, e = ES == 4 ? q : 0;
         acc[i][j] = mfma_part<T>(fragment<T, B_INNER>(bv[set], j, e), fragment<T, A_INNER>(av[set], i, e), acc[i][j], e);
         if (BETWEEN || t == SLOTS - 1) __builtin_amdgcn_sched_barrier(0);
+      }
+      if (SINGLE && (WHOLE || step + 1 < end)) {
+#pragma unroll
+        for (int r = q; r < READS; r += 4) read(step + 1, First{}, r);
       }
     }
   };
@@ -525,7 +531,7 @@ hipError_t launch_tiles(ProductArgs p, hipStream_t stream) {
 template <class T, bool A_INNER, bool B_INNER, Output OUT, bool TWO = false> hipError_t launch_sized(bool large, ProductArgs const& p, hipStream_t stream) {
   if constexpr (sizeof(T) == 2)
     if (large) return launch_tiles<T, A_INNER, B_INNER, OUT, TWO, 8, 4, 2, 4>(p, stream);
-  if constexpr (sizeof(T) == 4 && OUT == OUT_PAIR) return launch_tiles<T, A_INNER, B_INNER, OUT, TWO, 8, 4, 1, 2>(p, stream);
+  if constexpr (sizeof(T) == 4 && OUT == OUT_PAIR) return launch_tiles<T, A_INNER, B_INNER, OUT, TWO, 8, 4, 2, 2>(p, stream);
   else return launch_tiles<T, A_INNER, B_INNER, OUT, TWO, 4, 4, 2, 2>(p, stream);
 }
 
