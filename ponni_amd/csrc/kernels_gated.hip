@@ -67,7 +67,7 @@ int64_t own_stride(int64_t columns, int64_t es) { return round_to(columns, 128 /
 //   200 columns         53 + 149          32 + 71      105 + 260         54 + 116     34 + 71
 //   1000 columns        62 + 174          59 + 116     108 + 295         68 + 161     51 + 119
 //   16,000 columns      476 + 1114        462 + 1118   376 + 1183        377 + 835    384 + 839
-// and fp32 (128 x 128) 333-1001-77, 5000 columns: whole 178 + 818, chosen 140 + 233.
+// and fp32 (128 x 128) 333-1001-77, 5000 columns: whole 159 + 846, chosen 120 + 234.
 struct Choice {
   bool large;
   int parts;
@@ -188,10 +188,10 @@ Slices slices_of(int64_t es, int64_t k, int64_t outputs, int problems, int64_t g
   int64_t const held = std::min<int64_t>(each, 1024 / es);
   return {int((k + held - 1) / held), int(held)};
 }
-// Columns that they take at most.  fp32: up to 512 while tiles of the first products would leave half of the CUs idle.  us
-// so / in tiles, 1024-4096-1024: bf16 1 column 18 / 31, 32 columns 26 / 28; fp32 32 columns 33 / 161, 128 82 / 163, 256 (128
-// tiles) 139 / 168, 384 198 / 177; fp32 333-1001-77, 512 columns 40 / 69, 64-4096-64, 256 32 / 45, 4096-1024-4096, 512
-// 271 / 553.
+// Columns that they take at most.  fp32: up to 512 while tiles of the first products would leave half of the CUs idle (as
+// tiles of 64 features and 128 columns count).  us so / in tiles: bf16 1024-4096-1024 1 column 16 / 30, 32 columns 25 / 27;
+// fp16 256-700-256, 32 columns 20 / 17; fp32 1024-4096-1024 32 columns 33 / 154, 128 82 / 158, 256 (128 tiles) 143 / 163, 384 195 / 170;
+// 333-1001-77, 512 columns 40 / 65; 64-4096-64, 256 32 / 45; 4096-1024-4096, 512 270 / 528.
 int64_t most_thin(ponni_gated const& b) {
   constexpr int64_t kThin = 32, kMostThin = 512, kTiles = 128;
   if (element(b) == 2) return kThin;
