@@ -12,7 +12,7 @@
 // order.  The largest logits are lists in descending order, of equal values by
 // class; two lists are joined by a bitonic step.
 // Bound by the logits' way from memory; 11 VALU operations an element beside it.  bf16 65,536 classes x 4096: 150 + 5 us, 3.5
-// TB/s, the gradient 212, 5.1 TB/s read and written; fp32 10 x 4,194,304 with the 3 largest: 100, 3.4 TB/s of logits and
+// TB/s, the gradient 205, 5.2 TB/s read and written; fp32 10 x 4,194,304 with the 3 largest: 100, 3.4 TB/s of logits and
 // results; one bf16 column of 131,072 with the 8 largest: 15 + 7, latency.
 #include <cmath>
 
@@ -530,8 +530,9 @@ hipError_t launch_logp_backward(ponni_log_probs const& p, float const* d_log_pro
   int64_t const across = int64_t(nc) << a.lane_columns, turn = (kThreads >> a.lane_columns) * (nc >= 4 ? 4 : 8);
   a.tiles = (p.columns + across - 1) / across;
   int64_t const turns = (p.classes + turn - 1) / turn;
-  // A workgroup takes a few turns, unless the grid is small.
-  int64_t const parts = std::max<int64_t>(1, std::min(turns, std::max<int64_t>(2048 / a.tiles, (turns + 7) / 8)));
+  // A workgroup takes four turns, unless the grid is small (1 / 4 / 8 / 32 turns: bf16 65,536 x 4096 268 / 228 / 234 / 248 us,
+  // 1000 x 262,144 254 / 232 / 236 / 237, fp32 30,000 x 4000 165 / 177 / 185 / 184).
+  int64_t const parts = std::max<int64_t>(1, std::min(turns, std::max<int64_t>(2048 / a.tiles, (turns + 3) / 4)));
   a.rows = (turns + parts - 1) / parts * turn;
   int64_t const groups = a.tiles * ((p.classes + a.rows - 1) / a.rows);
   if (!launchable(groups)) return hipErrorInvalidConfiguration;
