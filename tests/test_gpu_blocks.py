@@ -19,10 +19,10 @@ def torch_dtype(name):
 
 
 def tensor(a, dtype, device, pad=0, shift=0):
-    """a [rows, columns] on the GPU in a wider array, `shift` columns in."""
+    """a [rows, columns] on the GPU in a wider array of NaN, `shift` columns in."""
     import torch
 
-    t = torch.full((a.shape[0], a.shape[1] + pad + shift), 7.0, dtype=torch_dtype(dtype), device=device)
+    t = torch.full((a.shape[0], a.shape[1] + pad + shift), float("nan"), dtype=torch_dtype(dtype), device=device)
     v = t[:, shift:shift + a.shape[1]]
     v.copy_(torch.from_numpy(np.ascontiguousarray(a)).to(device))
     return v
@@ -187,6 +187,26 @@ def test_log_probabilities_of_column_ranges(cuda, dtype):
         assert got.backward(g, g, g, out=x) is x
         assert torch.equal(x, d)
         assert bool(torch.isinf(a[:, :left]).all()) and bool(torch.isinf(a[:, left + b:]).all())
+
+
+def test_logits_beyond_four_gigabytes(cuda):
+    """Columns of an array of 2.4e9 elements: offsets past 2^31 elements and 2^32 bytes."""
+    import torch
+
+    c, ld = 40_000, 60_000
+    wide = torch.zeros((c, ld), dtype=torch.bfloat16, device=cuda)
+    for b in (1, 100):
+        x = wide[:, ld - b:]
+        x.copy_(torch.randn((c, b), device=cuda))
+        near = x.contiguous()
+        targets = torch.arange(c - b, c, dtype=torch.int32, device=cuda)
+        got, want = P.log_probabilities(x, targets, 5), P.log_probabilities(near, targets, 5)
+        for name in ("log_probs", "entropy", "log_normalizer", "top_classes", "top_log_probs"):
+            assert torch.equal(getattr(got, name), getattr(want, name)), name
+        g = torch.randn(b, device=cuda)
+        d = want.backward(g, g)
+        assert torch.equal(got.backward(g, g, out=x), d)
+    assert not wide[:, :ld - 100].any()
 
 
 def test_gradient_of_log_probabilities_by_differences(cuda):
@@ -368,7 +388,7 @@ def test_norm_results_leave_their_neighbours(cuda):
                 setattr(g, name, v.data_ptr())
                 setattr(g, "ld_" + name, a.stride(0))
             need = L.ponni_residual_norm_workspace_bytes(n, r.dtype, b)
-            work = torch.empty(need + 64, dtype=torch.uint8, device=cuda)
+            work = torch.full((need + 64,), 255, dtype=torch.uint8, device=cuda)  # (NaN)
             work[need:] = 7
             assert L.ponni_residual_norm_backward(ctypes.byref(r), ctypes.byref(g), work.data_ptr(), need, stream) == 0
             for (a, v), v2 in zip(out, (wanted.x, wanted.residual, wanted.gate)):
@@ -518,7 +538,7 @@ def test_gated_results_leave_their_neighbours(cuda, dtype):
         sa, sv = wide(3 * h, b)
         L = A.lib()
         need = L.ponni_gated_backward_workspace_bytes(model._ref, b)
-        work = torch.empty(need, dtype=torch.uint8, device=cuda)
+        work = torch.full((need,), 255, dtype=torch.uint8, device=cuda)  # (NaN)
         stream = torch.cuda.current_stream().cuda_stream
         assert L.ponni_gated_forward(model._ref, x.data_ptr(), b, y.data_ptr(), a.stride(0), sv.data_ptr(), sa.stride(0), b,
                                      work.data_ptr(), L.ponni_gated_workspace_bytes(model._ref, b), stream) == 0
@@ -557,7 +577,7 @@ def test_gated_gradients_that_are_asked_for(cuda):
         assert rest.x is None and torch.equal(rest.up, want.up) and torch.equal(rest.gate_bias, want.gate_bias)
         L = A.lib()
         need = L.ponni_gated_backward_workspace_bytes(model._ref, b)
-        work = torch.empty(need, dtype=torch.uint8, device=cuda)
+        work = torch.full((need,), 255, dtype=torch.uint8, device=cuda)  # (NaN)
         for name, ld in (("gate", h), ("up", h), ("down", o), ("gate_bias", 0), ("up_bias", 0), ("down_bias", 0)):
             v = torch.empty_like(getattr(want, name))
             g = A.GatedGradientArrays()
@@ -613,7 +633,7 @@ def test_gated_work_buffer_of_more_columns(cuda):
         model = P.create_gated_model(*ws, P.Silu(h))
         L = A.lib()
         need = L.ponni_gated_workspace_bytes(model._ref, most)
-        work = torch.empty(need + 64, dtype=torch.uint8, device=cuda)
+        work = torch.full((need + 64,), 255, dtype=torch.uint8, device=cuda)  # (NaN)
         work[need:] = 7
         for b in (1, 8, 9, 32, 33, 200, 512, 513, 1000, most):
             x = torch.randn((i, b), device=cuda).to(t)
