@@ -40,7 +40,7 @@ struct ProductArgs {
   float slope;
   void* states;  // [2 rows, columns]: OUT_PAIR writes them (null: not), OUT_STATES reads them
   int64_t ld_states;
-  float* sums;   // OUT_PARTS: [parts, problems, rows, ld_sums]
+  float* sums;   // OUT_PARTS: [parts, problems, rows, ld_sums], of FORM_PAIR one product's behind the other's
   int64_t ld_sums;
   // the grid, filled in by the launch
   int m_tiles, n_tiles, split_n, steps;

@@ -515,6 +515,63 @@ template <class T> __global__ __launch_bounds__(256) void join_parts(ProductArgs
   o.store(static_cast<T*>(p.y[second]) + m * p.ld[second] + n, p.columns - n < 4 ? int(p.columns - n) : 4);
 }
 
+// Four columns of a row of the parts' sum; grid (rows, columns / 1024).
+__device__ inline f32x4 sum_of_parts(ProductArgs const& p, float const* sums, int64_t m, int64_t n) {
+  f32x4 s = {0, 0, 0, 0};
+  for (int k = 0; k < p.parts; k++) s += *reinterpret_cast<f32x4 const*>(sums + (int64_t(k) * p.rows + m) * p.ld_sums + n);
+  return s;
+}
+// OUT_PAIR's outputs from the parts of the first product, then of the second.
+template <class T> __global__ __launch_bounds__(256) void join_pair(ProductArgs p) {
+  int64_t const n = (int64_t(blockIdx.y) * 256 + threadIdx.x) * 4, m = blockIdx.x;
+  if (n >= p.columns) return;
+  int const count = p.columns - n < 4 ? int(p.columns - n) : 4;
+  f32x4 v = sum_of_parts(p, p.sums, m, n), u = sum_of_parts(p, p.sums + p.parts * p.rows * p.ld_sums, m, n);
+  if (p.bias[0] != nullptr) v += float(static_cast<T const*>(p.bias[0])[m]);
+  if (p.bias[1] != nullptr) u += float(static_cast<T const*>(p.bias[1])[m]);
+  Pack<T, 4> o;
+  auto store = [&](f32x4 const& w, void* to, int64_t ld, int64_t row) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) o.set(e, w[e]);
+    o.store(static_cast<T*>(to) + row * ld + n, count);
+  };
+  if (p.states != nullptr) {
+    store(v, p.states, p.ld_states, m);
+    store(u, p.states, p.ld_states, p.rows + m);
+  }
+  with_activation<sizeof(T) == 4>(p.act, p.slope, [&](auto f) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      float a, d;
+      f(v[e], a, d);
+      v[e] = a * u[e];
+    }
+  });
+  store(v, p.y[0], p.ld[0], m);
+}
+// OUT_STATES' outputs from the parts.
+template <class T> __global__ __launch_bounds__(256) void join_states(ProductArgs p) {
+  int64_t const n = (int64_t(blockIdx.y) * 256 + threadIdx.x) * 4, m = blockIdx.x;
+  if (n >= p.columns) return;
+  int const count = p.columns - n < 4 ? int(p.columns - n) : 4;
+  f32x4 v = sum_of_parts(p, p.sums, m, n);
+  T const* const s = static_cast<T const*>(p.states) + m * p.ld_states + n;
+  Pack<T, 4> gate, up, dg, du;
+  gate.load(s, count, 0.0f);
+  up.load(s + p.rows * p.ld_states, count, 0.0f);
+  with_activation<sizeof(T) == 4>(p.act, p.slope, [&](auto f) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      float a, d;
+      f(gate[e], a, d);
+      dg.set(e, up[e] * (v[e] * d));
+      du.set(e, v[e] * a);
+    }
+  });
+  dg.store(static_cast<T*>(p.y[0]) + m * p.ld[0] + n, count);
+  du.store(static_cast<T*>(p.y[1]) + m * p.ld[0] + n, count);
+}
+
 template <class T, bool A_INNER, bool B_INNER, Output OUT, bool TWO, int MI, int NJ, int WM, int WN>
 hipError_t launch_tiles(ProductArgs p, hipStream_t stream) {
   constexpr int BM = 16 * MI * WM / (OUT == OUT_PAIR ? 2 : 1), BN = 16 * NJ * WN, STEP = 64 / sizeof(T);
@@ -544,10 +601,33 @@ template <class T, bool A_INNER, bool B_INNER, bool TWO = false> hipError_t laun
   return hipGetLastError();
 }
 
+// The first products of few tiles, each cut along k (choose_pair); then the one of D dy.
+template <class T> hipError_t launch_pair_in_parts(bool large, ProductArgs const& p, hipStream_t stream) {
+  for (int q = 0; q < 2; q++) {
+    ProductArgs one = p;
+    one.a[0] = p.a[q];
+    one.sums = p.sums + q * p.parts * p.rows * p.ld_sums;
+    hipError_t const err = launch_sized<T, false, false, OUT_PARTS>(large, one, stream);
+    if (err != hipSuccess) return err;
+  }
+  hipLaunchKernelGGL(join_pair<T>, dim3(unsigned(p.rows), unsigned((p.columns + 1023) / 1024)), dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+template <class T> hipError_t launch_states_in_parts(bool large, ProductArgs const& p, hipStream_t stream) {
+  hipError_t const err = launch_sized<T, true, false, OUT_PARTS>(large, p, stream);
+  if (err != hipSuccess) return err;
+  hipLaunchKernelGGL(join_states<T>, dim3(unsigned(p.rows), unsigned((p.columns + 1023) / 1024)), dim3(256), 0, stream, p);
+  return hipGetLastError();
+}
+
 template <class T> hipError_t launch_product_as(Form form, bool large, ProductArgs const& p, hipStream_t stream) {
   switch (form) {
-    case FORM_PAIR: return launch_sized<T, false, false, OUT_PAIR>(large, p, stream);
-    case FORM_STATES: return launch_sized<T, true, false, OUT_STATES>(large, p, stream);
+    case FORM_PAIR:
+      if (p.parts > 1) return launch_pair_in_parts<T>(large, p, stream);
+      return launch_sized<T, false, false, OUT_PAIR>(large, p, stream);
+    case FORM_STATES:
+      if (p.parts > 1) return launch_states_in_parts<T>(large, p, stream);
+      return launch_sized<T, true, false, OUT_STATES>(large, p, stream);
     case FORM_FORWARD: return launch_plain<T, false, false>(large, p, stream);
     case FORM_INPUT: return launch_plain<T, true, false, true>(large, p, stream);
     default: return launch_plain<T, true, true>(large, p, stream);

@@ -71,27 +71,35 @@ int64_t own_stride(int64_t columns, int64_t es) { return round_to(columns, 128 /
 struct Choice {
   bool large;
   int parts;
+  double time;
 };
 constexpr int kMostParts = 16, kLeastSteps = 8;
 constexpr int64_t kMostSums = int64_t(256) * 256 * 256 * 4;  // bytes: of as many tiles as run at once
 
 Choice choose(int64_t es, int64_t rows, int64_t columns, int problems, int64_t steps, bool pair, bool may_split) {
-  Choice best{false, 1};
-  double least = 1e300;
+  Choice best{false, 1, 1e300};
   for (int large = 0; large <= (es == 2 ? 1 : 0); large++) {
-    int64_t const bm = (large ? 256 : 128) / (pair ? 2 : 1), bn = large ? 256 : 128, at_once = large ? 256 : 512;
+    int64_t const bm = (large ? 256 : 128) / (pair && es == 2 ? 2 : 1), bn = large ? 256 : 128, at_once = large ? 256 : 512;
     int64_t const tiles = (rows + bm - 1) / bm * ((columns + bn - 1) / bn) * problems;
     for (int parts = 1; parts <= kMostParts; parts++) {
       if (parts > 1 && (!may_split || steps / parts < kLeastSteps || tiles * parts > at_once)) break;
       int64_t const groups = tiles * parts, rounds = (groups + at_once - 1) / at_once;
-      double const alone = es == 4 ? 1.3 : large ? 1.0 : 0.4, two = es == 4 ? 2.3 : 0.62;
+      // (a tile of a pair in fp32 is both of them)
+      double const alone = es == 4 ? (pair ? 2.2 : 1.3) : large ? 1.0 : 0.4, two = es == 4 ? (pair ? 3.6 : 2.3) : 0.62;
       double const step = large || groups <= 256 ? alone : two;
-      double time = double(rounds) * (double((steps + parts - 1) / parts) * step + 5.0);
+      double time = double(rounds) * (double((steps + parts - 1) / parts) * step + (pair && es == 4 ? 18.0 : 5.0));
       if (parts > 1) time += 4.0 + double(parts + 1) * double(rows * columns * problems) * 4.0 / 3e6;
-      if (time < least) least = time, best = {large != 0, parts};
+      if (time < best.time) best = {large != 0, parts, time};
     }
   }
   return best;
+}
+// Both first products: one kernel for whole sums, or cut along k one after the other (with states, us whole / cut: fp32
+// 4096-1024-4096, 64 columns 498 / 74, 512 528 / 140, 1024-4096-1024, 64 154 / 68).
+Choice choose_pair(int64_t es, int64_t rows, int64_t columns, int64_t steps) {
+  Choice const whole = choose(es, rows, columns, 1, steps, true, false);
+  Choice const cut = choose(es, rows, columns, 1, steps, false, true);
+  return cut.parts > 1 && 2 * cut.time < whole.time ? cut : whole;
 }
 
 // The caller's work buffer, taken piece by piece (base null: counted only).
@@ -153,14 +161,16 @@ template <class T> struct Run {
   void product(Form form, ProductArgs p) {
     if (err != hipSuccess) return;
     constexpr int64_t ES = sizeof(T), STEP = 64 / ES;
-    bool const pair = form == FORM_PAIR, plain = !pair && form != FORM_STATES;
     if (p.problems == 0) p.problems = 1;
-    Choice const c = choose(ES, p.rows, p.columns, p.problems, (form == FORM_INPUT ? 2 : 1) * ((p.k + STEP - 1) / STEP), pair, plain);
+    int64_t const steps = (form == FORM_INPUT ? 2 : 1) * ((p.k + STEP - 1) / STEP);
+    Choice const c = form == FORM_PAIR ? choose_pair(ES, p.rows, p.columns, steps)
+                                       : choose(ES, p.rows, p.columns, p.problems, steps, false, true);
     p.parts = c.parts;
     Taker const before = work;  // (the sums are read before the next product begins)
     if (c.parts > 1) {
       p.ld_sums = round_to(p.columns, 4);
-      p.sums = reinterpret_cast<float*>(work.take(c.parts * p.problems * p.rows * p.ld_sums * 4));
+      p.sums = reinterpret_cast<float*>(
+          work.take(c.parts * (form == FORM_PAIR ? 2 : p.problems) * p.rows * p.ld_sums * 4));
     }
     err = (std::is_same_v<T, float>      ? launch_product_f32
            : std::is_same_v<T, _Float16> ? launch_product_f16
@@ -188,14 +198,14 @@ Slices slices_of(int64_t es, int64_t k, int64_t outputs, int problems, int64_t g
   int64_t const held = std::min<int64_t>(each, 1024 / es);
   return {int((k + held - 1) / held), int(held)};
 }
-// Columns that they take at most.  fp32: up to 512 while tiles of the first products would leave half of the CUs idle (as
-// tiles of 64 features and 128 columns count).  us so / in tiles: bf16 1024-4096-1024 1 column 16 / 30, 32 columns 25 / 27;
-// fp16 256-700-256, 32 columns 20 / 17; fp32 1024-4096-1024 32 columns 33 / 154, 128 82 / 158, 256 (128 tiles) 143 / 163, 384 195 / 170;
-// 333-1001-77, 512 columns 40 / 65; 64-4096-64, 256 32 / 45; 4096-1024-4096, 512 270 / 528.
+// Columns that they take at most; in fp32 the fewer the more weights there are.  us so / in tiles: bf16 1024-4096-1024 1
+// column 17 / 30, 32 columns 25 / 28; fp16 256-700-256, 8 columns 16 / 20, 32 26 / 24; fp32 1024-4096-1024 (12.6 M weights) 64 columns
+// 51 / 67, 128 81 / 75, 4096-1024-4096 (12.6 M) 64 50 / 74, 128 80 / 84, 256 141 / 99; 2048-2000-300 (8.8 M) 128 60 / 69, 256
+// 104 / 81; 333-1001-77 (0.7 M) 512 40 / 57; 64-4096-64 (0.8 M) 512 44 / 45.
 int64_t most_thin(ponni_gated const& b) {
-  constexpr int64_t kThin = 32, kMostThin = 512, kTiles = 128;
+  constexpr int64_t kThin = 32, kMostThin = 512, kProducts = 1'400'000'000;
   if (element(b) == 2) return kThin;
-  return std::clamp(kTiles / ((b.n_hidden + 63) / 64) * 128, kThin, kMostThin);
+  return std::clamp(kProducts / ((2 * int64_t(b.n_in) + b.n_out) * b.n_hidden), kThin, kMostThin);
 }
 struct ThinPlan {
   Slices hidden, last;
@@ -228,7 +238,7 @@ int64_t gated_workspace_bytes(ponni_gated const& b, int64_t columns, bool backwa
   t.take(aligned_bytes(i, columns, es));
   t.take(aligned_bytes(h, columns, es));  // h itself, or a copy of the states'
   if (!backward) {
-    t.take(sums_bytes(o, columns, 1, steps_of(h, es)));
+    t.take(std::max(sums_bytes(o, columns, 1, steps_of(h, es)), 2 * sums_bytes(h, columns, 1, steps_of(i, es))));
     // (the slices become fewer past 8 columns)
     return std::max({t.used, thin_plan(b, std::min<int64_t>(columns, 8)).bytes(),
                      thin_plan(b, std::min(columns, most_thin(b))).bytes()});
@@ -236,7 +246,7 @@ int64_t gated_workspace_bytes(ponni_gated const& b, int64_t columns, bool backwa
   t.take(aligned_bytes(o, columns, es));
   t.take(aligned_bytes(2 * h, columns, es));  // dg, du
   t.take(std::max({sums_bytes(i, columns, 1, 2 * steps_of(h, es)), sums_bytes(i, h, 2, steps_of(columns, es)),
-                   sums_bytes(h, o, 1, steps_of(columns, es))}));
+                   sums_bytes(h, o, 1, steps_of(columns, es)), sums_bytes(h, columns, 1, steps_of(o, es))}));
   return t.used;
 }
 

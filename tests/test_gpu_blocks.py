@@ -487,6 +487,13 @@ def test_gated_large_tiles(cuda, sizes, b, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes,b", [((4099, 70, 40), 130), ((40, 70, 4099), 61), ((3001, 45, 2003), 35)])
+def test_gated_long_sums_of_few_tiles(cuda, sizes, b, dtype):
+    """Every product cut along k, both first ones and that of D dy among them."""
+    check_gated(cuda, sizes, b, "silu", dtype, bias=True, pad=3, shift=1)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("sizes", [(64, 256, 64), (1000, 600, 700), (130, 70, 33), (7, 1031, 5)])
 def test_gated_few_columns(cuda, sizes, dtype):
     """Either side of the numbers of columns where kernels change; a column's result is that of the column alone, but
