@@ -742,10 +742,11 @@ typedef struct ponni_residual_norm_gradients {
   int64_t ld_d_x;
   void* d_residual;
   int64_t ld_d_residual;
-  void* d_gate;          /* of a gate [n, columns]                                    */
+  void* d_gate;          /* of a gate [n, columns]; refused without one               */
   int64_t ld_d_gate;
-  float* d_feature_gate; /* [n], and                                                  */
-  float *d_after_weight, *d_after_bias, *d_before_weight, *d_before_bias; /* [n]       */
+  float* d_feature_gate; /* [n]; refused beside a gate [n, columns]                   */
+  float *d_after_weight, *d_after_bias;   /* [n], also of a norm that has no such      */
+  float *d_before_weight, *d_before_bias; /* array; refused without the norm itself    */
 } ponni_residual_norm_gradients;
 /* Reads x, residual, gate and statistics of r again. */
 int ponni_residual_norm_backward(const ponni_residual_norm* r, const ponni_residual_norm_gradients* gradients,

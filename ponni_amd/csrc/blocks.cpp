@@ -187,6 +187,20 @@ int residual_norm_backward_impl(ponni_residual_norm const* r, ponni_residual_nor
     return fail(PONNI_ERR_INVALID_ARGUMENT, "d_normed without a norm before the next block");
   if ((g->d_gate != nullptr) && r->gate == nullptr)
     return fail(PONNI_ERR_INVALID_ARGUMENT, "d_gate without a gate of every feature and column");
+  if (g->d_feature_gate != nullptr && r->gate != nullptr)
+    return fail(PONNI_ERR_INVALID_ARGUMENT, "d_feature_gate beside a gate of every feature and column");
+  // (a norm without a weight or bias has their gradients all the same, at ones and zeros)
+  struct Parameter {
+    char const* what;
+    float const* gradient;
+    int32_t kind;
+  };
+  for (Parameter const& p : {Parameter{"d_after_weight", g->d_after_weight, r->after.kind},
+                             Parameter{"d_after_bias", g->d_after_bias, r->after.kind},
+                             Parameter{"d_before_weight", g->d_before_weight, r->before.kind},
+                             Parameter{"d_before_bias", g->d_before_bias, r->before.kind}})
+    if (p.gradient != nullptr && p.kind == PONNI_NORM_NONE)
+      return fail(PONNI_ERR_INVALID_ARGUMENT, std::string(p.what) + " without such a norm");
   int64_t const es = element_bytes(r->dtype), n = r->n, c = r->columns, need = residual_norm_workspace_bytes(r->n, c);
   if ((st = check_workspace(workspace, workspace_bytes, need)) != PONNI_OK) return st;
   st = check_arrays({{"x", r->x, n, c, r->ld_x, es},

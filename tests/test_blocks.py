@@ -143,6 +143,24 @@ def test_refused_norm_parameters_and_gradients():
     assert sizes == sorted(sizes) and sizes[0] > 0
 
 
+@pytest.mark.parametrize("what", ["d_after_weight", "d_after_bias", "d_before_weight", "d_before_bias", "d_feature_gate"])
+def test_refused_gradients_of_what_is_not_there(what):
+    """A norm that the call has not, or one value per feature of a gate of every element: no gradient, so no array."""
+    L = A.lib()
+
+    def backward(r):
+        g = A.ResidualNormGradientArrays(fake(20), 10, None, 0, fake(22), 10, fake(23), 10)
+        setattr(g, what, fake(25))
+        return L.ponni_residual_norm_backward(ctypes.byref(r), ctypes.byref(g), fake(30), 0, None)
+
+    # what the call has passes, up to the work buffer that is missing
+    there = {"gate": None, "feature_gate": fake(7)}
+    assert backward(residual_norm(**there)) == A.PONNI_ERR_SHAPE and "workspace" in error()
+    missing = {"gate": fake(6)} if what == "d_feature_gate" else \
+        {"after": A.NORM_NONE} if "after" in what else {"before": A.NORM_NONE, "normed": None}
+    assert backward(residual_norm(**missing)) == A.PONNI_ERR_INVALID_ARGUMENT and what in error()
+
+
 def log_probs(classes=20, columns=10, dtype=A.F32, top_k=2, **kw):
     p = A.LogProbsArrays(classes, columns, fake(1), columns, dtype, top_k, *(fake(k) for k in range(2, 8)))
     for k, v in kw.items():
