@@ -74,7 +74,9 @@ template <bool Precise, class Each> __device__ inline void with_activation(int a
         constexpr float c = 2.0f * 0.79788456080286535588f;
         float const p = sigmoid(c * v * fmaf(0.044715f * v, v, 1.0f));
         a = Precise ? gelu_tanh_f32(v) : v * p;
-        d = p * fmaf(c * v * fmaf(3.0f * 0.044715f * v, v, 1.0f), 1.0f - p, 1.0f);
+        // (from 16 on p is 0 or 1; a square that overflows must not meet that zero)
+        float const w = __builtin_amdgcn_fmed3f(v, -64.0f, 64.0f);
+        d = p * fmaf(c * w * fmaf(3.0f * 0.044715f * w, w, 1.0f), 1.0f - p, 1.0f);
       });
       break;
     default:

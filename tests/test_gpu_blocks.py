@@ -450,6 +450,30 @@ def test_gated_activations(cuda, act, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", N.ACTS)
+def test_slopes_of_large_values(cuda, act, dtype):
+    """Far from zero a slope is 0, 1 or LeakyRelu's: no infinity meets a zero on the way, up to the largest floats.  (The
+    block hands out dg and du as they are: one input and one column of ones, D dy of ones.)"""
+    import torch
+
+    v = np.array([1e4, 6e4] if dtype == "f16" else [1e4, 1e8, 1e12, 1e13, 3e13, 1e19, 1e26, 3e38])
+    g = N.half(np.tile(np.concatenate([v, -v]), 5), dtype)
+    h = g.size
+    with np.errstate(over="ignore"):
+        a, slope = N.activation(act, g)
+    for o in (1, 4099):  # the product D dy in one piece, and cut along k
+        down = torch.zeros((h, o), dtype=torch_dtype(dtype), device=cuda)
+        down[:, 0] = 1
+        ones = torch.ones((o, 1), dtype=torch_dtype(dtype), device=cuda)
+        model = P.create_gated_model(*(torch.ones((1, h), dtype=ones.dtype, device=cuda) for _ in range(2)), down, act_layer(act, h))
+        states = vector(np.concatenate([g, np.ones(h), g])[:, None], cuda, dtype)
+        d = model.backward(ones[:1], states, ones)
+        # one product, 0.1 in fp32 and a rounding
+        for got, want in ((d.gate, slope), (d.up, a)):
+            close(got[0], want, 2 * N.E * np.abs(want) + N.rounding(want, dtype), f"{act} {o}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_gated_strides(cuda, dtype):
     """Weights, inputs and gradients as column ranges of wider arrays, at odd and even places."""
     for pad, shift, wpad in ((8, 0, 8), (3, 1, 0), (16, 8, 3), (0, 0, 1), (64, 2, 2)):
