@@ -40,6 +40,7 @@ struct NormArgs {
   int lane_columns;  // log2 of the lanes across a tile's columns
   int chunks;        // of STEPS * (threads down) rows; 1 where a lane holds all of its rows
   int64_t tiles;
+  int64_t first;     // tile of a forward launch
   float* parts;      // [workgroups, NORM_SUMS, n]
 };
 
@@ -124,7 +125,7 @@ __global__ __launch_bounds__(kThreads, (HELD && STEPS > 4) || GATE ? 2 : 4) void
   int const across = 1 << a.lane_columns, tx = threadIdx.x & (across - 1), ty = threadIdx.x >> a.lane_columns;
   int const down = kThreads >> a.lane_columns, n = r.n;
   Reducer<NC> reduce{lds, across, tx, 0};
-  int64_t const c0 = (by_xcd(blockIdx.x, gridDim.x) * across + tx) * NC, left = r.columns - c0;
+  int64_t const c0 = ((a.first + by_xcd(blockIdx.x, gridDim.x)) * across + tx) * NC, left = r.columns - c0;
   int const count = left < 1 ? 0 : left < NC ? int(left) : NC;
   float const inv_n = 1.0f / float(n);
   Rows<T> const rows_x(r.x, r.ld_x, ty, down, c0), rows_r(r.residual, r.ld_residual, ty, down, c0),
@@ -543,17 +544,21 @@ template <class T> hipError_t launch_norm(ponni_residual_norm const& r, hipStrea
   a.lane_columns = s.lane_columns;
   a.chunks = s.chunks;
   a.tiles = s.tiles;
-  if (s.tiles > int64_t(UINT32_MAX) / kThreads) return hipErrorInvalidConfiguration;
-  dim3 const grid(static_cast<unsigned>(s.tiles));
-  with_variant(s, r.gate != nullptr, has_layer(r), [&](auto steps, auto held, auto gate, auto layer) {
-    constexpr int S = decltype(steps)::value, NC = 16 / sizeof(T);
-    constexpr bool H = decltype(held)::value, G = decltype(gate)::value, L = decltype(layer)::value;
-    if constexpr (!(G && S == 16)) {  // (most_steps)
-      if (s.columns == 1) hipLaunchKernelGGL((residual_norm<T, 1, S, H, G, true>), grid, dim3(kThreads), 0, stream, a);
-      else hipLaunchKernelGGL((residual_norm<T, NC, S, H, G, L>), grid, dim3(kThreads), 0, stream, a);
-    }
-  });
-  return hipGetLastError();
+  constexpr int64_t kMost = int64_t(UINT32_MAX) / kThreads;  // workgroups of a launch
+  for (; a.first < s.tiles; a.first += kMost) {
+    dim3 const grid(static_cast<unsigned>(std::min(s.tiles - a.first, kMost)));
+    with_variant(s, r.gate != nullptr, has_layer(r), [&](auto steps, auto held, auto gate, auto layer) {
+      constexpr int S = decltype(steps)::value, NC = 16 / sizeof(T);
+      constexpr bool H = decltype(held)::value, G = decltype(gate)::value, L = decltype(layer)::value;
+      if constexpr (!(G && S == 16)) {  // (most_steps)
+        if (s.columns == 1) hipLaunchKernelGGL((residual_norm<T, 1, S, H, G, true>), grid, dim3(kThreads), 0, stream, a);
+        else hipLaunchKernelGGL((residual_norm<T, NC, S, H, G, L>), grid, dim3(kThreads), 0, stream, a);
+      }
+    });
+    hipError_t const err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  return hipSuccess;
 }
 
 template <class T>

@@ -345,6 +345,28 @@ def test_norm_rows_beyond_four_gigabytes(cuda):
     assert torch.equal(state[:, cols], want[0]) and torch.equal(normed[:, cols], want[1])
 
 
+@pytest.mark.parametrize("dtype,b", [("f32", 268_500_003), ("bf16", 536_900_005)])
+def test_norms_of_more_columns_than_a_launch_has(cuda, dtype, b):
+    """Tiles of 32 columns (16 bits: 64) by 512 threads, 2^32 threads a launch: a column's results are those of the column
+    among few, on either side of the border and at the end."""
+    import torch
+
+    t, n = torch_dtype(dtype), 2
+    x, res = (torch.empty((n, b), dtype=t, device=cuda).normal_() for _ in range(2))
+    model = P.create_residual_norm(n, after=P.BlockNorm("layer"), before=P.BlockNorm("rms"), scale=0.5, dtype=dtype)
+    state, normed, statistics = model.forward_with_statistics(x, res)
+    d = model.backward(x, res, None, statistics, None, normed)
+    border = (2 ** 32 // 512 - 1) * (32 if dtype == "f32" else 64)
+    for c in (0, 2 ** 27, border - 512, b - 1021):
+        near = x[:, c:c + 1021].contiguous(), res[:, c:c + 1021].contiguous()
+        want = model.forward_with_statistics(*near)
+        for got, w in zip((state, normed, statistics), want):
+            assert torch.equal(got[:, c:c + 1021], w)
+        wanted = model.backward(*near, None, want[2], None, want[1])
+        assert torch.equal(d.x[:, c:c + 1021], wanted.x) and torch.equal(d.residual[:, c:c + 1021], wanted.residual)
+    assert not torch.equal(state[:, border - 512:border], state[:, border:border + 512])
+
+
 def test_norm_results_leave_their_neighbours(cuda):
     """Column ranges of wider arrays for every result."""
     import ctypes
