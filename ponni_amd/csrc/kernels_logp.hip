@@ -33,6 +33,7 @@ struct LogpArgs {
   int lane_columns;       // log2 of the threads across a tile's columns
   int splits;             // workgroups that share a tile's columns
   int64_t rows;           // of one of them
+  int64_t first_tile;     // of this launch
   float* parts;           // [splits, 3, columns]: m, z, q
   float* part_values;     // [splits, K, columns]
   int32_t* part_classes;  // [splits, K, columns]
@@ -188,7 +189,7 @@ template <class T, int NC, int K> __global__ __launch_bounds__(kThreads) void lo
   int const across = 1 << a.lane_columns, tx = threadIdx.x & (across - 1), ty = threadIdx.x >> a.lane_columns;
   int const down = kThreads >> a.lane_columns;
   int const split = blockIdx.x % a.splits;
-  int64_t const tile = blockIdx.x / a.splits;
+  int64_t const tile = a.first_tile + blockIdx.x / a.splits;
   int64_t const c0 = (tile * across + tx) * NC, left = a.p.columns - c0;
   int const count = left < 1 ? 0 : left < NC ? int(left) : NC;
   int64_t const first = split * a.rows, end = first + a.rows < a.p.classes ? first + a.rows : a.p.classes;
@@ -357,8 +358,9 @@ struct LogpBackwardArgs {
   void* d_logits;
   int64_t ld_d;
   int lane_columns;
-  int64_t rows;  // of a workgroup
-  int64_t tiles;
+  int64_t rows;        // of a workgroup
+  int64_t first_tile;  // of this launch
+  int64_t tiles;       // of this launch
 };
 
 // p (gz - gl) - gh p (log p + entropy), and gl at the target.
@@ -367,7 +369,7 @@ template <class T, int NC> __global__ __launch_bounds__(kThreads) void logp_back
   constexpr bool EXACT = sizeof(T) == 4;
   int const across = 1 << a.lane_columns, tx = threadIdx.x & (across - 1), ty = threadIdx.x >> a.lane_columns;
   int const down = kThreads >> a.lane_columns;
-  int64_t const tile = blockIdx.x % a.tiles, c0 = (tile * across + tx) * NC, left = a.p.columns - c0;
+  int64_t const tile = a.first_tile + blockIdx.x % a.tiles, c0 = (tile * across + tx) * NC, left = a.p.columns - c0;
   int const count = left < 1 ? 0 : left < NC ? int(left) : NC;
   if (count == 0) return;
   int64_t const first = blockIdx.x / a.tiles * a.rows, end = first + a.rows < a.p.classes ? first + a.rows : a.p.classes;
@@ -463,7 +465,19 @@ template <class F> void with_list(int k, F&& f) {
   }
 }
 
-bool launchable(int64_t workgroups) { return workgroups <= int64_t(UINT32_MAX) / kThreads; }
+constexpr int64_t kMostWorkgroups = int64_t(UINT32_MAX) / kThreads;  // of a launch
+bool launchable(int64_t workgroups) { return workgroups <= kMostWorkgroups; }
+// f(first tile, tiles) for launches of whole tiles, each of `groups` workgroups.
+template <class F> hipError_t in_launches(int64_t tiles, int64_t groups, F&& f) {
+  if (!launchable(groups)) return hipErrorInvalidConfiguration;
+  int64_t const most = kMostWorkgroups / groups;
+  for (int64_t first = 0; first < tiles; first += most) {
+    f(first, std::min(tiles - first, most));
+    hipError_t const err = hipGetLastError();
+    if (err != hipSuccess) return err;
+  }
+  return hipSuccess;
+}
 
 }  // namespace
 
@@ -494,18 +508,18 @@ hipError_t launch_logp(ponni_log_probs const& p, void* workspace, hipStream_t st
   a.parts = static_cast<float*>(workspace);
   a.part_values = a.parts + int64_t(s.splits) * 3 * p.columns;
   a.part_classes = reinterpret_cast<int32_t*>(a.part_values + int64_t(s.splits) * k * p.columns);
-  int64_t const groups = s.tiles * s.splits;
-  if (!launchable(groups)) return hipErrorInvalidConfiguration;
-  with_dtype(p.dtype, [&](auto e) {
-    using T = decltype(e);
-    with_list(k, [&](auto list) {
-      constexpr int K = decltype(list)::value, NC = K == 0 ? 16 / sizeof(T) : K <= 8 ? 4 : 2;
-      dim3 const grid(static_cast<unsigned>(groups));
-      if (s.columns == 1) hipLaunchKernelGGL((logp<T, 1, K>), grid, dim3(kThreads), 0, stream, a);
-      else hipLaunchKernelGGL((logp<T, NC, K>), grid, dim3(kThreads), 0, stream, a);
+  hipError_t const err = in_launches(s.tiles, s.splits, [&](int64_t first, int64_t tiles) {
+    a.first_tile = first;
+    with_dtype(p.dtype, [&](auto e) {
+      using T = decltype(e);
+      with_list(k, [&](auto list) {
+        constexpr int K = decltype(list)::value, NC = K == 0 ? 16 / sizeof(T) : K <= 8 ? 4 : 2;
+        dim3 const grid(static_cast<unsigned>(tiles * s.splits));
+        if (s.columns == 1) hipLaunchKernelGGL((logp<T, 1, K>), grid, dim3(kThreads), 0, stream, a);
+        else hipLaunchKernelGGL((logp<T, NC, K>), grid, dim3(kThreads), 0, stream, a);
+      });
     });
   });
-  hipError_t err = hipGetLastError();
   if (err != hipSuccess || s.splits == 1) return err;
   a.lane_columns = 0;
   while (a.lane_columns < 6 && (1 << a.lane_columns) < s.splits) a.lane_columns++;
@@ -528,21 +542,22 @@ hipError_t launch_logp_backward(ponni_log_probs const& p, float const* d_log_pro
   if (p.classes <= 64 && lanes > 64) a.lane_columns = 8;  // (every lane takes all rows of its columns)
   while (a.lane_columns < 3 && (1 << a.lane_columns) < lanes) a.lane_columns++;
   int64_t const across = int64_t(nc) << a.lane_columns, turn = (kThreads >> a.lane_columns) * (nc >= 4 ? 4 : 8);
-  a.tiles = (p.columns + across - 1) / across;
+  int64_t const all_tiles = (p.columns + across - 1) / across;
   int64_t const turns = (p.classes + turn - 1) / turn;
   // A workgroup takes four turns, unless the grid is small (1 / 4 / 8 / 32 turns: bf16 65,536 x 4096 268 / 228 / 234 / 248 us,
   // 1000 x 262,144 254 / 232 / 236 / 237, fp32 30,000 x 4000 165 / 177 / 185 / 184).
-  int64_t const parts = std::max<int64_t>(1, std::min(turns, std::max<int64_t>(2048 / a.tiles, (turns + 3) / 4)));
+  int64_t const parts = std::max<int64_t>(1, std::min(turns, std::max<int64_t>(2048 / all_tiles, (turns + 3) / 4)));
   a.rows = (turns + parts - 1) / parts * turn;
-  int64_t const groups = a.tiles * ((p.classes + a.rows - 1) / a.rows);
-  if (!launchable(groups)) return hipErrorInvalidConfiguration;
-  with_dtype(p.dtype, [&](auto e) {
-    using T = decltype(e);
-    dim3 const grid(static_cast<unsigned>(groups));
-    if (nc == 1) hipLaunchKernelGGL((logp_backward<T, 1>), grid, dim3(kThreads), 0, stream, a);
-    else hipLaunchKernelGGL((logp_backward<T, 16 / sizeof(T)>), grid, dim3(kThreads), 0, stream, a);
+  int64_t const groups = (p.classes + a.rows - 1) / a.rows;
+  return in_launches(all_tiles, groups, [&](int64_t first, int64_t tiles) {
+    a.first_tile = first, a.tiles = tiles;
+    with_dtype(p.dtype, [&](auto e) {
+      using T = decltype(e);
+      dim3 const grid(static_cast<unsigned>(tiles * groups));
+      if (nc == 1) hipLaunchKernelGGL((logp_backward<T, 1>), grid, dim3(kThreads), 0, stream, a);
+      else hipLaunchKernelGGL((logp_backward<T, 16 / sizeof(T)>), grid, dim3(kThreads), 0, stream, a);
+    });
   });
-  return hipGetLastError();
 }
 
 }  // namespace ponni_hip

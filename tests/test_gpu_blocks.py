@@ -209,6 +209,34 @@ def test_logits_beyond_four_gigabytes(cuda):
     assert not wide[:, :ld - 100].any()
 
 
+def test_log_probabilities_of_more_columns_than_a_launch_has(cuda):
+    """Tiles of 32 fp32 columns by 256 threads, 2^32 threads a launch (65 classes: fewer take other tiles); the gradient into
+    the logits' place."""
+    import torch
+
+    c, b = 65, 536_900_005
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info(cuda)[0] < 170e9:
+        pytest.skip("150 GB of logits and results")
+    x = torch.empty((c, b), device=cuda).normal_()
+    targets = torch.randint(-1, c, (b,), dtype=torch.int32, device=cuda)
+    g = torch.empty(b, device=cuda).normal_()
+    border = (2 ** 32 // 256 - 1) * 32
+    pieces = [slice(k, k + 1021) for k in (0, 2 ** 28, border - 512, b - 1021)]
+    near = [(x[:, k].contiguous(), targets[k].contiguous(), g[k].contiguous()) for k in pieces]
+    got = P.log_probabilities(x, targets)
+    d = got.backward(g, out=x)
+    for k, (x2, t2, g2) in zip(pieces, near):
+        want = P.log_probabilities(x2, t2)
+        for name in ("log_probs", "entropy", "log_normalizer"):
+            # (sums in another order: a batch of few columns has tiles of its own)
+            close(getattr(got, name)[k], *N.log_probs(host(x2), host(t2).astype(int), 0)[name], name)
+            close(getattr(want, name), *N.log_probs(host(x2), host(t2).astype(int), 0)[name], name)
+        close(d[:, k], *N.log_probs_backward(N.log_probs(host(x2), host(t2).astype(int), 0), host(g2), None, None, "f32"), "d_logits")
+    del got, d, x
+    torch.cuda.empty_cache()
+
+
 def test_gradient_of_log_probabilities_by_differences(cuda):
     import torch
 
