@@ -317,6 +317,85 @@ def test_norms(cuda, n, b, after, before, gate, residual, dtype):
     check_norm(cuda, n, b, after, before, gate, residual, dtype, pad=b % 3, shift=b % 2)
 
 
+@pytest.mark.parametrize("n,b,after,before,gate,residual,dtype", [
+    # 16 bits: tiles of 64 columns, 516 of them; at most 8 rows of 64 threads' (4 beside a full gate or two layer norms) held
+    (500, 33_003, "rms", "rms", None, True, "bf16"), (300, 33_003, "layer", "layer", None, True, "f16"),
+    (250, 33_003, "layer", "rms", "full", True, "bf16"), (530, 33_003, None, "rms", "feature", True, "f16"),
+    (270, 33_003, "rms", "layer", "full", False, "f16"),
+    # fp32: tiles of 32 columns, 532 and more; held up to 512 rows at 128 bytes, read again from 1025 (2049 with a norm after)
+    (500, 17_003, "rms", "layer", "full", True, "f32"), (1030, 17_003, None, "layer", "feature", True, "f32"),
+    (2060, 16_390, "rms", "rms", None, True, "f32")])
+def test_norms_of_more_tiles_than_workgroups(cuda, n, b, after, before, gate, residual, dtype):
+    """The gradients' 512 workgroups add weights' gradients over several tiles, in registers and where columns are read
+    again, 128 bytes of a row across, with a last tile that is not whole.  (In pieces of columns: a term of a sum passes
+    fewer additions here, 16 in a lane, 6 across lanes and 48 behind the workgroups, than the pieces' bounds count.)"""
+    import torch
+
+    print(f"norms: n={n} b={b} {after} {before} {gate} {residual} {dtype}", flush=True)
+    assert b > 512 * (32 if dtype == "f32" else 64)
+    torch.manual_seed(n)
+    t = torch_dtype(dtype)
+
+    def normal(*shape, scale=1.0, shift=0.0):
+        return (torch.randn(shape, device=cuda) * scale + shift)
+
+    x, ds, dn = (normal(n, b).to(t) for _ in range(3))
+    res = normal(n, b, scale=2.0, shift=0.5).to(t) if residual else None
+    g = {"full": normal(n, b).to(t), "feature": normal(n), None: None}[gate]
+    w = [None if k is None else (k, normal(n, scale=0.3, shift=1.0), normal(n, scale=0.2)) for k in (after, before)]
+    model = P.create_residual_norm(n, *(None if k is None else P.BlockNorm(*k) for k in w), scale=0.7, dtype=dtype)
+    state, normed, statistics = model.forward_with_statistics(x, res, g)
+    d = model.backward(x, res, g, statistics, ds, dn)
+    norms = [None if k is None else (k[0], host(k[1]), host(k[2])) for k in w]
+    f, eps = float(np.float32(0.7)), float(np.float32(1e-5))
+    sums, step = {}, 509
+    for c in range(0, b, step):
+        at = slice(c, c + step)
+        px, pr, pds, pdn = (None if v is None else host(v[:, at]) for v in (x, res, ds, dn))
+        pg = host(g[:, at]) if gate == "full" else host(g)
+        want, s = N.norm_forward(px, pr, pg, *norms, f, eps, dtype)
+        close(state[:, at], *want["state"], "state")
+        close(normed[:, at], *want["normed"], "normed")
+        wanted = N.norm_backward(s, *norms, pds, pdn, f, pg, dtype)
+        for name, (v, e) in wanted.items():
+            got = getattr(d, name)
+            if got is not None and got.dim() == 2:
+                close(got[:, at], v, e, f"d_{name}")
+            elif got is not None:
+                total = sums.setdefault(name, [0.0, 0.0])
+                total[0], total[1] = total[0] + v, total[1] + e
+    assert len(sums) == 2 * sum(k is not None for k in w) + (gate == "feature")
+    for name, (v, e) in sums.items():
+        close(getattr(d, name), v, e, f"d_{name}")
+
+
+def test_gradients_of_weights_that_are_ones(cuda):
+    """A norm without a weight or bias has their gradients all the same, at ones and zeros; and a gate of ones."""
+    import ctypes
+
+    import torch
+
+    n, b = 77, 300
+    x, ds, dn = (torch.randn((n, b), device=cuda) for _ in range(3))
+    ones, zeros = torch.ones(n, device=cuda), torch.zeros(n, device=cuda)
+    given = P.create_residual_norm(n, P.BlockNorm("layer", ones, zeros), P.BlockNorm("rms", ones, zeros))
+    bare = P.create_residual_norm(n, P.BlockNorm("layer"), P.BlockNorm("rms"))
+    _, _, statistics = given.forward_with_statistics(x, x, ones)
+    want = given.backward(x, x, ones, statistics, ds, dn)
+    r = bare._arrays(x, x, None)
+    r.statistics = statistics.data_ptr()
+    out = {k: torch.empty(n, device=cuda) for k in ("feature_gate", "after_weight", "after_bias", "before_weight", "before_bias")}
+    g = A.ResidualNormGradientArrays(ds.data_ptr(), b, dn.data_ptr(), b)
+    for k, v in out.items():
+        setattr(g, "d_" + k, v.data_ptr())
+    need = A.lib().ponni_residual_norm_workspace_bytes(n, r.dtype, b)
+    work = torch.full((need,), 255, dtype=torch.uint8, device=cuda)  # (NaN)
+    assert A.lib().ponni_residual_norm_backward(ctypes.byref(r), ctypes.byref(g), work.data_ptr(), need,
+                                                torch.cuda.current_stream().cuda_stream) == 0
+    for k, v in out.items():
+        assert torch.equal(v, getattr(want, "gate" if k == "feature_gate" else k)), k
+
+
 def test_norms_without_weights(cuda):
     check_norm(cuda, 120, 50, "rms", "layer", None, True, "f16", weight=False, bias=False)
     check_norm(cuda, 120, 50, "layer", "rms", "full", False, "f32", weight=True, bias=False, scale=-1.0)
@@ -558,6 +637,14 @@ def test_gated_large_tiles(cuda, sizes, b, dtype):
     """Products large enough for the wider tiles, whole and cut along k, with ragged edges on every side."""
     print(f"gated: {sizes} b={b} {dtype}", flush=True)
     check_gated(cuda, sizes, b, "silu", dtype, bias=b % 2 == 1, pad=b % 5, shift=b % 2)
+
+
+@pytest.mark.parametrize("sizes,b", [((300, 400, 260), 17_003), ((20, 19, 18), 40_003), ((48, 38, 131), 30_011), ((700, 33, 57), 9_001),
+                                     ((64, 64, 64), 33_333)])
+def test_gated_fp32_of_many_tiles(cuda, sizes, b):
+    """More tiles than run at once, and narrow blocks over many columns."""
+    print(f"gated: {sizes} b={b}", flush=True)
+    check_gated(cuda, sizes, b, "silu", "f32", bias=b % 2 == 1, pad=b % 5, shift=b % 2)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
