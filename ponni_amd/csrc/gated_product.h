@@ -508,6 +508,7 @@ template <class T> __global__ __launch_bounds__(256) void join_parts(ProductArgs
   int const second = blockIdx.z;
   if (n >= p.columns) return;
   f32x4 s = {0, 0, 0, 0};
+#pragma unroll 8
   for (int k = 0; k < p.parts; k++)
     s += *reinterpret_cast<f32x4 const*>(p.sums + ((int64_t(k) * p.problems + second) * p.rows + m) * p.ld_sums + n);
   if (p.bias[0] != nullptr) s += float(static_cast<T const*>(p.bias[0])[m]);
@@ -520,6 +521,7 @@ template <class T> __global__ __launch_bounds__(256) void join_parts(ProductArgs
 // Four columns of a row of the parts' sum; grid (rows, columns / 1024).
 __device__ inline f32x4 sum_of_parts(ProductArgs const& p, float const* sums, int64_t m, int64_t n) {
   f32x4 s = {0, 0, 0, 0};
+#pragma unroll 8
   for (int k = 0; k < p.parts; k++) s += *reinterpret_cast<f32x4 const*>(sums + (int64_t(k) * p.rows + m) * p.ld_sums + n);
   return s;
 }

@@ -67,13 +67,15 @@ int64_t own_stride(int64_t columns, int64_t es) { return round_to(columns, 128 /
 //   200 columns         53 + 149          32 + 71      105 + 260         54 + 116     34 + 71
 //   1000 columns        62 + 174          59 + 116     108 + 295         68 + 161     51 + 119
 //   16,000 columns      476 + 1114        462 + 1118   376 + 1183        377 + 835    384 + 839
-// and fp32 (128 x 128) 333-1001-77, 5000 columns: whole 159 + 846, chosen 120 + 234.
+// and fp32 (128 x 128) 333-1001-77, 5000 columns: whole 159 + 846, chosen 120 + 234.  Gradients of narrow weights over many
+// columns are one or two tiles with a long sum: fp32 48-38-131, 274,418 columns, dG and dU in 16 parts 1138 + 6, in 218
+// 170 + 14.
 struct Choice {
   bool large;
   int parts;
   double time;
 };
-constexpr int kMostParts = 16, kLeastSteps = 8;
+constexpr int kMostParts = 256, kLeastSteps = 8;
 constexpr int64_t kMostSums = int64_t(256) * 256 * 256 * 4;  // bytes: of as many tiles as run at once
 
 Choice choose(int64_t es, int64_t rows, int64_t columns, int problems, int64_t steps, bool pair, bool may_split) {
@@ -81,14 +83,14 @@ Choice choose(int64_t es, int64_t rows, int64_t columns, int problems, int64_t s
   for (int large = 0; large <= (es == 2 ? 1 : 0); large++) {
     int64_t const bm = (large ? 256 : 128) / (pair && es == 2 ? 2 : 1), bn = large ? 256 : 128, at_once = large ? 256 : 512;
     int64_t const tiles = (rows + bm - 1) / bm * ((columns + bn - 1) / bn) * problems;
-    for (int parts = 1; parts <= kMostParts; parts++) {
+    for (int parts = 1; parts <= kMostParts; parts += parts < 16 ? 1 : parts / 4) {
       if (parts > 1 && (!may_split || steps / parts < kLeastSteps || tiles * parts > at_once)) break;
       int64_t const groups = tiles * parts, rounds = (groups + at_once - 1) / at_once;
       // (a tile of a pair in fp32 is both of them)
       double const alone = es == 4 ? (pair ? 2.2 : 1.3) : large ? 1.0 : 0.4, two = es == 4 ? (pair ? 3.6 : 2.3) : 0.62;
       double const step = large || groups <= 256 ? alone : two;
       double time = double(rounds) * (double((steps + parts - 1) / parts) * step + (pair && es == 4 ? 18.0 : 5.0));
-      if (parts > 1) time += 4.0 + double(parts + 1) * double(rows * columns * problems) * 4.0 / 3e6;
+      if (parts > 1) time += 4.0 + 0.05 * double(parts) + double(parts + 1) * double(rows * columns * problems) * 4.0 / 3e6;
       if (time < best.time) best = {large != 0, parts, time};
     }
   }

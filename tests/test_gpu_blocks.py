@@ -648,6 +648,42 @@ def test_gated_fp32_of_many_tiles(cuda, sizes, b):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sizes,b", [((20, 19, 18), 60_001), ((130, 40, 70), 30_002)])
+def test_gated_narrow_weights_over_many_columns(cuda, sizes, b, dtype):
+    """Weights' gradients in as many parts as there are workgroups to share them."""
+    print(f"gated: {sizes} b={b} {dtype}", flush=True)
+    check_gated(cuda, sizes, b, "tanh", dtype, bias=True, pad=b % 3, shift=b % 2)
+
+
+def test_gated_gradients_keep_to_their_work_buffer(cuda):
+    """What is needed for the columns of a call, and no byte behind it."""
+    import ctypes
+
+    import torch
+
+    i, h, o = 20, 19, 33
+    for dtype in DTYPES:
+        t = torch_dtype(dtype)
+        ws = [(torch.randn(s, device=cuda) / 4).to(t) for s in ((i, h), (i, h), (h, o))]
+        model = P.create_gated_model(*ws, P.Silu(h))
+        L = A.lib()
+        for b in (1, 7, 300, 4001, 20_000, 70_003):
+            x, dy = torch.randn((i, b), device=cuda).to(t), torch.randn((o, b), device=cuda).to(t)
+            _, states = model.forward_with_states(x)
+            want = model.backward(x, states, dy)
+            need = L.ponni_gated_backward_workspace_bytes(model._ref, b)
+            work = torch.full((need + 4096,), 255, dtype=torch.uint8, device=cuda)  # (NaN)
+            work[need:] = 7
+            out = [torch.empty_like(v) for v in (want.x, want.gate, want.up, want.down)]
+            g = A.GatedGradientArrays(out[0].data_ptr(), b, *(v.data_ptr() for v in out[1:]), h, h, o)
+            assert L.ponni_gated_backward(model._ref, x.data_ptr(), b, states.data_ptr(), states.stride(0), dy.data_ptr(), b, b,
+                                          ctypes.byref(g), work.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == 0
+            assert bool((work[need:] == 7).all())
+            for v, w in zip(out, (want.x, want.gate, want.up, want.down)):
+                assert torch.equal(v, w)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("sizes,b", [((4099, 70, 40), 130), ((40, 70, 4099), 61), ((3001, 45, 2003), 35)])
 def test_gated_long_sums_of_few_tiles(cuda, sizes, b, dtype):
     """Every product cut along k, both first ones and that of D dy among them."""
