@@ -15,10 +15,11 @@ struct Side {
 };
 
 enum Output {
-  OUT_PLAIN,   // y = C (+ bias)
-  OUT_PAIR,    // rows of two products: y = act(C) * C2, and both of them as states
-  OUT_STATES,  // from C and the states: y[0] = C u act'(g), y[1] = C act(g)
-  OUT_PARTS    // fp32 sums of a part of k
+  OUT_PLAIN,      // y = C (+ bias)
+  OUT_PAIR,       // rows of two products: y = act(C) * C2, and both of them as states
+  OUT_STATES,     // from C and the states: y[0] = C u act'(g), y[1] = C act(g)
+  OUT_PARTS,      // fp32 sums of a part of k
+  OUT_PAIR_PARTS  // the same of OUT_PAIR's two products
 };
 enum Form {
   FORM_PAIR,     // k outside in both; a: two arrays
@@ -33,6 +34,7 @@ struct ProductArgs {
   int64_t k, rows, columns;  // C [rows, columns]
   int problems;              // 2: a[0] b[0] and a[0] b[1], into y[0] and y[1]
   int parts;                 // workgroups that share a tile's k
+  bool pair_parts;           // a pair's parts of both products at a time (TILE_NARROW), else one product behind the other
   void* y[2];
   int64_t ld[2];
   void const* bias[2];
@@ -46,10 +48,15 @@ struct ProductArgs {
   int m_tiles, n_tiles, split_n, steps;
 };
 
-// large: tiles of 256 x 256 (16 bits), else of 128 x 128.
-hipError_t launch_product_f32(Form form, bool large, ProductArgs const& p, hipStream_t stream);
-hipError_t launch_product_f16(Form form, bool large, ProductArgs const& p, hipStream_t stream);
-hipError_t launch_product_bf16(Form form, bool large, ProductArgs const& p, hipStream_t stream);
+// Rows and columns of a workgroup's tile; of a pair in 16 bits, half the rows of each of two products.
+enum Tile {
+  TILE_128,    // 128 x 128
+  TILE_LARGE,  // 256 x 256, 16 bits
+  TILE_NARROW  // 64 x 256, fp32; of a pair, 32 rows of each product
+};
+hipError_t launch_product_f32(Form form, Tile tile, ProductArgs const& p, hipStream_t stream);
+hipError_t launch_product_f16(Form form, Tile tile, ProductArgs const& p, hipStream_t stream);
+hipError_t launch_product_bf16(Form form, Tile tile, ProductArgs const& p, hipStream_t stream);
 
 // A product of few columns (gated_thin.h): parts [slices, problems, columns, stride] of fp32.
 enum ThinInput { THIN_COLUMNS, THIN_PARTS, THIN_ROWS };

@@ -142,8 +142,10 @@ template <class T, bool INNER, int SIZE, int PANELS, int W> struct Loader {
   static constexpr int ROW = PANEL * ES;             // bytes of a k's row of a panel
   static constexpr int PLACES = ROW / 16;            // pieces of it
   static constexpr int PER_PANEL = PANEL * 64 / 1024;  // requests
-  static constexpr int BASES = INNER ? REQUESTS : PANELS;
-  static_assert(BYTES % (1024 * W) == 0 && 64 % PLACES == 0 && (PANELS == 1 || PER_PANEL % W == 0), "whole requests, of one panel each");
+  static constexpr bool APART = PANELS > 1 && PER_PANEL < W;  // a wave's one request is of its panel
+  static constexpr int BASES = INNER ? REQUESTS : APART ? 1 : PANELS;
+  static_assert(BYTES % (1024 * W) == 0 && 64 % PLACES == 0 && (PANELS == 1 || PER_PANEL % W == 0 || (APART && !INNER && REQUESTS == 1)),
+                "whole requests, of one panel each");
   unsigned offset[REQUESTS];  // of the lane's piece from the request's base
   int k[REQUESTS];            // INNER: the first k of the piece, within a step
   // Of the step that is asked for next, uniform: where each base lies, the bytes from there to the array's end, k's left.
@@ -181,7 +183,7 @@ template <class T, bool INNER, int SIZE, int PANELS, int W> struct Loader {
   __device__ void seek(int wave, Side const* s, int64_t first, int64_t k0, int64_t last) {
 #pragma unroll
     for (int b = 0; b < BASES; b++) {
-      Side const& from = s[INNER ? 0 : b];
+      Side const& from = s[INNER ? 0 : APART ? wave / PER_PANEL : b];
       uint64_t const o = INNER ? base_row(wave + W * b, from, first) * from.ld + k0 * ES : k0 * from.ld + first * ES;
       at[b] = uniform64(uint64_t(from.p) + o);
       left[b] = uniform64(from.bytes - o);
@@ -201,7 +203,7 @@ template <class T, bool INNER, int SIZE, int PANELS, int W> struct Loader {
     k_left = __builtin_amdgcn_readfirstlane(now ? int(last) : k_left);
   }
   __device__ void request(int r, int wave, unsigned lds) const {
-    int const base = INNER ? r : W * r / PER_PANEL;
+    int const base = INNER ? r : APART ? 0 : W * r / PER_PANEL;
     unsigned const o = INNER && k[r] >= k_left ? 0xfffffff0u : offset[r];
     dma16_in_range(resource_of(at[base], left[base]), o, lds + (wave + W * r) * 1024);
   }
@@ -210,6 +212,7 @@ template <class T, bool INNER, int SIZE, int PANELS, int W> struct Loader {
   static __device__ unsigned read_base(int first, int lane) {
     int const g = lane >> 4, c = lane & 15;
     if constexpr (INNER) return (first + c) * 64 + 16 * (g ^ twist(c));
+    else if constexpr (ES == 4 && APART) return c / 8 * (PANEL * 64) + 4 * g * ROW + 16 * (c % 8);  // (panels of 32 rows: a block of 64)
     else if constexpr (ES == 4) return 4 * g * ROW + first * 4 + 16 * c;
     else {
       int const row = 8 * g + c / 4;
@@ -276,18 +279,24 @@ template <class T> __device__ inline void load16(T const* x, int64_t left, float
   }
 }
 
+template <Output OUT> constexpr bool kPair = OUT == OUT_PAIR || OUT == OUT_PAIR_PARTS;
+
 // TWO: a sum of two products, of operands of the same shapes and strides.
 template <class T, bool A_INNER, bool B_INNER, Output OUT, bool TWO, int MI, int NJ, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, 2) void product(ProductArgs p) {
   constexpr int W = WM * WN, BM = 16 * MI * WM, BN = 16 * NJ * WN, ES = sizeof(T), STEP = 64 / ES;
-  constexpr bool PAIR = OUT == OUT_PAIR;
+  constexpr bool PAIR = kPair<OUT>;
+  // fp32, 32 features: a block of 64 rows is both products', lanes c < 8 hold the first one's features 4 c + i, others the
+  // second one's.
+  constexpr bool NARROW = PAIR && ES == 4 && MI == 4;
   using LA = Loader<T, A_INNER, BM, PAIR ? 2 : 1, W>;
   using LB = Loader<T, B_INNER, BN, 1, W>;
   // fp32, k outside: a quarter of k is done with behind its products, so that the next step's takes its registers and two
   // waves of both products fit a SIMD: 1024-4096-1024 x 16,384 2025 us for 2279, 333-1001 x 5,003 101 for 118.
   constexpr bool SINGLE = ES == 4 && !A_INNER && !B_INNER;
   constexpr int kSlots = SINGLE ? 3 : 4, SLOT = LA::BYTES + LB::BYTES, REQ = LA::REQUESTS + LB::REQUESTS;
-  static_assert(NJ % 4 == 0 && (ES == 2 || NJ == 4) && MI % (PAIR && ES == 4 ? 8 : 4) == 0 && !(PAIR && A_INNER), "blocks of 64");
+  static_assert(NJ % 4 == 0 && (ES == 2 || NJ == 4) && MI % (PAIR && ES == 4 && !NARROW ? 8 : 4) == 0 &&
+                    !(PAIR && A_INNER) && (!NARROW || WM == 1), "blocks of 64");
   __shared__ __attribute__((aligned(1024))) char lds[kSlots * SLOT];
   int const lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
   int const wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -345,8 +354,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void product(ProductArgs p) {
     constexpr int set = SINGLE ? 0 : decltype(at_set)::value;
     char const* slot = lds + unsigned(step - first_step) % kSlots * SLOT;
     if (r < MI) {
-      int const panel = r / HALF;
-      read_fragment<T, A_INNER, LA::ROW, MI>(slot + panel * LA::PANEL * 64, read_a, r % HALF, av[set], r);
+      int const panel = NARROW ? 0 : r / HALF;
+      read_fragment<T, A_INNER, LA::ROW, MI>(slot + panel * LA::PANEL * 64, read_a, NARROW ? r : r % HALF, av[set], r);
     } else {
       read_fragment<T, B_INNER, LB::ROW, NJ>(slot + LA::BYTES, read_b, r - MI, bv[set], r - MI);
     }
@@ -426,6 +435,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void product(ProductArgs p) {
 
   // Rows: of fragments of k outside in fp32 the four of a block of 64 are dealt one by one.
   auto row_of = [&](int i) {
+    if constexpr (NARROW) return m0 + 4 * (c % 8) + c / 8 * HALF + i;
     int const base = wm * 16 * HALF;
     return m0 + base + (ES == 4 && !A_INNER ? i / 4 * 64 + 4 * c + i % 4 : 16 * i + c);
   };
@@ -450,7 +460,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void product(ProductArgs p) {
       float v[16], u[16];
       columns(i, v);
       if constexpr (PAIR) columns(i + HALF, u);
+      if constexpr (NARROW) {
+        // Lanes c < 8 have features 4 c + i and 4 c + i + 2 of the first product, lanes c + 8 of the second: each takes both
+        // of one feature.
+        bool const first = c < 8;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+          float const other = __shfl_xor(first ? u[e] : v[e], 8);
+          u[e] = first ? other : u[e];
+          v[e] = first ? v[e] : other;
+        }
+      }
       if (m >= p.rows || left <= 0) continue;
+      if constexpr (OUT == OUT_PAIR_PARTS) {
+        float* at = p.sums + (int64_t(part) * p.rows + m) * p.ld_sums + n;
+        store16<float>(at, left, v);
+        store16<float>(at + int64_t(p.parts) * p.rows * p.ld_sums, left, u);
+        continue;
+      }
       if constexpr (OUT == OUT_PARTS) {
         float* at = p.sums + ((int64_t(part) * p.problems + second) * p.rows + m) * p.ld_sums + n;
         store16<float>(at, left, v);
@@ -578,7 +605,7 @@ template <class T> __global__ __launch_bounds__(256) void join_states(ProductArg
 
 template <class T, bool A_INNER, bool B_INNER, Output OUT, bool TWO, int MI, int NJ, int WM, int WN>
 hipError_t launch_tiles(ProductArgs p, hipStream_t stream) {
-  constexpr int BM = 16 * MI * WM / (OUT == OUT_PAIR ? 2 : 1), BN = 16 * NJ * WN, STEP = 64 / sizeof(T);
+  constexpr int BM = 16 * MI * WM / (kPair<OUT> ? 2 : 1), BN = 16 * NJ * WN, STEP = 64 / sizeof(T);
   int64_t const m_tiles = (p.rows + BM - 1) / BM, n_tiles = (p.columns + BN - 1) / BN * p.problems;
   p.m_tiles = int(m_tiles), p.n_tiles = int(n_tiles);
   p.split_n = p.problems == 2 ? p.n_tiles / 2 : 0;
@@ -589,52 +616,58 @@ hipError_t launch_tiles(ProductArgs p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <class T, bool A_INNER, bool B_INNER, Output OUT, bool TWO = false> hipError_t launch_sized(bool large, ProductArgs const& p, hipStream_t stream) {
+template <class T, bool A_INNER, bool B_INNER, Output OUT, bool TWO = false> hipError_t launch_sized(Tile tile, ProductArgs const& p, hipStream_t stream) {
+  if constexpr (sizeof(T) == 4)
+    if (tile == TILE_NARROW) return launch_tiles<T, A_INNER, B_INNER, OUT, TWO, 4, 4, 1, 4>(p, stream);
   if constexpr (sizeof(T) == 2)
-    if (large) return launch_tiles<T, A_INNER, B_INNER, OUT, TWO, 8, 4, 2, 4>(p, stream);
+    if (tile == TILE_LARGE) return launch_tiles<T, A_INNER, B_INNER, OUT, TWO, 8, 4, 2, 4>(p, stream);
   if constexpr (sizeof(T) == 4 && OUT == OUT_PAIR) return launch_tiles<T, A_INNER, B_INNER, OUT, TWO, 8, 4, 2, 2>(p, stream);
   else return launch_tiles<T, A_INNER, B_INNER, OUT, TWO, 4, 4, 2, 2>(p, stream);
 }
 
-template <class T, bool A_INNER, bool B_INNER, bool TWO = false> hipError_t launch_plain(bool large, ProductArgs const& p, hipStream_t stream) {
-  if (p.parts == 1) return launch_sized<T, A_INNER, B_INNER, OUT_PLAIN, TWO>(large, p, stream);
-  hipError_t const err = launch_sized<T, A_INNER, B_INNER, OUT_PARTS, TWO>(large, p, stream);
+template <class T, bool A_INNER, bool B_INNER, bool TWO = false> hipError_t launch_plain(Tile tile, ProductArgs const& p, hipStream_t stream) {
+  if (p.parts == 1) return launch_sized<T, A_INNER, B_INNER, OUT_PLAIN, TWO>(tile, p, stream);
+  hipError_t const err = launch_sized<T, A_INNER, B_INNER, OUT_PARTS, TWO>(tile, p, stream);
   if (err != hipSuccess) return err;
   hipLaunchKernelGGL(join_parts<T>, dim3(unsigned(p.rows), unsigned((p.columns + 1023) / 1024), unsigned(p.problems)), dim3(256),
                      0, stream, p);
   return hipGetLastError();
 }
 
-// The first products of few tiles, each cut along k (choose_pair); then the one of D dy.
-template <class T> hipError_t launch_pair_in_parts(bool large, ProductArgs const& p, hipStream_t stream) {
-  for (int q = 0; q < 2; q++) {
+// The first products of few tiles, cut along k, of wide tiles one after the other (choose_pair); then the one of D dy.
+template <class T> hipError_t launch_pair_in_parts(Tile tile, ProductArgs const& p, hipStream_t stream) {
+  hipError_t err = hipSuccess;
+  bool const together = sizeof(T) == 4 && p.pair_parts;
+  if constexpr (sizeof(T) == 4)
+    if (together) err = launch_tiles<T, false, false, OUT_PAIR_PARTS, false, 4, 4, 1, 4>(p, stream);
+  for (int q = 0; q < 2 && !together && err == hipSuccess; q++) {
     ProductArgs one = p;
     one.a[0] = p.a[q];
     one.sums = p.sums + q * p.parts * p.rows * p.ld_sums;
-    hipError_t const err = launch_sized<T, false, false, OUT_PARTS>(large, one, stream);
-    if (err != hipSuccess) return err;
+    err = launch_sized<T, false, false, OUT_PARTS>(tile, one, stream);
   }
+  if (err != hipSuccess) return err;
   hipLaunchKernelGGL(join_pair<T>, dim3(unsigned(p.rows), unsigned((p.columns + 1023) / 1024)), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
-template <class T> hipError_t launch_states_in_parts(bool large, ProductArgs const& p, hipStream_t stream) {
-  hipError_t const err = launch_sized<T, true, false, OUT_PARTS>(large, p, stream);
+template <class T> hipError_t launch_states_in_parts(Tile tile, ProductArgs const& p, hipStream_t stream) {
+  hipError_t const err = launch_sized<T, true, false, OUT_PARTS>(tile, p, stream);
   if (err != hipSuccess) return err;
   hipLaunchKernelGGL(join_states<T>, dim3(unsigned(p.rows), unsigned((p.columns + 1023) / 1024)), dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 
-template <class T> hipError_t launch_product_as(Form form, bool large, ProductArgs const& p, hipStream_t stream) {
+template <class T> hipError_t launch_product_as(Form form, Tile tile, ProductArgs const& p, hipStream_t stream) {
   switch (form) {
     case FORM_PAIR:
-      if (p.parts > 1) return launch_pair_in_parts<T>(large, p, stream);
-      return launch_sized<T, false, false, OUT_PAIR>(large, p, stream);
+      if (p.parts > 1) return launch_pair_in_parts<T>(tile, p, stream);
+      return launch_sized<T, false, false, OUT_PAIR>(tile, p, stream);
     case FORM_STATES:
-      if (p.parts > 1) return launch_states_in_parts<T>(large, p, stream);
-      return launch_sized<T, true, false, OUT_STATES>(large, p, stream);
-    case FORM_FORWARD: return launch_plain<T, false, false>(large, p, stream);
-    case FORM_INPUT: return launch_plain<T, true, false, true>(large, p, stream);
-    default: return launch_plain<T, true, true>(large, p, stream);
+      if (p.parts > 1) return launch_states_in_parts<T>(tile, p, stream);
+      return launch_sized<T, true, false, OUT_STATES>(tile, p, stream);
+    case FORM_FORWARD: return launch_plain<T, false, false>(tile, p, stream);
+    case FORM_INPUT: return launch_plain<T, true, false, true>(tile, p, stream);
+    default: return launch_plain<T, true, true>(tile, p, stream);
   }
 }
 

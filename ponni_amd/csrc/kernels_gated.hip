@@ -69,29 +69,37 @@ int64_t own_stride(int64_t columns, int64_t es) { return round_to(columns, 128 /
 //   16,000 columns      476 + 1114        462 + 1118   376 + 1183        377 + 835    384 + 839
 // and fp32 (128 x 128) 333-1001-77, 5000 columns: whole 159 + 846, chosen 120 + 234.  Gradients of narrow weights over many
 // columns are one or two tiles with a long sum: fp32 48-38-131, 274,418 columns, dG and dU in 16 parts 1138 + 6, in 218
-// 170 + 14.
+// 170 + 14.  Rows of a tile that are not there cost fp32 as much as others, so that narrow blocks take tiles of 64 rows (of a
+// pair 32 of each product) x 256 columns.  fp32, calls, tiles of 128 x 128 alone / with those (elementary products):
+//   2371-19-18 x 56,961 forward    558 / 176 (216)      64-64-64 x 500,000 forward     308 / 200 (655)
+//   2257-17-29 x 13,897 forward    152 / 54 (117)       800-20-600 x 46,000 training   811 / 486 (730)
 struct Choice {
-  bool large;
+  Tile tile;
   int parts;
+  bool pair;  // both products of a pair at a time
   double time;
 };
 constexpr int kMostParts = 256, kLeastSteps = 8;
 constexpr int64_t kMostSums = int64_t(256) * 256 * 256 * 4;  // bytes: of as many tiles as run at once
 
 Choice choose(int64_t es, int64_t rows, int64_t columns, int problems, int64_t steps, bool pair, bool may_split) {
-  Choice best{false, 1, 1e300};
-  for (int large = 0; large <= (es == 2 ? 1 : 0); large++) {
-    int64_t const bm = (large ? 256 : 128) / (pair && es == 2 ? 2 : 1), bn = large ? 256 : 128, at_once = large ? 256 : 512;
+  Choice best{TILE_128, 1, pair, 1e300};
+  for (Tile tile : {TILE_128, TILE_LARGE, TILE_NARROW}) {
+    bool const large = tile == TILE_LARGE, narrow = tile == TILE_NARROW;
+    if ((large && es != 2) || (narrow && es != 4)) continue;
+    int64_t const bm = narrow ? (pair ? 32 : 64) : (large ? 256 : 128) / (pair && es == 2 ? 2 : 1), bn = tile != TILE_128 ? 256 : 128,
+                  at_once = large ? 256 : 512;
     int64_t const tiles = (rows + bm - 1) / bm * ((columns + bn - 1) / bn) * problems;
     for (int parts = 1; parts <= kMostParts; parts += parts < 16 ? 1 : parts / 4) {
-      if (parts > 1 && (!may_split || steps / parts < kLeastSteps || tiles * parts > at_once)) break;
+      if (parts > 1 && (!(may_split || (pair && narrow)) || steps / parts < kLeastSteps || tiles * parts > at_once)) break;
       int64_t const groups = tiles * parts, rounds = (groups + at_once - 1) / at_once;
       // (a tile of a pair in fp32 is both of them)
-      double const alone = es == 4 ? (pair ? 2.2 : 1.3) : large ? 1.0 : 0.4, two = es == 4 ? (pair ? 3.6 : 2.3) : 0.62;
+      bool const both = pair && es == 4 && !narrow;
+      double const alone = es == 4 ? (both ? 2.2 : 1.3) : large ? 1.0 : 0.4, two = es == 4 ? (both ? 3.6 : 2.3) : 0.62;
       double const step = large || groups <= 256 ? alone : two;
-      double time = double(rounds) * (double((steps + parts - 1) / parts) * step + (pair && es == 4 ? 18.0 : 5.0));
-      if (parts > 1) time += 4.0 + 0.05 * double(parts) + double(parts + 1) * double(rows * columns * problems) * 4.0 / 3e6;
-      if (time < best.time) best = {large != 0, parts, time};
+      double time = double(rounds) * (double((steps + parts - 1) / parts) * step + (both ? 18.0 : pair && es == 4 ? 10.0 : 5.0));
+      if (parts > 1) time += 4.0 + 0.05 * double(parts) + double(parts + 1) * double(rows * columns * problems * (pair ? 2 : 1)) * 4.0 / 3e6;
+      if (time < best.time) best = {tile, parts, pair, time};
     }
   }
   return best;
@@ -167,7 +175,7 @@ template <class T> struct Run {
     int64_t const steps = (form == FORM_INPUT ? 2 : 1) * ((p.k + STEP - 1) / STEP);
     Choice const c = form == FORM_PAIR ? choose_pair(ES, p.rows, p.columns, steps)
                                        : choose(ES, p.rows, p.columns, p.problems, steps, false, true);
-    p.parts = c.parts;
+    p.parts = c.parts, p.pair_parts = c.pair && c.parts > 1;
     Taker const before = work;  // (the sums are read before the next product begins)
     if (c.parts > 1) {
       p.ld_sums = round_to(p.columns, 4);
@@ -176,7 +184,7 @@ template <class T> struct Run {
     }
     err = (std::is_same_v<T, float>      ? launch_product_f32
            : std::is_same_v<T, _Float16> ? launch_product_f16
-                                         : launch_product_bf16)(form, c.large, p, stream);
+                                         : launch_product_bf16)(form, c.tile, p, stream);
     work = before;
   }
   void sums(RowSums const& a, int64_t columns) {

@@ -2,8 +2,8 @@
 #include "gated_thin.h"
 
 namespace ponni_hip {
-hipError_t launch_product_f32(Form form, bool large, ProductArgs const& p, hipStream_t stream) {
-  return launch_product_as<float>(form, large, p, stream);
+hipError_t launch_product_f32(Form form, Tile tile, ProductArgs const& p, hipStream_t stream) {
+  return launch_product_as<float>(form, tile, p, stream);
 }
 hipError_t launch_thin_f32(ThinArgs const& hidden, ThinArgs const& last, hipStream_t stream) {
   return launch_thin_as<float>(hidden, last, stream);

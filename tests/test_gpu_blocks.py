@@ -647,6 +647,14 @@ def test_gated_fp32_of_many_tiles(cuda, sizes, b):
     check_gated(cuda, sizes, b, "silu", "f32", bias=b % 2 == 1, pad=b % 5, shift=b % 2)
 
 
+@pytest.mark.parametrize("sizes", [(40, 31, 33), (300, 32, 64), (333, 33, 65), (77, 64, 20), (900, 65, 5), (2100, 30, 127)])
+def test_gated_fp32_narrow_tiles(cuda, sizes):
+    """Tiles of 64 rows (of a pair 32 of each) by 256 columns: either side of their borders, in one piece and cut along k."""
+    for b in (255, 256, 257, 700, 3001):
+        for act in ("tanh", "gelu"):
+            check_gated(cuda, sizes, b, act, "f32", bias=b % 2 == 1, pad=b % 4, shift=b % 3, seed=b, wpad=b % 3)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("sizes,b", [((20, 19, 18), 60_001), ((130, 40, 70), 30_002)])
 def test_gated_narrow_weights_over_many_columns(cuda, sizes, b, dtype):
