@@ -696,6 +696,11 @@ int ponni_gated_backward(const ponni_gated* block, const void* x, int64_t ld_x, 
                          const void* dy, int64_t ld_dy, int64_t columns, const ponni_gated_gradients* gradients,
                          void* workspace, int64_t workspace_bytes, hipStream_t stream);
 int64_t ponni_gated_backward_workspace_bytes(const ponni_gated* block, int64_t columns);
+/* What one call with these arrays needs, which is less: of F16 and BF16 the queries above count copies of the arrays with
+ * columns, made of those whose rows do not all begin at multiples of 4 bytes, and of either type room for h, which is in the
+ * states where there are any.  dy null: of a forward call; states null: without states. */
+int64_t ponni_gated_call_workspace_bytes(const ponni_gated* block, const void* x, int64_t ld_x, const void* states,
+                                         int64_t ld_states, const void* dy, int64_t ld_dy, int64_t columns);
 
 /* What stands between two blocks, over columns of n features:
  *   state = residual + scale * gate * after(x),  normed = before(state)

@@ -321,6 +321,8 @@ def lib() -> ctypes.CDLL:
     L.ponni_gated_backward.argtypes = [gated, vp, i64, vp, i64, vp, i64, i64, ctypes.POINTER(GatedGradientArrays), vp, i64, vp]
     L.ponni_gated_backward_workspace_bytes.restype = i64
     L.ponni_gated_backward_workspace_bytes.argtypes = [gated, i64]
+    L.ponni_gated_call_workspace_bytes.restype = i64
+    L.ponni_gated_call_workspace_bytes.argtypes = [gated, vp, i64, vp, i64, vp, i64, i64]
     L.ponni_residual_norm_forward.restype = ctypes.c_int
     L.ponni_residual_norm_forward.argtypes = [norm, vp]
     L.ponni_residual_norm_backward.restype = ctypes.c_int

@@ -129,10 +129,10 @@ class GatedInference:
         else:
             ld_y = _array(y, "y", x, self.n_out, columns)
         L = A.lib()
-        need = L.ponni_gated_workspace_bytes(self._ref, columns)
+        at, ld_s = (None, 0) if states is None else (states.data_ptr(), states.stride(0))
+        need = L.ponni_gated_call_workspace_bytes(self._ref, x.data_ptr(), ld_x, at, ld_s, None, 0, columns)
         work, kept = _work(x, need)
-        _call(x, L.ponni_gated_forward, self._ref, x.data_ptr(), ld_x, y.data_ptr(), ld_y,
-              None if states is None else states.data_ptr(), 0 if states is None else states.stride(0), columns, work, need)
+        _call(x, L.ponni_gated_forward, self._ref, x.data_ptr(), ld_x, y.data_ptr(), ld_y, at, ld_s, columns, work, need)
         return y
 
     def forward_batch_parallel(self, x, y=None):
@@ -166,7 +166,8 @@ class GatedInference:
         at = [None if t is None else t.data_ptr() for t in (d.x, d.gate, d.up, d.down, d.gate_bias, d.up_bias, d.down_bias)]
         g = A.GatedGradientArrays(at[0], columns, *at[1:4], self.n_hidden, self.n_hidden, self.n_out, *at[4:])
         L = A.lib()
-        need = L.ponni_gated_backward_workspace_bytes(self._ref, columns)
+        need = L.ponni_gated_call_workspace_bytes(self._ref, x.data_ptr(), ld_x, states.data_ptr(), ld_s, dy.data_ptr(), ld_dy,
+                                                  columns)
         work, kept = _work(dy, need)
         _call(dy, L.ponni_gated_backward, self._ref, x.data_ptr(), ld_x, states.data_ptr(), ld_s, dy.data_ptr(), ld_dy,
               columns, ctypes.byref(g), work, need)

@@ -76,7 +76,8 @@ int gated_impl(ponni_gated const* b, void const* x, int64_t ld_x, void* y, int64
   if (st != PONNI_OK) return st;
   if (!b->gate || !b->up || !b->down) return fail(PONNI_ERR_INVALID_ARGUMENT, "a weight array is null");
   if (x == nullptr || y == nullptr) return fail(PONNI_ERR_INVALID_ARGUMENT, "input or output pointer is null");
-  int64_t const need = gated_workspace_bytes(*b, columns, false), es = element_bytes(b->dtype);
+  GatedArrays const arrays{x, ld_x, states, ld_states, nullptr, 0};
+  int64_t const need = gated_workspace_bytes(*b, columns, false, &arrays), es = element_bytes(b->dtype);
   if ((st = check_workspace(workspace, workspace_bytes, need)) != PONNI_OK) return st;
   if ((st = check_strides({ld_x, ld_y, states ? ld_states : 0, b->ld_gate, b->ld_up, b->ld_down})) != PONNI_OK) return st;
   st = check_arrays({{"x", x, b->n_in, columns, ld_x, es},
@@ -102,7 +103,8 @@ int gated_backward_impl(ponni_gated const* b, void const* x, int64_t ld_x, void 
   if (d == nullptr) return fail(PONNI_ERR_INVALID_ARGUMENT, "gradients is null");
   if (!b->gate || !b->up || !b->down) return fail(PONNI_ERR_INVALID_ARGUMENT, "a weight array is null");
   if (!x || !states || !dy) return fail(PONNI_ERR_INVALID_ARGUMENT, "x, states or dy is null");
-  int64_t const need = gated_workspace_bytes(*b, columns, true), es = element_bytes(b->dtype);
+  GatedArrays const arrays{x, ld_x, states, ld_states, dy, ld_dy};
+  int64_t const need = gated_workspace_bytes(*b, columns, true, &arrays), es = element_bytes(b->dtype);
   if ((st = check_workspace(workspace, workspace_bytes, need)) != PONNI_OK) return st;
   st = check_strides({ld_x, ld_states, ld_dy, b->ld_gate, b->ld_up, b->ld_down, d->x ? d->ld_x : 0, d->gate ? d->ld_gate : 0,
                       d->up ? d->ld_up : 0, d->down ? d->ld_down : 0});
@@ -333,6 +335,13 @@ int ponni_gated_backward(const ponni_gated* block, const void* x, int64_t ld_x, 
 int64_t ponni_gated_backward_workspace_bytes(const ponni_gated* block, int64_t columns) {
   return size_or_refusal([&] { return check_gated_sizes(block, columns); },
                          [&] { return gated_workspace_bytes(*block, columns, true); });
+}
+
+int64_t ponni_gated_call_workspace_bytes(const ponni_gated* block, const void* x, int64_t ld_x, const void* states,
+                                         int64_t ld_states, const void* dy, int64_t ld_dy, int64_t columns) {
+  GatedArrays const arrays{x, ld_x, states, ld_states, dy, ld_dy};
+  return size_or_refusal([&] { return check_gated_sizes(block, columns); },
+                         [&] { return gated_workspace_bytes(*block, columns, dy != nullptr, &arrays); });
 }
 
 int ponni_residual_norm_forward(const ponni_residual_norm* r, hipStream_t stream) {

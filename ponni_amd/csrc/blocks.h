@@ -35,7 +35,17 @@ hipError_t launch_residual_norm_backward(ponni_residual_norm const& r, ponni_res
 
 // -- gated blocks -----------------------------------------------------------------------
 
-int64_t gated_workspace_bytes(ponni_gated const& b, int64_t columns, bool backward);
+// The arrays with columns of a call (dy null: forward).
+struct GatedArrays {
+  void const* x;
+  int64_t ld_x;
+  void const* states;
+  int64_t ld_states;
+  void const* dy;
+  int64_t ld_dy;
+};
+// Of a call with those arrays; null: of any call.
+int64_t gated_workspace_bytes(ponni_gated const& b, int64_t columns, bool backward, GatedArrays const* arrays = nullptr);
 hipError_t launch_gated(ponni_gated const& b, int act, void const* x, int64_t ld_x, void* y, int64_t ld_y, void* states,
                         int64_t ld_states, int64_t columns, void* workspace, hipStream_t stream);
 hipError_t launch_gated_backward(ponni_gated const& b, int act, void const* x, int64_t ld_x, void const* states,

@@ -135,24 +135,30 @@ int64_t sums_bytes(int64_t rows, int64_t columns, int problems, int64_t steps) {
   return parts < 2 ? 0 : std::min(kMostSums, parts * problems * rows * round_to(columns, 4) * 4);
 }
 
+// Whether an array is read where it is: all rows at multiples of 4 bytes.
+bool in_place(void const* p, int64_t rows, int64_t ld, int64_t es) {
+  return reinterpret_cast<uint64_t>(p) % 4 == 0 && (rows == 1 || ld * es % 4 == 0);
+}
+// The same of two arrays of one shape, which are read at one stride.
+bool pair_in_place(void const* a, int64_t ld_a, void const* b, int64_t ld_b, int64_t rows, int64_t es) {
+  return in_place(a, rows, ld_a, es) && in_place(b, rows, ld_b, es) && (rows == 1 || ld_a == ld_b);
+}
+
 // One call's products.
 template <class T> struct Run {
   Taker work;
   hipStream_t stream;
   hipError_t err = hipSuccess;
 
-  static bool in_place(Matrix const& m) {
-    return reinterpret_cast<uint64_t>(m.p) % 4 == 0 && (m.rows == 1 || m.ld * int64_t(sizeof(T)) % 4 == 0);
-  }
   Side side(Matrix const& m) {
-    if (!in_place(m)) return copied(m);
+    if (!in_place(m.p, m.rows, m.ld, sizeof(T))) return copied(m);
     constexpr int64_t ES = sizeof(T);
     int64_t const ld = m.rows == 1 ? round_to(m.columns, 4 / ES) : m.ld;
     return {static_cast<char const*>(m.p), ld * ES, round_to(((m.rows - 1) * ld + m.columns) * ES, 4), m.rows};
   }
   // Two arrays of one shape, of one stride.
   void sides(Matrix const& a, Matrix const& b, Side (&out)[2]) {
-    bool const both = in_place(a) && in_place(b) && (a.rows == 1 || a.ld == b.ld);
+    bool const both = pair_in_place(a.p, a.ld, b.p, b.ld, a.rows, sizeof(T));
     out[0] = both ? side(a) : copied(a), out[1] = both ? side(b) : copied(b);
   }
   Side copied(Matrix const& m) {
@@ -238,22 +244,32 @@ int64_t steps_of(int64_t k, int64_t es) { return (k + 64 / es - 1) / (64 / es); 
 
 }  // namespace
 
-int64_t gated_workspace_bytes(ponni_gated const& b, int64_t columns, bool backward) {
+int64_t gated_workspace_bytes(ponni_gated const& b, int64_t columns, bool backward, GatedArrays const* arrays) {
   int64_t const es = element(b), i = b.n_in, h = b.n_hidden, o = b.n_out;
+  bool const states = arrays != nullptr && arrays->states != nullptr;
+  if (!backward && arrays != nullptr && !states && columns <= most_thin(b)) return thin_plan(b, columns).bytes();
   Taker t{nullptr};
-  // Copies of operands, for the arrays that need them.
-  t.take(aligned_bytes(i, h, es));
-  t.take(aligned_bytes(i, h, es));
-  t.take(aligned_bytes(h, o, es));
-  t.take(aligned_bytes(i, columns, es));
-  t.take(aligned_bytes(h, columns, es));  // h itself, or a copy of the states'
+  auto copy = [&](bool needed, int64_t rows, int64_t of) {
+    if (needed) t.take(aligned_bytes(rows, of, es));
+  };
+  // Of an array with columns: where it is not known, any of 16 bits may need a copy.
+  auto moved = [&](void const* p, int64_t rows, int64_t ld) { return arrays != nullptr ? !in_place(p, rows, ld, es) : es == 2; };
+  bool const pair = pair_in_place(b.gate, b.ld_gate, b.up, b.ld_up, i, es);
+  GatedArrays const a = arrays != nullptr ? *arrays : GatedArrays{};
+  copy(!pair, i, h);
+  copy(!pair, i, h);
+  copy(!in_place(b.down, h, b.ld_down, es), h, o);
+  copy(moved(a.x, i, a.ld_x), i, columns);
   if (!backward) {
+    copy(!states || moved(a.states, h, a.ld_states), h, columns);  // h itself, or a copy of the states'
     t.take(std::max(sums_bytes(o, columns, 1, steps_of(h, es)), 2 * sums_bytes(h, columns, 1, steps_of(i, es))));
+    if (arrays != nullptr) return t.used;
     // (the slices become fewer past 8 columns)
     return std::max({t.used, thin_plan(b, std::min<int64_t>(columns, 8)).bytes(),
                      thin_plan(b, std::min(columns, most_thin(b))).bytes()});
   }
-  t.take(aligned_bytes(o, columns, es));
+  copy(moved(a.states, h, a.ld_states), h, columns);
+  copy(moved(a.dy, o, a.ld_dy), o, columns);
   t.take(aligned_bytes(2 * h, columns, es));  // dg, du
   t.take(std::max({sums_bytes(i, columns, 1, 2 * steps_of(h, es)), sums_bytes(i, h, 2, steps_of(columns, es)),
                    sums_bytes(h, o, 1, steps_of(columns, es)), sums_bytes(h, columns, 1, steps_of(o, es))}));

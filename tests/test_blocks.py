@@ -91,6 +91,56 @@ def test_gated_work_buffers_serve_fewer_columns(dtype):
         assert L.ponni_gated_workspace_bytes(ctypes.byref(b), 0) == -1
 
 
+def gated_needs(b, columns, es, states=True, backward=True, odd=()):
+    """What a call needs: those arrays of `odd` have rows that do not all begin at multiples of 4 bytes."""
+    ld = {k: columns + columns % 2 + (k in odd) for k in ("x", "states", "dy")}
+    at = {"x": fake(4), "states": fake(5) if states else None, "dy": fake(6) if backward else None}
+    return A.lib().ponni_gated_call_workspace_bytes(ctypes.byref(b), *(v for k in ("x", "states", "dy") for v in (at[k], ld[k])), columns)
+
+
+@pytest.mark.parametrize("dtype,es", [(A.F32, 4), (A.F16, 2), (A.BF16, 2)])
+def test_gated_work_buffers_hold_what_is_used(dtype, es):
+    """Copies are counted where they are made: of 16-bit arrays at odd places, of pairs of other strides; room for h where
+    there are no states."""
+    L, columns = A.lib(), 32_768
+    i, h, o = 2048, 8192, 1024
+    b = block(i, h, o, dtype=dtype, act=P.Silu(h), ld_gate=h, ld_up=h, ld_down=o)
+    sums = 2 * 64 << 20  # most of a product's parts, both of a pair
+    forward, backward = h * columns * es, 2 * h * columns * es
+    assert gated_needs(b, columns, es, states=False, backward=False) <= forward + sums
+    assert gated_needs(b, columns, es, backward=False) <= sums
+    assert gated_needs(b, columns, es) <= backward + sums
+    for odd, rows in (("x", i), ("states", h), ("dy", o)):
+        more = gated_needs(b, columns, es, odd=(odd,)) - gated_needs(b, columns, es)
+        assert more == (0 if es == 4 else rows * columns * es)
+    # any call: of 16 bits with copies of all three
+    copies = 0 if es == 4 else (i + h + o) * columns * es
+    assert L.ponni_gated_backward_workspace_bytes(ctypes.byref(b), columns) == gated_needs(b, columns, es) + copies
+    # the weights: a 16-bit one at an odd place, and a pair of two strides, which is read at one
+    down = block(i, h, o, dtype=dtype, act=P.Silu(h), ld_gate=h, ld_up=h, ld_down=o + 1)
+    assert gated_needs(down, columns, es) - gated_needs(b, columns, es) == (0 if es == 4 else h * o * es)
+    pair = block(i, h, o, dtype=dtype, act=P.Silu(h), ld_gate=h, ld_up=h + 2, ld_down=o)
+    assert gated_needs(pair, columns, es) - gated_needs(b, columns, es) == 2 * i * h * es
+
+
+@pytest.mark.parametrize("dtype,es", [(A.F32, 4), (A.F16, 2), (A.BF16, 2)])
+def test_gated_work_buffers_of_calls(dtype, es):
+    """No call needs more than its number of columns says, and one of few columns needs no room of the weights' size."""
+    L = A.lib()
+    for sizes in ((8, 12, 6), (333, 1001, 77), (1024, 4096, 1024), (20, 19, 33)):
+        b = block(*sizes, dtype=dtype, act=P.Relu(sizes[1]), ld_gate=sizes[1], ld_up=sizes[1], ld_down=sizes[2])
+        for columns in (1, 8, 9, 32, 33, 200, 512, 513, 4097, 70_001, 1_000_000):
+            any_forward, any_backward = (size(ctypes.byref(b), columns) for size in
+                                         (L.ponni_gated_workspace_bytes, L.ponni_gated_backward_workspace_bytes))
+            for odd in ((), ("x",), ("x", "states"), ("x", "states", "dy")):
+                for states in (False, True):
+                    assert 0 <= gated_needs(b, columns, es, states, False, odd) <= any_forward
+                assert 0 <= gated_needs(b, columns, es, odd=odd) <= any_backward
+    b = block(1024, 4096, 1024, dtype=dtype, act=P.Relu(4096), ld_gate=4096, ld_up=4096, ld_down=1024)
+    assert gated_needs(b, 1, es, states=False, backward=False) < 3 << 20
+    assert gated_needs(b, 0, es) == -1
+
+
 def residual_norm(n=8, columns=10, dtype=A.F32, after=A.NORM_RMS, before=A.NORM_LAYER, **kw):
     r = A.ResidualNormArrays(n, dtype, columns, A.Norm(after, 1e-5), A.Norm(before, 1e-5), 1.0, fake(1), columns, fake(2),
                              columns, None, None, columns, fake(3), columns, fake(4), columns, fake(5))

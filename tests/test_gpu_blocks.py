@@ -856,6 +856,52 @@ def test_gated_work_buffer_of_more_columns(cuda):
         assert bool((work[need:] == 7).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gated_calls_keep_to_what_they_ask_for(cuda, dtype):
+    """The work buffer of a call with these arrays, whichever of them has to be copied first: enough, and no byte behind it
+    is written."""
+    import ctypes
+
+    import torch
+
+    t, L = torch_dtype(dtype), A.lib()
+    stream = torch.cuda.current_stream().cuda_stream
+    for (i, h, o), wpad in (((37, 70, 41), 1), ((300, 260, 50), 0), ((64, 33, 20), 3)):
+        ws = [tensor(np.random.default_rng(h).uniform(-0.3, 0.3, s), dtype, cuda, wpad) for s in ((i, h), (i, h), (h, o))]
+        model = P.create_gated_model(*ws, P.Gelu(h, True))
+        for b in (1, 20, 130, 1501):
+            for odd in ((), ("x",), ("states",), ("dy",), ("x", "states", "dy")):
+                def array(name, rows):
+                    return tensor(torch.randn((rows, b)).numpy(), dtype, cuda, b % 2, 1) if name in odd else \
+                        tensor(torch.randn((rows, b)).numpy(), dtype, cuda, b % 2, 0)
+
+                x, dy, states = array("x", i), array("dy", o), array("states", 3 * h)
+                y = torch.empty((o, b), dtype=t, device=cuda)
+
+                def call(fn, s, d, *args):
+                    need = L.ponni_gated_call_workspace_bytes(model._ref, x.data_ptr(), x.stride(0), s, states.stride(0), d,
+                                                              dy.stride(0), b)
+                    work = torch.full((need + 4096,), 255, dtype=torch.uint8, device=cuda)  # (NaN)
+                    work[need:] = 7
+                    assert fn(model._ref, x.data_ptr(), x.stride(0), *args, b, *rest, work.data_ptr(), need, stream) == 0
+                    assert bool((work[need:] == 7).all())
+
+                rest = ()
+                call(L.ponni_gated_forward, None, None, y.data_ptr(), b, None, 0)
+                assert torch.equal(y, model.forward_batch_parallel(x))
+                call(L.ponni_gated_forward, states.data_ptr(), None, y.data_ptr(), b, states.data_ptr(), states.stride(0))
+                y2, states2 = model.forward_with_states(x)
+                assert torch.equal(y, y2) and torch.equal(states, states2)
+                want = model.backward(x, states2, dy)
+                out = [torch.empty_like(v) for v in (want.x, want.gate, want.up, want.down)]
+                g = A.GatedGradientArrays(out[0].data_ptr(), b, *(v.data_ptr() for v in out[1:]), h, h, o)
+                rest = (ctypes.byref(g),)
+                call(L.ponni_gated_backward, states.data_ptr(), dy.data_ptr(), states.data_ptr(), states.stride(0), dy.data_ptr(),
+                     dy.stride(0))
+                for v, w in zip(out, (want.x, want.gate, want.up, want.down)):
+                    assert torch.equal(v, w)
+
+
 def test_gated_gradient_by_differences(cuda):
     r = np.random.default_rng(9)
     i, h, o, b = 6, 9, 5, 4
