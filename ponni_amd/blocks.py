@@ -368,23 +368,19 @@ def log_probabilities(logits, targets=None, top_k: int = 0) -> LogProbabilities:
         _vector(targets, "targets", columns, torch.int32, logits)
     L = A.lib()
     need = L.ponni_log_probs_workspace_bytes(classes, columns, top_k)
-    if need < 0:
-        raise A.PonniError(A.PONNI_ERR_INVALID_ARGUMENT, L.ponni_last_error().decode())
+    work, kept = _work(logits, need)  # (of its own: the results outlive it)
     r = LogProbabilities()
     r.logits, r.targets = logits.detach(), targets
-    # One allocation: the results, and a work buffer behind them at 16 bytes.
-    n = columns * (2 + (targets is not None) + 2 * top_k)
-    buffer = torch.empty((n + 3) // 4 * 4 + need // 4, dtype=torch.float32, device=logits.device)
-    rows = buffer[:n].view(-1, columns)
+    rows = torch.empty((2 + (targets is not None) + 2 * top_k, columns), dtype=torch.float32, device=logits.device)
     r.entropy, r.log_normalizer = rows[0], rows[1]
     r.log_probs = rows[2] if targets is not None else None
     first = 2 + (targets is not None)
     r.top_log_probs = rows[first:first + top_k] if top_k else None
     r.top_classes = rows[first + top_k:].view(torch.int32) if top_k else None
-    at = buffer.data_ptr()
+    at = rows.data_ptr()
     of = lambda row: at + 4 * columns * row  # noqa: E731
     r._p = A.LogProbsArrays(classes, columns, logits.data_ptr(), ld, codes[logits.dtype], top_k,
                             None if targets is None else targets.data_ptr(), None if targets is None else of(2), of(0), of(1),
                             of(first + top_k) if top_k else None, of(first) if top_k else None)
-    _call(logits, L.ponni_log_probs_forward, ctypes.byref(r._p), at + (n + 3) // 4 * 16, need)
+    _call(logits, L.ponni_log_probs_forward, ctypes.byref(r._p), work, need)
     return r

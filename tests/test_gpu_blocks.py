@@ -98,6 +98,21 @@ def test_log_probabilities_without_targets_or_masks(cuda):
     check_logp(cuda, 100, 1, 2, "f32", masked=0.0, targets=False)
 
 
+def test_log_probabilities_hold_no_work_buffer(cuda):
+    """What the results keep allocated is their own size (up to the allocator's blocks of 512 bytes)."""
+    import torch
+
+    for c, b, k in ((131_072, 1, 8), (65_536, 256, 0), (20_000, 40, 16)):
+        x = torch.randn((c, b), device=cuda).bfloat16()
+        targets = torch.zeros(b, dtype=torch.int32, device=cuda)
+        P.log_probabilities(x, targets, k)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated(cuda)
+        r = P.log_probabilities(x, targets, k)
+        assert torch.cuda.memory_allocated(cuda) - before <= 4 * b * (3 + 2 * k) + 512
+        assert r.log_probs.shape == (b,)
+
+
 def test_equal_logits(cuda):
     """Ties go to the lower class across lanes, waves and workgroups."""
     import torch
