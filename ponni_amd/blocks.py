@@ -336,7 +336,8 @@ class LogProbabilities:
 
     def backward(self, d_log_probs=None, d_entropy=None, d_log_normalizer=None, out=None):
         """The gradient of the logits from those of log_probs, entropy and log_normalizer (float32 [columns], None:
-        zero); out: a tensor for it, of the logits' shape and type, or the logits themselves."""
+        zero); out: a tensor for it, of the logits' shape and type, or the logits themselves, which every gradient reads:
+        then it is the last one."""
         import torch
 
         classes, columns = self.logits.shape

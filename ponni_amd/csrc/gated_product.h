@@ -22,10 +22,10 @@
 //
 // Bound by the matrix cores where k is long, and by the outputs (three or two arrays, with the states read)
 // beside them where it is short: all workgroups come to their outputs together.  bf16 1024-4096-1024, 16,384 columns, us (PFLOP/s):
-// g, u and h 315 (0.87), y 114 (1.21), dg and du 279 (0.49), dx 270 (1.02), dG and dU 256 + 12 (1.03),
+// g, u and h 306 (0.90), y 110 (1.25), dg and du 275 (0.50), dx 252 (1.09), dG and dU 256 + 12 (1.03),
 // dD 147 + 14 (0.85); a library's product of 8192 x 8192 x 8192 1.12.  fp16 2048-8192-2048,
-// 32,768: h 1961 (1.12), y 860 (1.28).  fp32 1024-4096-1024, 16,384: 136 to 142 TFLOP/s of 154; 333-1001-77, 5,003: 66 to
-// 83, few tiles and short sums.
+// 32,768: h 1848 (1.19), y 819 (1.34).  fp32 1024-4096-1024, 16,384: 136 to 142 TFLOP/s of 154; 333-1001-77, 5,003: 66 to
+// 83, few tiles and short sums; 2371-19, 56,961: 165 us, 3.3 TB/s of x.
 #pragma once
 
 #include <algorithm>

@@ -11,9 +11,14 @@
 // lanes, waves and workgroups that share columns join their (m, z, q) in a fixed
 // order.  The largest logits are lists in descending order, of equal values by
 // class; two lists are joined by a bitonic step.
-// Bound by the logits' way from memory; 11 VALU operations an element beside it.  bf16 65,536 classes x 4096: 150 + 5 us, 3.5
-// TB/s, the gradient 205, 5.2 TB/s read and written; fp32 10 x 4,194,304 with the 3 largest: 100, 3.4 TB/s of logits and
-// results; one bf16 column of 131,072 with the 8 largest: 15 + 7, latency.
+// The hardware's 2^x and log2 in every type, of a reference up to 4 below the largest: fp32 results are off by up to twice what
+// a sum of exact powers is (10 classes: 1.1e-7 of their size, where elementary operations are off by 6.4e-8); the gradient in
+// fp32 takes exp_f32.
+// Bound by the logits' way from memory; 11 VALU operations an element beside it.  By kernel (a trace, with the gradient between
+// two calls): bf16 65,536 classes x 4096: 154 + 5 us, 3.5 TB/s, the gradient 205, 5.2 TB/s read and written; fp32 10 x 4,194,304
+// with the 3 largest: 95, 3.5 TB/s of logits and results; one bf16 column of 131,072 with the 8 largest: 14 + 8, latency.
+// The figures beside the rules below are of calls of one kind one after the other, which leave part of the logits
+// in the caches: 135 us for the 154 + 5, and 229 for the gradient's 205.
 #include <cmath>
 
 #include "activations.h"
@@ -420,7 +425,7 @@ template <class T, int NC> __global__ __launch_bounds__(kThreads) void logp_back
 
 // -- launches -----------------------------------------------------------------------------
 
-// Workgroups that share columns, at most (1024 / 512 / 256: bf16 65,536 x 4096 123 / 142 / 239 us).
+// Workgroups that share columns, at most (1024 / 512 / 256: bf16 65,536 x 4096 135 / 146 / 248 us).
 constexpr int64_t kMostGroups = 1024, kMostParts = kMostGroups * 64;
 struct Shape {
   int columns;  // of a lane: 16 bytes of a row, half as many beside lists of 5 to 16
@@ -435,9 +440,9 @@ Shape shape_of(int64_t classes, int64_t columns, int32_t dtype, int32_t top_k) {
   Shape s{};
   s.columns = columns < wide ? 1 : k == 0 ? wide : k <= 8 ? 4 : 2;
   int64_t const lanes = (columns + s.columns - 1) / s.columns;
-  // Few classes: every lane takes all rows of its columns (us with / without: bf16 64 x 1,000,000 42 / 93, fp32 10 x
-  // 4,194,304 with the 3 largest 100 / 233, without them 87 / 79).  Else 128 bytes of a row across (128 / 64 / 32 bytes: bf16 65,536 x
-  // 4096 123 / 150 / 222, 1000 x 262,144 with the 4 largest 202 / 389 / 637).
+  // Few classes: every lane takes all rows of its columns (us with / without: bf16 64 x 1,000,000 43 / 91, fp32 10 x
+  // 4,194,304 with the 3 largest 96 / 226, without them 83 / 78).  Else 128 bytes of a row across (128 / 64 / 32 bytes: bf16 65,536 x
+  // 4096 135 / 149 / 221, 1000 x 262,144 with the 4 largest 212 / 250 / 388).
   int const line = s.columns == 1 || s.columns == wide ? 3 : s.columns * 2 == wide ? 4 : 5;
   if (classes <= 64 && lanes > 64) {
     s.lane_columns = 8;
@@ -544,8 +549,8 @@ hipError_t launch_logp_backward(ponni_log_probs const& p, float const* d_log_pro
   int64_t const across = int64_t(nc) << a.lane_columns, turn = (kThreads >> a.lane_columns) * (nc >= 4 ? 4 : 8);
   int64_t const all_tiles = (p.columns + across - 1) / across;
   int64_t const turns = (p.classes + turn - 1) / turn;
-  // A workgroup takes four turns, unless the grid is small (1 / 4 / 8 / 32 turns: bf16 65,536 x 4096 268 / 228 / 234 / 248 us,
-  // 1000 x 262,144 254 / 232 / 236 / 237, fp32 30,000 x 4000 165 / 177 / 185 / 184).
+  // A workgroup takes four turns, unless the grid is small (1 / 4 / 8 / 32 turns: bf16 65,536 x 4096 241 / 229 / 235 / 249 us,
+  // 1000 x 262,144 255 / 235 / 238 / 238, fp32 30,000 x 4000 165 / 178 / 186 / 186).
   int64_t const parts = std::max<int64_t>(1, std::min(turns, std::max<int64_t>(2048 / all_tiles, (turns + 3) / 4)));
   a.rows = (turns + parts - 1) / parts * turn;
   int64_t const groups = (p.classes + a.rows - 1) / a.rows;

@@ -17,9 +17,9 @@
 // Columns of more features than the registers hold (shape_of) are read again for each sum, 128 bytes of a row at a time.
 //
 // Bound by bytes: what a tile reads waits for its sums, which workgroups of the same CU fill up to where registers end.
-// bf16, 1024 features x 65,536, rms norms after and before, a gate for each feature: 170 us, 3.2 TB/s; its gradients 432.
-// fp32, 333 x 40,003 (rows at any 4 bytes), all inputs: 98 us, 2.7 TB/s; gradients 174 + 13.  fp16, 4096 x 16,384 (read
-// again): 170 us; gradients 280 + 9.  One column of 4096: 6.6 us.
+// By kernel: bf16, 1024 features x 65,536, rms norms after and before, a gate for each feature: 163 us, 3.3 TB/s; its gradients
+// 439 + 15.  fp32, 333 x 40,003 (rows at any 4 bytes), all inputs: 89 us, 3.0 TB/s; gradients 168 + 12.  fp16, 4096 x 16,384 (read
+// again): 172 us; gradients 284 + 9.  One column of 4096: 6.2 us.
 #pragma once
 
 #include <algorithm>
@@ -488,7 +488,7 @@ inline Shape shape_of(int32_t n, int64_t columns, int32_t dtype, int max_steps, 
   auto tiles_at = [&](int l) { return (lanes + (1 << l) - 1) >> l; };
   while (s.lane_columns > 0 && tiles_at(s.lane_columns) < 256) s.lane_columns--;
   // In registers at 128 bytes of a row or down to `narrowest` (3: 128, 1: 32): the kernel that reads whole lines again reads
-  // more, narrower pieces come slower.  us in registers / read again, 67 M elements: forward bf16, rms norms, n = 1024
+  // more, narrower pieces come slower.  us (calls one after the other) in registers / read again, 67 M elements: forward bf16, rms norms, n = 1024
   // (128 bytes) 151 / 170, 2048 (64) 162 / 179, 4096 (32) 285 / 191, with a gate layer norms 2048 (32) 274 / 322;
   // backward fp32 rms norms 1024 (64) 561 / 833, 2048 (32) 771 / 865, a norm before alone 1024 (64) 552 / 542, 2048 (32)
   // 673 / 589; backward bf16 rms norms 2048 (32) 498 / 413, layer norms 700 (64) 588 / 453, a norm before alone 4096 (16
